@@ -559,6 +559,87 @@ int dls_l1_mse_psnr(int n_images, int64_t n_per_image, const float* pred, const 
                     float w_l1, float w_mse, float* loss, float* grad, float* psnr, void* workspace,
                     void* stream);
 
+/* ---- view tokens ------------------------------------------------------------------------
+ * Operators of the token layer over all views' features (layer norm, dropout, rotary positions,
+ * attention over chosen blocks), forward and backward. Rows are f32, bf16 or f16 (DTK_* codes);
+ * sums, moments and softmax statistics are held in 32 bits, or more where said. */
+#define DTK_F32 0
+#define DTK_BF16 1
+#define DTK_F16 2
+#define DTK_I32 3
+#define DTK_I64 4
+
+/* Dropout from a counter: element n (row-major) is kept iff word n % 4 of Philox4x32-10 of the
+ * counter (n / 4 in two words, call, step) under the key (seed in two words) is >= p 2^32; kept
+ * values are scaled by 1 / (1 - p), dropped ones are 0 whatever they held. rng: device int64
+ * [2] = (seed, step), read when the kernel runs (a captured graph replays with the step it finds
+ * there). The mask is never stored: the backward is the same call on the gradient.
+ * y = dropout(x) (+ residual, when non-NULL), n elements, contiguous. */
+int dtk_dropout(int64_t n, int dtype, const void* x, const void* residual, double p, const int64_t* rng,
+                uint32_t call, void* y, void* stream);
+
+/* Layer norm over rows [rows, width], contiguous: z = x (residual NULL) or residual +
+ * dropout(x) (p > 0 needs rng), mean and 1 / sqrt(biased variance + eps) of z per row, y =
+ * (z - mean) rstd weight + bias (either may be NULL; wtype: dtype or DTK_F32). s (with a
+ * residual): z rounded to dtype; y is of z so rounded. mean, rstd [rows] f32, both or neither. */
+int dtk_layer_norm_fwd(int64_t rows, int width, int dtype, int wtype, const void* x, const void* residual,
+                       const void* weight, const void* bias, float eps, double p, const int64_t* rng,
+                       uint32_t call, void* s, void* y, float* mean, float* rstd, void* stream);
+/* Backward: z = x, or s of the forward with `add` (a residual was added); dy, ds: gradients of
+ * y and s, each may be NULL (zero). dx, dresidual, dweight, dbias overwritten when non-NULL; the
+ * weight's gradients are summed in a fixed order (the same bits every time) through `workspace`
+ * (dtk_layer_norm_bwd_workspace_size bytes; may be NULL without dweight and dbias). */
+size_t dtk_layer_norm_bwd_workspace_size(int64_t rows, int width, int dtype);
+int dtk_layer_norm_bwd(int64_t rows, int width, int dtype, int wtype, const void* z, const void* dy,
+                       const void* ds, const void* weight, const float* mean, const float* rstd, int add,
+                       double p, const int64_t* rng, uint32_t call, void* dx, void* dresidual,
+                       void* dweight, void* dbias, void* workspace, void* stream);
+
+/* Rotary positions of q [B,L,Hq,D] and k [B,L,Hk,D] (either with 0 heads) in one launch: pair i
+ * < F turns by positions[b,l,i / (F / axes)] freqs[i], times `factor`; pairs (2i, 2i + 1) if
+ * interleaved, else (i, i + F); channels from 2F on are copied. q, k: element strides (batch,
+ * token, head), channels contiguous; positions (ptype DTK_I64, DTK_I32 or DTK_F32): strides
+ * (batch, token, axis); freqs [F] double. Outputs contiguous. `backward`: the opposite angle. */
+int dtk_rotary(int64_t B, int64_t L, int Hq, int Hk, int D, int F, int axes, int interleaved, int backward,
+               int dtype, int ptype, const void* q, const int64_t* q_strides, const void* k,
+               const int64_t* k_strides, const void* positions, const int64_t* pos_strides,
+               const double* freqs, float factor, void* q_out, void* k_out, void* stream);
+
+/* The key blocks of each query tile: tiles and blocks of `block` (32, 64 or 128) tokens; score =
+ * (mean query row of the tile over the heads that share the key head) . (mean key row of the
+ * block), in 64 bits; index [B,Hkv,ceil(Lq/block),top] = the top blocks of the highest score among
+ * the allowed ones (allowed [ceil(Lq/block), ceil(Lk/block)] bytes, NULL: all) that hold a key, ties to
+ * the lowest block, ascending, -1 behind. A score that is no number ranks lowest. q_lengths,
+ * kv_lengths [B] (NULL: all of Lq, Lk): rows behind them do not count. D <= 256. */
+size_t dtk_select_blocks_workspace_size(int B, int64_t Lq, int64_t Lk, int Hkv, int D, int block);
+int dtk_select_blocks(int B, int64_t Lq, int64_t Lk, int Hq, int Hkv, int D, int block, int top, int dtype,
+                      const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
+                      const int32_t* q_lengths, const int32_t* kv_lengths, const uint8_t* allowed,
+                      int32_t* index, void* workspace, void* stream);
+
+/* Attention of the queries of tile t over the keys of the blocks index[b,hkv,t,:] (places that are
+ * no block of the sequence, or stand there a second time, are left out; top <= 1024). q
+ * [B,Lq,Hq,D], k and v [B,Lk,Hkv,D]: element strides (batch, token, head), channels contiguous, D a
+ * multiple of 8 up to 128; Hq a multiple of Hkv. o [B,Lq,Hq,D] contiguous: 0 for queries that see
+ * no key and behind q_lengths. lse [B,Hq,Lq] (base 2; NULL when no backward follows). Few tiles: the lists are
+ * split over workgroups and joined through the workspace. Backward: dout with its strides; dq,
+ * dk, dv contiguous, overwritten (0 behind the lengths), each sum in one order. */
+typedef struct dtk_attention {
+    int64_t Lq, Lk;
+    int32_t B, Hq, Hkv, D, block, top, dtype;
+    float scale;
+    const void *q, *k, *v;
+    int64_t q_strides[3], k_strides[3], v_strides[3];
+    const int32_t *index, *q_lengths, *kv_lengths;
+    void* o;
+    float* lse;
+} dtk_attention;
+size_t dtk_block_sparse_attention_fwd_workspace_size(const dtk_attention* a);
+int dtk_block_sparse_attention_fwd(const dtk_attention* a, void* workspace, void* stream);
+size_t dtk_block_sparse_attention_bwd_workspace_size(const dtk_attention* a);
+int dtk_block_sparse_attention_bwd(const dtk_attention* a, const void* dout, const int64_t* dout_strides,
+                                   void* dq, void* dk, void* dv, void* workspace, void* stream);
+
 /* ---- buffer sizing -------------------------------------------------------------------
  * Bytes of every caller-owned buffer of one rasterizer call sequence over V views of
  * W x H pixels and G gaussians per scene (T = ceil(W/16) * ceil(H/16) tiles per view), so a

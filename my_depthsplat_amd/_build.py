@@ -35,7 +35,9 @@ CFLAGS += ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 # FP32 is written out with explicit vector types); the SLP vectorizer re-packs the scalar
 # parts with register shuffles that cost more than they save (k_render_bwd 119 -> 109 us
 # without it at config B).
-FILE_FLAGS = {"dsr_raster.hip": ["-fno-slp-vectorize"]}
+FILE_FLAGS = {"dsr_raster.hip": ["-fno-slp-vectorize"],
+              # nothing there has to match another kernel bit for bit (the fused norm matches the plain one)
+              **{f: ["-ffp-contract=fast"] for f in ("dtk_rotary.hip", "dtk_attention.hip")}}
 
 
 def _sources() -> list[Path]:

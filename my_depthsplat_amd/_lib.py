@@ -20,6 +20,8 @@ LIB_PATH = Path(os.environ.get("DSPLAT_LIB") or Path(__file__).resolve().parent 
 # name -> (restype, argtypes); mirrors include/dsplat_hip.h exactly.
 _P = c_void_p
 _I = c_int
+_L = ctypes.c_int64
+_D = ctypes.c_double
 SIGNATURES: dict[str, tuple] = {
     "dsr_build_cameras": (_I, [_I, _P, _P, _P, _P, _P, _P, _I, _P, _P, c_uint32, _P]),
     "dsr_preprocess_fwd": (_I, [_I, _I, _I, _I, _I, _I, _I, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _P]),
@@ -76,6 +78,17 @@ SIGNATURES: dict[str, tuple] = {
                                   _P, _P, _P, _P, _P, _P]),
     "dls_loss_workspace_size": (ctypes.c_size_t, [_I, ctypes.c_int64]),
     "dls_l1_mse_psnr": (_I, [_I, ctypes.c_int64, _P, _P, c_float, c_float, _P, _P, _P, _P, _P]),
+    "dtk_dropout": (_I, [_L, _I, _P, _P, _D, _P, c_uint32, _P, _P]),
+    "dtk_layer_norm_fwd": (_I, [_L, _I, _I, _I, _P, _P, _P, _P, c_float, _D, _P, c_uint32, _P, _P, _P, _P, _P]),
+    "dtk_layer_norm_bwd_workspace_size": (ctypes.c_size_t, [_L, _I, _I]),
+    "dtk_layer_norm_bwd": (_I, [_L, _I, _I, _I, _P, _P, _P, _P, _P, _P, _I, _D, _P, c_uint32, _P, _P, _P, _P, _P, _P]),
+    "dtk_rotary": (_I, [_L, _L, _I, _I, _I, _I, _I, _I, _I, _I, _I, _P, _P, _P, _P, _P, _P, _P, c_float, _P, _P, _P]),
+    "dtk_select_blocks_workspace_size": (ctypes.c_size_t, [_I, _L, _L, _I, _I, _I]),
+    "dtk_select_blocks": (_I, [_I, _L, _L, _I, _I, _I, _I, _I, _I, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P]),
+    "dtk_block_sparse_attention_fwd_workspace_size": (ctypes.c_size_t, [_P]),
+    "dtk_block_sparse_attention_fwd": (_I, [_P, _P, _P]),
+    "dtk_block_sparse_attention_bwd_workspace_size": (ctypes.c_size_t, [_P]),
+    "dtk_block_sparse_attention_bwd": (_I, [_P, _P, _P, _P, _P, _P, _P, _P]),
     "dsplat_last_error": (ctypes.c_char_p, []),
     "dsplat_abi_version": (_I, []),
 }
@@ -86,6 +99,14 @@ class Workspace(ctypes.Structure):
         "cams_bytes", "geom_bytes", "radii_bytes", "seg_count_bytes", "seg_start_bytes", "keys_bytes",
         "scratch_bytes", "sort_ws_bytes", "color_bytes", "final_T_bytes", "n_contrib_bytes", "dgeom_bytes",
         "total_bytes")] + [("tiles", ctypes.c_int32), ("fixed_capacity", ctypes.c_int32)]
+
+
+class Attention(ctypes.Structure):
+    """dtk_attention (include/dsplat_hip.h)."""
+    _fields_ = ([("Lq", _L), ("Lk", _L)] + [(n, ctypes.c_int32) for n in ("B", "Hq", "Hkv", "D", "block", "top", "dtype")]
+                + [("scale", c_float)] + [(n, _P) for n in ("q", "k", "v")]
+                + [(n, _L * 3) for n in ("q_strides", "k_strides", "v_strides")]
+                + [(n, _P) for n in ("index", "q_lengths", "kv_lengths", "o", "lse")])
 
 
 _lib = None

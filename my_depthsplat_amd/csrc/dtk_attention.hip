@@ -1,0 +1,737 @@
+// dtk_attention.hip — attention of query tiles over their chosen key blocks, forward, backward
+// and the form for few queries, for gfx950.
+//
+//   tile t = queries t block .. t block + block - 1; its keys are those of the blocks index[t]
+//   x = scale q k^T, p = exp(x - lse), o = p v;  backward: dv = p^T do, dp = do v^T,
+//   ds = p (dp - sum_d do o), dq = scale ds k, dk = scale ds^T q
+//
+// All products are 32 x 32 matrix instructions, taken transposed (keys as rows, queries as
+// columns) in the forward and in dq: a lane then holds one query's scores, so the running
+// maximum and sum need one exchange between the two halves of the wave, and the probabilities
+// are already laid out as the second product's right operand: an instruction's k index may be
+// permuted as long as both operands agree, so the accumulator's rows (8 (r / 4) + 4 half + r % 4)
+// serve as they are and nothing is shuffled.
+
+#include "dtk_common.h"
+
+namespace {
+using namespace dtk;
+
+constexpr int NT = 256;
+constexpr float kLog2e = 1.44269504088896340736f;
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x8 __attribute__((ext_vector_type(8)));
+typedef bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef f16 f16x8 __attribute__((ext_vector_type(8)));
+
+// An operand fragment is 8 elements per lane: row (column) lane % 32, k = 8 (lane / 32) + j, or
+// any other k both operands share. f32 runs as eight k = 2 instructions over the same registers.
+template <typename T>
+struct Mma;
+template <>
+struct Mma<bf16> {
+  using Frag = bf16x8;
+  static __device__ __forceinline__ f32x16 mma(Frag a, Frag b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+  }
+};
+template <>
+struct Mma<f16> {
+  using Frag = f16x8;
+  static __device__ __forceinline__ f32x16 mma(Frag a, Frag b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+  }
+};
+template <>
+struct Mma<float> {
+  using Frag = f32x8;
+  static __device__ __forceinline__ f32x16 mma(Frag a, Frag b, f32x16 c) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[j], b[j], c, 0, 0, 0);
+    return c;
+  }
+};
+
+struct Strided {
+  const void* p;
+  int64_t b, l, h;
+};
+struct Args {
+  int64_t Lq, Lk;
+  int Hq, Hkv, G, D, block, top, Tq, Tk;
+  int Lt, rowtiles, splits;  // rows of a tile, workgroups per tile, parts of the key list
+  float scale;
+  Strided q, k, v, o, g;  // g: the output's gradient
+  const int32_t *index, *q_lengths, *kv_lengths;
+  void *out, *dq, *dk, *dv;  // contiguous
+  float *lse;                // [B, Hq, Lq], base 2; -inf for rows without a key
+  float *part, *part_m, *part_l;
+  float* delta;
+  uint32_t *bits, *gmax;
+};
+
+__device__ __forceinline__ int64_t length_of(const int32_t* lengths, int b, int64_t L) {
+  if (!lengths) return L;
+  const int64_t n = lengths[b];
+  return n < 0 ? 0 : n < L ? n : L;
+}
+
+// 8 channels of a row from d0 on, zeros behind D and for rows that do not count (what stands
+// there may be no number).
+template <typename T>
+__device__ __forceinline__ typename Mma<T>::Frag row_frag(const T* row, int d0, int D, bool valid) {
+  typename Mma<T>::Frag f = {};
+  if (valid && d0 < D) __builtin_memcpy(&f, row + d0, sizeof(f));
+  return f;
+}
+// The transposed fragment: channel d (this lane's) of the 8 rows 16 s + {4 half .. + 3, 8 + 4 half .. + 3}.
+template <typename T>
+__device__ __forceinline__ typename Mma<T>::Frag col_frag(const T* rows, int64_t stride, int s, int half, int d, int D,
+                                                         int n) {
+  typename Mma<T>::Frag f = {};
+  if (d < D)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int r = 16 * s + 4 * half + (j & 3) + 8 * (j >> 2);
+      if (r < n) f[j] = rows[r * stride + d];
+    }
+  return f;
+}
+template <typename T>
+__device__ __forceinline__ typename Mma<T>::Frag acc_frag(const f32x16& p, int s) {
+  typename Mma<T>::Frag f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) f[j] = (T)p[8 * s + j];
+  return f;
+}
+__device__ __forceinline__ int acc_row(int r, int half) { return 8 * (r >> 2) + 4 * half + (r & 3); }
+
+// The tile's list without places that are no block or stand in it already, in LDS, in order.
+__device__ __forceinline__ int block_list(const int32_t* idx, int top, int blocks, int32_t* list, int* count) {
+  if (threadIdx.x < 64) {
+    const int lane = threadIdx.x;
+    int n = 0;
+    for (int base = 0; base < top; base += 64) {
+      const int at = base + lane;
+      const int v = at < top ? idx[at] : -1;
+      bool ok = v >= 0 && v < blocks;
+      for (int j = 0; ok && j < at; ++j) ok = idx[j] != v;
+      const uint64_t m = __ballot(ok);
+      if (ok) list[n + __popcll(m & dsplat::lanemask_lt(lane))] = v;
+      n += __popcll(m);
+    }
+    if (lane == 0) *count = n;
+  }
+  __syncthreads();
+  return *count;
+}
+
+template <typename T>
+__device__ __forceinline__ void store4(T* p, float a, float b, float c, float d) {
+  T v[4] = {(T)a, (T)b, (T)c, (T)d};
+  __builtin_memcpy(p, v, sizeof(v));
+}
+
+// Where a workgroup works: tile, row group, key head, scene, part of the list.
+struct Where {
+  int t, rt, hk, b, split;
+};
+__device__ __forceinline__ Where where(const Args& a) {
+  Where w;
+  w.t = blockIdx.x / a.rowtiles;
+  w.rt = blockIdx.x % a.rowtiles;
+  w.hk = blockIdx.y;
+  w.b = blockIdx.z / a.splits;
+  w.split = blockIdx.z % a.splits;
+  return w;
+}
+
+// Forward. RW waves stand side by side over 32 rows each, 4 / RW take turns at the list's units
+// of 32 keys and are joined at the end. The rows of a tile are its queries of all heads that
+// share the key head (few queries: they fill the instruction's columns together).
+template <typename T, int DP, int RW>
+__global__ __launch_bounds__(NT) void k_attend_fwd(Args a) {
+  using M = Mma<T>;
+  using Frag = typename M::Frag;
+  constexpr int KW = 4 / RW, NS = DP / 16, ND = DP / 32;
+  extern __shared__ int32_t list[];
+  __shared__ int count;
+  __shared__ float join[KW > 1 ? RW * 32 * (DP + 1) : 1];
+  __shared__ float join_m[RW * 32], join_l[RW * 32];
+  const Where at = where(a);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, col = lane & 31;
+  const int rw = wave % RW, kw = wave / RW;
+  const int64_t nq = length_of(a.q_lengths, at.b, a.Lq), nk = length_of(a.kv_lengths, at.b, a.Lk);
+  const int row = (at.rt * RW + rw) * 32 + col;
+  const int g = row / a.Lt;
+  const int64_t i = (int64_t)at.t * a.block + row % a.Lt;
+  const bool exists = g < a.G && i < a.Lq, valid = exists && i < nq;
+  const int h = at.hk * a.G + (g < a.G ? g : 0);
+  const int blocks = (int)min((int64_t)a.Tk, (nk + a.block - 1) / a.block);
+  int n = 0;
+  if ((int64_t)at.t * a.block < nq)
+    n = block_list(a.index + (((int64_t)at.b * a.Hkv + at.hk) * a.Tq + at.t) * a.top, a.top, blocks, list, &count);
+
+  const T* qp = (const T*)a.q.p + at.b * a.q.b + (valid ? i : 0) * a.q.l + h * a.q.h;
+  Frag qf[NS];
+#pragma unroll
+  for (int s = 0; s < NS; ++s) qf[s] = row_frag<T>(qp, 16 * s + 8 * half, a.D, valid);
+  const T* kp = (const T*)a.k.p + at.b * a.k.b + at.hk * a.k.h;
+  const T* vp = (const T*)a.v.p + at.b * a.v.b + at.hk * a.v.h;
+
+  f32x16 o[ND] = {};
+  float m = -INFINITY, l = 0.f;
+  const float scale2 = a.scale * kLog2e;
+  const int upb = a.block / 32, units = n * upb;
+  const int per = (units + a.splits - 1) / a.splits;
+  const int u1 = min(units, (at.split + 1) * per);
+  for (int u = at.split * per + kw; u < u1; u += KW) {
+    const int64_t k0 = (int64_t)list[u / upb] * a.block + 32 * (u % upb);
+    if (k0 >= nk) continue;
+    const int left = (int)min((int64_t)32, nk - k0);
+    f32x16 x = {};
+#pragma unroll
+    for (int s = 0; s < NS; ++s)
+      x = M::mma(row_frag<T>(kp + (k0 + min(col, left - 1)) * a.k.l, 16 * s + 8 * half, a.D, col < left), qf[s], x);
+    float mx = -INFINITY;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      x[r] = acc_row(r, half) < left ? x[r] * scale2 : -INFINITY;
+      mx = fmaxf(mx, x[r]);
+    }
+    mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+    const float mn = fmaxf(m, mx), base = mn == -INFINITY ? 0.f : mn;
+    const float alpha = exp2f(m - base);
+    m = mn;
+    float sum = 0.f;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      x[r] = exp2f(x[r] - base);
+      sum += x[r];
+    }
+    l = l * alpha + sum;
+    const Frag p0 = acc_frag<T>(x, 0), p1 = acc_frag<T>(x, 1);
+#pragma unroll
+    for (int d = 0; d < ND; ++d) {
+      o[d] *= alpha;
+      o[d] = M::mma(col_frag<T>(vp + k0 * a.v.l, a.v.l, 0, half, 32 * d + col, a.D, left), p0, o[d]);
+      o[d] = M::mma(col_frag<T>(vp + k0 * a.v.l, a.v.l, 1, half, 32 * d + col, a.D, left), p1, o[d]);
+    }
+  }
+  l += __shfl_xor(l, 32, 64);
+  if constexpr (KW > 1) {
+    for (int k = 1; k < KW; ++k) {
+      float* jo = join + (rw * 32 + col) * (DP + 1);
+      __syncthreads();
+      if (kw == k) {
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) jo[32 * d + acc_row(r, half)] = o[d][r];
+        if (half == 0) {
+          join_m[rw * 32 + col] = m;
+          join_l[rw * 32 + col] = l;
+        }
+      }
+      __syncthreads();
+      if (kw == 0) {
+        const float mo = join_m[rw * 32 + col], lo = join_l[rw * 32 + col];
+        const float mn = fmaxf(m, mo), base = mn == -INFINITY ? 0.f : mn;
+        const float fa = exp2f(m - base), fb = exp2f(mo - base);
+        m = mn;
+        l = l * fa + lo * fb;
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) o[d][r] = o[d][r] * fa + jo[32 * d + acc_row(r, half)] * fb;
+      }
+    }
+  }
+  if (kw != 0 || !exists) return;
+  if (a.splits > 1) {
+    const int64_t r = ((int64_t)at.b * a.Hq + h) * a.Lq + i, rows = (int64_t)(gridDim.z / a.splits) * a.Hq * a.Lq;
+    float* po = a.part + (at.split * rows + r) * a.D;
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        if (32 * d + 8 * c + 4 * half < a.D)
+          store4<float>(po + 32 * d + 8 * c + 4 * half, o[d][4 * c], o[d][4 * c + 1], o[d][4 * c + 2], o[d][4 * c + 3]);
+    if (half == 0) {
+      a.part_m[at.split * rows + r] = m;
+      a.part_l[at.split * rows + r] = l;
+    }
+    return;
+  }
+  const float inv = valid && l > 0.f ? 1.f / l : (l != l ? l : 0.f);
+  T* op = (T*)a.out + (((int64_t)at.b * a.Lq + i) * a.Hq + h) * a.D;
+#pragma unroll
+  for (int d = 0; d < ND; ++d)
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+      if (32 * d + 8 * c + 4 * half < a.D)
+        store4<T>(op + 32 * d + 8 * c + 4 * half, o[d][4 * c] * inv, o[d][4 * c + 1] * inv, o[d][4 * c + 2] * inv,
+                  o[d][4 * c + 3] * inv);
+  if (half == 0 && a.lse) a.lse[((int64_t)at.b * a.Hq + h) * a.Lq + i] = valid ? m + log2f(l) : -INFINITY;
+}
+
+// Joins the parts of a split list: one row per group of D / 4 threads.
+template <typename T>
+__global__ __launch_bounds__(NT) void k_attend_join(Args a, int64_t rows) {
+  const int per = a.D / 4;
+  const int64_t id = (int64_t)blockIdx.x * NT + threadIdx.x;
+  const int64_t r = id / per;
+  const int d = (int)(id % per) * 4;
+  if (r >= rows) return;
+  float m = -INFINITY;
+  for (int s = 0; s < a.splits; ++s) m = fmaxf(m, a.part_m[s * rows + r]);
+  const float base = m == -INFINITY ? 0.f : m;
+  float l = 0.f, o[4] = {};
+  for (int s = 0; s < a.splits; ++s) {
+    const float f = exp2f(a.part_m[s * rows + r] - base);
+    l += a.part_l[s * rows + r] * f;
+    const float* p = a.part + (s * rows + r) * a.D + d;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] += p[e] * f;
+  }
+  const int64_t i = r % a.Lq, bh = r / a.Lq, b = bh / a.Hq, h = bh % a.Hq;
+  const bool valid = i < length_of(a.q_lengths, (int)b, a.Lq);
+  const float inv = valid && l > 0.f ? 1.f / l : (l != l ? l : 0.f);
+  store4<T>((T*)a.out + ((b * a.Lq + i) * a.Hq + h) * a.D + d, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
+  if (d == 0 && a.lse) a.lse[r] = valid ? m + log2f(l) : -INFINITY;
+}
+
+// delta = sum_d do o per row, and the largest |do| (its bits order as the numbers do).
+template <typename T>
+__global__ __launch_bounds__(NT) void k_attend_delta(Args a, int64_t rows) {
+  const int sub = threadIdx.x % 16;
+  const int64_t r = (int64_t)blockIdx.x * (NT / 16) + threadIdx.x / 16;
+  const bool in = r < rows;
+  const int64_t i = in ? r % a.Lq : 0, bh = in ? r / a.Lq : 0, b = bh / a.Hq, h = bh % a.Hq;
+  const bool valid = in && i < length_of(a.q_lengths, (int)b, a.Lq);
+  const T* op = (const T*)a.o.p + b * a.o.b + i * a.o.l + h * a.o.h;
+  const T* gp = (const T*)a.g.p + b * a.g.b + i * a.g.l + h * a.g.h;
+  float s = 0.f, mx = 0.f;
+  const auto of = row_frag<T>(op, 8 * sub, a.D, valid), gf = row_frag<T>(gp, 8 * sub, a.D, valid);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    s += (float)of[j] * (float)gf[j];
+    mx = fmaxf(mx, fabsf((float)gf[j]));
+  }
+#pragma unroll
+  for (int off = 8; off > 0; off >>= 1) s += __shfl_xor(s, off, 64);
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor(mx, off, 64));
+  if (in && sub == 0) a.delta[r] = s;
+  if ((threadIdx.x & 63) == 0 && mx > 0.f) atomicMax(a.gmax, __float_as_uint(mx));
+}
+
+// Which tiles chose a block: bits [B, Hkv, Tk, ceil(Tq / 32)].
+__global__ __launch_bounds__(NT) void k_attend_mark(Args a) {
+  const int t = blockIdx.x, hk = blockIdx.y, b = blockIdx.z;
+  if ((int64_t)t * a.block >= length_of(a.q_lengths, b, a.Lq)) return;
+  const int32_t* idx = a.index + (((int64_t)b * a.Hkv + hk) * a.Tq + t) * a.top;
+  const int words = (a.Tq + 31) / 32;
+  for (int j = threadIdx.x; j < a.top; j += NT) {
+    const int v = idx[j];
+    if (v >= 0 && v < a.Tk) atomicOr(a.bits + (((int64_t)b * a.Hkv + hk) * a.Tk + v) * words + t / 32, 1u << (t % 32));
+  }
+}
+
+// ds is rounded to the inputs' type for its products. f16 has few exponents, so it is taken
+// relative to the power of two at the largest |do| there (exact, undone in 32 bits).
+template <typename T>
+__device__ __forceinline__ void ds_scale(const uint32_t* gmax, float& down, float& up) {
+  down = up = 1.f;
+  if constexpr (sizeof(T) == 2 && !__is_same(T, bf16)) {
+    const int e = (int)((*gmax >> 23) & 255);
+    if (e > 27 && e < 227) {
+      down = __uint_as_float((uint32_t)(254 - e) << 23);
+      up = __uint_as_float((uint32_t)e << 23);
+    }
+  }
+}
+
+// dq: the forward's shape; p is taken from the saved lse.
+template <typename T, int DP, int RW>
+__global__ __launch_bounds__(NT) void k_attend_dq(Args a) {
+  using M = Mma<T>;
+  using Frag = typename M::Frag;
+  constexpr int KW = 4 / RW, NS = DP / 16, ND = DP / 32;
+  extern __shared__ int32_t list[];
+  __shared__ int count;
+  __shared__ float join[KW > 1 ? RW * 32 * (DP + 1) : 1];
+  const Where at = where(a);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, col = lane & 31;
+  const int rw = wave % RW, kw = wave / RW;
+  const int64_t nq = length_of(a.q_lengths, at.b, a.Lq), nk = length_of(a.kv_lengths, at.b, a.Lk);
+  const int row = (at.rt * RW + rw) * 32 + col;
+  const int g = row / a.Lt;
+  const int64_t i = (int64_t)at.t * a.block + row % a.Lt;
+  const bool exists = g < a.G && i < a.Lq, valid = exists && i < nq;
+  const int h = at.hk * a.G + (g < a.G ? g : 0);
+  const int blocks = (int)min((int64_t)a.Tk, (nk + a.block - 1) / a.block);
+  int n = 0;
+  if ((int64_t)at.t * a.block < nq)
+    n = block_list(a.index + (((int64_t)at.b * a.Hkv + at.hk) * a.Tq + at.t) * a.top, a.top, blocks, list, &count);
+
+  const int64_t ir = valid ? i : 0;
+  const T* qp = (const T*)a.q.p + at.b * a.q.b + ir * a.q.l + h * a.q.h;
+  const T* gp = (const T*)a.g.p + at.b * a.g.b + ir * a.g.l + h * a.g.h;
+  Frag qf[NS], gf[NS];
+#pragma unroll
+  for (int s = 0; s < NS; ++s) {
+    qf[s] = row_frag<T>(qp, 16 * s + 8 * half, a.D, valid);
+    gf[s] = row_frag<T>(gp, 16 * s + 8 * half, a.D, valid);
+  }
+  const int64_t stat = ((int64_t)at.b * a.Hq + h) * a.Lq + ir;
+  const float lse = valid ? a.lse[stat] : -INFINITY, delta = valid ? a.delta[stat] : 0.f;
+  const bool empty = lse == -INFINITY;
+  const T* kp = (const T*)a.k.p + at.b * a.k.b + at.hk * a.k.h;
+  const T* vp = (const T*)a.v.p + at.b * a.v.b + at.hk * a.v.h;
+  float down, up;
+  ds_scale<T>(a.gmax, down, up);
+
+  f32x16 dq[ND] = {};
+  const float scale2 = a.scale * kLog2e;
+  const int upb = a.block / 32, units = n * upb;
+  for (int u = kw; u < units; u += KW) {
+    const int64_t k0 = (int64_t)list[u / upb] * a.block + 32 * (u % upb);
+    if (k0 >= nk) continue;
+    const int left = (int)min((int64_t)32, nk - k0);
+    const int64_t kr = k0 + min(col, left - 1);
+    f32x16 x = {}, dp = {};
+#pragma unroll
+    for (int s = 0; s < NS; ++s) {
+      x = M::mma(row_frag<T>(kp + kr * a.k.l, 16 * s + 8 * half, a.D, col < left), qf[s], x);
+      dp = M::mma(row_frag<T>(vp + kr * a.v.l, 16 * s + 8 * half, a.D, col < left), gf[s], dp);
+    }
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const float p = !empty && acc_row(r, half) < left ? exp2f(x[r] * scale2 - lse) : 0.f;
+      x[r] = p * (dp[r] - delta) * down;
+    }
+    const Frag s0 = acc_frag<T>(x, 0), s1 = acc_frag<T>(x, 1);
+#pragma unroll
+    for (int d = 0; d < ND; ++d) {
+      dq[d] = M::mma(col_frag<T>(kp + k0 * a.k.l, a.k.l, 0, half, 32 * d + col, a.D, left), s0, dq[d]);
+      dq[d] = M::mma(col_frag<T>(kp + k0 * a.k.l, a.k.l, 1, half, 32 * d + col, a.D, left), s1, dq[d]);
+    }
+  }
+  if constexpr (KW > 1) {
+    for (int k = 1; k < KW; ++k) {
+      float* jo = join + (rw * 32 + col) * (DP + 1);
+      __syncthreads();
+      if (kw == k)
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) jo[32 * d + acc_row(r, half)] = dq[d][r];
+      __syncthreads();
+      if (kw == 0)
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) dq[d][r] += jo[32 * d + acc_row(r, half)];
+    }
+  }
+  if (kw != 0 || !exists) return;
+  T* op = (T*)a.dq + (((int64_t)at.b * a.Lq + i) * a.Hq + h) * a.D;
+  const float f = valid ? a.scale * up : 0.f;
+#pragma unroll
+  for (int d = 0; d < ND; ++d)
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+      if (32 * d + 8 * c + 4 * half < a.D)
+        store4<T>(op + 32 * d + 8 * c + 4 * half, dq[d][4 * c] * f, dq[d][4 * c + 1] * f, dq[d][4 * c + 2] * f,
+                  dq[d][4 * c + 3] * f);
+}
+
+// dk, dv of one key block: RW waves hold 32 keys each, 4 / RW take turns at the 32-query units of
+// the tiles that chose the block (their bits, some at a time) and are joined at the end. Every sum
+// has one order: no atomics on the gradients.
+constexpr int kTiles = 1024;  // tiles listed at a time
+template <typename T, int DP, int RW>
+__global__ __launch_bounds__(NT) void k_attend_dkv(Args a) {
+  using M = Mma<T>;
+  using Frag = typename M::Frag;
+  constexpr int QW = 4 / RW, NS = DP / 16, ND = DP / 32;
+  __shared__ int32_t tiles[kTiles];
+  __shared__ int count;
+  __shared__ float join[QW > 1 ? RW * 32 * (DP + 1) : 1];
+  const int blk = blockIdx.x, hk = blockIdx.y, b = blockIdx.z;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, col = lane & 31;
+  const int rw = wave % RW, qw = wave / RW;
+  const int64_t nq = length_of(a.q_lengths, b, a.Lq), nk = length_of(a.kv_lengths, b, a.Lk);
+  const int64_t key = (int64_t)blk * a.block + 32 * rw + col;
+  const bool exists = key < a.Lk, valid = key < nk;
+  const int64_t kr = valid ? key : 0;
+  const T* kp = (const T*)a.k.p + b * a.k.b + kr * a.k.l + hk * a.k.h;
+  const T* vp = (const T*)a.v.p + b * a.v.b + kr * a.v.l + hk * a.v.h;
+  Frag kf[NS], vf[NS];
+#pragma unroll
+  for (int s = 0; s < NS; ++s) {
+    kf[s] = row_frag<T>(kp, 16 * s + 8 * half, a.D, valid);
+    vf[s] = row_frag<T>(vp, 16 * s + 8 * half, a.D, valid);
+  }
+  float down, up;
+  ds_scale<T>(a.gmax, down, up);
+  f32x16 dk[ND] = {}, dv[ND] = {};
+  const float scale2 = a.scale * kLog2e;
+  const int upb = a.block / 32, words = (a.Tq + 31) / 32;
+  const uint32_t* bits = a.bits + (((int64_t)b * a.Hkv + hk) * a.Tk + blk) * words;
+  const bool any = (int64_t)blk * a.block < nk;
+  for (int w0 = 0; any && w0 < words; w0 += kTiles / 32) {
+    __syncthreads();
+    if (threadIdx.x < 64) {  // the first 32 lanes hold a word each
+      uint32_t m = lane < 32 && w0 + lane < words ? bits[w0 + lane] : 0u;
+      const uint32_t incl = dsplat::wave_incl_scan(__popc(m), lane);
+      int at = (int)incl - __popc(m);
+      while (m) {
+        tiles[at++] = 32 * (w0 + lane) + __ffs(m) - 1;
+        m &= m - 1;
+      }
+      if (lane == 63) count = (int)incl;
+    }
+    __syncthreads();
+    const int units = count * a.G * upb;
+    for (int u = qw; u < units; u += QW) {
+      const int64_t i0 = (int64_t)tiles[u / (a.G * upb)] * a.block + 32 * (u % upb);
+      const int h = hk * a.G + (u / upb) % a.G;
+      if (i0 >= nq) continue;
+      const int left = (int)min((int64_t)32, nq - i0);
+      const T* qp = (const T*)a.q.p + b * a.q.b + i0 * a.q.l + h * a.q.h;
+      const T* gp = (const T*)a.g.p + b * a.g.b + i0 * a.g.l + h * a.g.h;
+      const int qr = min(col, left - 1);
+      f32x16 x = {}, dp = {};
+#pragma unroll
+      for (int s = 0; s < NS; ++s) {
+        x = M::mma(row_frag<T>(qp + qr * a.q.l, 16 * s + 8 * half, a.D, col < left), kf[s], x);
+        dp = M::mma(row_frag<T>(gp + qr * a.g.l, 16 * s + 8 * half, a.D, col < left), vf[s], dp);
+      }
+      const int64_t stat = ((int64_t)b * a.Hq + h) * a.Lq + i0;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int ri = acc_row(r, half);
+        const float lse = ri < left ? a.lse[stat + ri] : -INFINITY, delta = ri < left ? a.delta[stat + ri] : 0.f;
+        const float p = valid && lse != -INFINITY ? exp2f(x[r] * scale2 - lse) : 0.f;
+        x[r] = p;
+        dp[r] = p * (dp[r] - delta) * down;
+      }
+      const Frag p0 = acc_frag<T>(x, 0), p1 = acc_frag<T>(x, 1), s0 = acc_frag<T>(dp, 0), s1 = acc_frag<T>(dp, 1);
+#pragma unroll
+      for (int d = 0; d < ND; ++d) {
+        dv[d] = M::mma(col_frag<T>(gp, a.g.l, 0, half, 32 * d + col, a.D, left), p0, dv[d]);
+        dv[d] = M::mma(col_frag<T>(gp, a.g.l, 1, half, 32 * d + col, a.D, left), p1, dv[d]);
+        dk[d] = M::mma(col_frag<T>(qp, a.q.l, 0, half, 32 * d + col, a.D, left), s0, dk[d]);
+        dk[d] = M::mma(col_frag<T>(qp, a.q.l, 1, half, 32 * d + col, a.D, left), s1, dk[d]);
+      }
+    }
+  }
+  if constexpr (QW > 1) {
+    float* jo = join + (rw * 32 + col) * (DP + 1);
+    for (int k = 1; k < QW; ++k)
+#pragma unroll
+      for (int which = 0; which < 2; ++which) {
+        f32x16* acc = which ? dv : dk;
+        __syncthreads();
+        if (qw == k)
+#pragma unroll
+          for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) jo[32 * d + acc_row(r, half)] = acc[d][r];
+        __syncthreads();
+        if (qw == 0)
+#pragma unroll
+          for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[d][r] += jo[32 * d + acc_row(r, half)];
+      }
+  }
+  if (qw != 0 || !exists) return;
+  const int64_t off = (((int64_t)b * a.Lk + key) * a.Hkv + hk) * a.D;
+  const float f = valid ? a.scale * up : 0.f, fv = valid ? 1.f : 0.f;
+#pragma unroll
+  for (int d = 0; d < ND; ++d)
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+      if (32 * d + 8 * c + 4 * half < a.D) {
+        const int e = 32 * d + 8 * c + 4 * half;
+        store4<T>((T*)a.dk + off + e, dk[d][4 * c] * f, dk[d][4 * c + 1] * f, dk[d][4 * c + 2] * f, dk[d][4 * c + 3] * f);
+        store4<T>((T*)a.dv + off + e, dv[d][4 * c] * fv, dv[d][4 * c + 1] * fv, dv[d][4 * c + 2] * fv, dv[d][4 * c + 3] * fv);
+      }
+}
+
+// 32-row waves side by side: as many as the tile's rows fill.
+inline int row_waves(const Args& a) {
+  const int rows = a.Lt * a.G;
+  return rows <= 32 ? 1 : rows <= 64 ? 2 : 4;
+}
+// Parts of the key list: enough workgroups for the chip when there are few tiles.
+inline int splits_of(int64_t workgroups, int units) {
+  int s = 1;
+  while (workgroups * s < 512 && s * 8 < units) s *= 2;
+  return s;
+}
+
+template <typename T, int DP, int RW>
+struct Fwd {
+  static int go(const Args& a, dim3 grid, size_t lds, hipStream_t st) {
+    k_attend_fwd<T, DP, RW><<<grid, NT, lds, st>>>(a);
+    return dsplat::check_launch("k_attend_fwd");
+  }
+};
+template <typename T, int DP, int RW>
+struct Dq {
+  static int go(const Args& a, dim3 grid, size_t lds, hipStream_t st) {
+    k_attend_dq<T, DP, RW><<<grid, NT, lds, st>>>(a);
+    return dsplat::check_launch("k_attend_dq");
+  }
+};
+template <typename T, int DP, int RW>
+struct Dkv {
+  static int go(const Args& a, dim3 grid, size_t, hipStream_t st) {
+    k_attend_dkv<T, DP, RW><<<grid, NT, 0, st>>>(a);
+    return dsplat::check_launch("k_attend_dkv");
+  }
+};
+template <template <typename, int, int> class F, typename T, int DP>
+int by_waves(int rw, const Args& a, dim3 grid, size_t lds, hipStream_t st) {
+  return rw == 1 ? F<T, DP, 1>::go(a, grid, lds, st) : rw == 2 ? F<T, DP, 2>::go(a, grid, lds, st) : F<T, DP, 4>::go(a, grid, lds, st);
+}
+template <template <typename, int, int> class F, typename T>
+int by_width(int rw, const Args& a, dim3 grid, size_t lds, hipStream_t st) {
+  if (a.D <= 32) return by_waves<F, T, 32>(rw, a, grid, lds, st);
+  if (a.D <= 64) return by_waves<F, T, 64>(rw, a, grid, lds, st);
+  if (a.D <= 96) return by_waves<F, T, 96>(rw, a, grid, lds, st);
+  return by_waves<F, T, 128>(rw, a, grid, lds, st);
+}
+template <template <typename, int, int> class F>
+int by_type(int dtype, int rw, const Args& a, dim3 grid, size_t lds, hipStream_t st) {
+  if (dtype == DTK_F32) return by_width<F, float>(rw, a, grid, lds, st);
+  if (dtype == DTK_BF16) return by_width<F, bf16>(rw, a, grid, lds, st);
+  return by_width<F, f16>(rw, a, grid, lds, st);
+}
+
+int check(const dtk_attention* c, const char* who) {
+  DSPLAT_REQUIRE(c, "%s: null pointer", who);
+  DSPLAT_REQUIRE(c->B >= 0 && c->Lq >= 0 && c->Lk >= 0 && c->Hkv > 0 && c->Hq > 0 && c->Hq % c->Hkv == 0 && c->top > 0 && c->top <= 1024,
+                 "%s: bad sizes", who);
+  DSPLAT_REQUIRE(c->D > 0 && c->D <= 128 && c->D % 8 == 0, "%s: the head size must be a multiple of 8 up to 128", who);
+  DSPLAT_REQUIRE(c->block == 32 || c->block == 64 || c->block == 128, "%s: block must be 32, 64 or 128", who);
+  DSPLAT_REQUIRE(type_ok(c->dtype), "%s: bad type", who);
+  DSPLAT_REQUIRE(c->Lq < (1LL << 31) && c->Lk < (1LL << 31) && c->Hq < 65536 && c->B < 65536, "%s: too large", who);
+  DSPLAT_REQUIRE(c->B == 0 || c->Lq == 0 || (c->q && c->o && c->index && (c->Lk == 0 || (c->k && c->v))), "%s: null pointer", who);
+  return 0;
+}
+Strided strided(const void* p, const int64_t* s) { return {p, s[0], s[1], s[2]}; }
+Args args_of(const dtk_attention* c) {
+  Args a = {};
+  a.Lq = c->Lq;
+  a.Lk = c->Lk;
+  a.Hq = c->Hq;
+  a.Hkv = c->Hkv;
+  a.G = c->Hq / c->Hkv;
+  a.D = c->D;
+  a.block = c->block;
+  a.top = c->top;
+  a.Tq = (int)((c->Lq + c->block - 1) / c->block);
+  a.Tk = (int)((c->Lk + c->block - 1) / c->block);
+  a.Lt = (int)(c->Lq < c->block ? (c->Lq > 0 ? c->Lq : 1) : c->block);
+  a.scale = c->scale;
+  a.q = strided(c->q, c->q_strides);
+  a.k = strided(c->k, c->k_strides);
+  a.v = strided(c->v, c->v_strides);
+  a.index = c->index;
+  a.q_lengths = c->q_lengths;
+  a.kv_lengths = c->kv_lengths;
+  a.out = c->o;
+  a.lse = c->lse;
+  const int per = 32 * row_waves(a);
+  a.rowtiles = (a.Lt * a.G + per - 1) / per;
+  a.splits = splits_of((int64_t)a.Tq * a.rowtiles * a.Hkv * c->B, a.top * (a.block / 32));
+  return a;
+}
+size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
+
+}  // namespace
+
+extern "C" {
+
+size_t dtk_block_sparse_attention_fwd_workspace_size(const dtk_attention* c) {
+  if (!c || c->B <= 0 || c->Lq <= 0 || c->Hq <= 0 || c->Hkv <= 0 || c->block <= 0) return 0;
+  const Args a = args_of(c);
+  if (a.splits == 1) return 0;
+  return (size_t)a.splits * c->B * c->Hq * c->Lq * (c->D + 2) * sizeof(float);
+}
+
+int dtk_block_sparse_attention_fwd(const dtk_attention* c, void* workspace, void* stream) {
+  if (int e = check(c, "dtk_block_sparse_attention_fwd")) return e;
+  if (c->B == 0 || c->Lq == 0) return 0;
+  Args a = args_of(c);
+  hipStream_t st = (hipStream_t)stream;
+  const int64_t rows = (int64_t)c->B * c->Hq * c->Lq;
+  if (a.splits > 1) {
+    DSPLAT_REQUIRE(workspace, "dtk_block_sparse_attention_fwd: null workspace");
+    a.part = (float*)workspace;
+    a.part_m = a.part + a.splits * rows * a.D;
+    a.part_l = a.part_m + a.splits * rows;
+  }
+  const dim3 grid(a.Tq * a.rowtiles, a.Hkv, c->B * a.splits);
+  if (int e = by_type<Fwd>(c->dtype, row_waves(a), a, grid, a.top * sizeof(int32_t), st)) return e;
+  if (a.splits == 1) return 0;
+  const unsigned blocks = (unsigned)((rows * (a.D / 4) + NT - 1) / NT);
+  if (c->dtype == DTK_F32) k_attend_join<float><<<blocks, NT, 0, st>>>(a, rows);
+  else if (c->dtype == DTK_BF16) k_attend_join<bf16><<<blocks, NT, 0, st>>>(a, rows);
+  else k_attend_join<f16><<<blocks, NT, 0, st>>>(a, rows);
+  return dsplat::check_launch("k_attend_join");
+}
+
+size_t dtk_block_sparse_attention_bwd_workspace_size(const dtk_attention* c) {
+  if (!c || c->B <= 0 || c->Lq < 0 || c->Lk < 0 || c->Hq <= 0 || c->Hkv <= 0 || c->block <= 0) return 0;
+  const Args a = args_of(c);
+  return align256((size_t)c->B * c->Hq * c->Lq * 4) + 256 +
+         (size_t)c->B * c->Hkv * a.Tk * ((a.Tq + 31) / 32) * 4;
+}
+
+int dtk_block_sparse_attention_bwd(const dtk_attention* c, const void* dout, const int64_t* dout_strides, void* dq,
+                                   void* dk, void* dv, void* workspace, void* stream) {
+  if (int e = check(c, "dtk_block_sparse_attention_bwd")) return e;
+  if (c->B == 0) return 0;
+  DSPLAT_REQUIRE((c->Lq == 0 || (dout && dout_strides && dq && c->lse && workspace)) && (c->Lk == 0 || (dk && dv && workspace)),
+                 "dtk_block_sparse_attention_bwd: null pointer");
+  Args a = args_of(c);
+  a.splits = 1;
+  hipStream_t st = (hipStream_t)stream;
+  const int64_t rows = (int64_t)c->B * c->Hq * c->Lq;
+  a.o = {c->o, c->Lq * c->Hq * c->D, (int64_t)c->Hq * c->D, c->D};
+  if (c->Lq) a.g = strided(dout, dout_strides);
+  a.dq = dq;
+  a.dk = dk;
+  a.dv = dv;
+  char* ws = (char*)workspace;
+  a.delta = (float*)ws;
+  ws += align256((size_t)rows * 4);
+  a.gmax = (uint32_t*)ws;
+  a.bits = (uint32_t*)(ws + 256);
+  const size_t nbits = (size_t)c->B * c->Hkv * a.Tk * ((a.Tq + 31) / 32);
+  if (int e = dsplat::zero_async(a.gmax, 256 + nbits * 4, st, "dtk_block_sparse_attention_bwd")) return e;
+  if (c->Lq) {
+    const unsigned blocks = (unsigned)((rows + NT / 16 - 1) / (NT / 16));
+    if (c->dtype == DTK_F32) k_attend_delta<float><<<blocks, NT, 0, st>>>(a, rows);
+    else if (c->dtype == DTK_BF16) k_attend_delta<bf16><<<blocks, NT, 0, st>>>(a, rows);
+    else k_attend_delta<f16><<<blocks, NT, 0, st>>>(a, rows);
+    if (int e = dsplat::check_launch("k_attend_delta")) return e;
+    const dim3 grid(a.Tq * a.rowtiles, a.Hkv, c->B);
+    if (int e = by_type<Dq>(c->dtype, row_waves(a), a, grid, a.top * sizeof(int32_t), st)) return e;
+    if (a.Tk) {
+      k_attend_mark<<<dim3(a.Tq, a.Hkv, c->B), NT, 0, st>>>(a);
+      if (int e = dsplat::check_launch("k_attend_mark")) return e;
+    }
+  }
+  if (!a.Tk) return 0;
+  return by_type<Dkv>(c->dtype, a.block / 32, a, dim3(a.Tk, a.Hkv, c->B), 0, st);
+}
+
+}  // extern "C"

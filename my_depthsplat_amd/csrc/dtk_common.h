@@ -1,0 +1,97 @@
+// Shared pieces of the view-token operators (dtk_*): element types, 16-byte vectors at any
+// alignment, the counter-based generator.
+#pragma once
+#include "dsplat_common.h"
+
+#include <hip/hip_bf16.h>
+#include <hip/hip_fp16.h>
+
+namespace dtk {
+
+using bf16 = __bf16;
+using f16 = _Float16;
+
+// One 16-byte vector of T. The loads and stores take any address (global memory accesses of
+// this ISA need no alignment beyond the element's), so rows of odd widths and strides move
+// as whole vectors too.
+template <typename T>
+struct Vec {
+  static constexpr int N = 16 / sizeof(T);
+  T v[N];
+};
+template <typename T>
+__device__ __forceinline__ Vec<T> load_vec(const T* p) {
+  Vec<T> r;
+  __builtin_memcpy(&r, p, 16);
+  return r;
+}
+template <typename T>
+__device__ __forceinline__ void store_vec(T* p, const Vec<T>& r) {
+  __builtin_memcpy(p, &r, 16);
+}
+
+// Philox4x32-10 (Salmon, Moraes, Dror, Shaw: "Parallel random numbers: as easy as 1, 2, 3",
+// SC 2011): ten rounds of two 32 x 32 -> 64 bit products of the counter, keyed. Counter: the
+// group's 64-bit number, the call's id, the step; key: the 64-bit seed.
+struct RngKey {
+  uint32_t k0, k1, call, step;
+};
+__device__ __forceinline__ RngKey rng_key(const int64_t* rng, uint32_t call) {
+  const uint64_t seed = (uint64_t)rng[0], step = (uint64_t)rng[1];
+  return {(uint32_t)seed, (uint32_t)(seed >> 32), call, (uint32_t)step};
+}
+__device__ __forceinline__ void philox(const RngKey& key, uint64_t group, uint32_t (&w)[4]) {
+  uint32_t c0 = (uint32_t)group, c1 = (uint32_t)(group >> 32), c2 = key.call, c3 = key.step;
+  uint32_t k0 = key.k0, k1 = key.k1;
+#pragma unroll
+  for (int r = 0; r < 10; ++r) {
+    const uint64_t a = (uint64_t)0xD2511F53u * c0, b = (uint64_t)0xCD9E8D57u * c2;
+    c0 = (uint32_t)(b >> 32) ^ c1 ^ k0;
+    c1 = (uint32_t)b;
+    c2 = (uint32_t)(a >> 32) ^ c3 ^ k1;
+    c3 = (uint32_t)a;
+    k0 += 0x9E3779B9u;
+    k1 += 0xBB67AE85u;
+  }
+  w[0] = c0;
+  w[1] = c1;
+  w[2] = c2;
+  w[3] = c3;
+}
+// keep[e] of the N elements n0 .. n0 + N - 1 (N a multiple of 4): element n takes word n % 4 of
+// group n / 4. A start inside a group costs one more group and a shift by selects.
+template <int N>
+__device__ __forceinline__ void keep_mask(const RngKey& key, uint64_t n0, uint64_t threshold, bool (&keep)[N]) {
+  constexpr int G = N / 4;
+  const uint64_t g0 = n0 >> 2;
+  const uint32_t sh = (uint32_t)n0 & 3u;
+  uint32_t w[4 * G + 4];
+#pragma unroll
+  for (int g = 0; g < G; ++g) {
+    uint32_t t[4];
+    philox(key, g0 + g, t);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[4 * g + i] = t[i];
+  }
+  if (sh) {
+    uint32_t t[4];
+    philox(key, g0 + G, t);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[4 * G + i] = t[i];
+#pragma unroll
+    for (int i = 0; i < 4 * G + 3; ++i) w[i] = (sh & 1) ? w[i + 1] : w[i];
+#pragma unroll
+    for (int i = 0; i < 4 * G + 1; ++i) w[i] = (sh & 2) ? w[i + 2] : w[i];
+  }
+#pragma unroll
+  for (int e = 0; e < N; ++e) keep[e] = w[e] >= threshold;  // 64-bit: a threshold of 2^32 keeps nothing
+}
+
+// p in [0, 1] -> the words that are kept are >= threshold; 1 / (1 - p), 0 for p = 1.
+inline uint64_t drop_threshold(double p) { return (uint64_t)__builtin_llrint(p * 4294967296.0); }
+inline float drop_scale(double p) { return p < 1.0 ? (float)(1.0 / (1.0 - p)) : 0.f; }
+
+inline bool type_ok(int t) { return t >= DTK_F32 && t <= DTK_F16; }
+inline size_t type_size(int t) { return t == DTK_F32 ? 4 : 2; }
+
+}  // namespace dtk
