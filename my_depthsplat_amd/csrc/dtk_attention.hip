@@ -85,19 +85,6 @@ __device__ __forceinline__ typename Mma<T>::Frag row_frag(const T* row, int d0, 
   if (valid && d0 < D) __builtin_memcpy(&f, row + d0, sizeof(f));
   return f;
 }
-// The transposed fragment: channel d (this lane's) of the 8 rows 16 s + {4 half .. + 3, 8 + 4 half .. + 3}.
-template <typename T>
-__device__ __forceinline__ typename Mma<T>::Frag col_frag(const T* rows, int64_t stride, int s, int half, int d, int D,
-                                                         int n) {
-  typename Mma<T>::Frag f = {};
-  if (d < D)
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int r = 16 * s + 4 * half + (j & 3) + 8 * (j >> 2);
-      if (r < n) f[j] = rows[r * stride + d];
-    }
-  return f;
-}
 template <typename T>
 __device__ __forceinline__ typename Mma<T>::Frag acc_frag(const f32x16& p, int s) {
   typename Mma<T>::Frag f;
@@ -105,6 +92,81 @@ __device__ __forceinline__ typename Mma<T>::Frag acc_frag(const f32x16& p, int s
   for (int j = 0; j < 8; ++j) f[j] = (T)p[8 * s + j];
   return f;
 }
+
+// A tile of rows in LDS, R rows of DP channels. The pitch keeps both ways of reading it nearly
+// free of bank conflicts: 16 rows' 16-byte pieces at one channel (the row fragments) fall on 16
+// different groups of four banks, and the transposed read's 8 rows x 64 bytes on each bank three
+// times at most (two is the least).
+template <typename T, int DP>
+struct Tile {
+  static constexpr int kPitch = DP * (int)sizeof(T) + (sizeof(T) == 2 && DP == 128 ? 48 : 16);  // bytes
+  static constexpr int kPieces = DP * (int)sizeof(T) / 16;                                      // per row
+  static constexpr int kUnit = 32 * kPitch;                                                     // bytes of 32 rows
+  using Frag = typename Mma<T>::Frag;
+
+  // channels 16 s + 8 half .. + 7 of row lane % 32
+  static __device__ __forceinline__ Frag row(const char* t, int s, int col, int half) {
+    Frag f;
+    __builtin_memcpy(&f, __builtin_assume_aligned(t + col * kPitch + (16 * s + 8 * half) * sizeof(T), 16), sizeof(f));
+    return f;
+  }
+  // channel 32 d + lane % 32 of the 8 rows 16 s + {4 half .. + 3, 8 + 4 half .. + 3}: the rows an accumulator
+  // holds. 16 bits: the transposing LDS read hands lane i of 16 the i-th column of the 4 rows of 16
+  // that the 16 lanes' 8-byte pieces make up.
+  static __device__ __forceinline__ Frag col(const char* t, int s, int d, int lane) {
+    Frag f;
+    const int half = lane >> 5;
+    if constexpr (sizeof(T) == 2) {
+      typedef short s16x4 __attribute__((ext_vector_type(4)));
+      typedef __attribute__((address_space(3))) s16x4* lds;
+      const int i = lane & 15;
+      const char* at = t + (16 * s + 4 * half + (i >> 2)) * kPitch + (32 * d + (lane & 16) + 4 * (i & 3)) * 2;
+      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds)at);
+      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds)(at + 8 * kPitch));
+      __builtin_memcpy(&f, &lo, 8);
+      __builtin_memcpy((char*)&f + 8, &hi, 8);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        f[j] = *(const T*)(t + (16 * s + 4 * half + (j & 3) + 8 * (j >> 2)) * kPitch + (32 * d + (lane & 31)) * 4);
+    }
+    return f;
+  }
+};
+
+// The workgroup's share of U units (32 rows each) on the way from memory to LDS: loaded into
+// registers while the tile before is worked on, then stored. Rows that do not count and channels
+// behind D become zeros.
+template <typename T, int DP, int U>
+struct Stage {
+  using L = Tile<T, DP>;
+  static constexpr int kPer = (U * 32 * L::kPieces + NT - 1) / NT;
+  Vec<T> v[kPer];
+  // first(j): where the j-th unit's first row starts (elements from base), count(j): its rows that count
+  template <typename F, typename C>
+  __device__ __forceinline__ void load(const T* base, int64_t stride, int D, F first, C count) {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int id = threadIdx.x + i * NT, r = id / L::kPieces, d = (id % L::kPieces) * Vec<T>::N, j = r / 32;
+      v[i] = Vec<T>{};
+      if (j < U && d < D && r % 32 < count(j)) v[i] = load_vec(base + first(j) + (r % 32) * stride + d);
+    }
+  }
+  __device__ __forceinline__ void store(char* t) const {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int id = threadIdx.x + i * NT, r = id / L::kPieces, c = id % L::kPieces;
+      if (r < U * 32) __builtin_memcpy(__builtin_assume_aligned(t + r * L::kPitch + c * 16, 16), &v[i], 16);
+    }
+  }
+};
+// Two buffers (one barrier per step) while they leave room for two workgroups per CU; f32 tiles are
+// twice as large and its products eight times as long: one.
+template <typename T, int DP, int U>
+constexpr int kBuffers = sizeof(T) == 2 && 4 * U * Tile<T, DP>::kUnit <= 80 * 1024 ? 2 : 1;
+template <typename T, int DP, int U>
+constexpr int kTileBytes = 2 * kBuffers<T, DP, U> * U * Tile<T, DP>::kUnit;
+
 __device__ __forceinline__ int acc_row(int r, int half) { return 8 * (r >> 2) + 4 * half + (r & 3); }
 
 // The tile's list without places that are no block or stand in it already, in LDS, in order.
@@ -147,18 +209,25 @@ __device__ __forceinline__ Where where(const Args& a) {
   return w;
 }
 
+// What a row's waves have in common at the end: wave kw = 0 takes in the others' sums through LDS.
+template <int RW, int DP>
+struct Join {
+  float o[RW * 32 * (DP + 1)];
+  float m[RW * 32], l[RW * 32];
+};
+
 // Forward. RW waves stand side by side over 32 rows each, 4 / RW take turns at the list's units
 // of 32 keys and are joined at the end. The rows of a tile are its queries of all heads that
 // share the key head (few queries: they fill the instruction's columns together).
 template <typename T, int DP, int RW>
 __global__ __launch_bounds__(NT) void k_attend_fwd(Args a) {
   using M = Mma<T>;
+  using L = Tile<T, DP>;
   using Frag = typename M::Frag;
-  constexpr int KW = 4 / RW, NS = DP / 16, ND = DP / 32;
-  extern __shared__ int32_t list[];
+  constexpr int KW = 4 / RW, NS = DP / 16, ND = DP / 32, NB = kBuffers<T, DP, KW>;
+  extern __shared__ __align__(16) char lds[];
   __shared__ int count;
-  __shared__ float join[KW > 1 ? RW * 32 * (DP + 1) : 1];
-  __shared__ float join_m[RW * 32], join_l[RW * 32];
+  int32_t* list = (int32_t*)(lds + kTileBytes<T, DP, KW>);
   const Where at = where(a);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, col = lane & 31;
   const int rw = wave % RW, kw = wave / RW;
@@ -174,55 +243,85 @@ __global__ __launch_bounds__(NT) void k_attend_fwd(Args a) {
     n = block_list(a.index + (((int64_t)at.b * a.Hkv + at.hk) * a.Tq + at.t) * a.top, a.top, blocks, list, &count);
 
   const T* qp = (const T*)a.q.p + at.b * a.q.b + (valid ? i : 0) * a.q.l + h * a.q.h;
+  const float scale2 = fabsf(a.scale) * kLog2e;
   Frag qf[NS];
 #pragma unroll
-  for (int s = 0; s < NS; ++s) qf[s] = row_frag<T>(qp, 16 * s + 8 * half, a.D, valid);
+  for (int s = 0; s < NS; ++s) {
+    qf[s] = row_frag<T>(qp, 16 * s + 8 * half, a.D, valid);
+    if (a.scale < 0.f) qf[s] = -qf[s];
+  }
   const T* kp = (const T*)a.k.p + at.b * a.k.b + at.hk * a.k.h;
   const T* vp = (const T*)a.v.p + at.b * a.v.b + at.hk * a.v.h;
 
   f32x16 o[ND] = {};
-  float m = -INFINITY, l = 0.f;
-  const float scale2 = a.scale * kLog2e;
+  // m: what the exponents are taken relative to, in units of x; it follows the running maximum only
+  // when that has risen by 8 powers of two (p stays below 2^8, and o is rarely rescaled)
+  float m = -INFINITY, base2 = 0.f, l = 0.f;
   const int upb = a.block / 32, units = n * upb;
   const int per = (units + a.splits - 1) / a.splits;
-  const int u1 = min(units, (at.split + 1) * per);
-  for (int u = at.split * per + kw; u < u1; u += KW) {
-    const int64_t k0 = (int64_t)list[u / upb] * a.block + 32 * (u % upb);
-    if (k0 >= nk) continue;
-    const int left = (int)min((int64_t)32, nk - k0);
+  const int u0 = min(units, at.split * per), u1 = min(units, u0 + per);
+  const auto key0 = [&](int u) { return (int64_t)list[u / upb] * a.block + 32 * (u % upb); };
+  const auto keys = [&](int u) { return u < u1 ? (int)max((int64_t)0, min((int64_t)32, nk - key0(u))) : 0; };
+  Stage<T, DP, KW> sk, sv;
+  const auto fetch = [&](int u) {
+    const auto have = [&](int j) { return keys(u + j); };
+    sk.load(kp, a.k.l, a.D, [&](int j) { return key0(u + j) * a.k.l; }, have);
+    sv.load(vp, a.v.l, a.D, [&](int j) { return key0(u + j) * a.v.l; }, have);
+  };
+  if (u0 < u1) fetch(u0);
+  for (int u = u0, step = 0; u < u1; u += KW, ++step) {
+    char* tk = lds + (step % NB) * 2 * KW * L::kUnit;
+    char* tv = tk + KW * L::kUnit;
+    if (NB == 1) __syncthreads();
+    sk.store(tk);
+    sv.store(tv);
+    __syncthreads();
+    if (u + KW < u1) fetch(u + KW);
+    tk += kw * L::kUnit;
+    tv += kw * L::kUnit;
+    const int left = keys(u + kw);
+    if (left == 0) continue;
     f32x16 x = {};
 #pragma unroll
-    for (int s = 0; s < NS; ++s)
-      x = M::mma(row_frag<T>(kp + (k0 + min(col, left - 1)) * a.k.l, 16 * s + 8 * half, a.D, col < left), qf[s], x);
-    float mx = -INFINITY;
+    for (int s = 0; s < NS; ++s) x = M::mma(L::row(tk, s, col, half), qf[s], x);
+    if (left < 32) {
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      x[r] = acc_row(r, half) < left ? x[r] * scale2 : -INFINITY;
-      mx = fmaxf(mx, x[r]);
+      for (int r = 0; r < 16; ++r) x[r] = acc_row(r, half) < left ? x[r] : -INFINITY;
     }
+    float mx = x[0];
+#pragma unroll
+    for (int r = 1; r < 16; ++r) mx = fmaxf(mx, x[r]);
     mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-    const float mn = fmaxf(m, mx), base = mn == -INFINITY ? 0.f : mn;
-    const float alpha = exp2f(m - base);
-    m = mn;
+    if (__any((mx - m) * scale2 > 8.f || m == -INFINITY)) {
+      const float mn = fmaxf(m, mx), b2 = mn == -INFINITY ? 0.f : mn * scale2;
+      const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(base2 - b2);
+      m = mn;
+      base2 = b2;
+      l *= alpha;
+#pragma unroll
+      for (int d = 0; d < ND; ++d) o[d] *= alpha;
+    }
     float sum = 0.f;
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
-      x[r] = exp2f(x[r] - base);
+      x[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[r], scale2, -base2));
+      if (left < 32) x[r] = acc_row(r, half) < left ? x[r] : 0.f;  // (a scale of 0: not -inf * 0)
       sum += x[r];
     }
-    l = l * alpha + sum;
+    l += sum;
     const Frag p0 = acc_frag<T>(x, 0), p1 = acc_frag<T>(x, 1);
 #pragma unroll
     for (int d = 0; d < ND; ++d) {
-      o[d] *= alpha;
-      o[d] = M::mma(col_frag<T>(vp + k0 * a.v.l, a.v.l, 0, half, 32 * d + col, a.D, left), p0, o[d]);
-      o[d] = M::mma(col_frag<T>(vp + k0 * a.v.l, a.v.l, 1, half, 32 * d + col, a.D, left), p1, o[d]);
+      o[d] = M::mma(L::col(tv, 0, d, lane), p0, o[d]);
+      o[d] = M::mma(L::col(tv, 1, d, lane), p1, o[d]);
     }
   }
   l += __shfl_xor(l, 32, 64);
   if constexpr (KW > 1) {
+    static_assert(sizeof(Join<RW, DP>) <= kTileBytes<T, DP, KW>, "joined in the tiles' place");
+    Join<RW, DP>& join = *(Join<RW, DP>*)lds;
+    float* jo = join.o + (rw * 32 + col) * (DP + 1);
     for (int k = 1; k < KW; ++k) {
-      float* jo = join + (rw * 32 + col) * (DP + 1);
       __syncthreads();
       if (kw == k) {
 #pragma unroll
@@ -230,16 +329,17 @@ __global__ __launch_bounds__(NT) void k_attend_fwd(Args a) {
 #pragma unroll
           for (int r = 0; r < 16; ++r) jo[32 * d + acc_row(r, half)] = o[d][r];
         if (half == 0) {
-          join_m[rw * 32 + col] = m;
-          join_l[rw * 32 + col] = l;
+          join.m[rw * 32 + col] = m == -INFINITY ? m : base2;
+          join.l[rw * 32 + col] = l;
         }
       }
       __syncthreads();
       if (kw == 0) {
-        const float mo = join_m[rw * 32 + col], lo = join_l[rw * 32 + col];
-        const float mn = fmaxf(m, mo), base = mn == -INFINITY ? 0.f : mn;
-        const float fa = exp2f(m - base), fb = exp2f(mo - base);
-        m = mn;
+        const float mo = join.m[rw * 32 + col], lo = join.l[rw * 32 + col], me = m == -INFINITY ? m : base2;
+        const float mn = fmaxf(me, mo), b2 = mn == -INFINITY ? 0.f : mn;
+        const float fa = __builtin_amdgcn_exp2f(me - b2), fb = __builtin_amdgcn_exp2f(mo - b2);
+        m = mn;  // from here on in powers of two
+        base2 = b2;
         l = l * fa + lo * fb;
 #pragma unroll
         for (int d = 0; d < ND; ++d)
@@ -249,6 +349,7 @@ __global__ __launch_bounds__(NT) void k_attend_fwd(Args a) {
     }
   }
   if (kw != 0 || !exists) return;
+  const float top2 = m == -INFINITY ? m : base2;
   if (a.splits > 1) {
     const int64_t r = ((int64_t)at.b * a.Hq + h) * a.Lq + i, rows = (int64_t)(gridDim.z / a.splits) * a.Hq * a.Lq;
     float* po = a.part + (at.split * rows + r) * a.D;
@@ -259,7 +360,7 @@ __global__ __launch_bounds__(NT) void k_attend_fwd(Args a) {
         if (32 * d + 8 * c + 4 * half < a.D)
           store4<float>(po + 32 * d + 8 * c + 4 * half, o[d][4 * c], o[d][4 * c + 1], o[d][4 * c + 2], o[d][4 * c + 3]);
     if (half == 0) {
-      a.part_m[at.split * rows + r] = m;
+      a.part_m[at.split * rows + r] = top2;
       a.part_l[at.split * rows + r] = l;
     }
     return;
@@ -273,7 +374,7 @@ __global__ __launch_bounds__(NT) void k_attend_fwd(Args a) {
       if (32 * d + 8 * c + 4 * half < a.D)
         store4<T>(op + 32 * d + 8 * c + 4 * half, o[d][4 * c] * inv, o[d][4 * c + 1] * inv, o[d][4 * c + 2] * inv,
                   o[d][4 * c + 3] * inv);
-  if (half == 0 && a.lse) a.lse[((int64_t)at.b * a.Hq + h) * a.Lq + i] = valid ? m + log2f(l) : -INFINITY;
+  if (half == 0 && a.lse) a.lse[((int64_t)at.b * a.Hq + h) * a.Lq + i] = valid ? top2 + log2f(l) : -INFINITY;
 }
 
 // Joins the parts of a split list: one row per group of D / 4 threads.
@@ -302,31 +403,6 @@ __global__ __launch_bounds__(NT) void k_attend_join(Args a, int64_t rows) {
   if (d == 0 && a.lse) a.lse[r] = valid ? m + log2f(l) : -INFINITY;
 }
 
-// delta = sum_d do o per row, and the largest |do| (its bits order as the numbers do).
-template <typename T>
-__global__ __launch_bounds__(NT) void k_attend_delta(Args a, int64_t rows) {
-  const int sub = threadIdx.x % 16;
-  const int64_t r = (int64_t)blockIdx.x * (NT / 16) + threadIdx.x / 16;
-  const bool in = r < rows;
-  const int64_t i = in ? r % a.Lq : 0, bh = in ? r / a.Lq : 0, b = bh / a.Hq, h = bh % a.Hq;
-  const bool valid = in && i < length_of(a.q_lengths, (int)b, a.Lq);
-  const T* op = (const T*)a.o.p + b * a.o.b + i * a.o.l + h * a.o.h;
-  const T* gp = (const T*)a.g.p + b * a.g.b + i * a.g.l + h * a.g.h;
-  float s = 0.f, mx = 0.f;
-  const auto of = row_frag<T>(op, 8 * sub, a.D, valid), gf = row_frag<T>(gp, 8 * sub, a.D, valid);
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    s += (float)of[j] * (float)gf[j];
-    mx = fmaxf(mx, fabsf((float)gf[j]));
-  }
-#pragma unroll
-  for (int off = 8; off > 0; off >>= 1) s += __shfl_xor(s, off, 64);
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor(mx, off, 64));
-  if (in && sub == 0) a.delta[r] = s;
-  if ((threadIdx.x & 63) == 0 && mx > 0.f) atomicMax(a.gmax, __float_as_uint(mx));
-}
-
 // Which tiles chose a block: bits [B, Hkv, Tk, ceil(Tq / 32)].
 __global__ __launch_bounds__(NT) void k_attend_mark(Args a) {
   const int t = blockIdx.x, hk = blockIdx.y, b = blockIdx.z;
@@ -339,29 +415,29 @@ __global__ __launch_bounds__(NT) void k_attend_mark(Args a) {
   }
 }
 
-// ds is rounded to the inputs' type for its products. f16 has few exponents, so it is taken
-// relative to the power of two at the largest |do| there (exact, undone in 32 bits).
+// ds is rounded to the inputs' type for its products. f16 has few exponents, so ds is taken there
+// relative to a power of two at the largest |do| (exact, undone in 32 bits): of the row in dq, of all rows
+// in dk.
 template <typename T>
-__device__ __forceinline__ void ds_scale(const uint32_t* gmax, float& down, float& up) {
-  down = up = 1.f;
-  if constexpr (sizeof(T) == 2 && !__is_same(T, bf16)) {
-    const int e = (int)((*gmax >> 23) & 255);
-    if (e > 27 && e < 227) {
-      down = __uint_as_float((uint32_t)(254 - e) << 23);
-      up = __uint_as_float((uint32_t)e << 23);
-    }
-  }
+constexpr bool kFewExponents = __is_same(T, f16);
+__device__ __forceinline__ void ds_scale(uint32_t largest, float& down, float& up) {
+  const int e = (int)((largest >> 23) & 255);
+  const bool ok = e > 27 && e < 227;
+  down = ok ? __uint_as_float((uint32_t)(254 - e) << 23) : 1.f;
+  up = ok ? __uint_as_float((uint32_t)e << 23) : 1.f;
 }
 
-// dq: the forward's shape; p is taken from the saved lse.
+// dq: the forward's shape; p is taken from the saved lse. delta = sum_d do o of each row on the
+// way, kept for dk.
 template <typename T, int DP, int RW>
 __global__ __launch_bounds__(NT) void k_attend_dq(Args a) {
   using M = Mma<T>;
+  using L = Tile<T, DP>;
   using Frag = typename M::Frag;
-  constexpr int KW = 4 / RW, NS = DP / 16, ND = DP / 32;
-  extern __shared__ int32_t list[];
+  constexpr int KW = 4 / RW, NS = DP / 16, ND = DP / 32, NB = kBuffers<T, DP, KW>;
+  extern __shared__ __align__(16) char lds[];
   __shared__ int count;
-  __shared__ float join[KW > 1 ? RW * 32 * (DP + 1) : 1];
+  int32_t* list = (int32_t*)(lds + kTileBytes<T, DP, KW>);
   const Where at = where(a);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, col = lane & 31;
   const int rw = wave % RW, kw = wave / RW;
@@ -379,49 +455,82 @@ __global__ __launch_bounds__(NT) void k_attend_dq(Args a) {
   const int64_t ir = valid ? i : 0;
   const T* qp = (const T*)a.q.p + at.b * a.q.b + ir * a.q.l + h * a.q.h;
   const T* gp = (const T*)a.g.p + at.b * a.g.b + ir * a.g.l + h * a.g.h;
+  const T* op = (const T*)a.o.p + at.b * a.o.b + ir * a.o.l + h * a.o.h;
   Frag qf[NS], gf[NS];
+  float delta = 0.f, most = 0.f;
 #pragma unroll
   for (int s = 0; s < NS; ++s) {
     qf[s] = row_frag<T>(qp, 16 * s + 8 * half, a.D, valid);
     gf[s] = row_frag<T>(gp, 16 * s + 8 * half, a.D, valid);
+    const Frag of = row_frag<T>(op, 16 * s + 8 * half, a.D, valid);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      delta += (float)gf[s][j] * (float)of[j];
+      if (kFewExponents<T>) most = fmaxf(most, fabsf((float)gf[s][j]));
+    }
+  }
+  delta += __shfl_xor(delta, 32, 64);
+  float down = 1.f, up = 1.f;
+  if constexpr (kFewExponents<T>) {
+    most = fmaxf(most, __shfl_xor(most, 32, 64));
+    ds_scale(__float_as_uint(most), down, up);
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) most = fmaxf(most, __shfl_xor(most, off, 64));
+    if (kw == 0 && lane == 0 && most > 0.f) atomicMax(a.gmax, __float_as_uint(most));  // any order, the same answer
   }
   const int64_t stat = ((int64_t)at.b * a.Hq + h) * a.Lq + ir;
-  const float lse = valid ? a.lse[stat] : -INFINITY, delta = valid ? a.delta[stat] : 0.f;
+  const float lse = valid ? a.lse[stat] : -INFINITY;
+  if (kw == 0 && half == 0 && valid) a.delta[stat] = delta;
   const bool empty = lse == -INFINITY;
   const T* kp = (const T*)a.k.p + at.b * a.k.b + at.hk * a.k.h;
   const T* vp = (const T*)a.v.p + at.b * a.v.b + at.hk * a.v.h;
-  float down, up;
-  ds_scale<T>(a.gmax, down, up);
 
   f32x16 dq[ND] = {};
   const float scale2 = a.scale * kLog2e;
   const int upb = a.block / 32, units = n * upb;
-  for (int u = kw; u < units; u += KW) {
-    const int64_t k0 = (int64_t)list[u / upb] * a.block + 32 * (u % upb);
-    if (k0 >= nk) continue;
-    const int left = (int)min((int64_t)32, nk - k0);
-    const int64_t kr = k0 + min(col, left - 1);
+  const auto key0 = [&](int u) { return (int64_t)list[u / upb] * a.block + 32 * (u % upb); };
+  const auto keys = [&](int u) { return u < units ? (int)max((int64_t)0, min((int64_t)32, nk - key0(u))) : 0; };
+  Stage<T, DP, KW> sk, sv;
+  const auto fetch = [&](int u) {
+    const auto have = [&](int j) { return keys(u + j); };
+    sk.load(kp, a.k.l, a.D, [&](int j) { return key0(u + j) * a.k.l; }, have);
+    sv.load(vp, a.v.l, a.D, [&](int j) { return key0(u + j) * a.v.l; }, have);
+  };
+  if (units) fetch(0);
+  for (int u = 0, step = 0; u < units; u += KW, ++step) {
+    char* tk = lds + (step % NB) * 2 * KW * L::kUnit;
+    char* tv = tk + KW * L::kUnit;
+    if (NB == 1) __syncthreads();
+    sk.store(tk);
+    sv.store(tv);
+    __syncthreads();
+    if (u + KW < units) fetch(u + KW);
+    tk += kw * L::kUnit;
+    tv += kw * L::kUnit;
+    const int left = keys(u + kw);
+    if (left == 0) continue;
     f32x16 x = {}, dp = {};
 #pragma unroll
     for (int s = 0; s < NS; ++s) {
-      x = M::mma(row_frag<T>(kp + kr * a.k.l, 16 * s + 8 * half, a.D, col < left), qf[s], x);
-      dp = M::mma(row_frag<T>(vp + kr * a.v.l, 16 * s + 8 * half, a.D, col < left), gf[s], dp);
+      x = M::mma(L::row(tk, s, col, half), qf[s], x);
+      dp = M::mma(L::row(tv, s, col, half), gf[s], dp);
     }
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
-      const float p = !empty && acc_row(r, half) < left ? exp2f(x[r] * scale2 - lse) : 0.f;
-      x[r] = p * (dp[r] - delta) * down;
+      float p = __builtin_amdgcn_exp2f(__builtin_fmaf(x[r], scale2, -lse));
+      if (left < 32) p = acc_row(r, half) < left ? p : 0.f;
+      x[r] = empty ? 0.f : p * ((dp[r] - delta) * down);
     }
     const Frag s0 = acc_frag<T>(x, 0), s1 = acc_frag<T>(x, 1);
 #pragma unroll
     for (int d = 0; d < ND; ++d) {
-      dq[d] = M::mma(col_frag<T>(kp + k0 * a.k.l, a.k.l, 0, half, 32 * d + col, a.D, left), s0, dq[d]);
-      dq[d] = M::mma(col_frag<T>(kp + k0 * a.k.l, a.k.l, 1, half, 32 * d + col, a.D, left), s1, dq[d]);
+      dq[d] = M::mma(L::col(tk, 0, d, lane), s0, dq[d]);
+      dq[d] = M::mma(L::col(tk, 1, d, lane), s1, dq[d]);
     }
   }
   if constexpr (KW > 1) {
+    float* jo = (float*)lds + (rw * 32 + col) * (DP + 1);
     for (int k = 1; k < KW; ++k) {
-      float* jo = join + (rw * 32 + col) * (DP + 1);
       __syncthreads();
       if (kw == k)
 #pragma unroll
@@ -437,15 +546,19 @@ __global__ __launch_bounds__(NT) void k_attend_dq(Args a) {
     }
   }
   if (kw != 0 || !exists) return;
-  T* op = (T*)a.dq + (((int64_t)at.b * a.Lq + i) * a.Hq + h) * a.D;
-  const float f = valid ? a.scale * up : 0.f;
+  T* out = (T*)a.dq + (((int64_t)at.b * a.Lq + i) * a.Hq + h) * a.D;
+  const float f = a.scale * up;
 #pragma unroll
   for (int d = 0; d < ND; ++d)
 #pragma unroll
     for (int c = 0; c < 4; ++c)
-      if (32 * d + 8 * c + 4 * half < a.D)
-        store4<T>(op + 32 * d + 8 * c + 4 * half, dq[d][4 * c] * f, dq[d][4 * c + 1] * f, dq[d][4 * c + 2] * f,
-                  dq[d][4 * c + 3] * f);
+      if (32 * d + 8 * c + 4 * half < a.D) {
+        if (valid)
+          store4<T>(out + 32 * d + 8 * c + 4 * half, dq[d][4 * c] * f, dq[d][4 * c + 1] * f, dq[d][4 * c + 2] * f,
+                    dq[d][4 * c + 3] * f);
+        else
+          store4<T>(out + 32 * d + 8 * c + 4 * half, 0.f, 0.f, 0.f, 0.f);
+      }
 }
 
 // dk, dv of one key block: RW waves hold 32 keys each, 4 / RW take turns at the 32-query units of
@@ -455,11 +568,13 @@ constexpr int kTiles = 1024;  // tiles listed at a time
 template <typename T, int DP, int RW>
 __global__ __launch_bounds__(NT) void k_attend_dkv(Args a) {
   using M = Mma<T>;
+  using L = Tile<T, DP>;
   using Frag = typename M::Frag;
-  constexpr int QW = 4 / RW, NS = DP / 16, ND = DP / 32;
+  constexpr int QW = 4 / RW, NS = DP / 16, ND = DP / 32, NB = kBuffers<T, DP, QW>;
+  extern __shared__ __align__(16) char lds[];
   __shared__ int32_t tiles[kTiles];
   __shared__ int count;
-  __shared__ float join[QW > 1 ? RW * 32 * (DP + 1) : 1];
+  __shared__ float stats[NB][2][QW * 32];  // lse and delta of the staged rows
   const int blk = blockIdx.x, hk = blockIdx.y, b = blockIdx.z;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, col = lane & 31;
   const int rw = wave % RW, qw = wave / RW;
@@ -475,13 +590,14 @@ __global__ __launch_bounds__(NT) void k_attend_dkv(Args a) {
     kf[s] = row_frag<T>(kp, 16 * s + 8 * half, a.D, valid);
     vf[s] = row_frag<T>(vp, 16 * s + 8 * half, a.D, valid);
   }
-  float down, up;
-  ds_scale<T>(a.gmax, down, up);
+  float down = 1.f, up = 1.f;
+  if constexpr (kFewExponents<T>) ds_scale(*a.gmax, down, up);
   f32x16 dk[ND] = {}, dv[ND] = {};
   const float scale2 = a.scale * kLog2e;
-  const int upb = a.block / 32, words = (a.Tq + 31) / 32;
+  const int upb = a.block / 32, upt = a.G * upb, words = (a.Tq + 31) / 32;  // units per tile
   const uint32_t* bits = a.bits + (((int64_t)b * a.Hkv + hk) * a.Tk + blk) * words;
   const bool any = (int64_t)blk * a.block < nk;
+  int step = 0;
   for (int w0 = 0; any && w0 < words; w0 += kTiles / 32) {
     __syncthreads();
     if (threadIdx.x < 64) {  // the first 32 lanes hold a word each
@@ -495,42 +611,69 @@ __global__ __launch_bounds__(NT) void k_attend_dkv(Args a) {
       if (lane == 63) count = (int)incl;
     }
     __syncthreads();
-    const int units = count * a.G * upb;
-    for (int u = qw; u < units; u += QW) {
-      const int64_t i0 = (int64_t)tiles[u / (a.G * upb)] * a.block + 32 * (u % upb);
-      const int h = hk * a.G + (u / upb) % a.G;
-      if (i0 >= nq) continue;
-      const int left = (int)min((int64_t)32, nq - i0);
-      const T* qp = (const T*)a.q.p + b * a.q.b + i0 * a.q.l + h * a.q.h;
-      const T* gp = (const T*)a.g.p + b * a.g.b + i0 * a.g.l + h * a.g.h;
-      const int qr = min(col, left - 1);
+    const int units = count * upt;
+    const auto row0 = [&](int u) { return (int64_t)tiles[u / upt] * a.block + 32 * (u % upb); };
+    const auto head = [&](int u) { return hk * a.G + (u / upb) % a.G; };
+    const auto rows = [&](int u) { return u < units ? (int)max((int64_t)0, min((int64_t)32, nq - row0(u))) : 0; };
+    Stage<T, DP, QW> sq, sg;
+    float st_lse = -INFINITY, st_delta = 0.f;
+    const auto fetch = [&](int u) {
+      const auto have = [&](int j) { return rows(u + j); };
+      sq.load((const T*)a.q.p + b * a.q.b, a.q.l, a.D, [&](int j) { return row0(u + j) * a.q.l + head(u + j) * a.q.h; }, have);
+      sg.load((const T*)a.g.p + b * a.g.b, a.g.l, a.D, [&](int j) { return row0(u + j) * a.g.l + head(u + j) * a.g.h; }, have);
+      if (threadIdx.x < QW * 32) {
+        const int j = threadIdx.x / 32, r = threadIdx.x % 32;
+        st_lse = -INFINITY;
+        if (r < rows(u + j)) {
+          const int64_t stat = ((int64_t)b * a.Hq + head(u + j)) * a.Lq + row0(u + j) + r;
+          st_lse = a.lse[stat];
+          st_delta = a.delta[stat];
+        }
+      }
+    };
+    if (units) fetch(0);
+    for (int u = 0; u < units; u += QW, ++step) {
+      char* tq = lds + (step % NB) * 2 * QW * L::kUnit;
+      char* tg = tq + QW * L::kUnit;
+      if (NB == 1) __syncthreads();
+      sq.store(tq);
+      sg.store(tg);
+      if (threadIdx.x < QW * 32) {
+        stats[step % NB][0][threadIdx.x] = st_lse;
+        stats[step % NB][1][threadIdx.x] = st_delta;
+      }
+      __syncthreads();
+      if (u + QW < units) fetch(u + QW);
+      if (rows(u + qw) == 0) continue;
+      tq += qw * L::kUnit;
+      tg += qw * L::kUnit;
       f32x16 x = {}, dp = {};
 #pragma unroll
       for (int s = 0; s < NS; ++s) {
-        x = M::mma(row_frag<T>(qp + qr * a.q.l, 16 * s + 8 * half, a.D, col < left), kf[s], x);
-        dp = M::mma(row_frag<T>(gp + qr * a.g.l, 16 * s + 8 * half, a.D, col < left), vf[s], dp);
+        x = M::mma(L::row(tq, s, col, half), kf[s], x);
+        dp = M::mma(L::row(tg, s, col, half), vf[s], dp);
       }
-      const int64_t stat = ((int64_t)b * a.Hq + h) * a.Lq + i0;
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         const int ri = acc_row(r, half);
-        const float lse = ri < left ? a.lse[stat + ri] : -INFINITY, delta = ri < left ? a.delta[stat + ri] : 0.f;
-        const float p = valid && lse != -INFINITY ? exp2f(x[r] * scale2 - lse) : 0.f;
-        x[r] = p;
-        dp[r] = p * (dp[r] - delta) * down;
+        const float lse = stats[step % NB][0][qw * 32 + ri], delta = stats[step % NB][1][qw * 32 + ri];
+        const bool on = valid && lse != -INFINITY;
+        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(x[r], scale2, -lse));
+        x[r] = on ? p : 0.f;
+        dp[r] = on ? p * ((dp[r] - delta) * down) : 0.f;
       }
       const Frag p0 = acc_frag<T>(x, 0), p1 = acc_frag<T>(x, 1), s0 = acc_frag<T>(dp, 0), s1 = acc_frag<T>(dp, 1);
 #pragma unroll
       for (int d = 0; d < ND; ++d) {
-        dv[d] = M::mma(col_frag<T>(gp, a.g.l, 0, half, 32 * d + col, a.D, left), p0, dv[d]);
-        dv[d] = M::mma(col_frag<T>(gp, a.g.l, 1, half, 32 * d + col, a.D, left), p1, dv[d]);
-        dk[d] = M::mma(col_frag<T>(qp, a.q.l, 0, half, 32 * d + col, a.D, left), s0, dk[d]);
-        dk[d] = M::mma(col_frag<T>(qp, a.q.l, 1, half, 32 * d + col, a.D, left), s1, dk[d]);
+        dv[d] = M::mma(L::col(tg, 0, d, lane), p0, dv[d]);
+        dv[d] = M::mma(L::col(tg, 1, d, lane), p1, dv[d]);
+        dk[d] = M::mma(L::col(tq, 0, d, lane), s0, dk[d]);
+        dk[d] = M::mma(L::col(tq, 1, d, lane), s1, dk[d]);
       }
     }
   }
   if constexpr (QW > 1) {
-    float* jo = join + (rw * 32 + col) * (DP + 1);
+    float* jo = (float*)lds + (rw * 32 + col) * (DP + 1);
     for (int k = 1; k < QW; ++k)
 #pragma unroll
       for (int which = 0; which < 2; ++which) {
@@ -563,6 +706,14 @@ __global__ __launch_bounds__(NT) void k_attend_dkv(Args a) {
       }
 }
 
+template <typename K>
+int launch(K kernel, const Args& a, dim3 grid, size_t lds, hipStream_t st, const char* what) {
+  if (lds > 32 * 1024)
+    if (int e = dsplat::ensure_dyn_lds((const void*)kernel, lds, what)) return e;
+  kernel<<<grid, NT, lds, st>>>(a);
+  return dsplat::check_launch(what);
+}
+
 // 32-row waves side by side: as many as the tile's rows fill.
 inline int row_waves(const Args& a) {
   const int rows = a.Lt * a.G;
@@ -577,41 +728,38 @@ inline int splits_of(int64_t workgroups, int units) {
 
 template <typename T, int DP, int RW>
 struct Fwd {
-  static int go(const Args& a, dim3 grid, size_t lds, hipStream_t st) {
-    k_attend_fwd<T, DP, RW><<<grid, NT, lds, st>>>(a);
-    return dsplat::check_launch("k_attend_fwd");
+  static int go(const Args& a, dim3 grid, hipStream_t st) {
+    return launch(k_attend_fwd<T, DP, RW>, a, grid, kTileBytes<T, DP, 4 / RW> + a.top * sizeof(int32_t), st, "k_attend_fwd");
   }
 };
 template <typename T, int DP, int RW>
 struct Dq {
-  static int go(const Args& a, dim3 grid, size_t lds, hipStream_t st) {
-    k_attend_dq<T, DP, RW><<<grid, NT, lds, st>>>(a);
-    return dsplat::check_launch("k_attend_dq");
+  static int go(const Args& a, dim3 grid, hipStream_t st) {
+    return launch(k_attend_dq<T, DP, RW>, a, grid, kTileBytes<T, DP, 4 / RW> + a.top * sizeof(int32_t), st, "k_attend_dq");
   }
 };
 template <typename T, int DP, int RW>
 struct Dkv {
-  static int go(const Args& a, dim3 grid, size_t, hipStream_t st) {
-    k_attend_dkv<T, DP, RW><<<grid, NT, 0, st>>>(a);
-    return dsplat::check_launch("k_attend_dkv");
+  static int go(const Args& a, dim3 grid, hipStream_t st) {
+    return launch(k_attend_dkv<T, DP, RW>, a, grid, kTileBytes<T, DP, 4 / RW>, st, "k_attend_dkv");
   }
 };
 template <template <typename, int, int> class F, typename T, int DP>
-int by_waves(int rw, const Args& a, dim3 grid, size_t lds, hipStream_t st) {
-  return rw == 1 ? F<T, DP, 1>::go(a, grid, lds, st) : rw == 2 ? F<T, DP, 2>::go(a, grid, lds, st) : F<T, DP, 4>::go(a, grid, lds, st);
+int by_waves(int rw, const Args& a, dim3 grid, hipStream_t st) {
+  return rw == 1 ? F<T, DP, 1>::go(a, grid, st) : rw == 2 ? F<T, DP, 2>::go(a, grid, st) : F<T, DP, 4>::go(a, grid, st);
 }
 template <template <typename, int, int> class F, typename T>
-int by_width(int rw, const Args& a, dim3 grid, size_t lds, hipStream_t st) {
-  if (a.D <= 32) return by_waves<F, T, 32>(rw, a, grid, lds, st);
-  if (a.D <= 64) return by_waves<F, T, 64>(rw, a, grid, lds, st);
-  if (a.D <= 96) return by_waves<F, T, 96>(rw, a, grid, lds, st);
-  return by_waves<F, T, 128>(rw, a, grid, lds, st);
+int by_width(int rw, const Args& a, dim3 grid, hipStream_t st) {
+  if (a.D <= 32) return by_waves<F, T, 32>(rw, a, grid, st);
+  if (a.D <= 64) return by_waves<F, T, 64>(rw, a, grid, st);
+  if (a.D <= 96) return by_waves<F, T, 96>(rw, a, grid, st);
+  return by_waves<F, T, 128>(rw, a, grid, st);
 }
 template <template <typename, int, int> class F>
-int by_type(int dtype, int rw, const Args& a, dim3 grid, size_t lds, hipStream_t st) {
-  if (dtype == DTK_F32) return by_width<F, float>(rw, a, grid, lds, st);
-  if (dtype == DTK_BF16) return by_width<F, bf16>(rw, a, grid, lds, st);
-  return by_width<F, f16>(rw, a, grid, lds, st);
+int by_type(int dtype, int rw, const Args& a, dim3 grid, hipStream_t st) {
+  if (dtype == DTK_F32) return by_width<F, float>(rw, a, grid, st);
+  if (dtype == DTK_BF16) return by_width<F, bf16>(rw, a, grid, st);
+  return by_width<F, f16>(rw, a, grid, st);
 }
 
 int check(const dtk_attention* c, const char* who) {
@@ -679,7 +827,7 @@ int dtk_block_sparse_attention_fwd(const dtk_attention* c, void* workspace, void
     a.part_l = a.part_m + a.splits * rows;
   }
   const dim3 grid(a.Tq * a.rowtiles, a.Hkv, c->B * a.splits);
-  if (int e = by_type<Fwd>(c->dtype, row_waves(a), a, grid, a.top * sizeof(int32_t), st)) return e;
+  if (int e = by_type<Fwd>(c->dtype, row_waves(a), a, grid, st)) return e;
   if (a.splits == 1) return 0;
   const unsigned blocks = (unsigned)((rows * (a.D / 4) + NT - 1) / NT);
   if (c->dtype == DTK_F32) k_attend_join<float><<<blocks, NT, 0, st>>>(a, rows);
@@ -718,20 +866,15 @@ int dtk_block_sparse_attention_bwd(const dtk_attention* c, const void* dout, con
   const size_t nbits = (size_t)c->B * c->Hkv * a.Tk * ((a.Tq + 31) / 32);
   if (int e = dsplat::zero_async(a.gmax, 256 + nbits * 4, st, "dtk_block_sparse_attention_bwd")) return e;
   if (c->Lq) {
-    const unsigned blocks = (unsigned)((rows + NT / 16 - 1) / (NT / 16));
-    if (c->dtype == DTK_F32) k_attend_delta<float><<<blocks, NT, 0, st>>>(a, rows);
-    else if (c->dtype == DTK_BF16) k_attend_delta<bf16><<<blocks, NT, 0, st>>>(a, rows);
-    else k_attend_delta<f16><<<blocks, NT, 0, st>>>(a, rows);
-    if (int e = dsplat::check_launch("k_attend_delta")) return e;
     const dim3 grid(a.Tq * a.rowtiles, a.Hkv, c->B);
-    if (int e = by_type<Dq>(c->dtype, row_waves(a), a, grid, a.top * sizeof(int32_t), st)) return e;
+    if (int e = by_type<Dq>(c->dtype, row_waves(a), a, grid, st)) return e;
     if (a.Tk) {
       k_attend_mark<<<dim3(a.Tq, a.Hkv, c->B), NT, 0, st>>>(a);
       if (int e = dsplat::check_launch("k_attend_mark")) return e;
     }
   }
   if (!a.Tk) return 0;
-  return by_type<Dkv>(c->dtype, a.block / 32, a, dim3(a.Tk, a.Hkv, c->B), 0, st);
+  return by_type<Dkv>(c->dtype, a.block / 32, a, dim3(a.Tk, a.Hkv, c->B), st);
 }
 
 }  // extern "C"
