@@ -26,53 +26,98 @@ __device__ __forceinline__ int64_t length_of(const int32_t* lengths, int b, int6
   return n < 0 ? 0 : n < L ? n : L;
 }
 
-// grid (tiles, Hkv, B): out[b][hkv][tile][D] = mean over the tile's rows and the group's heads
-template <typename T>
-__global__ __launch_bounds__(NT) void k_pool(Rows x, int64_t L, int D, int group, int block, double* __restrict__ out) {
-  __shared__ double red[NT];
-  const int t = blockIdx.x, hk = blockIdx.y, b = blockIdx.z;
-  const int64_t lo = (int64_t)t * block;
-  const int n = (int)max((int64_t)0, min((int64_t)block, length_of(x.lengths, b, L) - lo));
-  const int lanes = min(NT, 1 << (32 - __clz(D - 1)));  // threads per row, a power of two >= D (D <= 256)
-  const int c = threadIdx.x % lanes, part = threadIdx.x / lanes, parts = NT / lanes;
-  double s = 0.0;
-  if (c < D) {
-    const T* p = (const T*)x.p + (int64_t)b * x.b + (int64_t)hk * group * x.h + c;
-    for (int i = part; i < n * group; i += parts) s += (double)(float)p[(lo + i / group) * x.l + (i % group) * x.h];
+// What the pooled rows of q (grid.x < Tq) and k (behind them) are made of; both in one launch.
+struct PoolArgs {
+  Rows x[2];
+  int64_t L[2];
+  int group[2];  // heads that share a pooled row
+  int Tq, D, pitch, block;
+  double* out[2];  // [B, Hkv, tiles, pitch]: zeros from D on
+};
+inline int pitch_of(int D) { return (D + 7) & ~7; }
+
+// One workgroup per tile: a thread sums one 16-byte piece of every (256 / pieces)-th row, the
+// threads of a piece are folded through LDS in a fixed order.
+template <typename T, bool VEC>
+__global__ __launch_bounds__(NT) void k_pool(PoolArgs a) {
+  constexpr int N = VEC ? Vec<T>::N : 1;
+  __shared__ double red[NT * N];
+  const int which = (int)blockIdx.x >= a.Tq, t = (int)blockIdx.x - (which ? a.Tq : 0);
+  const int hk = blockIdx.y, b = blockIdx.z, tiles = which ? gridDim.x - a.Tq : a.Tq, group = a.group[which];
+  const Rows x = a.x[which];
+  const int64_t lo = (int64_t)t * a.block;
+  const int n = (int)max((int64_t)0, min((int64_t)a.block, length_of(x.lengths, b, a.L[which]) - lo));
+  const int pieces = a.D / N, parts = NT / pieces;  // D <= 256
+  const int c = threadIdx.x % pieces, part = threadIdx.x / pieces;
+  const T* p = (const T*)x.p + (int64_t)b * x.b + (int64_t)hk * group * x.h + lo * x.l + c * N;
+  double s[N] = {};
+  if (part < parts) {
+    if constexpr (VEC) {
+      for (int g = 0; g < group; ++g)
+#pragma unroll 4
+        for (int i = part; i < n; i += parts) {
+          const Vec<T> v = load_vec(p + i * x.l + g * x.h);
+#pragma unroll
+          for (int e = 0; e < N; ++e) s[e] += (double)(float)v.v[e];
+        }
+    } else {
+      for (int i = part; i < n * group; i += parts) s[0] += (double)(float)p[(i / group) * x.l + (i % group) * x.h];
+    }
   }
-  red[threadIdx.x] = s;
+#pragma unroll
+  for (int e = 0; e < N; ++e) red[e * NT + threadIdx.x] = s[e];
   __syncthreads();
-  if (part == 0 && c < D) {
-    for (int k = 1; k < parts; ++k) s += red[k * lanes + c];
-    out[(((int64_t)b * gridDim.y + hk) * gridDim.x + t) * D + c] = n ? s / (double)(n * group) : 0.0;
+  double* out = a.out[which] + (((int64_t)b * gridDim.y + hk) * tiles + t) * a.pitch;
+  const double inv = n ? 1.0 / (double)(n * group) : 0.0;
+  for (int d = threadIdx.x; d < a.pitch; d += NT) {
+    double v = 0.0;
+    if (d < a.D)
+      for (int k = 0; k < parts; ++k) v += red[(d % N) * NT + k * pieces + d / N];
+    out[d] = v * inv;
   }
 }
 
-// grid (Tk / 64, Tq / 16, B * Hkv): 16 x 64 scores per workgroup, the pooled rows staged in LDS
-constexpr int SQ = 16, SK = 64, SD = 16;
-__global__ __launch_bounds__(NT) void k_scores(int Tq, int Tk, int D, const double* __restrict__ qm,
+// Scores on the 64-bit matrix instruction (16 x 16 x 4): a wave takes 32 query tiles x 64 key
+// blocks, the workgroup's 4 waves stand side by side over 256 blocks. Lane group lane / 16 takes a
+// quarter of the channels in order, so each lane reads its pooled rows as 16-byte vectors.
+typedef double f64x4 __attribute__((ext_vector_type(4)));
+typedef double f64x2 __attribute__((ext_vector_type(2)));
+__global__ __launch_bounds__(NT) void k_scores(int Tq, int Tk, int pitch, const double* __restrict__ qm,
                                                const double* __restrict__ km, double* __restrict__ score) {
-  __shared__ double sq[SQ][SD + 1], sk[SK][SD + 1];
   const int64_t z = blockIdx.z;
-  const int q0 = blockIdx.y * SQ, k0 = blockIdx.x * SK;
-  const int tk = threadIdx.x % 16, tq = threadIdx.x / 16;  // row q0 + tq, columns k0 + tk + 16 j
-  double acc[4] = {};
-  for (int d0 = 0; d0 < D; d0 += SD) {
-    __syncthreads();
-    const int d = threadIdx.x % 16, r = threadIdx.x / 16;
-    sq[r][d] = q0 + r < Tq && d0 + d < D ? qm[(z * Tq + q0 + r) * D + d0 + d] : 0.0;
+  const int lane = threadIdx.x & 63, col = lane & 15, quarter = lane >> 4;
+  const int q0 = blockIdx.y * 32, k0 = (blockIdx.x * 4 + (threadIdx.x >> 6)) * 64;
+  if (k0 >= Tk) return;
+  const int per = pitch / 4;
+  const double *ap[2], *bp[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      sk[r + 16 * j][d] = k0 + r + 16 * j < Tk && d0 + d < D ? km[(z * Tk + k0 + r + 16 * j) * D + d0 + d] : 0.0;
-    __syncthreads();
+  for (int i = 0; i < 2; ++i) ap[i] = qm + (z * Tq + min(q0 + 16 * i + col, Tq - 1)) * pitch + quarter * per;
 #pragma unroll
-    for (int i = 0; i < SD; ++i)
+  for (int j = 0; j < 4; ++j) bp[j] = km + (z * Tk + min(k0 + 16 * j + col, Tk - 1)) * pitch + quarter * per;
+  f64x4 acc[2][4] = {};
+#pragma unroll 2
+  for (int d = 0; d < per; d += 2) {
+    f64x2 av[2], bv[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) acc[j] = __builtin_fma(sq[tq][i], sk[tk + 16 * j][i], acc[j]);
+    for (int i = 0; i < 2; ++i) av[i] = *(const f64x2*)(ap[i] + d);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) bv[j] = *(const f64x2*)(bp[j] + d);
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[i][j] = __builtin_amdgcn_mfma_f64_16x16x4f64(av[i][e], bv[j][e], acc[i][j], 0, 0, 0);
   }
-  if (q0 + tq < Tq)
-    for (int j = 0; j < 4; ++j)
-      if (k0 + tk + 16 * j < Tk) score[(z * Tq + q0 + tq) * Tk + k0 + tk + 16 * j] = acc[j];
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int q = q0 + 16 * i + 4 * r + quarter;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (q < Tq && k0 + 16 * j + col < Tk) score[(z * Tq + q) * Tk + k0 + 16 * j + col] = acc[i][j][r];
+    }
 }
 
 // The order of doubles as unsigned numbers; 0 is kept for blocks that may not be chosen. A score
@@ -84,68 +129,147 @@ __device__ __forceinline__ uint64_t order_key(double v) {
   return (u >> 63) ? ~u : (u | 0x8000000000000000ull);
 }
 
-// grid (Tq, B * Hkv): a radix descent over the row's keys, 8 bits at a time, finds the key of the
-// last chosen place and how many equal ones are taken; a scan over the row writes the places.
-__global__ __launch_bounds__(NT) void k_choose(int Tq, int Tk, int Hkv, int64_t Lq, int64_t Lk, int block, int top,
-                                               const int32_t* __restrict__ q_lengths,
-                                               const int32_t* __restrict__ kv_lengths,
-                                               const uint8_t* __restrict__ allowed, const double* __restrict__ score,
-                                               int32_t* __restrict__ index) {
-  __shared__ uint32_t hist[256];
-  __shared__ uint64_t s_key;
-  __shared__ int s_need, s_any;
-  __shared__ int wave_n[2][NT / 64];
-  const int t = blockIdx.x, z = blockIdx.y, b = z / Hkv;
-  const int64_t nq = length_of(q_lengths, b, Lq), nk = length_of(kv_lengths, b, Lk);
-  int32_t* out = index + ((int64_t)z * Tq + t) * top;
-  const int blocks = (int)((nk + block - 1) / block);  // blocks with a key
-  if ((int64_t)t * block >= nq || blocks == 0) {
-    for (int i = threadIdx.x; i < top; i += NT) out[i] = -1;
-    return;
+struct ChooseArgs {
+  int Tq, Tk, Hkv, block, top;
+  int64_t Lq, Lk, rows;
+  const int32_t *q_lengths, *kv_lengths;
+  const uint8_t* allowed;
+  const double* score;
+  int32_t* index;
+};
+
+// A wave per tile, 64 NV >= Tk keys in registers (place 64 j + lane in slot j). The key of the last chosen
+// place is found from its highest bit down: a bit is kept if at least `top` keys reach the number with
+// it. As soon as exactly `top` do, they are the answer: for scores that differ early, as they
+// do, well before the lower 32 bits are looked at.
+template <int NV>
+__global__ __launch_bounds__(NT) void k_choose(ChooseArgs a) {
+  const int64_t row = (int64_t)blockIdx.x * (NT / 64) + (threadIdx.x >> 6);
+  if (row >= a.rows) return;
+  const int lane = threadIdx.x & 63, t = (int)(row % a.Tq), b = (int)(row / a.Tq / a.Hkv);
+  const int64_t nq = length_of(a.q_lengths, b, a.Lq), nk = length_of(a.kv_lengths, b, a.Lk);
+  int32_t* out = a.index + row * a.top;
+  const int blocks = (int64_t)t * a.block < nq ? (int)((nk + a.block - 1) / a.block) : 0;  // blocks with a key
+  const double* score = a.score + row * a.Tk;
+  const uint8_t* may = a.allowed ? a.allowed + (int64_t)t * a.Tk : nullptr;
+  uint32_t hi[NV], lo[NV];
+  int have = 0;
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    const int i = 64 * j + lane;
+    const uint64_t k = i < blocks && (!may || may[i]) ? order_key(score[i]) : 0;
+    hi[j] = (uint32_t)(k >> 32);
+    lo[j] = (uint32_t)k;
+    have += __popcll(__ballot(k != 0));
   }
-  const double* row = score + ((int64_t)z * Tq + t) * Tk;
-  const uint8_t* may = allowed ? allowed + (int64_t)t * Tk : nullptr;
-  auto key_at = [&](int i) -> uint64_t { return (i < blocks && (!may || may[i])) ? order_key(row[i]) : 0ull; };
-  if (threadIdx.x == 0) s_any = 0;
+  uint32_t th = 0, tl = 1;  // every allowed block, if no more are allowed than wanted
+  int reach = have;         // keys at or above (th, tl)
+  if (have > a.top) {
+    tl = 0;
+    for (int bit = 31; bit >= 0 && reach != a.top; --bit) {
+      const uint32_t c = th | (1u << bit);
+      int n = 0;
+#pragma unroll
+      for (int j = 0; j < NV; ++j) n += __popcll(__ballot(hi[j] >= c));
+      if (n >= a.top) {
+        th = c;
+        reach = n;
+      }
+    }
+    if (reach != a.top) {
+      int above = 0;  // keys whose upper half is larger
+#pragma unroll
+      for (int j = 0; j < NV; ++j) above += __popcll(__ballot(hi[j] > th));
+      for (int bit = 31; bit >= 0 && reach != a.top; --bit) {
+        const uint32_t c = tl | (1u << bit);
+        int n = above;
+#pragma unroll
+        for (int j = 0; j < NV; ++j) n += __popcll(__ballot(hi[j] == th && lo[j] >= c));
+        if (n >= a.top) {
+          tl = c;
+          reach = n;
+        }
+      }
+    }
+  }
+  // equal keys beyond `top`: the lowest places of them are taken
+  int ties = reach - min(reach, a.top), equal = 0;
+  if (ties > 0) {
+#pragma unroll
+    for (int j = 0; j < NV; ++j) equal += __popcll(__ballot(hi[j] == th && lo[j] == tl));
+  }
+  const int taken = equal - ties;
+  int at = 0, tied = 0;
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    const bool tie = ties > 0 && hi[j] == th && lo[j] == tl;
+    const bool up = !tie && (hi[j] > th || (hi[j] == th && lo[j] >= tl));
+    const uint64_t mt = __ballot(tie), mu = __ballot(up);
+    const int before = tied + __popcll(mt & dsplat::lanemask_lt(lane));
+    if (up || (tie && before < taken)) out[at + __popcll(mu & dsplat::lanemask_lt(lane)) + min(before, taken)] = 64 * j + lane;
+    at += __popcll(mu);
+    tied += __popcll(mt);
+  }
+  for (int i = min(have, a.top) + lane; i < a.top; i += 64) out[i] = -1;
+}
+
+// More blocks than registers hold: a workgroup per tile, a radix descent over the row's keys 8 bits at a
+// time; then a scan over the row writes the places.
+__global__ __launch_bounds__(NT) void k_choose_long(ChooseArgs a) {
+  __shared__ int hist[256], wave_n[2][NT / 64];
+  __shared__ int s_digit, s_need, s_have;
+  const int64_t row = blockIdx.x;
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, t = (int)(row % a.Tq), b = (int)(row / a.Tq / a.Hkv);
+  const int64_t nq = length_of(a.q_lengths, b, a.Lq), nk = length_of(a.kv_lengths, b, a.Lk);
+  int32_t* out = a.index + row * a.top;
+  const int blocks = (int64_t)t * a.block < nq ? (int)((nk + a.block - 1) / a.block) : 0;
+  const double* score = a.score + row * a.Tk;
+  const uint8_t* may = a.allowed ? a.allowed + (int64_t)t * a.Tk : nullptr;
+  const auto key_at = [&](int i) -> uint64_t { return (i < blocks && (!may || may[i])) ? order_key(score[i]) : 0ull; };
+  if (threadIdx.x == 0) s_have = 0;
   __syncthreads();
-  int any = 0;
-  for (int i = threadIdx.x; i < blocks; i += NT) any += key_at(i) != 0;
-  atomicAdd(&s_any, any);
+  int mine = 0;
+  for (int i = threadIdx.x; i < blocks; i += NT) mine += key_at(i) != 0;
+  atomicAdd(&s_have, mine);
   __syncthreads();
-  const int have = s_any;
-  const int want = min(top, have);
-  uint64_t key = 1;   // every allowed block, if no more are allowed than wanted
-  int equal = blocks;
-  if (have > top) {
-    uint64_t prefix = 0;
-    int need = top;
+  const int have = s_have;
+  uint64_t key = 0;
+  int equal = 0;  // of the blocks with exactly this key, the lowest `equal` are taken
+  if (have > a.top) {
+    equal = a.top;
     for (int shift = 56; shift >= 0; shift -= 8) {
       hist[threadIdx.x] = 0;
       __syncthreads();
       for (int i = threadIdx.x; i < blocks; i += NT) {
         const uint64_t k = key_at(i);
-        if (k && (shift == 56 || (k >> (shift + 8)) == prefix)) atomicAdd(&hist[(k >> shift) & 255], 1u);
+        if (k && (shift == 56 || (k >> (shift + 8)) == key)) atomicAdd(&hist[(k >> shift) & 255], 1);
       }
       __syncthreads();
-      if (threadIdx.x == 0) {
-        int d = 255, n = need;
-        while (d > 0 && (int)hist[d] < n) n -= hist[d--];
-        s_key = (prefix << 8) | (uint64_t)d;
-        s_need = n;
+      // keys in this digit or above it: the digit where that passes `equal`
+      int from = hist[threadIdx.x];
+#pragma unroll
+      for (int off = 1; off < 64; off <<= 1) {
+        const int v = __shfl_down(from, off, 64);
+        if (lane + off < 64) from += v;
+      }
+      if (lane == 0) wave_n[0][w] = from;
+      __syncthreads();
+      for (int j = w + 1; j < NT / 64; ++j) from += wave_n[0][j];
+      const int over = from - hist[threadIdx.x];
+      if (from >= equal && over < equal) {
+        s_digit = threadIdx.x;
+        s_need = equal - over;
       }
       __syncthreads();
-      prefix = s_key;
-      need = s_need;
+      key = (key << 8) | (uint64_t)s_digit;
+      equal = s_need;
+      __syncthreads();
     }
-    key = prefix;
-    equal = need;  // of the blocks with exactly this key, the lowest `need`
   }
-  // ascending places: above = key greater, tie = key equal (the first `equal` of them)
   int above0 = 0, tie0 = 0;  // before this chunk
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   for (int base = 0; base < blocks; base += NT) {
-    const uint64_t k = base + (int)threadIdx.x < blocks ? key_at(base + threadIdx.x) : 0ull;
-    const bool up = have > top ? k > key : k != 0, tie = have > top && k == key;
+    const uint64_t k = key_at(base + (int)threadIdx.x);
+    const bool up = have > a.top ? k > key : k != 0, tie = have > a.top && k == key;
     const uint64_t mu = __ballot(up), mt = __ballot(tie);
     if (lane == 0) {
       wave_n[0][w] = __popcll(mu);
@@ -164,14 +288,15 @@ __global__ __launch_bounds__(NT) void k_choose(int Tq, int Tk, int Hkv, int64_t 
     if (up || (tie && e < equal)) out[u + min(e, equal)] = base + threadIdx.x;
     __syncthreads();
   }
-  for (int i = want + threadIdx.x; i < top; i += NT) out[i] = -1;
+  for (int i = min(have, a.top) + threadIdx.x; i < a.top; i += NT) out[i] = -1;
 }
 
 inline int64_t tiles_of(int64_t L, int block) { return (L + block - 1) / block; }
 
 template <typename T>
-void pool(const Rows& x, int64_t L, int D, int group, int block, int tiles, int Hkv, int B, double* out, hipStream_t st) {
-  k_pool<T><<<dim3(tiles, Hkv, B), NT, 0, st>>>(x, L, D, group, block, out);
+void pool(const PoolArgs& a, dim3 grid, hipStream_t st) {
+  if (a.D % Vec<T>::N == 0) k_pool<T, true><<<grid, NT, 0, st>>>(a);
+  else k_pool<T, false><<<grid, NT, 0, st>>>(a);
 }
 
 }  // namespace
@@ -181,7 +306,7 @@ extern "C" {
 size_t dtk_select_blocks_workspace_size(int B, int64_t Lq, int64_t Lk, int Hkv, int D, int block) {
   if (B <= 0 || Lq <= 0 || Lk <= 0 || Hkv <= 0 || D <= 0 || block <= 0) return 0;
   const size_t tq = tiles_of(Lq, block), tk = tiles_of(Lk, block);
-  return (size_t)B * Hkv * ((tq + tk) * D + tq * tk) * sizeof(double);
+  return (size_t)B * Hkv * ((tq + tk) * pitch_of(D) + tq * tk) * sizeof(double);
 }
 
 int dtk_select_blocks(int B, int64_t Lq, int64_t Lk, int Hq, int Hkv, int D, int block, int top, int dtype,
@@ -195,31 +320,31 @@ int dtk_select_blocks(int B, int64_t Lq, int64_t Lk, int Hq, int Hkv, int D, int
   DSPLAT_REQUIRE(Lq < (1LL << 31) && Lk < (1LL << 31) && (int64_t)B * Hkv < 65536 && Hq < 65536, "dtk_select_blocks: too large");
   if (B == 0 || Lq == 0) return 0;
   const int Tq = (int)tiles_of(Lq, block), Tk = (int)tiles_of(Lk, block);
-  DSPLAT_REQUIRE(Tq <= 16 * 65535, "dtk_select_blocks: too large");
+  DSPLAT_REQUIRE(Tq <= 32 * 65535 && Hkv < 65536 && B < 65536, "dtk_select_blocks: too large");
   DSPLAT_REQUIRE(index && (Lk == 0 || (q && k && q_strides && k_strides && workspace)), "dtk_select_blocks: null pointer");
   hipStream_t st = (hipStream_t)stream;
+  const int pitch = pitch_of(D);
   double* qm = (double*)workspace;
-  double* km = qm + (size_t)B * Hkv * Tq * D;
-  double* score = km + (size_t)B * Hkv * Tk * D;
+  double* km = qm + (size_t)B * Hkv * Tq * pitch;
+  double* score = km + (size_t)B * Hkv * Tk * pitch;
   if (Lk > 0) {
-    const Rows rq = {q, q_strides[0], q_strides[1], q_strides[2], q_lengths};
-    const Rows rk = {k, k_strides[0], k_strides[1], k_strides[2], kv_lengths};
-    const int group = Hq / Hkv;
-    if (dtype == DTK_F32) {
-      pool<float>(rq, Lq, D, group, block, Tq, Hkv, B, qm, st);
-      pool<float>(rk, Lk, D, 1, block, Tk, Hkv, B, km, st);
-    } else if (dtype == DTK_BF16) {
-      pool<bf16>(rq, Lq, D, group, block, Tq, Hkv, B, qm, st);
-      pool<bf16>(rk, Lk, D, 1, block, Tk, Hkv, B, km, st);
-    } else {
-      pool<f16>(rq, Lq, D, group, block, Tq, Hkv, B, qm, st);
-      pool<f16>(rk, Lk, D, 1, block, Tk, Hkv, B, km, st);
-    }
+    const PoolArgs a = {{{q, q_strides[0], q_strides[1], q_strides[2], q_lengths}, {k, k_strides[0], k_strides[1], k_strides[2], kv_lengths}},
+                        {Lq, Lk}, {Hq / Hkv, 1}, Tq, D, pitch, block, {qm, km}};
+    const dim3 grid(Tq + Tk, Hkv, B);
+    if (dtype == DTK_F32) pool<float>(a, grid, st);
+    else if (dtype == DTK_BF16) pool<bf16>(a, grid, st);
+    else pool<f16>(a, grid, st);
     if (int e = dsplat::check_launch("k_pool")) return e;
-    k_scores<<<dim3((Tk + SK - 1) / SK, (Tq + SQ - 1) / SQ, B * Hkv), NT, 0, st>>>(Tq, Tk, D, qm, km, score);
+    k_scores<<<dim3((Tk + 255) / 256, (Tq + 31) / 32, B * Hkv), NT, 0, st>>>(Tq, Tk, pitch, qm, km, score);
     if (int e = dsplat::check_launch("k_scores")) return e;
   }
-  k_choose<<<dim3(Tq, B * Hkv), NT, 0, st>>>(Tq, Tk, Hkv, Lq, Lk, block, top, q_lengths, kv_lengths, allowed, score, index);
+  const ChooseArgs a = {Tq, Tk, Hkv, block, top, Lq, Lk, (int64_t)B * Hkv * Tq, q_lengths, kv_lengths, allowed, score, index};
+  DSPLAT_REQUIRE(a.rows < (1LL << 31), "dtk_select_blocks: too large");
+  const unsigned waves = (unsigned)((a.rows + NT / 64 - 1) / (NT / 64));
+  if (Tk <= 64 * 2) k_choose<2><<<waves, NT, 0, st>>>(a);
+  else if (Tk <= 64 * 8) k_choose<8><<<waves, NT, 0, st>>>(a);
+  else if (Tk <= 64 * 32) k_choose<32><<<waves, NT, 0, st>>>(a);
+  else k_choose_long<<<(unsigned)a.rows, NT, 0, st>>>(a);
   return dsplat::check_launch("k_choose");
 }
 

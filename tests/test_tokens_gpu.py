@@ -303,7 +303,7 @@ def test_rotary_of_slices(gpu):
 @pytest.mark.parametrize("t", TYPES)
 @pytest.mark.parametrize("B,Lq,Lk,Hq,Hkv,D,block,top", [
     (2, 70, 200, 4, 2, 16, 32, 3), (1, 1, 1000, 8, 2, 64, 64, 5), (2, 300, 130, 2, 1, 72, 128, 4), (1, 65, 2100, 1, 1, 8, 32, 20),
-    (1, 33, 31, 3, 3, 130, 32, 2), (1, 10, 9000, 1, 1, 1, 32, 300)])
+    (1, 33, 31, 3, 3, 130, 32, 2), (1, 10, 9000, 1, 1, 1, 32, 300), (2, 40, 20001, 2, 1, 12, 32, 7), (1, 33, 66000, 1, 1, 8, 32, 40)])
 def test_select_blocks(gpu, t, B, Lq, Lk, Hq, Hkv, D, block, top):
     T = tokens()
     rnd = make(gpu, Lq + Lk)
@@ -323,6 +323,15 @@ def test_select_blocks_ties_padding_and_no_numbers(gpu):
     k = torch.randn(1, 32, 1, 16, device=gpu).repeat(1, 40, 1, 1)
     q = torch.randn(1, 64, 1, 16, device=gpu)
     assert T.select_blocks(q, k, 5, block=32).flatten().tolist() == [0, 1, 2, 3, 4] * 2
+    for blocks in (700, 2100):  # ties and fewer choices than wanted on every path
+        k = torch.zeros(1, 32 * blocks, 1, 16, device=gpu)
+        k[:, 32 * 5:32 * 6] = q.mean(1, keepdim=True)
+        one = q.mean(1, keepdim=True).expand(1, 32, 1, 16)
+        assert T.select_blocks(one, k, 4, block=32).flatten().tolist() == [0, 1, 2, 5]
+        assert T.select_blocks(-one, -k, 4, block=32).flatten().tolist() == [0, 1, 2, 5]
+        may = torch.zeros(1, blocks, dtype=torch.bool, device=gpu)
+        may[0, 600], may[0, 650] = True, True
+        assert T.select_blocks(one, k, 4, block=32, allowed=may).flatten().tolist() == [600, 650, -1, -1]
     k = torch.randn(1, 320, 1, 16, device=gpu)
     want = T.select_blocks(q[:, :40], k[:, :250], 3, block=32)
     bad_k, bad_q = k.clone(), q.clone()
