@@ -60,8 +60,11 @@ struct Strided {
 struct Args {
   int64_t Lq, Lk;
   int Hq, Hkv, G, D, block, top, Tq, Tk;
+  int lg;                    // block = 32 << lg
+  uint32_t group_magic;      // ceil(2^32 / G)
   int Lt, rowtiles, splits;  // rows of a tile, workgroups per tile, parts of the key list
-  float scale;
+  float scale, scale2;       // scale2: |scale| log2 e, at least the smallest normal number (masked scores are
+                             // -inf, and a scale of 0 must not make them no number)
   Strided q, k, v, o, g;  // g: the output's gradient
   const int32_t *index, *q_lengths, *kv_lengths;
   void *out, *dq, *dk, *dv;  // contiguous
@@ -134,29 +137,44 @@ struct Tile {
   }
 };
 
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
 // The workgroup's share of U units (32 rows each) on the way from memory to LDS: loaded into
 // registers while the tile before is worked on, then stored. Rows that do not count and channels
-// behind D become zeros.
+// behind D become zeros. A wave's pieces are all of one unit, so where that starts is scalar work and a
+// load adds one 32-bit offset to it (31 rows' strides fit: the host checks).
 template <typename T, int DP, int U>
 struct Stage {
   using L = Tile<T, DP>;
   static constexpr int kPer = (U * 32 * L::kPieces + NT - 1) / NT;
+  static constexpr int kWaves = 32 * L::kPieces / 64;  // waves of pieces per unit
   Vec<T> v[kPer];
-  // first(j): where the j-th unit's first row starts (elements from base), count(j): its rows that count
+  // from(j): where the j-th unit's first row starts, count(j): its rows that count
   template <typename F, typename C>
-  __device__ __forceinline__ void load(const T* base, int64_t stride, int D, F first, C count) {
+  __device__ __forceinline__ void load(int64_t stride, int D, F from, C count) {
+    const int wave = uniform(threadIdx.x >> 6);
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-      const int id = threadIdx.x + i * NT, r = id / L::kPieces, d = (id % L::kPieces) * Vec<T>::N, j = r / 32;
-      v[i] = Vec<T>{};
-      if (j < U && d < D && r % 32 < count(j)) v[i] = load_vec(base + first(j) + (r % 32) * stride + d);
+      const int j = (wave + i * (NT / 64)) / kWaves;
+      if (j >= U) break;
+      const int id = threadIdx.x + i * NT, r = id / L::kPieces % 32, d = id % L::kPieces * Vec<T>::N;
+      const uint32_t off = (uint32_t)r * (uint32_t)stride + (uint32_t)d;
+      const int n = count(j);
+      const T* p = from(j);
+      if (n == 32 && D == DP) {
+        v[i] = load_vec(p + off);
+      } else {
+        v[i] = Vec<T>{};
+        if (r < n && d < D) v[i] = load_vec(p + off);
+      }
     }
   }
   __device__ __forceinline__ void store(char* t) const {
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
       const int id = threadIdx.x + i * NT, r = id / L::kPieces, c = id % L::kPieces;
-      if (r < U * 32) __builtin_memcpy(__builtin_assume_aligned(t + r * L::kPitch + c * 16, 16), &v[i], 16);
+      if ((i + 1) * NT <= U * 32 * L::kPieces || r < U * 32)
+        __builtin_memcpy(__builtin_assume_aligned(t + r * L::kPitch + c * 16, 16), &v[i], 16);
     }
   }
 };
@@ -186,7 +204,7 @@ __device__ __forceinline__ int block_list(const int32_t* idx, int top, int block
     if (lane == 0) *count = n;
   }
   __syncthreads();
-  return *count;
+  return __builtin_amdgcn_readfirstlane(*count);
 }
 
 template <typename T>
@@ -209,6 +227,19 @@ __device__ __forceinline__ Where where(const Args& a) {
   return w;
 }
 
+// A tile's units of 32 keys: unit u is part u % (block / 32) of the list's block u / (block / 32).
+struct Keys {
+  const int32_t* list;
+  int block, lg, units;
+  int64_t nk;
+  __device__ __forceinline__ int64_t first(int u) const {
+    return (int64_t)uniform(list[u >> lg]) * block + 32 * (u & ((1 << lg) - 1));
+  }
+  __device__ __forceinline__ int count(int u) const {
+    return u < units ? (int)max((int64_t)0, min((int64_t)32, nk - first(u))) : 0;
+  }
+};
+
 // What a row's waves have in common at the end: wave kw = 0 takes in the others' sums through LDS.
 template <int RW, int DP>
 struct Join {
@@ -220,7 +251,7 @@ struct Join {
 // of 32 keys and are joined at the end. The rows of a tile are its queries of all heads that
 // share the key head (few queries: they fill the instruction's columns together).
 template <typename T, int DP, int RW>
-__global__ __launch_bounds__(NT) void k_attend_fwd(Args a) {
+__global__ __launch_bounds__(NT, (sizeof(T) == 2 && DP <= 64 ? 4 : 1)) void k_attend_fwd(Args a) {
   using M = Mma<T>;
   using L = Tile<T, DP>;
   using Frag = typename M::Frag;
@@ -230,7 +261,7 @@ __global__ __launch_bounds__(NT) void k_attend_fwd(Args a) {
   int32_t* list = (int32_t*)(lds + kTileBytes<T, DP, KW>);
   const Where at = where(a);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, col = lane & 31;
-  const int rw = wave % RW, kw = wave / RW;
+  const int rw = uniform(wave) % RW, kw = uniform(wave) / RW;
   const int64_t nq = length_of(a.q_lengths, at.b, a.Lq), nk = length_of(a.kv_lengths, at.b, a.Lk);
   const int row = (at.rt * RW + rw) * 32 + col;
   const int g = row / a.Lt;
@@ -243,7 +274,6 @@ __global__ __launch_bounds__(NT) void k_attend_fwd(Args a) {
     n = block_list(a.index + (((int64_t)at.b * a.Hkv + at.hk) * a.Tq + at.t) * a.top, a.top, blocks, list, &count);
 
   const T* qp = (const T*)a.q.p + at.b * a.q.b + (valid ? i : 0) * a.q.l + h * a.q.h;
-  const float scale2 = fabsf(a.scale) * kLog2e;
   Frag qf[NS];
 #pragma unroll
   for (int s = 0; s < NS; ++s) {
@@ -254,21 +284,22 @@ __global__ __launch_bounds__(NT) void k_attend_fwd(Args a) {
   const T* vp = (const T*)a.v.p + at.b * a.v.b + at.hk * a.v.h;
 
   f32x16 o[ND] = {};
-  // m: what the exponents are taken relative to, in units of x; it follows the running maximum only
-  // when that has risen by 8 powers of two (p stays below 2^8, and o is rarely rescaled)
+  // The exponents are taken relative to base2, which follows the running maximum m only when a sum of 16
+  // has passed 2^12: p stays in every type's range, the fast path needs no maximum, and o is
+  // rarely rescaled. (l <= 2^12 x keys, o likewise: far inside 32 bits.)
   float m = -INFINITY, base2 = 0.f, l = 0.f;
-  const int upb = a.block / 32, units = n * upb;
+  const int units = n << a.lg;
   const int per = (units + a.splits - 1) / a.splits;
   const int u0 = min(units, at.split * per), u1 = min(units, u0 + per);
-  const auto key0 = [&](int u) { return (int64_t)list[u / upb] * a.block + 32 * (u % upb); };
-  const auto keys = [&](int u) { return u < u1 ? (int)max((int64_t)0, min((int64_t)32, nk - key0(u))) : 0; };
+  const Keys where_ = {list, a.block, a.lg, u1, nk};
   Stage<T, DP, KW> sk, sv;
   const auto fetch = [&](int u) {
-    const auto have = [&](int j) { return keys(u + j); };
-    sk.load(kp, a.k.l, a.D, [&](int j) { return key0(u + j) * a.k.l; }, have);
-    sv.load(vp, a.v.l, a.D, [&](int j) { return key0(u + j) * a.v.l; }, have);
+    const auto have = [&](int j) { return where_.count(u + j); };
+    sk.load(a.k.l, a.D, [&](int j) { return kp + where_.first(u + j) * a.k.l; }, have);
+    sv.load(a.v.l, a.D, [&](int j) { return vp + where_.first(u + j) * a.v.l; }, have);
   };
   if (u0 < u1) fetch(u0);
+  bool begun = false;
   for (int u = u0, step = 0; u < u1; u += KW, ++step) {
     char* tk = lds + (step % NB) * 2 * KW * L::kUnit;
     char* tv = tk + KW * L::kUnit;
@@ -279,7 +310,7 @@ __global__ __launch_bounds__(NT) void k_attend_fwd(Args a) {
     if (u + KW < u1) fetch(u + KW);
     tk += kw * L::kUnit;
     tv += kw * L::kUnit;
-    const int left = keys(u + kw);
+    const int left = where_.count(u + kw);
     if (left == 0) continue;
     f32x16 x = {};
 #pragma unroll
@@ -288,28 +319,37 @@ __global__ __launch_bounds__(NT) void k_attend_fwd(Args a) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) x[r] = acc_row(r, half) < left ? x[r] : -INFINITY;
     }
-    float mx = x[0];
+    f32x16 p;
+    float sum = 0.f;
+    if (begun) {
 #pragma unroll
-    for (int r = 1; r < 16; ++r) mx = fmaxf(mx, x[r]);
-    mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-    if (__any((mx - m) * scale2 > 8.f || m == -INFINITY)) {
-      const float mn = fmaxf(m, mx), b2 = mn == -INFINITY ? 0.f : mn * scale2;
+      for (int r = 0; r < 16; ++r) {
+        p[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[r], a.scale2, -base2));
+        sum += p[r];
+      }
+    }
+    if (!begun || __any(!(sum <= 4096.f))) {
+      begun = true;
+      float mx = x[0];
+#pragma unroll
+      for (int r = 1; r < 16; ++r) mx = fmaxf(mx, x[r]);
+      mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+      const float mn = fmaxf(m, mx), b2 = mn == -INFINITY ? 0.f : mn * a.scale2;
       const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(base2 - b2);
       m = mn;
       base2 = b2;
       l *= alpha;
 #pragma unroll
       for (int d = 0; d < ND; ++d) o[d] *= alpha;
-    }
-    float sum = 0.f;
+      sum = 0.f;
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      x[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[r], scale2, -base2));
-      if (left < 32) x[r] = acc_row(r, half) < left ? x[r] : 0.f;  // (a scale of 0: not -inf * 0)
-      sum += x[r];
+      for (int r = 0; r < 16; ++r) {
+        p[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[r], a.scale2, -base2));
+        sum += p[r];
+      }
     }
     l += sum;
-    const Frag p0 = acc_frag<T>(x, 0), p1 = acc_frag<T>(x, 1);
+    const Frag p0 = acc_frag<T>(p, 0), p1 = acc_frag<T>(p, 1);
 #pragma unroll
     for (int d = 0; d < ND; ++d) {
       o[d] = M::mma(L::col(tv, 0, d, lane), p0, o[d]);
@@ -440,7 +480,7 @@ __global__ __launch_bounds__(NT) void k_attend_dq(Args a) {
   int32_t* list = (int32_t*)(lds + kTileBytes<T, DP, KW>);
   const Where at = where(a);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, col = lane & 31;
-  const int rw = wave % RW, kw = wave / RW;
+  const int rw = uniform(wave) % RW, kw = uniform(wave) / RW;
   const int64_t nq = length_of(a.q_lengths, at.b, a.Lq), nk = length_of(a.kv_lengths, at.b, a.Lk);
   const int row = (at.rt * RW + rw) * 32 + col;
   const int g = row / a.Lt;
@@ -461,6 +501,7 @@ __global__ __launch_bounds__(NT) void k_attend_dq(Args a) {
 #pragma unroll
   for (int s = 0; s < NS; ++s) {
     qf[s] = row_frag<T>(qp, 16 * s + 8 * half, a.D, valid);
+    if (a.scale < 0.f) qf[s] = -qf[s];
     gf[s] = row_frag<T>(gp, 16 * s + 8 * half, a.D, valid);
     const Frag of = row_frag<T>(op, 16 * s + 8 * half, a.D, valid);
 #pragma unroll
@@ -479,22 +520,20 @@ __global__ __launch_bounds__(NT) void k_attend_dq(Args a) {
     if (kw == 0 && lane == 0 && most > 0.f) atomicMax(a.gmax, __float_as_uint(most));  // any order, the same answer
   }
   const int64_t stat = ((int64_t)at.b * a.Hq + h) * a.Lq + ir;
-  const float lse = valid ? a.lse[stat] : -INFINITY;
+  // rows that see nothing: relative to +inf every p is 0
+  const float saved = valid ? a.lse[stat] : -INFINITY, lse = saved == -INFINITY ? INFINITY : saved;
   if (kw == 0 && half == 0 && valid) a.delta[stat] = delta;
-  const bool empty = lse == -INFINITY;
   const T* kp = (const T*)a.k.p + at.b * a.k.b + at.hk * a.k.h;
   const T* vp = (const T*)a.v.p + at.b * a.v.b + at.hk * a.v.h;
 
   f32x16 dq[ND] = {};
-  const float scale2 = a.scale * kLog2e;
-  const int upb = a.block / 32, units = n * upb;
-  const auto key0 = [&](int u) { return (int64_t)list[u / upb] * a.block + 32 * (u % upb); };
-  const auto keys = [&](int u) { return u < units ? (int)max((int64_t)0, min((int64_t)32, nk - key0(u))) : 0; };
+  const int units = n << a.lg;
+  const Keys where_ = {list, a.block, a.lg, units, nk};
   Stage<T, DP, KW> sk, sv;
   const auto fetch = [&](int u) {
-    const auto have = [&](int j) { return keys(u + j); };
-    sk.load(kp, a.k.l, a.D, [&](int j) { return key0(u + j) * a.k.l; }, have);
-    sv.load(vp, a.v.l, a.D, [&](int j) { return key0(u + j) * a.v.l; }, have);
+    const auto have = [&](int j) { return where_.count(u + j); };
+    sk.load(a.k.l, a.D, [&](int j) { return kp + where_.first(u + j) * a.k.l; }, have);
+    sv.load(a.v.l, a.D, [&](int j) { return vp + where_.first(u + j) * a.v.l; }, have);
   };
   if (units) fetch(0);
   for (int u = 0, step = 0; u < units; u += KW, ++step) {
@@ -507,7 +546,7 @@ __global__ __launch_bounds__(NT) void k_attend_dq(Args a) {
     if (u + KW < units) fetch(u + KW);
     tk += kw * L::kUnit;
     tv += kw * L::kUnit;
-    const int left = keys(u + kw);
+    const int left = where_.count(u + kw);
     if (left == 0) continue;
     f32x16 x = {}, dp = {};
 #pragma unroll
@@ -515,11 +554,14 @@ __global__ __launch_bounds__(NT) void k_attend_dq(Args a) {
       x = M::mma(L::row(tk, s, col, half), qf[s], x);
       dp = M::mma(L::row(tv, s, col, half), gf[s], dp);
     }
+    if (left < 32) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) x[r] = acc_row(r, half) < left ? x[r] : -INFINITY;
+    }
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
-      float p = __builtin_amdgcn_exp2f(__builtin_fmaf(x[r], scale2, -lse));
-      if (left < 32) p = acc_row(r, half) < left ? p : 0.f;
-      x[r] = empty ? 0.f : p * ((dp[r] - delta) * down);
+      const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(x[r], a.scale2, -lse));
+      x[r] = p * (kFewExponents<T> ? (dp[r] - delta) * down : dp[r] - delta);
     }
     const Frag s0 = acc_frag<T>(x, 0), s1 = acc_frag<T>(x, 1);
 #pragma unroll
@@ -574,10 +616,10 @@ __global__ __launch_bounds__(NT) void k_attend_dkv(Args a) {
   extern __shared__ __align__(16) char lds[];
   __shared__ int32_t tiles[kTiles];
   __shared__ int count;
-  __shared__ float stats[NB][2][QW * 32];  // lse and delta of the staged rows
+  __shared__ __align__(16) float stats[NB][2][QW * 32];  // lse and delta of the staged rows
   const int blk = blockIdx.x, hk = blockIdx.y, b = blockIdx.z;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, col = lane & 31;
-  const int rw = wave % RW, qw = wave / RW;
+  const int rw = uniform(wave) % RW, qw = uniform(wave) / RW;
   const int64_t nq = length_of(a.q_lengths, b, a.Lq), nk = length_of(a.kv_lengths, b, a.Lk);
   const int64_t key = (int64_t)blk * a.block + 32 * rw + col;
   const bool exists = key < a.Lk, valid = key < nk;
@@ -588,13 +630,13 @@ __global__ __launch_bounds__(NT) void k_attend_dkv(Args a) {
 #pragma unroll
   for (int s = 0; s < NS; ++s) {
     kf[s] = row_frag<T>(kp, 16 * s + 8 * half, a.D, valid);
+    if (a.scale < 0.f) kf[s] = -kf[s];
     vf[s] = row_frag<T>(vp, 16 * s + 8 * half, a.D, valid);
   }
   float down = 1.f, up = 1.f;
   if constexpr (kFewExponents<T>) ds_scale(*a.gmax, down, up);
   f32x16 dk[ND] = {}, dv[ND] = {};
-  const float scale2 = a.scale * kLog2e;
-  const int upb = a.block / 32, upt = a.G * upb, words = (a.Tq + 31) / 32;  // units per tile
+  const int upt = a.G << a.lg, words = (a.Tq + 31) / 32;  // units per tile
   const uint32_t* bits = a.bits + (((int64_t)b * a.Hkv + hk) * a.Tk + blk) * words;
   const bool any = (int64_t)blk * a.block < nk;
   int step = 0;
@@ -611,24 +653,33 @@ __global__ __launch_bounds__(NT) void k_attend_dkv(Args a) {
       if (lane == 63) count = (int)incl;
     }
     __syncthreads();
-    const int units = count * upt;
-    const auto row0 = [&](int u) { return (int64_t)tiles[u / upt] * a.block + 32 * (u % upb); };
-    const auto head = [&](int u) { return hk * a.G + (u / upb) % a.G; };
+    const int units = uniform(count) * upt;
+    // unit u: 32 rows (part u % (block / 32)) of a head of the group of a listed tile
+    const auto pos = [&](int u) {  // exact: u >> lg < 2^20 and G <= 1024
+      return a.G == 1 ? u >> a.lg : (int)__umulhi((uint32_t)(u >> a.lg), a.group_magic);
+    };
+    const auto row0 = [&](int u) { return (int64_t)uniform(tiles[pos(u)]) * a.block + 32 * (u & ((1 << a.lg) - 1)); };
+    const auto head = [&](int u) { return hk * a.G + (u >> a.lg) - pos(u) * a.G; };
     const auto rows = [&](int u) { return u < units ? (int)max((int64_t)0, min((int64_t)32, nq - row0(u))) : 0; };
     Stage<T, DP, QW> sq, sg;
-    float st_lse = -INFINITY, st_delta = 0.f;
+    float st_lse = INFINITY, st_delta = 0.f;
     const auto fetch = [&](int u) {
       const auto have = [&](int j) { return rows(u + j); };
-      sq.load((const T*)a.q.p + b * a.q.b, a.q.l, a.D, [&](int j) { return row0(u + j) * a.q.l + head(u + j) * a.q.h; }, have);
-      sg.load((const T*)a.g.p + b * a.g.b, a.g.l, a.D, [&](int j) { return row0(u + j) * a.g.l + head(u + j) * a.g.h; }, have);
+      sq.load(a.q.l, a.D, [&](int j) { return (const T*)a.q.p + b * a.q.b + row0(u + j) * a.q.l + head(u + j) * a.q.h; }, have);
+      sg.load(a.g.l, a.D, [&](int j) { return (const T*)a.g.p + b * a.g.b + row0(u + j) * a.g.l + head(u + j) * a.g.h; }, have);
       if (threadIdx.x < QW * 32) {
-        const int j = threadIdx.x / 32, r = threadIdx.x % 32;
+        const int r = threadIdx.x % 32, uj = u + threadIdx.x / 32;
         st_lse = -INFINITY;
-        if (r < rows(u + j)) {
-          const int64_t stat = ((int64_t)b * a.Hq + head(u + j)) * a.Lq + row0(u + j) + r;
-          st_lse = a.lse[stat];
-          st_delta = a.delta[stat];
+        if (uj < units) {
+          const int at = pos(uj);
+          const int64_t i = (int64_t)tiles[at] * a.block + 32 * (uj & ((1 << a.lg) - 1)) + r;
+          if (i < nq) {
+            const int64_t stat = ((int64_t)b * a.Hq + hk * a.G + (uj >> a.lg) - at * a.G) * a.Lq + i;
+            st_lse = a.lse[stat];
+            st_delta = a.delta[stat];
+          }
         }
+        st_lse = st_lse == -INFINITY ? INFINITY : st_lse;  // rows that see nothing, or are none: every p is 0
       }
     };
     if (units) fetch(0);
@@ -653,14 +704,19 @@ __global__ __launch_bounds__(NT) void k_attend_dkv(Args a) {
         x = M::mma(L::row(tq, s, col, half), kf[s], x);
         dp = M::mma(L::row(tg, s, col, half), vf[s], dp);
       }
+      // (lanes whose key is none hold columns that are not written)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int ri = acc_row(r, half);
-        const float lse = stats[step % NB][0][qw * 32 + ri], delta = stats[step % NB][1][qw * 32 + ri];
-        const bool on = valid && lse != -INFINITY;
-        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(x[r], scale2, -lse));
-        x[r] = on ? p : 0.f;
-        dp[r] = on ? p * ((dp[r] - delta) * down) : 0.f;
+      for (int c = 0; c < 4; ++c) {
+        const float4 lse = *(const float4*)&stats[step % NB][0][qw * 32 + 8 * c + 4 * half];
+        const float4 delta = *(const float4*)&stats[step % NB][1][qw * 32 + 8 * c + 4 * half];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int r = 4 * c + e;
+          const float ls = e == 0 ? lse.x : e == 1 ? lse.y : e == 2 ? lse.z : lse.w;
+          const float de = e == 0 ? delta.x : e == 1 ? delta.y : e == 2 ? delta.z : delta.w;
+          x[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[r], a.scale2, -ls));
+          dp[r] = x[r] * (kFewExponents<T> ? (dp[r] - de) * down : dp[r] - de);
+        }
       }
       const Frag p0 = acc_frag<T>(x, 0), p1 = acc_frag<T>(x, 1), s0 = acc_frag<T>(dp, 0), s1 = acc_frag<T>(dp, 1);
 #pragma unroll
@@ -694,16 +750,21 @@ __global__ __launch_bounds__(NT) void k_attend_dkv(Args a) {
   }
   if (qw != 0 || !exists) return;
   const int64_t off = (((int64_t)b * a.Lk + key) * a.Hkv + hk) * a.D;
-  const float f = valid ? a.scale * up : 0.f, fv = valid ? 1.f : 0.f;
+  const float f = a.scale * up;
 #pragma unroll
   for (int d = 0; d < ND; ++d)
 #pragma unroll
-    for (int c = 0; c < 4; ++c)
-      if (32 * d + 8 * c + 4 * half < a.D) {
-        const int e = 32 * d + 8 * c + 4 * half;
+    for (int c = 0; c < 4; ++c) {
+      const int e = 32 * d + 8 * c + 4 * half;
+      if (e >= a.D) continue;
+      if (valid) {
         store4<T>((T*)a.dk + off + e, dk[d][4 * c] * f, dk[d][4 * c + 1] * f, dk[d][4 * c + 2] * f, dk[d][4 * c + 3] * f);
-        store4<T>((T*)a.dv + off + e, dv[d][4 * c] * fv, dv[d][4 * c + 1] * fv, dv[d][4 * c + 2] * fv, dv[d][4 * c + 3] * fv);
+        store4<T>((T*)a.dv + off + e, dv[d][4 * c], dv[d][4 * c + 1], dv[d][4 * c + 2], dv[d][4 * c + 3]);
+      } else {
+        store4<T>((T*)a.dk + off + e, 0.f, 0.f, 0.f, 0.f);
+        store4<T>((T*)a.dv + off + e, 0.f, 0.f, 0.f, 0.f);
       }
+    }
 }
 
 template <typename K>
@@ -769,6 +830,9 @@ int check(const dtk_attention* c, const char* who) {
   DSPLAT_REQUIRE(c->D > 0 && c->D <= 128 && c->D % 8 == 0, "%s: the head size must be a multiple of 8 up to 128", who);
   DSPLAT_REQUIRE(c->block == 32 || c->block == 64 || c->block == 128, "%s: block must be 32, 64 or 128", who);
   DSPLAT_REQUIRE(type_ok(c->dtype), "%s: bad type", who);
+  DSPLAT_REQUIRE(c->Hq / c->Hkv <= 1024, "%s: more than 1024 query heads per key head", who);
+  for (const int64_t* s : {c->q_strides, c->k_strides, c->v_strides})
+    DSPLAT_REQUIRE(s[1] >= 0 && s[1] < (1LL << 24), "%s: a token stride must be below 2^24 elements", who);
   DSPLAT_REQUIRE(c->Lq < (1LL << 31) && c->Lk < (1LL << 31) && c->Hq < 65536 && c->B < 65536, "%s: too large", who);
   DSPLAT_REQUIRE(c->B == 0 || c->Lq == 0 || (c->q && c->o && c->index && (c->Lk == 0 || (c->k && c->v))), "%s: null pointer", who);
   return 0;
@@ -787,7 +851,10 @@ Args args_of(const dtk_attention* c) {
   a.Tq = (int)((c->Lq + c->block - 1) / c->block);
   a.Tk = (int)((c->Lk + c->block - 1) / c->block);
   a.Lt = (int)(c->Lq < c->block ? (c->Lq > 0 ? c->Lq : 1) : c->block);
+  a.lg = c->block == 32 ? 0 : c->block == 64 ? 1 : 2;
+  a.group_magic = (uint32_t)((0x100000000ull + a.G - 1) / a.G);
   a.scale = c->scale;
+  a.scale2 = fmaxf(fabsf(c->scale) * kLog2e, 1.17549435e-38f);
   a.q = strided(c->q, c->q_strides);
   a.k = strided(c->k, c->k_strides);
   a.v = strided(c->v, c->v_strides);
@@ -849,6 +916,8 @@ int dtk_block_sparse_attention_bwd(const dtk_attention* c, const void* dout, con
   if (c->B == 0) return 0;
   DSPLAT_REQUIRE((c->Lq == 0 || (dout && dout_strides && dq && c->lse && workspace)) && (c->Lk == 0 || (dk && dv && workspace)),
                  "dtk_block_sparse_attention_bwd: null pointer");
+  DSPLAT_REQUIRE(c->Lq == 0 || (dout_strides[1] >= 0 && dout_strides[1] < (1LL << 24)),
+                 "dtk_block_sparse_attention_bwd: a token stride must be below 2^24 elements");
   Args a = args_of(c);
   a.splits = 1;
   hipStream_t st = (hipStream_t)stream;
