@@ -149,24 +149,28 @@ struct Stage {
   static constexpr int kPer = (U * 32 * L::kPieces + NT - 1) / NT;
   static constexpr int kWaves = 32 * L::kPieces / 64;  // waves of pieces per unit
   Vec<T> v[kPer];
-  // from(j): where the j-th unit's first row starts, count(j): its rows that count
-  template <typename F, typename C>
-  __device__ __forceinline__ void load(int64_t stride, int D, F from, C count) {
+  // from[j]: where the j-th unit's first row starts, n[j]: its rows that count
+  __device__ __forceinline__ void load(const T* const (&from)[U], const int (&n)[U], int64_t stride, int D) {
     const int wave = uniform(threadIdx.x >> 6);
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-      const int j = (wave + i * (NT / 64)) / kWaves;
-      if (j >= U) break;
       const int id = threadIdx.x + i * NT, r = id / L::kPieces % 32, d = id % L::kPieces * Vec<T>::N;
       const uint32_t off = (uint32_t)r * (uint32_t)stride + (uint32_t)d;
-      const int n = count(j);
-      const T* p = from(j);
-      if (n == 32 && D == DP) {
-        v[i] = load_vec(p + off);
+      int have = 0;
+      const T* p = nullptr;
+      if constexpr (kWaves % (NT / 64) == 0) {
+        have = n[i / (kWaves / (NT / 64))];
+        p = from[i / (kWaves / (NT / 64))];
       } else {
-        v[i] = Vec<T>{};
-        if (r < n && d < D) v[i] = load_vec(p + off);
+#pragma unroll
+        for (int j = 0; j < U; ++j)
+          if ((wave + i * (NT / 64)) / kWaves == j) {
+            have = n[j];
+            p = from[j];
+          }
       }
+      v[i] = Vec<T>{};
+      if (r < have && d < D) v[i] = load_vec(p + off);
     }
   }
   __device__ __forceinline__ void store(char* t) const {
@@ -228,17 +232,38 @@ __device__ __forceinline__ Where where(const Args& a) {
 }
 
 // A tile's units of 32 keys: unit u is part u % (block / 32) of the list's block u / (block / 32).
+template <int U>
+struct Span {
+  int64_t first[U];
+  int n[U];  // keys that count
+};
 struct Keys {
   const int32_t* list;
   int block, lg, units;
   int64_t nk;
-  __device__ __forceinline__ int64_t first(int u) const {
-    return (int64_t)uniform(list[u >> lg]) * block + 32 * (u & ((1 << lg) - 1));
-  }
-  __device__ __forceinline__ int count(int u) const {
-    return u < units ? (int)max((int64_t)0, min((int64_t)32, nk - first(u))) : 0;
+  template <int U>
+  __device__ __forceinline__ Span<U> span(int u) const {
+    int b[U];
+    Span<U> s;
+#pragma unroll
+    for (int j = 0; j < U; ++j) b[j] = list[min(u + j, units - 1) >> lg];
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+      s.first[j] = (int64_t)uniform(b[j]) * block + 32 * ((u + j) & ((1 << lg) - 1));
+      const int64_t left = nk - s.first[j];
+      s.n[j] = u + j < units ? (int)max((int64_t)0, min((int64_t)32, left)) : 0;
+    }
+    return s;
   }
 };
+// The unit of this wave (its number among U is uniform).
+template <int U>
+__device__ __forceinline__ int pick(const int (&n)[U], int w) {
+  int v = n[0];
+#pragma unroll
+  for (int j = 1; j < U; ++j) v = w == j ? n[j] : v;
+  return v;
+}
 
 // What a row's waves have in common at the end: wave kw = 0 takes in the others' sums through LDS.
 template <int RW, int DP>
@@ -294,11 +319,18 @@ __global__ __launch_bounds__(NT, (sizeof(T) == 2 && DP <= 64 ? 4 : 1)) void k_at
   const Keys where_ = {list, a.block, a.lg, u1, nk};
   Stage<T, DP, KW> sk, sv;
   const auto fetch = [&](int u) {
-    const auto have = [&](int j) { return where_.count(u + j); };
-    sk.load(a.k.l, a.D, [&](int j) { return kp + where_.first(u + j) * a.k.l; }, have);
-    sv.load(a.v.l, a.D, [&](int j) { return vp + where_.first(u + j) * a.v.l; }, have);
+    const Span<KW> s = where_.span<KW>(u);
+    const T *pk[KW], *pv[KW];
+#pragma unroll
+    for (int j = 0; j < KW; ++j) {
+      pk[j] = kp + s.first[j] * a.k.l;
+      pv[j] = vp + s.first[j] * a.v.l;
+    }
+    sk.load(pk, s.n, a.k.l, a.D);
+    sv.load(pv, s.n, a.v.l, a.D);
+    return pick(s.n, kw);
   };
-  if (u0 < u1) fetch(u0);
+  int ahead = u0 < u1 ? fetch(u0) : 0;
   bool begun = false;
   for (int u = u0, step = 0; u < u1; u += KW, ++step) {
     char* tk = lds + (step % NB) * 2 * KW * L::kUnit;
@@ -307,10 +339,10 @@ __global__ __launch_bounds__(NT, (sizeof(T) == 2 && DP <= 64 ? 4 : 1)) void k_at
     sk.store(tk);
     sv.store(tv);
     __syncthreads();
-    if (u + KW < u1) fetch(u + KW);
+    const int left = ahead;
+    if (u + KW < u1) ahead = fetch(u + KW);
     tk += kw * L::kUnit;
     tv += kw * L::kUnit;
-    const int left = where_.count(u + kw);
     if (left == 0) continue;
     f32x16 x = {};
 #pragma unroll
@@ -531,11 +563,18 @@ __global__ __launch_bounds__(NT) void k_attend_dq(Args a) {
   const Keys where_ = {list, a.block, a.lg, units, nk};
   Stage<T, DP, KW> sk, sv;
   const auto fetch = [&](int u) {
-    const auto have = [&](int j) { return where_.count(u + j); };
-    sk.load(a.k.l, a.D, [&](int j) { return kp + where_.first(u + j) * a.k.l; }, have);
-    sv.load(a.v.l, a.D, [&](int j) { return vp + where_.first(u + j) * a.v.l; }, have);
+    const Span<KW> s = where_.span<KW>(u);
+    const T *pk[KW], *pv[KW];
+#pragma unroll
+    for (int j = 0; j < KW; ++j) {
+      pk[j] = kp + s.first[j] * a.k.l;
+      pv[j] = vp + s.first[j] * a.v.l;
+    }
+    sk.load(pk, s.n, a.k.l, a.D);
+    sv.load(pv, s.n, a.v.l, a.D);
+    return pick(s.n, kw);
   };
-  if (units) fetch(0);
+  int ahead = units ? fetch(0) : 0;
   for (int u = 0, step = 0; u < units; u += KW, ++step) {
     char* tk = lds + (step % NB) * 2 * KW * L::kUnit;
     char* tv = tk + KW * L::kUnit;
@@ -543,10 +582,10 @@ __global__ __launch_bounds__(NT) void k_attend_dq(Args a) {
     sk.store(tk);
     sv.store(tv);
     __syncthreads();
-    if (u + KW < units) fetch(u + KW);
+    const int left = ahead;
+    if (u + KW < units) ahead = fetch(u + KW);
     tk += kw * L::kUnit;
     tv += kw * L::kUnit;
-    const int left = where_.count(u + kw);
     if (left == 0) continue;
     f32x16 x = {}, dp = {};
 #pragma unroll
@@ -658,15 +697,23 @@ __global__ __launch_bounds__(NT) void k_attend_dkv(Args a) {
     const auto pos = [&](int u) {  // exact: u >> lg < 2^20 and G <= 1024
       return a.G == 1 ? u >> a.lg : (int)__umulhi((uint32_t)(u >> a.lg), a.group_magic);
     };
-    const auto row0 = [&](int u) { return (int64_t)uniform(tiles[pos(u)]) * a.block + 32 * (u & ((1 << a.lg) - 1)); };
-    const auto head = [&](int u) { return hk * a.G + (u >> a.lg) - pos(u) * a.G; };
-    const auto rows = [&](int u) { return u < units ? (int)max((int64_t)0, min((int64_t)32, nq - row0(u))) : 0; };
     Stage<T, DP, QW> sq, sg;
     float st_lse = INFINITY, st_delta = 0.f;
     const auto fetch = [&](int u) {
-      const auto have = [&](int j) { return rows(u + j); };
-      sq.load(a.q.l, a.D, [&](int j) { return (const T*)a.q.p + b * a.q.b + row0(u + j) * a.q.l + head(u + j) * a.q.h; }, have);
-      sg.load(a.g.l, a.D, [&](int j) { return (const T*)a.g.p + b * a.g.b + row0(u + j) * a.g.l + head(u + j) * a.g.h; }, have);
+      const T *pq[QW], *pg[QW];
+      int tile[QW], have[QW];
+#pragma unroll
+      for (int j = 0; j < QW; ++j) tile[j] = tiles[pos(min(u + j, units - 1))];
+#pragma unroll
+      for (int j = 0; j < QW; ++j) {
+        const int64_t i0 = (int64_t)uniform(tile[j]) * a.block + 32 * ((u + j) & ((1 << a.lg) - 1));
+        const int h = hk * a.G + ((u + j) >> a.lg) - pos(u + j) * a.G;
+        pq[j] = (const T*)a.q.p + b * a.q.b + i0 * a.q.l + h * a.q.h;
+        pg[j] = (const T*)a.g.p + b * a.g.b + i0 * a.g.l + h * a.g.h;
+        have[j] = u + j < units ? (int)max((int64_t)0, min((int64_t)32, nq - i0)) : 0;
+      }
+      sq.load(pq, have, a.q.l, a.D);
+      sg.load(pg, have, a.g.l, a.D);
       if (threadIdx.x < QW * 32) {
         const int r = threadIdx.x % 32, uj = u + threadIdx.x / 32;
         st_lse = -INFINITY;
@@ -681,8 +728,9 @@ __global__ __launch_bounds__(NT) void k_attend_dkv(Args a) {
         }
         st_lse = st_lse == -INFINITY ? INFINITY : st_lse;  // rows that see nothing, or are none: every p is 0
       }
+      return pick(have, qw);
     };
-    if (units) fetch(0);
+    int ahead = units ? fetch(0) : 0;
     for (int u = 0; u < units; u += QW, ++step) {
       char* tq = lds + (step % NB) * 2 * QW * L::kUnit;
       char* tg = tq + QW * L::kUnit;
@@ -694,8 +742,9 @@ __global__ __launch_bounds__(NT) void k_attend_dkv(Args a) {
         stats[step % NB][1][threadIdx.x] = st_delta;
       }
       __syncthreads();
-      if (u + QW < units) fetch(u + QW);
-      if (rows(u + qw) == 0) continue;
+      const int live = ahead;
+      if (u + QW < units) ahead = fetch(u + QW);
+      if (live == 0) continue;
       tq += qw * L::kUnit;
       tg += qw * L::kUnit;
       f32x16 x = {}, dp = {};
