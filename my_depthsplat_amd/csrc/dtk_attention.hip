@@ -71,7 +71,8 @@ struct Args {
   float *lse;                // [B, Hq, Lq], base 2; -inf for rows without a key
   float *part, *part_m, *part_l;
   float* delta;
-  uint32_t *bits, *gmax;
+  uint32_t *bits, *gmax, *chosen;  // chosen, order: NULL where every workgroup of dk/dv fits the chip at once
+  int32_t* order;
 };
 
 __device__ __forceinline__ int64_t length_of(const int32_t* lengths, int b, int64_t L) {
@@ -475,7 +476,8 @@ __global__ __launch_bounds__(NT) void k_attend_join(Args a, int64_t rows) {
   if (d == 0 && a.lse) a.lse[r] = valid ? m + log2f(l) : -INFINITY;
 }
 
-// Which tiles chose a block: bits [B, Hkv, Tk, ceil(Tq / 32)].
+// Which tiles chose a block: bits [B, Hkv, Tk, ceil(Tq / 32)]; and how many did (a block named twice counts
+// once: whoever sets the bit counts it).
 __global__ __launch_bounds__(NT) void k_attend_mark(Args a) {
   const int t = blockIdx.x, hk = blockIdx.y, b = blockIdx.z;
   if ((int64_t)t * a.block >= length_of(a.q_lengths, b, a.Lq)) return;
@@ -483,8 +485,40 @@ __global__ __launch_bounds__(NT) void k_attend_mark(Args a) {
   const int words = (a.Tq + 31) / 32;
   for (int j = threadIdx.x; j < a.top; j += NT) {
     const int v = idx[j];
-    if (v >= 0 && v < a.Tk) atomicOr(a.bits + (((int64_t)b * a.Hkv + hk) * a.Tk + v) * words + t / 32, 1u << (t % 32));
+    if (v < 0 || v >= a.Tk) continue;
+    const int64_t item = ((int64_t)b * a.Hkv + hk) * a.Tk + v;
+    const uint32_t bit = 1u << (t % 32);
+    if (!(atomicOr(a.bits + item * words + t / 32, bit) & bit) && a.chosen) atomicAdd(a.chosen + item, 1u);
   }
+}
+
+// The blocks with the longest lists first: they are workgroups of dk/dv, the longest of which would
+// otherwise run on alone at the end (a popular block is chosen several times as often as the mean). One
+// workgroup sorts by the list's length, eight steps to a power of two; the order within a step does not matter.
+constexpr int kSteps = 264, kOrderThreads = 1024;
+__device__ __forceinline__ int length_step(uint32_t n) {  // 0 for the longest
+  if (n < 8) return kSteps - 1 - (int)n;
+  const int e = 31 - __clz(n);
+  return kSteps - 1 - (8 * (e - 2) + (int)((n >> (e - 3)) & 7));
+}
+__global__ __launch_bounds__(kOrderThreads) void k_attend_order(Args a, int items) {
+  __shared__ int at[kSteps];
+  for (int i = threadIdx.x; i < kSteps; i += kOrderThreads) at[i] = 0;
+  __syncthreads();
+  for (int i = threadIdx.x; i < items; i += kOrderThreads) atomicAdd(&at[length_step(a.chosen[i])], 1);
+  __syncthreads();
+  if (threadIdx.x < 64) {  // exclusive sums, 64 steps at a time
+    int before = 0;
+    for (int base = 0; base < kSteps; base += 64) {
+      const int i = base + (int)threadIdx.x;
+      const int n = i < kSteps ? at[i] : 0;
+      const int incl = (int)dsplat::wave_incl_scan((uint32_t)n, threadIdx.x);
+      if (i < kSteps) at[i] = before + incl - n;
+      before += __shfl(incl, 63, 64);
+    }
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < items; i += kOrderThreads) a.order[atomicAdd(&at[length_step(a.chosen[i])], 1)] = i;
 }
 
 // ds is rounded to the inputs' type for its products. f16 has few exponents, so ds is taken there
@@ -502,7 +536,7 @@ __device__ __forceinline__ void ds_scale(uint32_t largest, float& down, float& u
 // dq: the forward's shape; p is taken from the saved lse. delta = sum_d do o of each row on the
 // way, kept for dk.
 template <typename T, int DP, int RW>
-__global__ __launch_bounds__(NT) void k_attend_dq(Args a) {
+__global__ __launch_bounds__(NT, (sizeof(T) == 2 && DP <= 64 ? 3 : 1)) void k_attend_dq(Args a) {
   using M = Mma<T>;
   using L = Tile<T, DP>;
   using Frag = typename M::Frag;
@@ -656,7 +690,8 @@ __global__ __launch_bounds__(NT) void k_attend_dkv(Args a) {
   __shared__ int32_t tiles[kTiles];
   __shared__ int count;
   __shared__ __align__(16) float stats[NB][2][QW * 32];  // lse and delta of the staged rows
-  const int blk = blockIdx.x, hk = blockIdx.y, b = blockIdx.z;
+  const int item = a.order ? a.order[blockIdx.x] : (int)blockIdx.x;
+  const int blk = item % a.Tk, hk = item / a.Tk % a.Hkv, b = item / a.Tk / a.Hkv;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, col = lane & 31;
   const int rw = uniform(wave) % RW, qw = uniform(wave) / RW;
   const int64_t nq = length_of(a.q_lengths, b, a.Lq), nk = length_of(a.kv_lengths, b, a.Lk);
@@ -919,6 +954,24 @@ Args args_of(const dtk_attention* c) {
 }
 size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
 
+// The backward's workspace: delta, then what is cleared (the largest |do|, the lists' bits and lengths), the order.
+struct BwdLayout {
+  size_t gmax, bits, chosen, order, end;
+  int64_t items;
+  bool sorted;
+};
+BwdLayout layout_of(const dtk_attention* c, const Args& a) {
+  BwdLayout l;
+  l.items = (int64_t)c->B * c->Hkv * a.Tk;
+  l.sorted = l.items > 512;
+  l.gmax = align256((size_t)c->B * c->Hq * c->Lq * 4);
+  l.bits = l.gmax + 256;
+  l.chosen = l.bits + (size_t)l.items * ((a.Tq + 31) / 32) * 4;
+  l.order = l.chosen + (l.sorted ? (size_t)l.items * 4 : 0);
+  l.end = l.order + (l.sorted ? (size_t)l.items * 4 : 0);
+  return l;
+}
+
 }  // namespace
 
 extern "C" {
@@ -955,8 +1008,7 @@ int dtk_block_sparse_attention_fwd(const dtk_attention* c, void* workspace, void
 size_t dtk_block_sparse_attention_bwd_workspace_size(const dtk_attention* c) {
   if (!c || c->B <= 0 || c->Lq < 0 || c->Lk < 0 || c->Hq <= 0 || c->Hkv <= 0 || c->block <= 0) return 0;
   const Args a = args_of(c);
-  return align256((size_t)c->B * c->Hq * c->Lq * 4) + 256 +
-         (size_t)c->B * c->Hkv * a.Tk * ((a.Tq + 31) / 32) * 4;
+  return layout_of(c, a).end;
 }
 
 int dtk_block_sparse_attention_bwd(const dtk_attention* c, const void* dout, const int64_t* dout_strides, void* dq,
@@ -970,19 +1022,22 @@ int dtk_block_sparse_attention_bwd(const dtk_attention* c, const void* dout, con
   Args a = args_of(c);
   a.splits = 1;
   hipStream_t st = (hipStream_t)stream;
-  const int64_t rows = (int64_t)c->B * c->Hq * c->Lq;
   a.o = {c->o, c->Lq * c->Hq * c->D, (int64_t)c->Hq * c->D, c->D};
   if (c->Lq) a.g = strided(dout, dout_strides);
   a.dq = dq;
   a.dk = dk;
   a.dv = dv;
   char* ws = (char*)workspace;
+  const BwdLayout l = layout_of(c, a);
+  DSPLAT_REQUIRE(l.items < (1LL << 31), "dtk_block_sparse_attention_bwd: too large");
   a.delta = (float*)ws;
-  ws += align256((size_t)rows * 4);
-  a.gmax = (uint32_t*)ws;
-  a.bits = (uint32_t*)(ws + 256);
-  const size_t nbits = (size_t)c->B * c->Hkv * a.Tk * ((a.Tq + 31) / 32);
-  if (int e = dsplat::zero_async(a.gmax, 256 + nbits * 4, st, "dtk_block_sparse_attention_bwd")) return e;
+  a.gmax = (uint32_t*)(ws + l.gmax);
+  a.bits = (uint32_t*)(ws + l.bits);
+  if (l.sorted) {
+    a.chosen = (uint32_t*)(ws + l.chosen);
+    a.order = (int32_t*)(ws + l.order);
+  }
+  if (int e = dsplat::zero_async(a.gmax, l.order - l.gmax, st, "dtk_block_sparse_attention_bwd")) return e;
   if (c->Lq) {
     const dim3 grid(a.Tq * a.rowtiles, a.Hkv, c->B);
     if (int e = by_type<Dq>(c->dtype, row_waves(a), a, grid, st)) return e;
@@ -992,7 +1047,11 @@ int dtk_block_sparse_attention_bwd(const dtk_attention* c, const void* dout, con
     }
   }
   if (!a.Tk) return 0;
-  return by_type<Dkv>(c->dtype, a.block / 32, a, dim3(a.Tk, a.Hkv, c->B), st);
+  if (l.sorted) {
+    k_attend_order<<<1, kOrderThreads, 0, st>>>(a, (int)l.items);
+    if (int e = dsplat::check_launch("k_attend_order")) return e;
+  }
+  return by_type<Dkv>(c->dtype, a.block / 32, a, dim3((unsigned)l.items), st);
 }
 
 }  // extern "C"
