@@ -686,6 +686,7 @@ __global__ __launch_bounds__(NT) void k_attend_dkv(Args a) {
   using L = Tile<T, DP>;
   using Frag = typename M::Frag;
   constexpr int QW = 4 / RW, NS = DP / 16, ND = DP / 32, NB = kBuffers<T, DP, QW>;
+  constexpr int kAhead = sizeof(T) == 2 && DP <= 64 ? 2 : 1;  // steps whose rows are on their way
   extern __shared__ __align__(16) char lds[];
   __shared__ int32_t tiles[kTiles];
   __shared__ int count;
@@ -732,9 +733,13 @@ __global__ __launch_bounds__(NT) void k_attend_dkv(Args a) {
     const auto pos = [&](int u) {  // exact: u >> lg < 2^20 and G <= 1024
       return a.G == 1 ? u >> a.lg : (int)__umulhi((uint32_t)(u >> a.lg), a.group_magic);
     };
-    Stage<T, DP, QW> sq, sg;
-    float st_lse = INFINITY, st_delta = 0.f;
-    const auto fetch = [&](int u) {
+    // What is on its way: the rows of the units u .. u + QW - 1 and their statistics.
+    struct Ahead {
+      Stage<T, DP, QW> q, g;
+      float lse, delta;
+      int live;
+    };
+    const auto fetch = [&](Ahead& f, int u) {
       const T *pq[QW], *pg[QW];
       int tile[QW], have[QW];
 #pragma unroll
@@ -747,39 +752,38 @@ __global__ __launch_bounds__(NT) void k_attend_dkv(Args a) {
         pg[j] = (const T*)a.g.p + b * a.g.b + i0 * a.g.l + h * a.g.h;
         have[j] = u + j < units ? (int)max((int64_t)0, min((int64_t)32, nq - i0)) : 0;
       }
-      sq.load(pq, have, a.q.l, a.D);
-      sg.load(pg, have, a.g.l, a.D);
+      f.q.load(pq, have, a.q.l, a.D);
+      f.g.load(pg, have, a.g.l, a.D);
       if (threadIdx.x < QW * 32) {
         const int r = threadIdx.x % 32, uj = u + threadIdx.x / 32;
-        st_lse = -INFINITY;
+        f.lse = -INFINITY;
         if (uj < units) {
           const int at = pos(uj);
           const int64_t i = (int64_t)tiles[at] * a.block + 32 * (uj & ((1 << a.lg) - 1)) + r;
           if (i < nq) {
             const int64_t stat = ((int64_t)b * a.Hq + hk * a.G + (uj >> a.lg) - at * a.G) * a.Lq + i;
-            st_lse = a.lse[stat];
-            st_delta = a.delta[stat];
+            f.lse = a.lse[stat];
+            f.delta = a.delta[stat];
           }
         }
-        st_lse = st_lse == -INFINITY ? INFINITY : st_lse;  // rows that see nothing, or are none: every p is 0
       }
-      return pick(have, qw);
+      f.live = pick(have, qw);
     };
-    int ahead = units ? fetch(0) : 0;
-    for (int u = 0; u < units; u += QW, ++step) {
+    const auto turn = [&](Ahead& f, int u) {
       char* tq = lds + (step % NB) * 2 * QW * L::kUnit;
       char* tg = tq + QW * L::kUnit;
       if (NB == 1) __syncthreads();
-      sq.store(tq);
-      sg.store(tg);
+      f.q.store(tq);
+      f.g.store(tg);
       if (threadIdx.x < QW * 32) {
-        stats[step % NB][0][threadIdx.x] = st_lse;
-        stats[step % NB][1][threadIdx.x] = st_delta;
+        // rows that see nothing, or are none: relative to +inf every p is 0
+        stats[step % NB][0][threadIdx.x] = f.lse == -INFINITY ? INFINITY : f.lse;
+        stats[step % NB][1][threadIdx.x] = f.delta;
       }
       __syncthreads();
-      const int live = ahead;
-      if (u + QW < units) ahead = fetch(u + QW);
-      if (live == 0) continue;
+      const int live = f.live, buffer = step++ % NB;
+      if (u + kAhead * QW < units) fetch(f, u + kAhead * QW);
+      if (live == 0) return;
       tq += qw * L::kUnit;
       tg += qw * L::kUnit;
       f32x16 x = {}, dp = {};
@@ -791,8 +795,8 @@ __global__ __launch_bounds__(NT) void k_attend_dkv(Args a) {
       // (lanes whose key is none hold columns that are not written)
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
-        const float4 lse = *(const float4*)&stats[step % NB][0][qw * 32 + 8 * c + 4 * half];
-        const float4 delta = *(const float4*)&stats[step % NB][1][qw * 32 + 8 * c + 4 * half];
+        const float4 lse = *(const float4*)&stats[buffer][0][qw * 32 + 8 * c + 4 * half];
+        const float4 delta = *(const float4*)&stats[buffer][1][qw * 32 + 8 * c + 4 * half];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int r = 4 * c + e;
@@ -810,7 +814,15 @@ __global__ __launch_bounds__(NT) void k_attend_dkv(Args a) {
         dk[d] = M::mma(L::col(tq, 0, d, lane), s0, dk[d]);
         dk[d] = M::mma(L::col(tq, 1, d, lane), s1, dk[d]);
       }
-    }
+    };
+    Ahead f[kAhead] = {};
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k)
+      if (k * QW < units) fetch(f[k], k * QW);
+    for (int u = 0; u < units; u += kAhead * QW)
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k)
+        if (u + k * QW < units) turn(f[k], u + k * QW);
   }
   if constexpr (QW > 1) {
     float* jo = (float*)lds + (rw * 32 + col) * (DP + 1);
