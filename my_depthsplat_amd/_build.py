@@ -37,7 +37,8 @@ CFLAGS += ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 # without it at config B).
 FILE_FLAGS = {"dsr_raster.hip": ["-fno-slp-vectorize"],
               # nothing there has to match another kernel bit for bit (the fused norm matches the plain one)
-              **{f: ["-ffp-contract=fast"] for f in ("dtk_rotary.hip", "dtk_attention.hip")}}
+              **{f: ["-ffp-contract=fast"] for f in ("dtk_rotary.hip", "dtk_attention.hip", "dtk_attention_f32.hip",
+                                                   "dtk_attention_bf16.hip", "dtk_attention_f16.hip")}}
 
 
 def _sources() -> list[Path]:

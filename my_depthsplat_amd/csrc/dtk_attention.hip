@@ -1,454 +1,11 @@
-// dtk_attention.hip — attention of query tiles over their chosen key blocks, forward, backward
-// and the form for few queries, for gfx950.
-//
-//   tile t = queries t block .. t block + block - 1; its keys are those of the blocks index[t]
-//   x = scale q k^T, p = exp(x - lse), o = p v;  backward: dv = p^T do, dp = do v^T,
-//   ds = p (dp - sum_d do o), dq = scale ds k, dk = scale ds^T q
-//
-// All products are 32 x 32 matrix instructions, taken transposed (keys as rows, queries as
-// columns) in the forward and in dq: a lane then holds one query's scores, so the running
-// maximum and sum need one exchange between the two halves of the wave, and the probabilities
-// are already laid out as the second product's right operand: an instruction's k index may be
-// permuted as long as both operands agree, so the accumulator's rows (8 (r / 4) + 4 half + r % 4)
-// serve as they are and nothing is shuffled.
-
-#include "dtk_common.h"
+// dtk_attention.hip — the C ABI of attention over chosen blocks (kernels: dtk_attention.h), the join of
+// split lists, and who chose which block for the backward.
+#include "dtk_attention.h"
 
 namespace {
 using namespace dtk;
 
-constexpr int NT = 256;
-constexpr float kLog2e = 1.44269504088896340736f;
-
-typedef float f32x16 __attribute__((ext_vector_type(16)));
-typedef float f32x8 __attribute__((ext_vector_type(8)));
-typedef bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef f16 f16x8 __attribute__((ext_vector_type(8)));
-
-// An operand fragment is 8 elements per lane: row (column) lane % 32, k = 8 (lane / 32) + j, or
-// any other k both operands share. f32 runs as eight k = 2 instructions over the same registers.
-template <typename T>
-struct Mma;
-template <>
-struct Mma<bf16> {
-  using Frag = bf16x8;
-  static __device__ __forceinline__ f32x16 mma(Frag a, Frag b, f32x16 c) {
-    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
-  }
-};
-template <>
-struct Mma<f16> {
-  using Frag = f16x8;
-  static __device__ __forceinline__ f32x16 mma(Frag a, Frag b, f32x16 c) {
-    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
-  }
-};
-template <>
-struct Mma<float> {
-  using Frag = f32x8;
-  static __device__ __forceinline__ f32x16 mma(Frag a, Frag b, f32x16 c) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[j], b[j], c, 0, 0, 0);
-    return c;
-  }
-};
-
-struct Strided {
-  const void* p;
-  int64_t b, l, h;
-};
-struct Args {
-  int64_t Lq, Lk;
-  int Hq, Hkv, G, D, block, top, Tq, Tk;
-  int lg;                    // block = 32 << lg
-  uint32_t group_magic;      // ceil(2^32 / G)
-  int Lt, rowtiles, splits;  // rows of a tile, workgroups per tile, parts of the key list
-  float scale, scale2;       // scale2: |scale| log2 e, at least the smallest normal number (masked scores are
-                             // -inf, and a scale of 0 must not make them no number)
-  Strided q, k, v, o, g;  // g: the output's gradient
-  const int32_t *index, *q_lengths, *kv_lengths;
-  void *out, *dq, *dk, *dv;  // contiguous
-  float *lse;                // [B, Hq, Lq], base 2; -inf for rows without a key
-  float *part, *part_m, *part_l;
-  float* delta;
-  uint32_t *bits, *gmax, *chosen;  // chosen, order: NULL where every workgroup of dk/dv fits the chip at once
-  int32_t* order;
-};
-
-__device__ __forceinline__ int64_t length_of(const int32_t* lengths, int b, int64_t L) {
-  if (!lengths) return L;
-  const int64_t n = lengths[b];
-  return n < 0 ? 0 : n < L ? n : L;
-}
-
-// 8 channels of a row from d0 on, zeros behind D and for rows that do not count (what stands
-// there may be no number).
-template <typename T>
-__device__ __forceinline__ typename Mma<T>::Frag row_frag(const T* row, int d0, int D, bool valid) {
-  typename Mma<T>::Frag f = {};
-  if (valid && d0 < D) __builtin_memcpy(&f, row + d0, sizeof(f));
-  return f;
-}
-template <typename T>
-__device__ __forceinline__ typename Mma<T>::Frag acc_frag(const f32x16& p, int s) {
-  typename Mma<T>::Frag f;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) f[j] = (T)p[8 * s + j];
-  return f;
-}
-
-// A tile of rows in LDS, R rows of DP channels. The pitch keeps both ways of reading it nearly
-// free of bank conflicts: 16 rows' 16-byte pieces at one channel (the row fragments) fall on 16
-// different groups of four banks, and the transposed read's 8 rows x 64 bytes on each bank three
-// times at most (two is the least).
-template <typename T, int DP>
-struct Tile {
-  static constexpr int kPitch = DP * (int)sizeof(T) + (sizeof(T) == 2 && DP == 128 ? 48 : 16);  // bytes
-  static constexpr int kPieces = DP * (int)sizeof(T) / 16;                                      // per row
-  static constexpr int kUnit = 32 * kPitch;                                                     // bytes of 32 rows
-  using Frag = typename Mma<T>::Frag;
-
-  // channels 16 s + 8 half .. + 7 of row lane % 32
-  static __device__ __forceinline__ Frag row(const char* t, int s, int col, int half) {
-    Frag f;
-    __builtin_memcpy(&f, __builtin_assume_aligned(t + col * kPitch + (16 * s + 8 * half) * sizeof(T), 16), sizeof(f));
-    return f;
-  }
-  // channel 32 d + lane % 32 of the 8 rows 16 s + {4 half .. + 3, 8 + 4 half .. + 3}: the rows an accumulator
-  // holds. 16 bits: the transposing LDS read hands lane i of 16 the i-th column of the 4 rows of 16
-  // that the 16 lanes' 8-byte pieces make up.
-  static __device__ __forceinline__ Frag col(const char* t, int s, int d, int lane) {
-    Frag f;
-    const int half = lane >> 5;
-    if constexpr (sizeof(T) == 2) {
-      typedef short s16x4 __attribute__((ext_vector_type(4)));
-      typedef __attribute__((address_space(3))) s16x4* lds;
-      const int i = lane & 15;
-      const char* at = t + (16 * s + 4 * half + (i >> 2)) * kPitch + (32 * d + (lane & 16) + 4 * (i & 3)) * 2;
-      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds)at);
-      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds)(at + 8 * kPitch));
-      __builtin_memcpy(&f, &lo, 8);
-      __builtin_memcpy((char*)&f + 8, &hi, 8);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        f[j] = *(const T*)(t + (16 * s + 4 * half + (j & 3) + 8 * (j >> 2)) * kPitch + (32 * d + (lane & 31)) * 4);
-    }
-    return f;
-  }
-};
-
-__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
-
-// The workgroup's share of U units (32 rows each) on the way from memory to LDS: loaded into
-// registers while the tile before is worked on, then stored. Rows that do not count and channels
-// behind D become zeros. A wave's pieces are all of one unit, so where that starts is scalar work and a
-// load adds one 32-bit offset to it (31 rows' strides fit: the host checks).
-template <typename T, int DP, int U>
-struct Stage {
-  using L = Tile<T, DP>;
-  static constexpr int kPer = (U * 32 * L::kPieces + NT - 1) / NT;
-  static constexpr int kWaves = 32 * L::kPieces / 64;  // waves of pieces per unit
-  Vec<T> v[kPer];
-  // from[j]: where the j-th unit's first row starts, n[j]: its rows that count
-  __device__ __forceinline__ void load(const T* const (&from)[U], const int (&n)[U], int64_t stride, int D) {
-    const int wave = uniform(threadIdx.x >> 6);
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      const int id = threadIdx.x + i * NT, r = id / L::kPieces % 32, d = id % L::kPieces * Vec<T>::N;
-      const uint32_t off = (uint32_t)r * (uint32_t)stride + (uint32_t)d;
-      int have = 0;
-      const T* p = nullptr;
-      if constexpr (kWaves % (NT / 64) == 0) {
-        have = n[i / (kWaves / (NT / 64))];
-        p = from[i / (kWaves / (NT / 64))];
-      } else {
-#pragma unroll
-        for (int j = 0; j < U; ++j)
-          if ((wave + i * (NT / 64)) / kWaves == j) {
-            have = n[j];
-            p = from[j];
-          }
-      }
-      v[i] = Vec<T>{};
-      if (r < have && d < D) v[i] = load_vec(p + off);
-    }
-  }
-  __device__ __forceinline__ void store(char* t) const {
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      const int id = threadIdx.x + i * NT, r = id / L::kPieces, c = id % L::kPieces;
-      if ((i + 1) * NT <= U * 32 * L::kPieces || r < U * 32)
-        __builtin_memcpy(__builtin_assume_aligned(t + r * L::kPitch + c * 16, 16), &v[i], 16);
-    }
-  }
-};
-// Two buffers (one barrier per step) while they leave room for two workgroups per CU; f32 tiles are
-// twice as large and its products eight times as long: one.
-template <typename T, int DP, int U>
-constexpr int kBuffers = sizeof(T) == 2 && 4 * U * Tile<T, DP>::kUnit <= 80 * 1024 ? 2 : 1;
-template <typename T, int DP, int U>
-constexpr int kTileBytes = 2 * kBuffers<T, DP, U> * U * Tile<T, DP>::kUnit;
-
-__device__ __forceinline__ int acc_row(int r, int half) { return 8 * (r >> 2) + 4 * half + (r & 3); }
-
-// The tile's list without places that are no block or stand in it already, in LDS, in order.
-__device__ __forceinline__ int block_list(const int32_t* idx, int top, int blocks, int32_t* list, int* count) {
-  if (threadIdx.x < 64) {
-    const int lane = threadIdx.x;
-    int n = 0;
-    for (int base = 0; base < top; base += 64) {
-      const int at = base + lane;
-      const int v = at < top ? idx[at] : -1;
-      bool ok = v >= 0 && v < blocks;
-      for (int j = 0; ok && j < at; ++j) ok = idx[j] != v;
-      const uint64_t m = __ballot(ok);
-      if (ok) list[n + __popcll(m & dsplat::lanemask_lt(lane))] = v;
-      n += __popcll(m);
-    }
-    if (lane == 0) *count = n;
-  }
-  __syncthreads();
-  return __builtin_amdgcn_readfirstlane(*count);
-}
-
-template <typename T>
-__device__ __forceinline__ void store4(T* p, float a, float b, float c, float d) {
-  T v[4] = {(T)a, (T)b, (T)c, (T)d};
-  __builtin_memcpy(p, v, sizeof(v));
-}
-
-// Where a workgroup works: tile, row group, key head, scene, part of the list.
-struct Where {
-  int t, rt, hk, b, split;
-};
-__device__ __forceinline__ Where where(const Args& a) {
-  Where w;
-  w.t = blockIdx.x / a.rowtiles;
-  w.rt = blockIdx.x % a.rowtiles;
-  w.hk = blockIdx.y;
-  w.b = blockIdx.z / a.splits;
-  w.split = blockIdx.z % a.splits;
-  return w;
-}
-
-// A tile's units of 32 keys: unit u is part u % (block / 32) of the list's block u / (block / 32).
-template <int U>
-struct Span {
-  int64_t first[U];
-  int n[U];  // keys that count
-};
-struct Keys {
-  const int32_t* list;
-  int block, lg, units;
-  int64_t nk;
-  template <int U>
-  __device__ __forceinline__ Span<U> span(int u) const {
-    int b[U];
-    Span<U> s;
-#pragma unroll
-    for (int j = 0; j < U; ++j) b[j] = list[min(u + j, units - 1) >> lg];
-#pragma unroll
-    for (int j = 0; j < U; ++j) {
-      s.first[j] = (int64_t)uniform(b[j]) * block + 32 * ((u + j) & ((1 << lg) - 1));
-      const int64_t left = nk - s.first[j];
-      s.n[j] = u + j < units ? (int)max((int64_t)0, min((int64_t)32, left)) : 0;
-    }
-    return s;
-  }
-};
-// The unit of this wave (its number among U is uniform).
-template <int U>
-__device__ __forceinline__ int pick(const int (&n)[U], int w) {
-  int v = n[0];
-#pragma unroll
-  for (int j = 1; j < U; ++j) v = w == j ? n[j] : v;
-  return v;
-}
-
-// What a row's waves have in common at the end: wave kw = 0 takes in the others' sums through LDS.
-template <int RW, int DP>
-struct Join {
-  float o[RW * 32 * (DP + 1)];
-  float m[RW * 32], l[RW * 32];
-};
-
-// Forward. RW waves stand side by side over 32 rows each, 4 / RW take turns at the list's units
-// of 32 keys and are joined at the end. The rows of a tile are its queries of all heads that
-// share the key head (few queries: they fill the instruction's columns together).
-template <typename T, int DP, int RW>
-__global__ __launch_bounds__(NT, (sizeof(T) == 2 && DP <= 64 ? 4 : 1)) void k_attend_fwd(Args a) {
-  using M = Mma<T>;
-  using L = Tile<T, DP>;
-  using Frag = typename M::Frag;
-  constexpr int KW = 4 / RW, NS = DP / 16, ND = DP / 32, NB = kBuffers<T, DP, KW>;
-  extern __shared__ __align__(16) char lds[];
-  __shared__ int count;
-  int32_t* list = (int32_t*)(lds + kTileBytes<T, DP, KW>);
-  const Where at = where(a);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, col = lane & 31;
-  const int rw = uniform(wave) % RW, kw = uniform(wave) / RW;
-  const int64_t nq = length_of(a.q_lengths, at.b, a.Lq), nk = length_of(a.kv_lengths, at.b, a.Lk);
-  const int row = (at.rt * RW + rw) * 32 + col;
-  const int g = row / a.Lt;
-  const int64_t i = (int64_t)at.t * a.block + row % a.Lt;
-  const bool exists = g < a.G && i < a.Lq, valid = exists && i < nq;
-  const int h = at.hk * a.G + (g < a.G ? g : 0);
-  const int blocks = (int)min((int64_t)a.Tk, (nk + a.block - 1) / a.block);
-  int n = 0;
-  if ((int64_t)at.t * a.block < nq)
-    n = block_list(a.index + (((int64_t)at.b * a.Hkv + at.hk) * a.Tq + at.t) * a.top, a.top, blocks, list, &count);
-
-  const T* qp = (const T*)a.q.p + at.b * a.q.b + (valid ? i : 0) * a.q.l + h * a.q.h;
-  Frag qf[NS];
-#pragma unroll
-  for (int s = 0; s < NS; ++s) {
-    qf[s] = row_frag<T>(qp, 16 * s + 8 * half, a.D, valid);
-    if (a.scale < 0.f) qf[s] = -qf[s];
-  }
-  const T* kp = (const T*)a.k.p + at.b * a.k.b + at.hk * a.k.h;
-  const T* vp = (const T*)a.v.p + at.b * a.v.b + at.hk * a.v.h;
-
-  f32x16 o[ND] = {};
-  // The exponents are taken relative to base2, which follows the running maximum m only when a sum of 16
-  // has passed 2^12: p stays in every type's range, the fast path needs no maximum, and o is
-  // rarely rescaled. (l <= 2^12 x keys, o likewise: far inside 32 bits.)
-  float m = -INFINITY, base2 = 0.f, l = 0.f;
-  const int units = n << a.lg;
-  const int per = (units + a.splits - 1) / a.splits;
-  const int u0 = min(units, at.split * per), u1 = min(units, u0 + per);
-  const Keys where_ = {list, a.block, a.lg, u1, nk};
-  Stage<T, DP, KW> sk, sv;
-  const auto fetch = [&](int u) {
-    const Span<KW> s = where_.span<KW>(u);
-    const T *pk[KW], *pv[KW];
-#pragma unroll
-    for (int j = 0; j < KW; ++j) {
-      pk[j] = kp + s.first[j] * a.k.l;
-      pv[j] = vp + s.first[j] * a.v.l;
-    }
-    sk.load(pk, s.n, a.k.l, a.D);
-    sv.load(pv, s.n, a.v.l, a.D);
-    return pick(s.n, kw);
-  };
-  int ahead = u0 < u1 ? fetch(u0) : 0;
-  bool begun = false;
-  for (int u = u0, step = 0; u < u1; u += KW, ++step) {
-    char* tk = lds + (step % NB) * 2 * KW * L::kUnit;
-    char* tv = tk + KW * L::kUnit;
-    if (NB == 1) __syncthreads();
-    sk.store(tk);
-    sv.store(tv);
-    __syncthreads();
-    const int left = ahead;
-    if (u + KW < u1) ahead = fetch(u + KW);
-    tk += kw * L::kUnit;
-    tv += kw * L::kUnit;
-    if (left == 0) continue;
-    f32x16 x = {};
-#pragma unroll
-    for (int s = 0; s < NS; ++s) x = M::mma(L::row(tk, s, col, half), qf[s], x);
-    if (left < 32) {
-#pragma unroll
-      for (int r = 0; r < 16; ++r) x[r] = acc_row(r, half) < left ? x[r] : -INFINITY;
-    }
-    f32x16 p;
-    float sum = 0.f;
-    if (begun) {
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        p[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[r], a.scale2, -base2));
-        sum += p[r];
-      }
-    }
-    if (!begun || __any(!(sum <= 4096.f))) {
-      begun = true;
-      float mx = x[0];
-#pragma unroll
-      for (int r = 1; r < 16; ++r) mx = fmaxf(mx, x[r]);
-      mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-      const float mn = fmaxf(m, mx), b2 = mn == -INFINITY ? 0.f : mn * a.scale2;
-      const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(base2 - b2);
-      m = mn;
-      base2 = b2;
-      l *= alpha;
-#pragma unroll
-      for (int d = 0; d < ND; ++d) o[d] *= alpha;
-      sum = 0.f;
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        p[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[r], a.scale2, -base2));
-        sum += p[r];
-      }
-    }
-    l += sum;
-    const Frag p0 = acc_frag<T>(p, 0), p1 = acc_frag<T>(p, 1);
-#pragma unroll
-    for (int d = 0; d < ND; ++d) {
-      o[d] = M::mma(L::col(tv, 0, d, lane), p0, o[d]);
-      o[d] = M::mma(L::col(tv, 1, d, lane), p1, o[d]);
-    }
-  }
-  l += __shfl_xor(l, 32, 64);
-  if constexpr (KW > 1) {
-    static_assert(sizeof(Join<RW, DP>) <= kTileBytes<T, DP, KW>, "joined in the tiles' place");
-    Join<RW, DP>& join = *(Join<RW, DP>*)lds;
-    float* jo = join.o + (rw * 32 + col) * (DP + 1);
-    for (int k = 1; k < KW; ++k) {
-      __syncthreads();
-      if (kw == k) {
-#pragma unroll
-        for (int d = 0; d < ND; ++d)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) jo[32 * d + acc_row(r, half)] = o[d][r];
-        if (half == 0) {
-          join.m[rw * 32 + col] = m == -INFINITY ? m : base2;
-          join.l[rw * 32 + col] = l;
-        }
-      }
-      __syncthreads();
-      if (kw == 0) {
-        const float mo = join.m[rw * 32 + col], lo = join.l[rw * 32 + col], me = m == -INFINITY ? m : base2;
-        const float mn = fmaxf(me, mo), b2 = mn == -INFINITY ? 0.f : mn;
-        const float fa = __builtin_amdgcn_exp2f(me - b2), fb = __builtin_amdgcn_exp2f(mo - b2);
-        m = mn;  // from here on in powers of two
-        base2 = b2;
-        l = l * fa + lo * fb;
-#pragma unroll
-        for (int d = 0; d < ND; ++d)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) o[d][r] = o[d][r] * fa + jo[32 * d + acc_row(r, half)] * fb;
-      }
-    }
-  }
-  if (kw != 0 || !exists) return;
-  const float top2 = m == -INFINITY ? m : base2;
-  if (a.splits > 1) {
-    const int64_t r = ((int64_t)at.b * a.Hq + h) * a.Lq + i, rows = (int64_t)(gridDim.z / a.splits) * a.Hq * a.Lq;
-    float* po = a.part + (at.split * rows + r) * a.D;
-#pragma unroll
-    for (int d = 0; d < ND; ++d)
-#pragma unroll
-      for (int c = 0; c < 4; ++c)
-        if (32 * d + 8 * c + 4 * half < a.D)
-          store4<float>(po + 32 * d + 8 * c + 4 * half, o[d][4 * c], o[d][4 * c + 1], o[d][4 * c + 2], o[d][4 * c + 3]);
-    if (half == 0) {
-      a.part_m[at.split * rows + r] = top2;
-      a.part_l[at.split * rows + r] = l;
-    }
-    return;
-  }
-  const float inv = valid && l > 0.f ? 1.f / l : (l != l ? l : 0.f);
-  T* op = (T*)a.out + (((int64_t)at.b * a.Lq + i) * a.Hq + h) * a.D;
-#pragma unroll
-  for (int d = 0; d < ND; ++d)
-#pragma unroll
-    for (int c = 0; c < 4; ++c)
-      if (32 * d + 8 * c + 4 * half < a.D)
-        store4<T>(op + 32 * d + 8 * c + 4 * half, o[d][4 * c] * inv, o[d][4 * c + 1] * inv, o[d][4 * c + 2] * inv,
-                  o[d][4 * c + 3] * inv);
-  if (half == 0 && a.lse) a.lse[((int64_t)at.b * a.Hq + h) * a.Lq + i] = valid ? top2 + log2f(l) : -INFINITY;
-}
+constexpr int NT = kThreads;
 
 // Joins the parts of a split list: one row per group of D / 4 threads.
 template <typename T>
@@ -521,402 +78,9 @@ __global__ __launch_bounds__(kOrderThreads) void k_attend_order(Args a, int item
   for (int i = threadIdx.x; i < items; i += kOrderThreads) a.order[atomicAdd(&at[length_step(a.chosen[i])], 1)] = i;
 }
 
-// ds is rounded to the inputs' type for its products. f16 has few exponents, so ds is taken there
-// relative to a power of two at the largest |do| (exact, undone in 32 bits): of the row in dq, of all rows
-// in dk.
-template <typename T>
-constexpr bool kFewExponents = __is_same(T, f16);
-__device__ __forceinline__ void ds_scale(uint32_t largest, float& down, float& up) {
-  const int e = (int)((largest >> 23) & 255);
-  const bool ok = e > 27 && e < 227;
-  down = ok ? __uint_as_float((uint32_t)(254 - e) << 23) : 1.f;
-  up = ok ? __uint_as_float((uint32_t)e << 23) : 1.f;
-}
-
-// dq: the forward's shape; p is taken from the saved lse. delta = sum_d do o of each row on the
-// way, kept for dk.
-template <typename T, int DP, int RW>
-__global__ __launch_bounds__(NT, (sizeof(T) == 2 && DP <= 64 ? 3 : 1)) void k_attend_dq(Args a) {
-  using M = Mma<T>;
-  using L = Tile<T, DP>;
-  using Frag = typename M::Frag;
-  constexpr int KW = 4 / RW, NS = DP / 16, ND = DP / 32, NB = kBuffers<T, DP, KW>;
-  extern __shared__ __align__(16) char lds[];
-  __shared__ int count;
-  int32_t* list = (int32_t*)(lds + kTileBytes<T, DP, KW>);
-  const Where at = where(a);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, col = lane & 31;
-  const int rw = uniform(wave) % RW, kw = uniform(wave) / RW;
-  const int64_t nq = length_of(a.q_lengths, at.b, a.Lq), nk = length_of(a.kv_lengths, at.b, a.Lk);
-  const int row = (at.rt * RW + rw) * 32 + col;
-  const int g = row / a.Lt;
-  const int64_t i = (int64_t)at.t * a.block + row % a.Lt;
-  const bool exists = g < a.G && i < a.Lq, valid = exists && i < nq;
-  const int h = at.hk * a.G + (g < a.G ? g : 0);
-  const int blocks = (int)min((int64_t)a.Tk, (nk + a.block - 1) / a.block);
-  int n = 0;
-  if ((int64_t)at.t * a.block < nq)
-    n = block_list(a.index + (((int64_t)at.b * a.Hkv + at.hk) * a.Tq + at.t) * a.top, a.top, blocks, list, &count);
-
-  const int64_t ir = valid ? i : 0;
-  const T* qp = (const T*)a.q.p + at.b * a.q.b + ir * a.q.l + h * a.q.h;
-  const T* gp = (const T*)a.g.p + at.b * a.g.b + ir * a.g.l + h * a.g.h;
-  const T* op = (const T*)a.o.p + at.b * a.o.b + ir * a.o.l + h * a.o.h;
-  Frag qf[NS], gf[NS];
-  float delta = 0.f, most = 0.f;
-#pragma unroll
-  for (int s = 0; s < NS; ++s) {
-    qf[s] = row_frag<T>(qp, 16 * s + 8 * half, a.D, valid);
-    if (a.scale < 0.f) qf[s] = -qf[s];
-    gf[s] = row_frag<T>(gp, 16 * s + 8 * half, a.D, valid);
-    const Frag of = row_frag<T>(op, 16 * s + 8 * half, a.D, valid);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      delta += (float)gf[s][j] * (float)of[j];
-      if (kFewExponents<T>) most = fmaxf(most, fabsf((float)gf[s][j]));
-    }
-  }
-  delta += __shfl_xor(delta, 32, 64);
-  float down = 1.f, up = 1.f;
-  if constexpr (kFewExponents<T>) {
-    most = fmaxf(most, __shfl_xor(most, 32, 64));
-    ds_scale(__float_as_uint(most), down, up);
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) most = fmaxf(most, __shfl_xor(most, off, 64));
-    if (kw == 0 && lane == 0 && most > 0.f) atomicMax(a.gmax, __float_as_uint(most));  // any order, the same answer
-  }
-  const int64_t stat = ((int64_t)at.b * a.Hq + h) * a.Lq + ir;
-  // rows that see nothing: relative to +inf every p is 0
-  const float saved = valid ? a.lse[stat] : -INFINITY, lse = saved == -INFINITY ? INFINITY : saved;
-  if (kw == 0 && half == 0 && valid) a.delta[stat] = delta;
-  const T* kp = (const T*)a.k.p + at.b * a.k.b + at.hk * a.k.h;
-  const T* vp = (const T*)a.v.p + at.b * a.v.b + at.hk * a.v.h;
-
-  f32x16 dq[ND] = {};
-  const int units = n << a.lg;
-  const Keys where_ = {list, a.block, a.lg, units, nk};
-  Stage<T, DP, KW> sk, sv;
-  const auto fetch = [&](int u) {
-    const Span<KW> s = where_.span<KW>(u);
-    const T *pk[KW], *pv[KW];
-#pragma unroll
-    for (int j = 0; j < KW; ++j) {
-      pk[j] = kp + s.first[j] * a.k.l;
-      pv[j] = vp + s.first[j] * a.v.l;
-    }
-    sk.load(pk, s.n, a.k.l, a.D);
-    sv.load(pv, s.n, a.v.l, a.D);
-    return pick(s.n, kw);
-  };
-  int ahead = units ? fetch(0) : 0;
-  for (int u = 0, step = 0; u < units; u += KW, ++step) {
-    char* tk = lds + (step % NB) * 2 * KW * L::kUnit;
-    char* tv = tk + KW * L::kUnit;
-    if (NB == 1) __syncthreads();
-    sk.store(tk);
-    sv.store(tv);
-    __syncthreads();
-    const int left = ahead;
-    if (u + KW < units) ahead = fetch(u + KW);
-    tk += kw * L::kUnit;
-    tv += kw * L::kUnit;
-    if (left == 0) continue;
-    f32x16 x = {}, dp = {};
-#pragma unroll
-    for (int s = 0; s < NS; ++s) {
-      x = M::mma(L::row(tk, s, col, half), qf[s], x);
-      dp = M::mma(L::row(tv, s, col, half), gf[s], dp);
-    }
-    if (left < 32) {
-#pragma unroll
-      for (int r = 0; r < 16; ++r) x[r] = acc_row(r, half) < left ? x[r] : -INFINITY;
-    }
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(x[r], a.scale2, -lse));
-      x[r] = p * (kFewExponents<T> ? (dp[r] - delta) * down : dp[r] - delta);
-    }
-    const Frag s0 = acc_frag<T>(x, 0), s1 = acc_frag<T>(x, 1);
-#pragma unroll
-    for (int d = 0; d < ND; ++d) {
-      dq[d] = M::mma(L::col(tk, 0, d, lane), s0, dq[d]);
-      dq[d] = M::mma(L::col(tk, 1, d, lane), s1, dq[d]);
-    }
-  }
-  if constexpr (KW > 1) {
-    float* jo = (float*)lds + (rw * 32 + col) * (DP + 1);
-    for (int k = 1; k < KW; ++k) {
-      __syncthreads();
-      if (kw == k)
-#pragma unroll
-        for (int d = 0; d < ND; ++d)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) jo[32 * d + acc_row(r, half)] = dq[d][r];
-      __syncthreads();
-      if (kw == 0)
-#pragma unroll
-        for (int d = 0; d < ND; ++d)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) dq[d][r] += jo[32 * d + acc_row(r, half)];
-    }
-  }
-  if (kw != 0 || !exists) return;
-  T* out = (T*)a.dq + (((int64_t)at.b * a.Lq + i) * a.Hq + h) * a.D;
-  const float f = a.scale * up;
-#pragma unroll
-  for (int d = 0; d < ND; ++d)
-#pragma unroll
-    for (int c = 0; c < 4; ++c)
-      if (32 * d + 8 * c + 4 * half < a.D) {
-        if (valid)
-          store4<T>(out + 32 * d + 8 * c + 4 * half, dq[d][4 * c] * f, dq[d][4 * c + 1] * f, dq[d][4 * c + 2] * f,
-                    dq[d][4 * c + 3] * f);
-        else
-          store4<T>(out + 32 * d + 8 * c + 4 * half, 0.f, 0.f, 0.f, 0.f);
-      }
-}
-
-// dk, dv of one key block: RW waves hold 32 keys each, 4 / RW take turns at the 32-query units of
-// the tiles that chose the block (their bits, some at a time) and are joined at the end. Every sum
-// has one order: no atomics on the gradients.
-constexpr int kTiles = 1024;  // tiles listed at a time
-template <typename T, int DP, int RW>
-__global__ __launch_bounds__(NT) void k_attend_dkv(Args a) {
-  using M = Mma<T>;
-  using L = Tile<T, DP>;
-  using Frag = typename M::Frag;
-  constexpr int QW = 4 / RW, NS = DP / 16, ND = DP / 32, NB = kBuffers<T, DP, QW>;
-  constexpr int kAhead = sizeof(T) == 2 && DP <= 64 ? 2 : 1;  // steps whose rows are on their way
-  extern __shared__ __align__(16) char lds[];
-  __shared__ int32_t tiles[kTiles];
-  __shared__ int count;
-  __shared__ __align__(16) float stats[NB][2][QW * 32];  // lse and delta of the staged rows
-  const int item = a.order ? a.order[blockIdx.x] : (int)blockIdx.x;
-  const int blk = item % a.Tk, hk = item / a.Tk % a.Hkv, b = item / a.Tk / a.Hkv;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, col = lane & 31;
-  const int rw = uniform(wave) % RW, qw = uniform(wave) / RW;
-  const int64_t nq = length_of(a.q_lengths, b, a.Lq), nk = length_of(a.kv_lengths, b, a.Lk);
-  const int64_t key = (int64_t)blk * a.block + 32 * rw + col;
-  const bool exists = key < a.Lk, valid = key < nk;
-  const int64_t kr = valid ? key : 0;
-  const T* kp = (const T*)a.k.p + b * a.k.b + kr * a.k.l + hk * a.k.h;
-  const T* vp = (const T*)a.v.p + b * a.v.b + kr * a.v.l + hk * a.v.h;
-  Frag kf[NS], vf[NS];
-#pragma unroll
-  for (int s = 0; s < NS; ++s) {
-    kf[s] = row_frag<T>(kp, 16 * s + 8 * half, a.D, valid);
-    if (a.scale < 0.f) kf[s] = -kf[s];
-    vf[s] = row_frag<T>(vp, 16 * s + 8 * half, a.D, valid);
-  }
-  float down = 1.f, up = 1.f;
-  if constexpr (kFewExponents<T>) ds_scale(*a.gmax, down, up);
-  f32x16 dk[ND] = {}, dv[ND] = {};
-  const int upt = a.G << a.lg, words = (a.Tq + 31) / 32;  // units per tile
-  const uint32_t* bits = a.bits + (((int64_t)b * a.Hkv + hk) * a.Tk + blk) * words;
-  const bool any = (int64_t)blk * a.block < nk;
-  int step = 0;
-  for (int w0 = 0; any && w0 < words; w0 += kTiles / 32) {
-    __syncthreads();
-    if (threadIdx.x < 64) {  // the first 32 lanes hold a word each
-      uint32_t m = lane < 32 && w0 + lane < words ? bits[w0 + lane] : 0u;
-      const uint32_t incl = dsplat::wave_incl_scan(__popc(m), lane);
-      int at = (int)incl - __popc(m);
-      while (m) {
-        tiles[at++] = 32 * (w0 + lane) + __ffs(m) - 1;
-        m &= m - 1;
-      }
-      if (lane == 63) count = (int)incl;
-    }
-    __syncthreads();
-    const int units = uniform(count) * upt;
-    // unit u: 32 rows (part u % (block / 32)) of a head of the group of a listed tile
-    const auto pos = [&](int u) {  // exact: u >> lg < 2^20 and G <= 1024
-      return a.G == 1 ? u >> a.lg : (int)__umulhi((uint32_t)(u >> a.lg), a.group_magic);
-    };
-    // What is on its way: the rows of the units u .. u + QW - 1 and their statistics.
-    struct Ahead {
-      Stage<T, DP, QW> q, g;
-      float lse, delta;
-      int live;
-    };
-    const auto fetch = [&](Ahead& f, int u) {
-      const T *pq[QW], *pg[QW];
-      int tile[QW], have[QW];
-#pragma unroll
-      for (int j = 0; j < QW; ++j) tile[j] = tiles[pos(min(u + j, units - 1))];
-#pragma unroll
-      for (int j = 0; j < QW; ++j) {
-        const int64_t i0 = (int64_t)uniform(tile[j]) * a.block + 32 * ((u + j) & ((1 << a.lg) - 1));
-        const int h = hk * a.G + ((u + j) >> a.lg) - pos(u + j) * a.G;
-        pq[j] = (const T*)a.q.p + b * a.q.b + i0 * a.q.l + h * a.q.h;
-        pg[j] = (const T*)a.g.p + b * a.g.b + i0 * a.g.l + h * a.g.h;
-        have[j] = u + j < units ? (int)max((int64_t)0, min((int64_t)32, nq - i0)) : 0;
-      }
-      f.q.load(pq, have, a.q.l, a.D);
-      f.g.load(pg, have, a.g.l, a.D);
-      if (threadIdx.x < QW * 32) {
-        const int r = threadIdx.x % 32, uj = u + threadIdx.x / 32;
-        f.lse = -INFINITY;
-        if (uj < units) {
-          const int at = pos(uj);
-          const int64_t i = (int64_t)tiles[at] * a.block + 32 * (uj & ((1 << a.lg) - 1)) + r;
-          if (i < nq) {
-            const int64_t stat = ((int64_t)b * a.Hq + hk * a.G + (uj >> a.lg) - at * a.G) * a.Lq + i;
-            f.lse = a.lse[stat];
-            f.delta = a.delta[stat];
-          }
-        }
-      }
-      f.live = pick(have, qw);
-    };
-    const auto turn = [&](Ahead& f, int u) {
-      char* tq = lds + (step % NB) * 2 * QW * L::kUnit;
-      char* tg = tq + QW * L::kUnit;
-      if (NB == 1) __syncthreads();
-      f.q.store(tq);
-      f.g.store(tg);
-      if (threadIdx.x < QW * 32) {
-        // rows that see nothing, or are none: relative to +inf every p is 0
-        stats[step % NB][0][threadIdx.x] = f.lse == -INFINITY ? INFINITY : f.lse;
-        stats[step % NB][1][threadIdx.x] = f.delta;
-      }
-      __syncthreads();
-      const int live = f.live, buffer = step++ % NB;
-      if (u + kAhead * QW < units) fetch(f, u + kAhead * QW);
-      if (live == 0) return;
-      tq += qw * L::kUnit;
-      tg += qw * L::kUnit;
-      f32x16 x = {}, dp = {};
-#pragma unroll
-      for (int s = 0; s < NS; ++s) {
-        x = M::mma(L::row(tq, s, col, half), kf[s], x);
-        dp = M::mma(L::row(tg, s, col, half), vf[s], dp);
-      }
-      // (lanes whose key is none hold columns that are not written)
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const float4 lse = *(const float4*)&stats[buffer][0][qw * 32 + 8 * c + 4 * half];
-        const float4 delta = *(const float4*)&stats[buffer][1][qw * 32 + 8 * c + 4 * half];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int r = 4 * c + e;
-          const float ls = e == 0 ? lse.x : e == 1 ? lse.y : e == 2 ? lse.z : lse.w;
-          const float de = e == 0 ? delta.x : e == 1 ? delta.y : e == 2 ? delta.z : delta.w;
-          x[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[r], a.scale2, -ls));
-          dp[r] = x[r] * (kFewExponents<T> ? (dp[r] - de) * down : dp[r] - de);
-        }
-      }
-      const Frag p0 = acc_frag<T>(x, 0), p1 = acc_frag<T>(x, 1), s0 = acc_frag<T>(dp, 0), s1 = acc_frag<T>(dp, 1);
-#pragma unroll
-      for (int d = 0; d < ND; ++d) {
-        dv[d] = M::mma(L::col(tg, 0, d, lane), p0, dv[d]);
-        dv[d] = M::mma(L::col(tg, 1, d, lane), p1, dv[d]);
-        dk[d] = M::mma(L::col(tq, 0, d, lane), s0, dk[d]);
-        dk[d] = M::mma(L::col(tq, 1, d, lane), s1, dk[d]);
-      }
-    };
-    Ahead f[kAhead] = {};
-#pragma unroll
-    for (int k = 0; k < kAhead; ++k)
-      if (k * QW < units) fetch(f[k], k * QW);
-    for (int u = 0; u < units; u += kAhead * QW)
-#pragma unroll
-      for (int k = 0; k < kAhead; ++k)
-        if (u + k * QW < units) turn(f[k], u + k * QW);
-  }
-  if constexpr (QW > 1) {
-    float* jo = (float*)lds + (rw * 32 + col) * (DP + 1);
-    for (int k = 1; k < QW; ++k)
-#pragma unroll
-      for (int which = 0; which < 2; ++which) {
-        f32x16* acc = which ? dv : dk;
-        __syncthreads();
-        if (qw == k)
-#pragma unroll
-          for (int d = 0; d < ND; ++d)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) jo[32 * d + acc_row(r, half)] = acc[d][r];
-        __syncthreads();
-        if (qw == 0)
-#pragma unroll
-          for (int d = 0; d < ND; ++d)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) acc[d][r] += jo[32 * d + acc_row(r, half)];
-      }
-  }
-  if (qw != 0 || !exists) return;
-  const int64_t off = (((int64_t)b * a.Lk + key) * a.Hkv + hk) * a.D;
-  const float f = a.scale * up;
-#pragma unroll
-  for (int d = 0; d < ND; ++d)
-#pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      const int e = 32 * d + 8 * c + 4 * half;
-      if (e >= a.D) continue;
-      if (valid) {
-        store4<T>((T*)a.dk + off + e, dk[d][4 * c] * f, dk[d][4 * c + 1] * f, dk[d][4 * c + 2] * f, dk[d][4 * c + 3] * f);
-        store4<T>((T*)a.dv + off + e, dv[d][4 * c], dv[d][4 * c + 1], dv[d][4 * c + 2], dv[d][4 * c + 3]);
-      } else {
-        store4<T>((T*)a.dk + off + e, 0.f, 0.f, 0.f, 0.f);
-        store4<T>((T*)a.dv + off + e, 0.f, 0.f, 0.f, 0.f);
-      }
-    }
-}
-
-template <typename K>
-int launch(K kernel, const Args& a, dim3 grid, size_t lds, hipStream_t st, const char* what) {
-  if (lds > 32 * 1024)
-    if (int e = dsplat::ensure_dyn_lds((const void*)kernel, lds, what)) return e;
-  kernel<<<grid, NT, lds, st>>>(a);
-  return dsplat::check_launch(what);
-}
-
-// 32-row waves side by side: as many as the tile's rows fill.
-inline int row_waves(const Args& a) {
-  const int rows = a.Lt * a.G;
-  return rows <= 32 ? 1 : rows <= 64 ? 2 : 4;
-}
-// Parts of the key list: enough workgroups for the chip when there are few tiles.
-inline int splits_of(int64_t workgroups, int units) {
-  int s = 1;
-  while (workgroups * s < 512 && s * 8 < units) s *= 2;
-  return s;
-}
-
-template <typename T, int DP, int RW>
-struct Fwd {
-  static int go(const Args& a, dim3 grid, hipStream_t st) {
-    return launch(k_attend_fwd<T, DP, RW>, a, grid, kTileBytes<T, DP, 4 / RW> + a.top * sizeof(int32_t), st, "k_attend_fwd");
-  }
-};
-template <typename T, int DP, int RW>
-struct Dq {
-  static int go(const Args& a, dim3 grid, hipStream_t st) {
-    return launch(k_attend_dq<T, DP, RW>, a, grid, kTileBytes<T, DP, 4 / RW> + a.top * sizeof(int32_t), st, "k_attend_dq");
-  }
-};
-template <typename T, int DP, int RW>
-struct Dkv {
-  static int go(const Args& a, dim3 grid, hipStream_t st) {
-    return launch(k_attend_dkv<T, DP, RW>, a, grid, kTileBytes<T, DP, 4 / RW>, st, "k_attend_dkv");
-  }
-};
-template <template <typename, int, int> class F, typename T, int DP>
-int by_waves(int rw, const Args& a, dim3 grid, hipStream_t st) {
-  return rw == 1 ? F<T, DP, 1>::go(a, grid, st) : rw == 2 ? F<T, DP, 2>::go(a, grid, st) : F<T, DP, 4>::go(a, grid, st);
-}
-template <template <typename, int, int> class F, typename T>
-int by_width(int rw, const Args& a, dim3 grid, hipStream_t st) {
-  if (a.D <= 32) return by_waves<F, T, 32>(rw, a, grid, st);
-  if (a.D <= 64) return by_waves<F, T, 64>(rw, a, grid, st);
-  if (a.D <= 96) return by_waves<F, T, 96>(rw, a, grid, st);
-  return by_waves<F, T, 128>(rw, a, grid, st);
-}
-template <template <typename, int, int> class F>
-int by_type(int dtype, int rw, const Args& a, dim3 grid, hipStream_t st) {
-  if (dtype == DTK_F32) return by_width<F, float>(rw, a, grid, st);
-  if (dtype == DTK_BF16) return by_width<F, bf16>(rw, a, grid, st);
-  return by_width<F, f16>(rw, a, grid, st);
+template <typename F>
+F* by_type(int dtype, F* f32, F* b16, F* h16) {
+  return dtype == DTK_F32 ? f32 : dtype == DTK_BF16 ? b16 : h16;
 }
 
 int check(const dtk_attention* c, const char* who) {
@@ -1008,7 +172,7 @@ int dtk_block_sparse_attention_fwd(const dtk_attention* c, void* workspace, void
     a.part_l = a.part_m + a.splits * rows;
   }
   const dim3 grid(a.Tq * a.rowtiles, a.Hkv, c->B * a.splits);
-  if (int e = by_type<Fwd>(c->dtype, row_waves(a), a, grid, st)) return e;
+  if (int e = by_type(c->dtype, attend_fwd<float>, attend_fwd<bf16>, attend_fwd<f16>)(a, row_waves(a), grid, st)) return e;
   if (a.splits == 1) return 0;
   const unsigned blocks = (unsigned)((rows * (a.D / 4) + NT - 1) / NT);
   if (c->dtype == DTK_F32) k_attend_join<float><<<blocks, NT, 0, st>>>(a, rows);
@@ -1052,7 +216,7 @@ int dtk_block_sparse_attention_bwd(const dtk_attention* c, const void* dout, con
   if (int e = dsplat::zero_async(a.gmax, l.order - l.gmax, st, "dtk_block_sparse_attention_bwd")) return e;
   if (c->Lq) {
     const dim3 grid(a.Tq * a.rowtiles, a.Hkv, c->B);
-    if (int e = by_type<Dq>(c->dtype, row_waves(a), a, grid, st)) return e;
+    if (int e = by_type(c->dtype, attend_dq<float>, attend_dq<bf16>, attend_dq<f16>)(a, row_waves(a), grid, st)) return e;
     if (a.Tk) {
       k_attend_mark<<<dim3(a.Tq, a.Hkv, c->B), NT, 0, st>>>(a);
       if (int e = dsplat::check_launch("k_attend_mark")) return e;
@@ -1063,7 +227,7 @@ int dtk_block_sparse_attention_bwd(const dtk_attention* c, const void* dout, con
     k_attend_order<<<1, kOrderThreads, 0, st>>>(a, (int)l.items);
     if (int e = dsplat::check_launch("k_attend_order")) return e;
   }
-  return by_type<Dkv>(c->dtype, a.block / 32, a, dim3((unsigned)l.items), st);
+  return by_type(c->dtype, attend_dkv<float>, attend_dkv<bf16>, attend_dkv<f16>)(a, a.block / 32, dim3((unsigned)l.items), st);
 }
 
 }  // extern "C"

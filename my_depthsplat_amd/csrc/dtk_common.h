@@ -32,7 +32,8 @@ __device__ __forceinline__ void store_vec(T* p, const Vec<T>& r) {
 
 // Philox4x32-10 (Salmon, Moraes, Dror, Shaw: "Parallel random numbers: as easy as 1, 2, 3",
 // SC 2011): ten rounds of two 32 x 32 -> 64 bit products of the counter, keyed. Counter: the
-// group's 64-bit number, the call's id, the step; key: the 64-bit seed.
+// group's 64-bit number, the call's id, the step; key: the 64-bit seed. A round is two v_mad_u64_u32 (8 cycles a
+// wave; separate upper and lower halves take half as long again) and two three-way exclusive ors.
 struct RngKey {
   uint32_t k0, k1, call, step;
 };
@@ -46,9 +47,9 @@ __device__ __forceinline__ void philox(const RngKey& key, uint64_t group, uint32
 #pragma unroll
   for (int r = 0; r < 10; ++r) {
     const uint64_t a = (uint64_t)0xD2511F53u * c0, b = (uint64_t)0xCD9E8D57u * c2;
-    c0 = (uint32_t)(b >> 32) ^ c1 ^ k0;
+    c0 = __builtin_amdgcn_bitop3_b32((uint32_t)(b >> 32), c1, k0, 0x96);  // the three's exclusive or
     c1 = (uint32_t)b;
-    c2 = (uint32_t)(a >> 32) ^ c3 ^ k1;
+    c2 = __builtin_amdgcn_bitop3_b32((uint32_t)(a >> 32), c3, k1, 0x96);
     c3 = (uint32_t)a;
     k0 += 0x9E3779B9u;
     k1 += 0xBB67AE85u;
@@ -58,38 +59,18 @@ __device__ __forceinline__ void philox(const RngKey& key, uint64_t group, uint32
   w[2] = c2;
   w[3] = c3;
 }
-// keep[e] of the N elements n0 .. n0 + N - 1 (N a multiple of 4): element n takes word n % 4 of
-// group n / 4. A start inside a group costs one more group and a shift by selects.
+// keep[e] of the N elements from n0 on (both multiples of 4): element n takes word n % 4 of group n / 4, and
+// is kept if that is above `least`.
 template <int N>
-__device__ __forceinline__ void keep_mask(const RngKey& key, uint64_t n0, uint64_t threshold, bool (&keep)[N]) {
-  constexpr int G = N / 4;
-  const uint64_t g0 = n0 >> 2;
-  const uint32_t sh = (uint32_t)n0 & 3u;
-  uint32_t w[4 * G + 4];
+__device__ __forceinline__ void keep_mask(const RngKey& key, uint64_t n0, uint32_t least, bool (&keep)[N]) {
 #pragma unroll
-  for (int g = 0; g < G; ++g) {
-    uint32_t t[4];
-    philox(key, g0 + g, t);
+  for (int g = 0; g < N / 4; ++g) {
+    uint32_t w[4];
+    philox(key, (n0 >> 2) + g, w);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) w[4 * g + i] = t[i];
+    for (int i = 0; i < 4; ++i) keep[4 * g + i] = w[i] > least;
   }
-  if (sh) {
-    uint32_t t[4];
-    philox(key, g0 + G, t);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) w[4 * G + i] = t[i];
-#pragma unroll
-    for (int i = 0; i < 4 * G + 3; ++i) w[i] = (sh & 1) ? w[i + 1] : w[i];
-#pragma unroll
-    for (int i = 0; i < 4 * G + 1; ++i) w[i] = (sh & 2) ? w[i + 2] : w[i];
-  }
-#pragma unroll
-  for (int e = 0; e < N; ++e) keep[e] = w[e] >= threshold;  // 64-bit: a threshold of 2^32 keeps nothing
 }
-
-// p in [0, 1] -> the words that are kept are >= threshold; 1 / (1 - p), 0 for p = 1.
-inline uint64_t drop_threshold(double p) { return (uint64_t)__builtin_llrint(p * 4294967296.0); }
-inline float drop_scale(double p) { return p < 1.0 ? (float)(1.0 / (1.0 - p)) : 0.f; }
 
 inline bool type_ok(int t) { return t >= DTK_F32 && t <= DTK_F16; }
 inline size_t type_size(int t) { return t == DTK_F32 ? 4 : 2; }

@@ -1,0 +1,7 @@
+// The layer norm's kernels for bf16 rows.
+#include "dtk_norm.h"
+
+namespace dtk {
+template void run_fwd<bf16>(const FwdArgs&, const Shape&, hipStream_t);
+template void run_bwd<bf16>(const BwdArgs&, int, const Shape&, bool, hipStream_t);
+}  // namespace dtk
