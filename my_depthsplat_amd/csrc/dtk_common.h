@@ -30,6 +30,14 @@ __device__ __forceinline__ void store_vec(T* p, const Vec<T>& r) {
   __builtin_memcpy(p, &r, 16);
 }
 
+// The 32-bit value rounded to T. Without the empty statement a last f32 operation and f16's rounding become one
+// instruction that rounds once, in some kernels and not in others; the plain and the fused norm give the same bits.
+template <typename T>
+__device__ __forceinline__ T rounded(float f) {
+  if constexpr (__is_same(T, f16)) asm("" : "+v"(f));
+  return (T)f;
+}
+
 // Philox4x32-10 (Salmon, Moraes, Dror, Shaw: "Parallel random numbers: as easy as 1, 2, 3",
 // SC 2011): ten rounds of two 32 x 32 -> 64 bit products of the counter, keyed. Counter: the
 // group's 64-bit number, the call's id, the step; key: the 64-bit seed. A round is two v_mad_u64_u32 (8 cycles a
@@ -70,6 +78,29 @@ __device__ __forceinline__ void keep_mask(const RngKey& key, uint64_t n0, uint32
 #pragma unroll
     for (int i = 0; i < 4; ++i) keep[4 * g + i] = w[i] > least;
   }
+}
+
+// The same from any element on: one group more where n0 lies inside one, and the bits shifted by its place.
+template <int N>
+__device__ __forceinline__ void keep_mask_anywhere(const RngKey& key, uint64_t n0, uint32_t least, bool (&keep)[N]) {
+  const uint32_t sh = (uint32_t)n0 & 3u;
+  uint32_t bits = 0;
+#pragma unroll
+  for (int g = 0; g < N / 4; ++g) {
+    uint32_t w[4];
+    philox(key, (n0 >> 2) + g, w);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) bits |= w[i] > least ? 1u << (4 * g + i) : 0u;
+  }
+  if (sh) {
+    uint32_t w[4];
+    philox(key, (n0 >> 2) + N / 4, w);
+#pragma unroll
+    for (int i = 0; i < 3; ++i) bits |= w[i] > least ? 1u << (N + i) : 0u;
+  }
+  bits >>= sh;
+#pragma unroll
+  for (int e = 0; e < N; ++e) keep[e] = (bits >> e) & 1u;
 }
 
 inline bool type_ok(int t) { return t >= DTK_F32 && t <= DTK_F16; }

@@ -61,70 +61,82 @@ __device__ __forceinline__ float row_sum(float v, float* red) {
   return v;
 }
 
-// LPR lanes share a row, each holds NI vectors of N elements (16 bytes); vector i of a lane is
-// number lane + i LPR. The vectors lie on multiples of N of the whole array, not of the row: a row whose width
-// N does not divide (ODD) begins and ends inside one. So every load and whole store is an
-// aligned vector and every vector is made of whole groups of the generator, at any width; the elements of
-// the neighbour rows are read and left out.
-template <int N, bool ODD>
+// LPR lanes share a row, each holds NI vectors of N elements (16 bytes); vector i of a lane is number lane +
+// i LPR of the row. How the row's width meets the vectors: kWhole: N divides it; kRagged: the last vector ends with the
+// row, so its first `lo` elements are the one before's too: left out of the sums, and stored twice with the same value;
+// kTiny: the row is shorter than a vector. (Vectors on multiples of N of the whole array instead, which
+// read aligned and need a third less of the generator, lose more at the rows' partial stores: 1001 f16, fused forward 55
+// us against 48.)
+enum Fit { kWhole, kRagged, kTiny };
+template <int N, Fit FIT>
 struct Cols {
-  int c0, lo, hi;  // the vector's first column (may be negative); its elements lo .. hi - 1 are the row's
-  __device__ __forceinline__ Cols(int vec, int shift, int width)
-      : c0(vec * N - (ODD ? shift : 0)), lo(ODD ? max(0, -c0) : 0), hi(ODD ? min(N, width - c0) : (c0 < width ? N : 0)) {}
-  __device__ __forceinline__ bool live() const { return hi > lo; }
-  __device__ __forceinline__ bool mine(int e) const { return !ODD || (e >= lo && e < hi); }
+  int c0, lo, width;
+  bool live;
+  __device__ __forceinline__ Cols(int vec, int width)
+      : c0(FIT == kRagged ? min(vec * N, width - N) : vec * N), lo(vec * N - c0), width(width), live(vec * N < width) {}
+  __device__ __forceinline__ bool there(int e) const { return FIT != kTiny || e < width; }  // the row has this element
+  __device__ __forceinline__ bool first(int e) const { return FIT == kWhole || (e >= lo && there(e)); }  // and it is this vector's
+  // the sum over the elements that are this vector's
+  template <typename F>
+  __device__ __forceinline__ float sum(F value) const {
+    float t = 0.f;
+    if (FIT == kWhole || (FIT == kRagged && lo == 0)) {
+#pragma unroll
+      for (int e = 0; e < N; ++e) t += value(e);
+    } else {
+#pragma unroll
+      for (int e = 0; e < N; ++e) t += first(e) ? value(e) : 0.f;
+    }
+    return live ? t : 0.f;
+  }
 };
-template <int N, bool ODD>
-__device__ __forceinline__ int shift_of(int64_t row, int width) {
-  return ODD ? (int)((row * width) & (N - 1)) : 0;
-}
-
-// n0: the vector's first element in the array of `total`
-template <typename T, int N, bool ODD>
-__device__ __forceinline__ Vec<T> load_row(const T* p, int64_t n0, int64_t total) {
-  if (!ODD || n0 + N <= total) return load_vec(p + n0);
-  Vec<T> v = {};  // the last row's last vector
+template <typename T, int N, Fit FIT>
+__device__ __forceinline__ Vec<T> load_row(const T* row, const Cols<N, FIT>& c) {
+  Vec<T> v = {};
+  if (!c.live) return v;
+  if constexpr (FIT != kTiny) return load_vec(row + c.c0);
 #pragma unroll
   for (int e = 0; e < N; ++e)
-    if (n0 + e < total) v.v[e] = p[n0 + e];
+    if (c.there(e)) v.v[e] = row[e];
   return v;
 }
-template <typename T, int N, bool ODD>
-__device__ __forceinline__ void store_row(T* p, int64_t n0, const Cols<N, ODD>& c, const float (&f)[N]) {
+template <typename T, int N, Fit FIT>
+__device__ __forceinline__ void store_row(T* row, const Cols<N, FIT>& c, const float (&f)[N]) {
   Vec<T> v;
 #pragma unroll
-  for (int e = 0; e < N; ++e) v.v[e] = (T)f[e];
-  if (!ODD || (c.lo == 0 && c.hi == N)) {
-    store_vec(p + n0, v);
+  for (int e = 0; e < N; ++e) v.v[e] = rounded<T>(f[e]);
+  if (!c.live) return;
+  if constexpr (FIT != kTiny) {
+    store_vec(row + c.c0, v);
   } else {
 #pragma unroll
     for (int e = 0; e < N; ++e)
-      if (c.mine(e)) p[n0 + e] = v.v[e];
+      if (c.there(e)) row[e] = v.v[e];
   }
 }
-template <typename T, int N, bool ODD>
-__device__ __forceinline__ void load_w(const void* p, bool f32, const Cols<N, ODD>& c, float none, float (&f)[N]) {
+template <typename T, int N, Fit FIT>
+__device__ __forceinline__ void load_w(const void* p, bool f32, const Cols<N, FIT>& c, float none, float (&f)[N]) {
 #pragma unroll
   for (int e = 0; e < N; ++e) f[e] = none;
-  if (!p) return;
-  if (!ODD || (c.lo == 0 && c.hi == N)) {
-    if (sizeof(T) == 4 || !f32) {
-      const Vec<T> v = load_vec((const T*)p + c.c0);
+  if (!p || !c.live) return;
+  if (sizeof(T) == 4 || !f32) {
+    const Vec<T> v = load_row<T, N, FIT>((const T*)p, c);
 #pragma unroll
-      for (int e = 0; e < N; ++e) f[e] = (float)v.v[e];
-    } else {
-      const Vec<float> v0 = load_vec((const float*)p + c.c0), v1 = load_vec((const float*)p + c.c0 + N / 2);
-#pragma unroll
-      for (int e = 0; e < N / 2; ++e) {
-        f[e] = v0.v[e];
-        f[e + N / 2] = v1.v[e];
-      }
-    }
+    for (int e = 0; e < N; ++e) f[e] = (float)v.v[e];
   } else {
 #pragma unroll
     for (int e = 0; e < N; ++e)
-      if (c.mine(e)) f[e] = f32 ? ((const float*)p)[c.c0 + e] : (float)((const T*)p)[c.c0 + e];
+      if (c.there(e)) f[e] = ((const float*)p)[c.c0 + e];
   }
+}
+template <int N, Fit FIT>
+__device__ __forceinline__ void drop_row(const Drop& drop, const RngKey& key, uint64_t n0, float (&f)[N]) {
+  if (!drop.rng) return;
+  bool keep[N];
+  if constexpr (FIT == kWhole) keep_mask<N>(key, n0, drop.least, keep);
+  else keep_mask_anywhere<N>(key, n0, drop.least, keep);
+#pragma unroll
+  for (int e = 0; e < N; ++e) f[e] = keep[e] ? f[e] * drop.scale : 0.f;
 }
 
 struct FwdArgs {
@@ -138,75 +150,85 @@ struct FwdArgs {
   float *mean, *rstd;
 };
 
-template <typename T, int NI, int LPR, bool ADD, bool ODD>
-__global__ __launch_bounds__(kThreads) void k_norm_fwd(FwdArgs a) {
+// Waves per SIMD that the registers of NI vectors leave room for (all: the fused backward, which holds a third
+// gradient and the generator's words; at 3 waves it would spill: 77 us against 55 for 20001 x 1001 f16).
+constexpr int waves_of(int ni, bool all) { return ni <= 1 ? 4 : ni > 2 ? 1 : all ? 2 : 3; }
+
+// A group of LPR lanes walks rows with the stride of the grid; the next row is on its way while one is worked on,
+// the weights stay in registers.
+template <typename T, int NI, int LPR, bool ADD, Fit FIT>
+__global__ __launch_bounds__(kThreads, waves_of(NI, false)) void k_norm_fwd(FwdArgs a) {
   constexpr int N = Vec<T>::N, RPB = kThreads / LPR;
+  using C = Cols<N, FIT>;
   __shared__ float red[kThreads / 64];
   const T *x = (const T*)a.x, *residual = (const T*)a.residual;
   const int lane = threadIdx.x % LPR, width = a.width;
-  const int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / LPR, total = a.rows * width;
-  if (LPR <= 64 && row >= a.rows) return;  // whole groups of lanes
-  const int shift = shift_of<N, ODD>(row, width);
+  const int64_t step = (int64_t)gridDim.x * RPB;
+  int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / LPR;
   const float inv = 1.f / (float)width;
-  float z[NI][N];
-  float sum = 0.f;
   RngKey key = {};
   if (ADD && a.drop.rng) key = rng_key(a.drop.rng, a.drop.call);
+  struct Row {
+    Vec<T> x[NI], r[ADD ? NI : 1];
+  };
+  const auto fetch = [&](Row& f, int64_t row) {
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      const C c(lane + i * LPR, width);
+      f.x[i] = load_row<T, N, FIT>(x + row * width, c);
+      if (ADD) f.r[i] = load_row<T, N, FIT>(residual + row * width, c);
+    }
+  };
+  Row next;
+  if (row < a.rows) fetch(next, row);
+  float w[NI][N], b[NI][N];
 #pragma unroll
   for (int i = 0; i < NI; ++i) {
-    const Cols<N, ODD> c(lane + i * LPR, shift, width);
-    const int64_t n0 = row * width + c.c0;
+    const C c(lane + i * LPR, width);
+    load_w<T, N, FIT>(a.wb.w, a.wb.f32, c, 1.f, w[i]);
+    load_w<T, N, FIT>(a.wb.b, a.wb.f32, c, 0.f, b[i]);
+  }
+  while (row < a.rows) {
+    const Row cur = next;
+    const int64_t at = row;
+    row += step;
+    if (row < a.rows) fetch(next, row);
+    float z[NI][N];
+    float sum = 0.f;
 #pragma unroll
-    for (int e = 0; e < N; ++e) z[i][e] = 0.f;
-    if (!c.live()) continue;
-    const Vec<T> v = load_row<T, N, ODD>(x, n0, total);
-    if constexpr (ADD) {
-      const Vec<T> r = load_row<T, N, ODD>(residual, n0, total);
-      bool keep[N];
-      if (a.drop.rng) keep_mask<N>(key, (uint64_t)n0, a.drop.least, keep);
+    for (int i = 0; i < NI; ++i) {
+      const C c(lane + i * LPR, width);
 #pragma unroll
-      for (int e = 0; e < N; ++e) {
-        float d = (float)v.v[e];
-        if (a.drop.rng) d = keep[e] ? d * a.drop.scale : 0.f;
-        z[i][e] = (float)(T)(d + (float)r.v[e]);
+      for (int e = 0; e < N; ++e) z[i][e] = (float)cur.x[i].v[e];
+      if constexpr (ADD) {
+        drop_row<N, FIT>(a.drop, key, (uint64_t)(at * width + c.c0), z[i]);
+#pragma unroll
+        for (int e = 0; e < N; ++e) z[i][e] = (float)rounded<T>(z[i][e] + (float)cur.r[i].v[e]);
+        store_row<T, N, FIT>((T*)a.s + at * width, c, z[i]);
       }
-      store_row<T, N, ODD>((T*)a.s, n0, c, z[i]);
-    } else {
+      sum += c.sum([&](int e) { return z[i][e]; });
+    }
+    const float mu = row_sum<LPR>(sum, red) * inv;
+    float sq = 0.f;
 #pragma unroll
-      for (int e = 0; e < N; ++e) z[i][e] = (float)v.v[e];
+    for (int i = 0; i < NI; ++i) {
+      const C c(lane + i * LPR, width);
+#pragma unroll
+      for (int e = 0; e < N; ++e) z[i][e] -= mu;
+      sq += c.sum([&](int e) { return z[i][e] * z[i][e]; });
+    }
+    const float r = 1.f / sqrtf(row_sum<LPR>(sq, red) * inv + a.eps);
+    if (lane == 0 && a.mean) {
+      a.mean[at] = mu;
+      a.rstd[at] = r;
     }
 #pragma unroll
-    for (int e = 0; e < N; ++e) {
-      z[i][e] = c.mine(e) ? z[i][e] : 0.f;
-      sum += z[i][e];
+    for (int i = 0; i < NI; ++i) {
+      float o[N];
+#pragma unroll
+      for (int e = 0; e < N; ++e) o[e] = __builtin_fmaf(z[i][e] * r, w[i][e], b[i][e]);
+      store_row<T, N, FIT>((T*)a.y + at * width, C(lane + i * LPR, width), o);
     }
-  }
-  const float mu = row_sum<LPR>(sum, red) * inv;
-  float sq = 0.f;
-#pragma unroll
-  for (int i = 0; i < NI; ++i) {
-    const Cols<N, ODD> c(lane + i * LPR, shift, width);
-#pragma unroll
-    for (int e = 0; e < N; ++e) {
-      z[i][e] -= mu;
-      sq += c.live() && c.mine(e) ? z[i][e] * z[i][e] : 0.f;
-    }
-  }
-  const float r = 1.f / sqrtf(row_sum<LPR>(sq, red) * inv + a.eps);
-  if (lane == 0 && a.mean) {
-    a.mean[row] = mu;
-    a.rstd[row] = r;
-  }
-#pragma unroll
-  for (int i = 0; i < NI; ++i) {
-    const Cols<N, ODD> c(lane + i * LPR, shift, width);
-    if (!c.live()) continue;
-    float w[N], b[N], o[N];
-    load_w<T, N, ODD>(a.wb.w, a.wb.f32, c, 1.f, w);
-    load_w<T, N, ODD>(a.wb.b, a.wb.f32, c, 0.f, b);
-#pragma unroll
-    for (int e = 0; e < N; ++e) o[e] = z[i][e] * r * w[e] + b[e];
-    store_row<T, N, ODD>((T*)a.y, row * width + c.c0, c, o);
   }
 }
 
@@ -221,27 +243,25 @@ struct BwdArgs {
   float* part;  // [2, gridDim, width]: the workgroups' sums of dy xh and of dy
 };
 
-// Backward: a group of LPR lanes walks rows with the stride of the grid and keeps its columns' sums
-// of dy xh and dy in registers; the next row is on its way while one is worked on. (ODD: the stride is a multiple
-// of N rows, so the columns of a lane stay the same.) The groups of a workgroup are folded through LDS in
-// turn into one row of `part`, which k_norm_fold sums in a fixed order: no atomics, the same bits every time.
-template <typename T, int NI, int LPR, bool ADD, bool ODD>
-__global__ __launch_bounds__(kThreads) void k_norm_bwd(BwdArgs a) {
+// Backward: the same walk; a lane keeps its columns' sums of dy xh and dy in registers. The groups of a workgroup are
+// folded through LDS in turn into one row of `part`, which k_norm_fold sums in a fixed order: no atomics,
+// the same bits every time.
+template <typename T, int NI, int LPR, bool ADD, Fit FIT>
+__global__ __launch_bounds__(kThreads, waves_of(NI, ADD)) void k_norm_bwd(BwdArgs a) {
   constexpr int N = Vec<T>::N, RPB = kThreads / LPR;
-  constexpr int kFold = LPR <= 64 ? (NI * LPR + 1) * N : 1;  // columns of a row
+  using C = Cols<N, FIT>;
   __shared__ float red[kThreads / 64];
-  __shared__ float fold[2][kFold];
+  __shared__ float fold[2][LPR <= 64 ? NI * LPR * N : 1];
   const T *z = (const T*)a.z, *dy = (const T*)a.dy, *ds = (const T*)a.ds;
   const int lane = threadIdx.x % LPR, group = threadIdx.x / LPR, width = a.width;
-  const int64_t total = a.rows * width, step = (int64_t)gridDim.x * RPB;
+  const int64_t step = (int64_t)gridDim.x * RPB;
   int64_t row = (int64_t)blockIdx.x * RPB + group;
-  const int shift = shift_of<N, ODD>(row, width);
   const float inv = 1.f / (float)width;
   float dw[NI][N] = {}, db[NI][N] = {};
   RngKey key = {};
   if (ADD && a.drop.rng) key = rng_key(a.drop.rng, a.drop.call);
   struct Row {
-    Vec<T> z[NI], dy[NI], ds[ADD ? NI : 1];
+    Vec<T> z[NI], dy[NI];
     float mu, r;
   };
   const auto fetch = [&](Row& f, int64_t row) {
@@ -249,64 +269,59 @@ __global__ __launch_bounds__(kThreads) void k_norm_bwd(BwdArgs a) {
     f.r = a.rstd[row];
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
-      const Cols<N, ODD> c(lane + i * LPR, shift, width);
-      const int64_t n0 = row * width + c.c0;
-      f.z[i] = f.dy[i] = Vec<T>{};
-      if (ADD) f.ds[i] = Vec<T>{};
-      if (!c.live()) continue;
-      f.z[i] = load_row<T, N, ODD>(z, n0, total);
-      if (dy) f.dy[i] = load_row<T, N, ODD>(dy, n0, total);
-      if (ADD && ds) f.ds[i] = load_row<T, N, ODD>(ds, n0, total);
+      const C c(lane + i * LPR, width);
+      f.z[i] = load_row<T, N, FIT>(z + row * width, c);
+      f.dy[i] = dy ? load_row<T, N, FIT>(dy + row * width, c) : Vec<T>{};
     }
   };
   Row next;
   if (row < a.rows) fetch(next, row);
+  float w[NI][N];
+#pragma unroll
+  for (int i = 0; i < NI; ++i) load_w<T, N, FIT>(a.wb.w, a.wb.f32, C(lane + i * LPR, width), 1.f, w[i]);
   while (row < a.rows) {
     const Row cur = next;
     const int64_t at = row;
     row += step;
+    Vec<T> add[ADD ? NI : 1];
+    if constexpr (ADD) {
+#pragma unroll
+      for (int i = 0; i < NI; ++i)
+        add[i] = ds ? load_row<T, N, FIT>(ds + at * width, C(lane + i * LPR, width)) : Vec<T>{};
+    }
     if (row < a.rows) fetch(next, row);
     float xh[NI][N], g[NI][N];
     float s1 = 0.f, s2 = 0.f;
+    const float shift = -cur.mu * cur.r;
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
-      const Cols<N, ODD> c(lane + i * LPR, shift, width);
-      float w[N];
-      if (c.live()) load_w<T, N, ODD>(a.wb.w, a.wb.f32, c, 1.f, w);
+      const C c(lane + i * LPR, width);
 #pragma unroll
       for (int e = 0; e < N; ++e) {
-        const bool on = c.live() && c.mine(e);
-        xh[i][e] = on ? ((float)cur.z[i].v[e] - cur.mu) * cur.r : 0.f;
-        const float d = on ? (float)cur.dy[i].v[e] : 0.f;
-        dw[i][e] += d * xh[i][e];
+        xh[i][e] = __builtin_fmaf((float)cur.z[i].v[e], cur.r, shift);
+        const float d = (float)cur.dy[i].v[e];
+        dw[i][e] = __builtin_fmaf(d, xh[i][e], dw[i][e]);
         db[i][e] += d;
-        g[i][e] = on ? d * w[e] : 0.f;
-        s1 += g[i][e];
-        s2 += g[i][e] * xh[i][e];
+        g[i][e] = d * w[i][e];
       }
+      s1 += c.sum([&](int e) { return g[i][e]; });
+      s2 += c.sum([&](int e) { return g[i][e] * xh[i][e]; });
     }
     s1 = row_sum<LPR>(s1, red) * inv;
     s2 = row_sum<LPR>(s2, red) * inv;
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
-      const Cols<N, ODD> c(lane + i * LPR, shift, width);
-      if (!c.live()) continue;
-      const int64_t n0 = at * width + c.c0;
+      const C c(lane + i * LPR, width);
       float o[N];
 #pragma unroll
-      for (int e = 0; e < N; ++e) o[e] = cur.r * (g[i][e] - s1 - xh[i][e] * s2);
+      for (int e = 0; e < N; ++e) o[e] = cur.r * __builtin_fmaf(-xh[i][e], s2, g[i][e] - s1);
       if constexpr (ADD) {
 #pragma unroll
-        for (int e = 0; e < N; ++e) o[e] += ds ? (float)cur.ds[i].v[e] : 0.f;
-        if (a.dres) store_row<T, N, ODD>((T*)a.dres, n0, c, o);
-        if (a.dx && a.drop.rng) {
-          bool keep[N];
-          keep_mask<N>(key, (uint64_t)n0, a.drop.least, keep);
-#pragma unroll
-          for (int e = 0; e < N; ++e) o[e] = keep[e] ? o[e] * a.drop.scale : 0.f;
-        }
+        for (int e = 0; e < N; ++e) o[e] += (float)add[i].v[e];
+        if (a.dres) store_row<T, N, FIT>((T*)a.dres + at * width, c, o);
+        if (a.dx) drop_row<N, FIT>(a.drop, key, (uint64_t)(at * width + c.c0), o);
       }
-      if (a.dx) store_row<T, N, ODD>((T*)a.dx, n0, c, o);
+      if (a.dx) store_row<T, N, FIT>((T*)a.dx + at * width, c, o);
     }
   }
   if (!a.part) return;
@@ -315,10 +330,10 @@ __global__ __launch_bounds__(kThreads) void k_norm_bwd(BwdArgs a) {
   if constexpr (LPR > 64) {
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
-      const Cols<N, ODD> c(lane + i * LPR, shift, width);
+      const C c(lane + i * LPR, width);
 #pragma unroll
       for (int e = 0; e < N; ++e)
-        if (c.live() && c.mine(e)) {
+        if (c.live && c.first(e)) {
           pw[c.c0 + e] = dw[i][e];
           pb[c.c0 + e] = db[i][e];
         }
@@ -329,10 +344,10 @@ __global__ __launch_bounds__(kThreads) void k_norm_bwd(BwdArgs a) {
       if (group != gq) continue;
 #pragma unroll
       for (int i = 0; i < NI; ++i) {
-        const Cols<N, ODD> c(lane + i * LPR, shift, width);
+        const C c(lane + i * LPR, width);
 #pragma unroll
         for (int e = 0; e < N; ++e)
-          if (c.live() && c.mine(e)) {
+          if (c.live && c.first(e)) {
             fold[0][c.c0 + e] = (gq ? fold[0][c.c0 + e] : 0.f) + dw[i][e];
             fold[1][c.c0 + e] = (gq ? fold[1][c.c0 + e] : 0.f) + db[i][e];
           }
@@ -373,7 +388,7 @@ __global__ __launch_bounds__(kThreads) void k_norm_fwd_wide(FwdArgs a) {
     float v = (float)x[c];
     if constexpr (ADD) {
       if (a.drop.rng) v = keep_one(a.drop, key, (uint64_t)row * width + c) ? v * a.drop.scale : 0.f;
-      v = (float)(T)(v + (float)residual[c]);
+      v = (float)rounded<T>(v + (float)residual[c]);
       s[c] = (T)v;
     }
     sum += v;
@@ -390,8 +405,8 @@ __global__ __launch_bounds__(kThreads) void k_norm_fwd_wide(FwdArgs a) {
     a.rstd[row] = r;
   }
   for (int c = threadIdx.x; c < width; c += kThreads)
-    ((T*)a.y)[row * width + c] = (T)(((float)z[c] - mu) * r * weight_at<T>(a.wb.w, a.wb.f32, c, 1.f) +
-                                     weight_at<T>(a.wb.b, a.wb.f32, c, 0.f));
+    ((T*)a.y)[row * width + c] = rounded<T>(__builtin_fmaf(((float)z[c] - mu) * r, weight_at<T>(a.wb.w, a.wb.f32, c, 1.f),
+                                                          weight_at<T>(a.wb.b, a.wb.f32, c, 0.f)));
 }
 template <typename T, bool ADD>
 __global__ __launch_bounds__(kThreads) void k_norm_bwd_wide(BwdArgs a) {
@@ -419,10 +434,10 @@ __global__ __launch_bounds__(kThreads) void k_norm_bwd_wide(BwdArgs a) {
       float g = r * (d * weight_at<T>(a.wb.w, a.wb.f32, c, 1.f) - s1 - xh * s2);
       if constexpr (ADD) {
         if (ds) g += (float)ds[row * width + c];
-        if (a.dres) ((T*)a.dres)[row * width + c] = (T)g;
+        if (a.dres) ((T*)a.dres)[row * width + c] = rounded<T>(g);
         if (a.dx && a.drop.rng) g = keep_one(a.drop, key, (uint64_t)row * width + c) ? g * a.drop.scale : 0.f;
       }
-      if (a.dx) ((T*)a.dx)[row * width + c] = (T)g;
+      if (a.dx) ((T*)a.dx)[row * width + c] = rounded<T>(g);
       if (a.part) {  // each thread owns its columns of the workgroup's partial row
         float* pw = a.part + (int64_t)blockIdx.x * width + c;
         float* pb = a.part + ((int64_t)gridDim.x + blockIdx.x) * width + c;
@@ -434,41 +449,44 @@ __global__ __launch_bounds__(kThreads) void k_norm_bwd_wide(BwdArgs a) {
 }
 
 // The registers' layout of a row: LPR lanes x NI vectors. Up to 32 vectors the smallest group that holds
-// the row, so narrow rows share a wave; up to 256 one wave; up to 2048 the workgroup; wider rows are
+// the row, so narrow rows share a wave; up to 128 one wave; up to 1024 the workgroup; wider rows are
 // walked (lpr 0).
 struct Shape {
   int lpr, ni;
-  bool odd;
+  Fit fit;
 };
 inline Shape shape_of(int width, int dtype) {
-  const int n = dtype == DTK_F32 ? 4 : 8;
-  const bool odd = width % n != 0;
-  const int vecs = odd ? (width + 2 * n - 2) / n : width / n;  // odd: whatever the row's place in its first vector
-  if (vecs <= 8) return {8, 1, odd};
-  if (vecs <= 16) return {16, 1, odd};
-  if (vecs <= 32) return {32, 1, odd};
-  if (vecs <= 256) return {64, (vecs + 63) / 64, odd};
-  if (vecs <= 1024) return {256, (vecs + 255) / 256, odd};
-  return {0, 0, odd};
+  const int n = dtype == DTK_F32 ? 4 : 8, vecs = (width + n - 1) / n;
+  const Fit fit = width < n ? kTiny : width % n ? kRagged : kWhole;
+  if (vecs <= 8) return {8, 1, fit};
+  if (vecs <= 16) return {16, 1, fit};
+  if (vecs <= 32) return {32, 1, fit};
+  if (vecs <= 128) return {64, (vecs + 63) / 64, fit};
+  if (vecs <= 1024) return {256, vecs <= 256 ? 1 : vecs <= 512 ? 2 : 4, fit};
+  return {0, 0, fit};
 }
-inline int rows_per_block(const Shape& s) { return s.lpr ? kThreads / s.lpr : 1; }
-// Workgroups of the backward: enough to fill 256 CUs four times, few enough that their partial rows stay small; a
-// multiple of 8 where that keeps a lane's columns (k_norm_bwd, ODD).
-inline int bwd_grid(int64_t rows, const Shape& s) {
-  const int64_t need = (rows + rows_per_block(s) - 1) / rows_per_block(s);
-  return (int)(need >= 1024 ? 1024 : s.lpr && s.odd ? (need + 7) / 8 * 8 : need);
+// Workgroups that walk the rows: no more than the chip holds at once (waves_of() per CU), and so many
+// that each walks the same number of rows.
+inline int walk_grid(int64_t rows, const Shape& s, bool all) {
+  const int per_block = s.lpr ? kThreads / s.lpr : 1;
+  const int64_t need = (rows + per_block - 1) / per_block;
+  const int most = 256 * waves_of(s.ni, all);
+  const int64_t turns = (need + most - 1) / most;
+  return (int)((need + turns - 1) / turns);
 }
 
 template <typename T, int NI, int LPR, bool ADD>
-void launch_fwd(const FwdArgs& a, bool odd, hipStream_t st) {
-  const unsigned grid = (unsigned)((a.rows + kThreads / LPR - 1) / (kThreads / LPR));
-  if (odd) k_norm_fwd<T, NI, LPR, ADD, true><<<grid, kThreads, 0, st>>>(a);
-  else k_norm_fwd<T, NI, LPR, ADD, false><<<grid, kThreads, 0, st>>>(a);
+void launch_fwd(const FwdArgs& a, Fit fit, hipStream_t st) {
+  const int grid = walk_grid(a.rows, {LPR, NI, fit}, false);
+  if (fit == kWhole) k_norm_fwd<T, NI, LPR, ADD, kWhole><<<grid, kThreads, 0, st>>>(a);
+  else if (LPR > 8 || fit == kRagged) k_norm_fwd<T, NI, LPR, ADD, kRagged><<<grid, kThreads, 0, st>>>(a);
+  else k_norm_fwd<T, 1, 8, ADD, kTiny><<<grid, kThreads, 0, st>>>(a);
 }
 template <typename T, int NI, int LPR, bool ADD>
-void launch_bwd(const BwdArgs& a, int grid, bool odd, hipStream_t st) {
-  if (odd) k_norm_bwd<T, NI, LPR, ADD, true><<<grid, kThreads, 0, st>>>(a);
-  else k_norm_bwd<T, NI, LPR, ADD, false><<<grid, kThreads, 0, st>>>(a);
+void launch_bwd(const BwdArgs& a, int grid, Fit fit, hipStream_t st) {
+  if (fit == kWhole) k_norm_bwd<T, NI, LPR, ADD, kWhole><<<grid, kThreads, 0, st>>>(a);
+  else if (LPR > 8 || fit == kRagged) k_norm_bwd<T, NI, LPR, ADD, kRagged><<<grid, kThreads, 0, st>>>(a);
+  else k_norm_bwd<T, 1, 8, ADD, kTiny><<<grid, kThreads, 0, st>>>(a);
 }
 #define DTK_BY_SHAPE(GO, WIDE)                     \
   switch (s.lpr) {                                 \
@@ -477,23 +495,22 @@ void launch_bwd(const BwdArgs& a, int grid, bool odd, hipStream_t st) {
     case 32: return GO(1, 32);                     \
     case 64:                                       \
       if (s.ni == 1) return GO(1, 64);             \
-      if (s.ni == 2) return GO(2, 64);             \
-      if (s.ni == 3) return GO(3, 64);             \
-      return GO(4, 64);                            \
+      return GO(2, 64);                            \
     case 256:                                      \
+      if (s.ni == 1) return GO(1, 256);            \
       if (s.ni == 2) return GO(2, 256);            \
       return GO(4, 256);                           \
   }                                                \
   WIDE
 template <typename T, bool ADD>
 void run_fwd(const FwdArgs& a, const Shape& s, hipStream_t st) {
-#define DTK_GO(NI, LPR) launch_fwd<T, NI, LPR, ADD>(a, s.odd, st)
+#define DTK_GO(NI, LPR) launch_fwd<T, NI, LPR, ADD>(a, s.fit, st)
   DTK_BY_SHAPE(DTK_GO, (k_norm_fwd_wide<T, ADD><<<(unsigned)a.rows, kThreads, 0, st>>>(a)));
 #undef DTK_GO
 }
 template <typename T, bool ADD>
 void run_bwd(const BwdArgs& a, int grid, const Shape& s, hipStream_t st) {
-#define DTK_GO(NI, LPR) launch_bwd<T, NI, LPR, ADD>(a, grid, s.odd, st)
+#define DTK_GO(NI, LPR) launch_bwd<T, NI, LPR, ADD>(a, grid, s.fit, st)
   DTK_BY_SHAPE(DTK_GO, (k_norm_bwd_wide<T, ADD><<<grid, kThreads, 0, st>>>(a)));
 #undef DTK_GO
 }

@@ -38,7 +38,7 @@ __device__ __forceinline__ void drop_vec(Vec<T>& v, const Vec<T>& r, const Drop&
   for (int e = 0; e < N; ++e) {
     float f = (float)v.v[e];
     if (drop.rng) f = keep[e] ? f * drop.scale : 0.f;
-    v.v[e] = (T)(add ? f + (float)r.v[e] : f);
+    v.v[e] = rounded<T>(add ? f + (float)r.v[e] : f);
   }
 }
 // One vector per thread. The generator's 20 products per vector (f32: 10) come to about half the time that the
@@ -101,7 +101,7 @@ int dtk_layer_norm_fwd(int64_t rows, int width, int dtype, int wtype, const void
 
 size_t dtk_layer_norm_bwd_workspace_size(int64_t rows, int width, int dtype) {
   if (rows <= 0 || width <= 0) return 0;
-  return (size_t)2 * bwd_grid(rows, shape_of(width, dtype)) * width * sizeof(float);
+  return (size_t)2 * walk_grid(rows, shape_of(width, dtype), false) * width * sizeof(float);
 }
 
 int dtk_layer_norm_bwd(int64_t rows, int width, int dtype, int wtype, const void* z, const void* dy, const void* ds,
@@ -115,7 +115,7 @@ int dtk_layer_norm_bwd(int64_t rows, int width, int dtype, int wtype, const void
   const bool sums = dweight || dbias;
   DSPLAT_REQUIRE(rows == 0 || (z && mean && rstd && (!sums || workspace)), "dtk_layer_norm_bwd: null pointer");
   const Shape sh = shape_of(width, dtype);
-  const int grid = rows ? bwd_grid(rows, sh) : 0;
+  const int grid = rows ? walk_grid(rows, sh, add != 0) : 0;
   hipStream_t st = (hipStream_t)stream;
   const BwdArgs a = {rows, width, z, dy, ds, {weight, nullptr, wtype == DTK_F32}, mean, rstd, drop_of(p, rng, call), dx, dresidual,
                      sums ? (float*)workspace : nullptr};
