@@ -15,6 +15,7 @@ PKG = Path(__file__).resolve().parent
 ROOT = PKG.parent
 CSRC = PKG / "csrc"
 LIB = PKG / "lib" / "libdsplat_hip.so"
+TORCH_LIB = PKG / "lib" / "dsplat_torch.so"
 OBJ = PKG / "lib" / "obj"
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
@@ -83,6 +84,28 @@ def build_hip(force: bool = False, verbose: bool = False) -> Path:
     return LIB
 
 
+def build_torch(force: bool = False) -> Path:
+    """The operators' torch layer (csrc/dtk_torch.cpp): host code against this torch's headers. It needs no
+    HIP library to link to (its functions are bound by address when it is loaded)."""
+    src = CSRC / "dtk_torch.cpp"
+    OBJ.mkdir(parents=True, exist_ok=True)
+    if not force and not _needs(TORCH_LIB, [src, ROOT / "include" / "dsplat_hip.h", Path(__file__)]):
+        return TORCH_LIB
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension as ext
+    libdir = Path(torch.__file__).resolve().parent / "lib"
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-D__HIP_PLATFORM_AMD__", "-DUSE_ROCM",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           *(f"-isystem{p}" for p in (*ext.include_paths("cuda"), sysconfig.get_paths()["include"])),
+           str(src), "-o", str(TORCH_LIB), f"-L{libdir}", "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_python"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"g++ failed for {src.name}:\n{r.stderr}")
+    return TORCH_LIB
+
+
 def build_oracle() -> Path:
     r = subprocess.run(["make", "-s", "-C", str(ROOT / "oracle")], capture_output=True, text=True)
     if r.returncode != 0:
@@ -92,4 +115,5 @@ def build_oracle() -> Path:
 
 if __name__ == "__main__":
     print(build_hip(force="--force" in sys.argv, verbose=True))
+    print(build_torch(force="--force" in sys.argv))
     print(build_oracle())

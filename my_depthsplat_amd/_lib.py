@@ -8,6 +8,8 @@ the library shares torch's streams and device allocations.
 from __future__ import annotations
 
 import ctypes
+import importlib.machinery
+import importlib.util
 import os
 from ctypes import c_float, c_int, c_uint32, c_void_p
 from pathlib import Path
@@ -16,6 +18,8 @@ import torch  # noqa: F401  (must be loaded before the HIP library)
 
 # (DSPLAT_LIB: another build of the same ABI, e.g. a tools/ab_build.py A/B variant)
 LIB_PATH = Path(os.environ.get("DSPLAT_LIB") or Path(__file__).resolve().parent / "lib" / "libdsplat_hip.so")
+
+TORCH_LIB_PATH = Path(__file__).resolve().parent / "lib" / "dsplat_torch.so"
 
 # name -> (restype, argtypes); mirrors include/dsplat_hip.h exactly.
 _P = c_void_p
@@ -134,6 +138,26 @@ def load(path: Path | str | None = None) -> ctypes.CDLL:
     if path is None:
         _lib = lib
     return lib
+
+
+_torch_lib = None
+
+
+def load_torch():
+    """The operators with a C++ torch layer (csrc/dtk_torch.cpp), bound to the library that load() loads."""
+    global _torch_lib
+    if _torch_lib is None:
+        p = TORCH_LIB_PATH
+        if not p.exists():
+            raise DsplatError(f"HIP extension not built: {p} is missing. Run `python -c 'import __graft_entry__ as g; "
+                              "g.build()'`. There is no CPU fallback.")
+        lib = load()
+        loader = importlib.machinery.ExtensionFileLoader("dsplat_torch", str(p))
+        module = importlib.util.module_from_spec(importlib.util.spec_from_loader("dsplat_torch", loader))
+        loader.exec_module(module)
+        module.bind({name: ctypes.cast(getattr(lib, name), c_void_p).value for name in SIGNATURES})
+        _torch_lib = module
+    return _torch_lib
 
 
 def check(status: int, what: str) -> None:

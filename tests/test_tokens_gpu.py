@@ -287,14 +287,17 @@ def test_rotary_of_slices(gpu):
     pos = T.view_positions(2, 5, 5, gpu)
     fr = T.rotary_frequencies(64, 2, device=gpu)
     q, k = T.rotary(qkv[:, :, :4], qkv[:, :, 4:5], pos, fr)
-    pq, pk = T.rotary(qkv[:, :, :4].contiguous(), qkv[:, :, 4:5].contiguous(), pos.expand(2, -1, -1).contiguous(), fr)
+    packed = [qkv[:, :, :4].detach().contiguous().requires_grad_(True), qkv[:, :, 4:5].detach().contiguous().requires_grad_(True)]
+    pq, pk = T.rotary(*packed, pos.expand(2, -1, -1).contiguous(), fr)
     assert torch.equal(q, pq) and torch.equal(k, pk)
     (g,) = torch.autograd.grad(q.float().sum() + 2 * k.float().sum(), qkv)
     one = torch.ones(2, 50, 4, 64, device=gpu, dtype=BF16)
-    want = torch.zeros_like(qkv)
-    dq, dk = T._rotary(one, 2 * one[:, :, :1], pos, fr, False, 1.0, True)
-    want[:, :, :4], want[:, :, 4:5] = dq, dk
-    assert torch.equal(g, want)
+    dq, dk = torch.autograd.grad((pq, pk), packed, (one, 2 * one[:, :, :1].contiguous()))
+    assert torch.equal(g, torch.cat([dq, dk, torch.zeros_like(dk)], 2))
+    (only,) = torch.autograd.grad(T.rotary(*packed, pos, fr)[1].sum(), packed[1])  # q' unused
+    assert only.shape == dk.shape
+    (none,) = torch.autograd.grad(T.rotary(packed[0], None, pos, fr)[0], packed[0], one)
+    assert torch.equal(none, dq) and T.rotary(packed[0], None, pos, fr)[1] is None
 
 
 # ---- block choice ---------------------------------------------------------------------------
@@ -466,6 +469,14 @@ def test_attention_of_slices_and_same_bits(gpu):
     for _ in range(3):
         (g,) = torch.autograd.grad(T.block_sparse_attention(q, k, v, index), qkv, do)
         assert torch.equal(g, want)
+
+
+def test_gradients_are_not_differentiable_twice(gpu):
+    T = tokens()
+    x = torch.randn(4, 8, device=gpu, requires_grad=True)
+    (g,) = torch.autograd.grad(T.layer_norm(x).square().sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError):
+        g.sum().backward()
 
 
 def test_attention_empty_calls(gpu):

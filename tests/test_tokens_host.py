@@ -149,6 +149,7 @@ idx = torch.zeros(2, 2, 1, 3, dtype=torch.int32)
     lambda: tokens.block_sparse_attention(q4, k4, k4, idx.expand(2, 2, 1, 3).repeat(1, 1, 1, 342)),
     lambda: tokens.block_sparse_attention(q4[..., :12], k4[..., :12], k4[..., :12], idx),
     lambda: tokens.block_sparse_attention(q4.repeat(1, 1, 1, 9), k4.repeat(1, 1, 1, 9), k4.repeat(1, 1, 1, 9), idx),
+    lambda: tokens.block_sparse_attention(torch.zeros(1, 2, 1025, 8), torch.zeros(1, 2, 1, 8), torch.zeros(1, 2, 1, 8), idx[:1, :1]),
     lambda: tokens.block_sparse_attention(q4, k4, k4, idx, block=48),
     lambda: tokens.block_sparse_attention(q4, k4, k4, idx, kv_lengths=torch.zeros(1, 2, dtype=torch.int32)),
 ])
@@ -208,7 +209,8 @@ def test_abi_refusals():
     at = lambda **kw: _lib.Attention(**{**dict(Lq=9, Lk=9, B=1, Hq=2, Hkv=1, D=8, block=64, top=2, dtype=0, scale=1.0), **kw})  # noqa: E731
     for kw, text in ((dict(Hq=3, Hkv=2), b"bad sizes"), (dict(top=1025), b"bad sizes"), (dict(D=12), b"multiple of 8"),
                      (dict(D=136), b"multiple of 8"), (dict(block=16), b"block must be"), (dict(dtype=4), b"bad type"),
-                     (dict(), b"null pointer")):
+                     (dict(Hq=1025), b"more than 1024"), (dict(k_strides=(0, 1 << 24, 8)), b"token stride"),
+                     (dict(v_strides=(0, -8, 8)), b"token stride"), (dict(), b"null pointer")):
         refused(lib.dtk_block_sparse_attention_fwd(ctypes.byref(at(**kw)), None, None), text)
         refused(lib.dtk_block_sparse_attention_bwd(ctypes.byref(at(**kw)), None, None, None, None, None, None, None), text)
     refused(lib.dtk_block_sparse_attention_fwd(None, None, None), b"null pointer")
