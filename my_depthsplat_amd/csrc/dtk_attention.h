@@ -192,16 +192,19 @@ constexpr int kTileBytes = 2 * kBuffers<T, DP, U> * U * Tile<T, DP>::kUnit;
 
 __device__ __forceinline__ int acc_row(int r, int half) { return 8 * (r >> 2) + 4 * half + (r & 3); }
 
-// The tile's list without places that are no block or stand in it already, in LDS, in order.
+// The tile's list without places that are no block or stand in it already, in LDS, in order. One wave, 64 places at
+// a time: each is compared with those before it by broadcasts within the wave (from memory, one after the other, it took
+// longer than the attention of few queries itself), and with the list so far.
 __device__ __forceinline__ int block_list(const int32_t* idx, int top, int blocks, int32_t* list, int* count) {
   if (threadIdx.x < 64) {
     const int lane = threadIdx.x;
     int n = 0;
     for (int base = 0; base < top; base += 64) {
-      const int at = base + lane;
-      const int v = at < top ? idx[at] : -1;
+      const int v = base + lane < top ? idx[base + lane] : -1;
       bool ok = v >= 0 && v < blocks;
-      for (int j = 0; ok && j < at; ++j) ok = idx[j] != v;
+      const int here = min(64, top - base);
+      for (int j = 0; j < here; ++j) ok = ok && !(j < lane && __builtin_amdgcn_readlane(v, j) == v);
+      for (int j = 0; j < n; ++j) ok = ok && list[j] != v;
       const uint64_t m = __ballot(ok);
       if (ok) list[n + __popcll(m & dsplat::lanemask_lt(lane))] = v;
       n += __popcll(m);

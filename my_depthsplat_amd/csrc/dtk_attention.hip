@@ -7,7 +7,7 @@ using namespace dtk;
 
 constexpr int NT = kThreads;
 
-// Joins the parts of a split list: one row per group of D / 4 threads.
+// Joins the parts of a split list: four channels of a row per thread.
 template <typename T>
 __global__ __launch_bounds__(NT) void k_attend_join(Args a, int64_t rows) {
   const int per = a.D / 4;
@@ -15,16 +15,34 @@ __global__ __launch_bounds__(NT) void k_attend_join(Args a, int64_t rows) {
   const int64_t r = id / per;
   const int d = (int)(id % per) * 4;
   if (r >= rows) return;
-  float m = -INFINITY;
-  for (int s = 0; s < a.splits; ++s) m = fmaxf(m, a.part_m[s * rows + r]);
-  const float base = m == -INFINITY ? 0.f : m;
-  float l = 0.f, o[4] = {};
-  for (int s = 0; s < a.splits; ++s) {
-    const float f = exp2f(a.part_m[s * rows + r] - base);
-    l += a.part_l[s * rows + r] * f;
-    const float* p = a.part + (s * rows + r) * a.D + d;
+  float m = -INFINITY, l = 0.f, o[4] = {};
+  for (int s0 = 0; s0 < a.splits; s0 += 8) {  // eight parts' values on their way together
+    float pm[8], pl[8];
+    float4 po[8];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) o[e] += p[e] * f;
+    for (int k = 0; k < 8; ++k) {
+      const int64_t at = (int64_t)min(s0 + k, a.splits - 1) * rows + r;
+      pm[k] = a.part_m[at];
+      pl[k] = a.part_l[at];
+      po[k] = *(const float4*)(a.part + at * a.D + d);
+    }
+    float mn = m;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) mn = fmaxf(mn, pm[k]);
+    const float base = mn == -INFINITY ? 0.f : mn, f0 = exp2f(m - base);
+    m = mn;
+    l *= f0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] *= f0;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const float f = s0 + k < a.splits ? exp2f(pm[k] - base) : 0.f;
+      l += pl[k] * f;
+      o[0] += po[k].x * f;
+      o[1] += po[k].y * f;
+      o[2] += po[k].z * f;
+      o[3] += po[k].w * f;
+    }
   }
   const int64_t i = r % a.Lq, bh = r / a.Lq, b = bh / a.Hq, h = bh % a.Hq;
   const bool valid = i < length_of(a.q_lengths, (int)b, a.Lq);

@@ -38,6 +38,17 @@ __device__ __forceinline__ void angle(const RotaryArgs& a, const P* pos, int i, 
   s = (back ? -sn : sn) * a.factor;
 }
 
+template <typename T, int N>
+struct Piece {
+  T v[N];
+  static __device__ __forceinline__ Piece load(const T* p) {
+    Piece r;
+    __builtin_memcpy(&r, p, sizeof(r));
+    return r;
+  }
+  __device__ __forceinline__ void store(T* p) const { __builtin_memcpy(p, this, sizeof(*this)); }
+};
+
 // N = channels of a vector (16 bytes) or 1. Units of a token: halves: the F / N vector pairs,
 // then the copied vectors; interleaved: the vectors (N = 1: the pairs, then the copied channels).
 template <typename T, typename P, int N, bool INTER, bool BACK>
@@ -56,49 +67,48 @@ __global__ __launch_bounds__(NT) void k_rotary(RotaryArgs a) {
   const int c0 = copy ? (PAIR ? 2 * a.F + (u - turning) * N : u * N) : (INTER ? (N == 1 ? 2 * u : u * N) : u * N);
   const int step = INTER ? 1 : a.F;  // from a pair's first channel (vector) to its second
   constexpr int NP = PAIR ? N : N / 2;
+  constexpr int K = 4;  // heads whose channels are on their way together
+  const int h1 = min((g + 1) * a.heads_per, a.Hq + a.Hk);
+  const auto in = [&](int h) {
+    return h < a.Hq ? (const T*)a.q + b * a.qb + l * a.ql + h * a.qh : (const T*)a.k + b * a.kb + l * a.kl + (h - a.Hq) * a.kh;
+  };
+  const auto out = [&](int h) {
+    return h < a.Hq ? (T*)a.oq + (token * a.Hq + h) * a.D : (T*)a.ok + (token * a.Hk + (h - a.Hq)) * a.D;
+  };
+  using V = Piece<T, N>;
+  V x[K], y[K];
+  const auto fetch = [&](int h) {
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+      if (h + k < h1) {
+        x[k] = V::load(in(h + k) + c0);
+        if (PAIR && !copy) y[k] = V::load(in(h + k) + c0 + step);
+      }
+  };
+  fetch(g * a.heads_per);
   float c[NP], s[NP];
   if (!copy) {
 #pragma unroll
     for (int i = 0; i < NP; ++i) angle<P>(a, pos, (INTER ? c0 / 2 : c0) + i, BACK, c[i], s[i]);
   }
-  const int h1 = min((g + 1) * a.heads_per, a.Hq + a.Hk);
-  for (int h = g * a.heads_per; h < h1; ++h) {
-    const bool isq = h < a.Hq;
-    const T* in = isq ? (const T*)a.q + b * a.qb + l * a.ql + h * a.qh
-                      : (const T*)a.k + b * a.kb + l * a.kl + (h - a.Hq) * a.kh;
-    T* out = isq ? (T*)a.oq + (token * a.Hq + h) * a.D : (T*)a.ok + (token * a.Hk + (h - a.Hq)) * a.D;
-    if constexpr (N == 1) {
-      if (copy) {
-        out[c0] = in[c0];
-      } else {
-        const float x = (float)in[c0], y = (float)in[c0 + step];
-        out[c0] = (T)(x * c[0] - y * s[0]);
-        out[c0 + step] = (T)(x * s[0] + y * c[0]);
-      }
-    } else if (copy) {
-      store_vec(out + c0, load_vec(in + c0));
-    } else if constexpr (INTER) {
-      const Vec<T> v = load_vec(in + c0);
-      Vec<T> o;
+  for (int h = g * a.heads_per; h < h1; h += K) {
 #pragma unroll
-      for (int i = 0; i < NP; ++i) {
-        const float x = (float)v.v[2 * i], y = (float)v.v[2 * i + 1];
-        o.v[2 * i] = (T)(x * c[i] - y * s[i]);
-        o.v[2 * i + 1] = (T)(x * s[i] + y * c[i]);
-      }
-      store_vec(out + c0, o);
-    } else {
-      const Vec<T> v = load_vec(in + c0), w = load_vec(in + c0 + a.F);
-      Vec<T> o, q;
+    for (int k = 0; k < K; ++k) {
+      if (h + k >= h1) break;
+      if (!copy) {
 #pragma unroll
-      for (int i = 0; i < NP; ++i) {
-        const float x = (float)v.v[i], y = (float)w.v[i];
-        o.v[i] = (T)(x * c[i] - y * s[i]);
-        q.v[i] = (T)(x * s[i] + y * c[i]);
+        for (int i = 0; i < NP; ++i) {
+          T& p = PAIR ? x[k].v[i] : x[k].v[2 * i % N];
+          T& q = PAIR ? y[k].v[i] : x[k].v[(2 * i + 1) % N];
+          const float f = (float)p, t = (float)q;
+          p = (T)(f * c[i] - t * s[i]);
+          q = (T)(f * s[i] + t * c[i]);
+        }
+        if (PAIR) y[k].store(out(h + k) + c0 + step);
       }
-      store_vec(out + c0, o);
-      store_vec(out + c0 + a.F, q);
+      x[k].store(out(h + k) + c0);
     }
+    if (h + K < h1) fetch(h + K);
   }
 }
 
