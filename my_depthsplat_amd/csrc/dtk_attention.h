@@ -280,7 +280,7 @@ struct Join {
 // of 32 keys and are joined at the end. The rows of a tile are its queries of all heads that
 // share the key head (few queries: they fill the instruction's columns together).
 template <typename T, int DP, int RW>
-__global__ __launch_bounds__(kThreads, (sizeof(T) == 2 && DP <= 64 ? 4 : 1)) void k_attend_fwd(Args a) {
+__global__ __launch_bounds__(kThreads, (sizeof(T) == 2 && DP <= 64 ? (RW == 1 ? 2 : 4) : 1)) void k_attend_fwd(Args a) {
   using M = Mma<T>;
   using L = Tile<T, DP>;
   using Frag = typename M::Frag;
@@ -468,7 +468,7 @@ __device__ __forceinline__ void ds_scale(uint32_t largest, float& down, float& u
 // dq: the forward's shape; p is taken from the saved lse. delta = sum_d do o of each row on the
 // way, kept for dk.
 template <typename T, int DP, int RW>
-__global__ __launch_bounds__(kThreads, (sizeof(T) == 2 && DP <= 64 ? 3 : 1)) void k_attend_dq(Args a) {
+__global__ __launch_bounds__(kThreads, (sizeof(T) == 2 && DP <= 64 ? (RW == 1 ? 2 : 3) : 1)) void k_attend_dq(Args a) {
   using M = Mma<T>;
   using L = Tile<T, DP>;
   using Frag = typename M::Frag;

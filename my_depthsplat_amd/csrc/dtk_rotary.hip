@@ -18,8 +18,8 @@ using namespace dtk;
 constexpr int NT = 256;
 
 struct RotaryArgs {
-  int64_t L, units;        // tokens per sequence; units per token
-  int64_t total;           // B * L * units * head groups
+  int64_t L, tokens;  // tokens per sequence; of all sequences
+  int units;          // per token
   int Hq, Hk, D, F, per_axis, axes, groups, heads_per;
   const void *q, *k, *pos;
   int64_t qb, ql, qh, kb, kl, kh, pb, pl, pa;  // strides in elements
@@ -28,14 +28,23 @@ struct RotaryArgs {
   void *oq, *ok;  // contiguous [B, L, H, D]
 };
 
-template <typename P>
-__device__ __forceinline__ void angle(const RotaryArgs& a, const P* pos, int i, bool back, float& c, float& s) {
-  const double f = a.freqs[i] * 0.15915494309189533577;  // turns per position
-  const double t = (double)pos[(i / a.per_axis) * a.pa] * f;
-  float sn, cs;
-  sincospif((float)(2.0 * (t - rint(t))), &sn, &cs);
-  c = cs * a.factor;
-  s = (back ? -sn : sn) * a.factor;
+// The sines of pairs i .. i + NP - 1 at a token. A vector's pairs have one axis where the frequencies of an axis are
+// whole vectors (same).
+template <typename P, int NP>
+__device__ __forceinline__ void angles(const RotaryArgs& a, const P* pos, int i, bool same, bool back, float (&c)[NP], float (&s)[NP]) {
+  double f[NP];
+#pragma unroll
+  for (int k = 0; k < NP; ++k) f[k] = a.freqs[i + k];
+  const double p0 = (double)pos[(i / a.per_axis) * a.pa];
+#pragma unroll
+  for (int k = 0; k < NP; ++k) {
+    const double p = same ? p0 : (double)pos[((i + k) / a.per_axis) * a.pa];
+    const double t = p * (f[k] * 0.15915494309189533577);  // turns
+    float sn, cs;
+    sincospif((float)(2.0 * (t - rint(t))), &sn, &cs);
+    c[k] = cs * a.factor;
+    s[k] = (back ? -sn : sn) * a.factor;
+  }
 }
 
 template <typename T, int N>
@@ -52,15 +61,7 @@ struct Piece {
 // N = channels of a vector (16 bytes) or 1. Units of a token: halves: the F / N vector pairs,
 // then the copied vectors; interleaved: the vectors (N = 1: the pairs, then the copied channels).
 template <typename T, typename P, int N, bool INTER, bool BACK>
-__global__ __launch_bounds__(NT) void k_rotary(RotaryArgs a) {
-  const int64_t id = (int64_t)blockIdx.x * NT + threadIdx.x;
-  if (id >= a.total) return;
-  const int u = (int)(id % a.units);
-  const int64_t r = id / a.units;
-  const int g = (int)(r % a.groups);
-  const int64_t token = r / a.groups;
-  const int64_t b = token / a.L, l = token % a.L;
-  const P* pos = (const P*)a.pos + b * a.pb + l * a.pl;
+__device__ __forceinline__ void turn_unit(const RotaryArgs& a, const P* pos, int64_t token, int64_t b, int64_t l, int g, int u) {
   constexpr bool PAIR = !INTER || N == 1;  // the unit holds both ends of its pairs as two vectors
   const int turning = PAIR ? a.F / N : 2 * a.F / N;
   const bool copy = u >= turning;
@@ -87,10 +88,7 @@ __global__ __launch_bounds__(NT) void k_rotary(RotaryArgs a) {
   };
   fetch(g * a.heads_per);
   float c[NP], s[NP];
-  if (!copy) {
-#pragma unroll
-    for (int i = 0; i < NP; ++i) angle<P>(a, pos, (INTER ? c0 / 2 : c0) + i, BACK, c[i], s[i]);
-  }
+  if (!copy) angles<P, NP>(a, pos, INTER ? c0 / 2 : c0, a.per_axis % NP == 0, BACK, c, s);
   for (int h = g * a.heads_per; h < h1; h += K) {
 #pragma unroll
     for (int k = 0; k < K; ++k) {
@@ -112,13 +110,24 @@ __global__ __launch_bounds__(NT) void k_rotary(RotaryArgs a) {
   }
 }
 
+template <typename T, typename P, int N, bool INTER, bool BACK>
+__global__ __launch_bounds__(NT) void k_rotary(RotaryArgs a) {
+  const int g = blockIdx.y;
+  const int64_t token = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
+  if (token >= a.tokens) return;
+  const int64_t b = (uint32_t)token / (uint32_t)a.L, l = token - b * a.L;  // fewer than 2^31 tokens (the host checks)
+  const P* pos = (const P*)a.pos + b * a.pb + l * a.pl;
+  for (int u = threadIdx.x; u < a.units; u += blockDim.x) turn_unit<T, P, N, INTER, BACK>(a, pos, token, b, l, g, u);
+}
+
 template <typename T, typename P, int N>
 void launch(const RotaryArgs& a, bool inter, bool back, hipStream_t st) {
-  const unsigned grid = (unsigned)((a.total + NT - 1) / NT);
+  const int ux = a.units < NT ? a.units : NT, ty = NT / ux;  // a token's units side by side, tokens above each other
+  const dim3 block(ux, ty), grid((unsigned)((a.tokens + ty - 1) / ty), a.groups);
   if (inter)
-    back ? k_rotary<T, P, N, true, true><<<grid, NT, 0, st>>>(a) : k_rotary<T, P, N, true, false><<<grid, NT, 0, st>>>(a);
+    back ? k_rotary<T, P, N, true, true><<<grid, block, 0, st>>>(a) : k_rotary<T, P, N, true, false><<<grid, block, 0, st>>>(a);
   else
-    back ? k_rotary<T, P, N, false, true><<<grid, NT, 0, st>>>(a) : k_rotary<T, P, N, false, false><<<grid, NT, 0, st>>>(a);
+    back ? k_rotary<T, P, N, false, true><<<grid, block, 0, st>>>(a) : k_rotary<T, P, N, false, false><<<grid, block, 0, st>>>(a);
 }
 template <typename T>
 void by_pos(const RotaryArgs& a, int ptype, bool vec, bool inter, bool back, hipStream_t st) {
@@ -134,7 +143,7 @@ extern "C" int dtk_rotary(int64_t B, int64_t L, int Hq, int Hk, int D, int F, in
                           int dtype, int ptype, const void* q, const int64_t* q_strides, const void* k,
                           const int64_t* k_strides, const void* positions, const int64_t* pos_strides,
                           const double* freqs, float factor, void* q_out, void* k_out, void* stream) {
-  DSPLAT_REQUIRE(B >= 0 && L >= 0 && Hq >= 0 && Hk >= 0 && D > 0 && Hq < 65536 && Hk < 65536 && D < (1 << 20),
+  DSPLAT_REQUIRE(B >= 0 && L >= 0 && (L == 0 || B < (1LL << 31) / L) && Hq >= 0 && Hk >= 0 && D > 0 && Hq < 65536 && Hk < 65536 && D < (1 << 20),
                  "dtk_rotary: bad sizes");
   DSPLAT_REQUIRE(F >= 0 && 2 * F <= D && axes > 0 && F % axes == 0, "dtk_rotary: bad number of frequencies");
   DSPLAT_REQUIRE(type_ok(dtype) && (ptype == DTK_I64 || ptype == DTK_I32 || ptype == DTK_F32), "dtk_rotary: bad types");
@@ -171,8 +180,8 @@ extern "C" int dtk_rotary(int64_t B, int64_t L, int Hq, int Hk, int D, int F, in
   while (groups < heads && threads * groups < 256 * 1024) groups *= 2;
   a.heads_per = (heads + groups - 1) / groups;
   a.groups = (heads + a.heads_per - 1) / a.heads_per;
-  a.total = threads * a.groups;
-  DSPLAT_REQUIRE(a.total < (int64_t)NT * 2147483647LL, "dtk_rotary: too large");
+  a.tokens = B * L;
+  DSPLAT_REQUIRE(a.tokens < (1LL << 31) && a.groups < 65536, "dtk_rotary: too large");
   hipStream_t st = (hipStream_t)stream;
   if (dtype == DTK_F32) by_pos<float>(a, ptype, vec, interleaved != 0, backward != 0, st);
   else if (dtype == DTK_BF16) by_pos<bf16>(a, ptype, vec, interleaved != 0, backward != 0, st);
