@@ -10,5 +10,7 @@ reference's own operator names:
   my_depthsplat_amd.decoder        Decoder, DecoderOutput, DecoderSplattingCUDA, DECODERS, get_decoder
   my_depthsplat_amd.matching       warp_with_pose_depth_candidates, plane_sweep_cost_volume
   my_depthsplat_amd.gaussian_adapter  GaussianAdapter, GaussianAdapterCfg
+  my_depthsplat_amd.tokens         layer_norm, dropout, dropout_add_layer_norm, rotary, select_blocks,
+                                   block_sparse_attention (+ token_layer.ViewTokenLayer made of them)
 """
 __version__ = "0.1.0"

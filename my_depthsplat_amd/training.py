@@ -79,9 +79,15 @@ def head_rows(x: torch.Tensor, C: int, r: int) -> torch.Tensor:
 class GaussianHead(nn.Module):
     """Trainable stand-in for the Gaussian regressor + head: context image + depth ->
     per-pixel head channels [B, V, H*W, d_out] (d_out = 1 opacity + 2 offsets + adapter.d_in).
-    Works at 1/`down` resolution and pixel-shuffles back to full resolution."""
+    Works at 1/`down` resolution and pixel-shuffles back to full resolution.
 
-    def __init__(self, d_out: int, width: int = 108, down: int = 8):
+    token_layers > 0: that many ViewTokenLayers over the tokens of all views of a scene between the body
+    and the output (GPU only), with `token_heads` heads, `token_top` key blocks per tile and dropout
+    `token_dropout` from the generator state `rng` (seed, step): a buffer, so a checkpoint resumes it; the step
+    goes up with every training forward."""
+
+    def __init__(self, d_out: int, width: int = 108, down: int = 8, token_layers: int = 0, token_heads: int = 3,
+                 token_top: int = 16, token_dropout: float = 0.0, seed: int = 0):
         super().__init__()
         self.down = down
         self.d_out = d_out
@@ -91,12 +97,36 @@ class GaussianHead(nn.Module):
         self.out = nn.Conv2d(2 * width, d_out * down * down, 1)
         nn.init.normal_(self.out.weight, std=1e-3)
         nn.init.zeros_(self.out.bias)
+        self.layers = None
+        if token_layers:
+            from .token_layer import ViewTokenLayer
+            from .tokens import rotary_frequencies
+            self.layers = nn.ModuleList(ViewTokenLayer(2 * width, token_heads, top=token_top, p=token_dropout)
+                                        for _ in range(token_layers))
+            self.register_buffer("freqs", rotary_frequencies(self.layers[0].part(2), 2, device="cpu"), persistent=False)
+            self.register_buffer("rng", torch.tensor([seed, 0], dtype=torch.int64))
+
+    def _view_tokens(self, x: torch.Tensor, views: int) -> torch.Tensor:
+        """[BV, C, h, w] -> the same, through the token layers over the V h w tokens of each scene."""
+        from .tokens import view_positions
+        BV, C, h, w = x.shape
+        t = x.view(BV // views, views, C, h * w).transpose(2, 3).reshape(BV // views, views * h * w, C)
+        positions = view_positions(views, h, w, x.device)
+        rng = self.rng.clone()  # the backward reads it again, after the step below
+        for i, layer in enumerate(self.layers):
+            t = layer(t, positions, self.freqs, rng, 2 * i)
+        if self.training:
+            self.rng[1] += 1
+        return t.view(BV, h * w, C).transpose(1, 2).reshape(BV, C, h, w)
 
     def forward(self, images: torch.Tensor, depths: torch.Tensor) -> torch.Tensor:
         B, V, _, H, W = images.shape
         x = torch.cat([images, depths.reshape(B, V, 1, H, W)], 2).reshape(B * V, 4, H, W)
         x = F.avg_pool2d(x, self.down)
-        x = self.out(self.body(self.stem(x)))                   # [BV, d_out r^2, h, w], r = down
+        x = self.body(self.stem(x))
+        if self.layers is not None:
+            x = self._view_tokens(x, V)
+        x = self.out(x)                                         # [BV, d_out r^2, h, w], r = down
         # pixel shuffle + "(b v) c h w -> b v (h w) c" in one pass (head_rows):
         # out[b, v, (hh r + i) W + ww r + j, c] = x[bv, c r^2 + i r + j, hh, ww]
         return head_rows(x, self.d_out, self.down).view(B, V, H * W, self.d_out)
