@@ -174,6 +174,12 @@ struct Stage {
       if (r < have && d < D) v[i] = load_vec(p + off);
     }
   }
+  __device__ __forceinline__ void negate() {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+#pragma unroll
+      for (int e = 0; e < Vec<T>::N; ++e) v[i].v[e] = -v[i].v[e];
+  }
   __device__ __forceinline__ void store(char* t) const {
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
@@ -281,7 +287,7 @@ struct Join {
 // of 32 keys and are joined at the end. The rows of a tile are its queries of all heads that
 // share the key head (few queries: they fill the instruction's columns together).
 template <typename T, int DP, int RW>
-__global__ __launch_bounds__(kThreads, (sizeof(T) == 2 && DP <= 64 ? (RW == 1 ? 2 : 4) : 1)) void k_attend_fwd(Args a) {
+__global__ __launch_bounds__(kThreads, (sizeof(T) == 2 ? (DP > 64 || RW == 1 ? 2 : 4) : 1)) void k_attend_fwd(Args a) {
   using M = Mma<T>;
   using L = Tile<T, DP>;
   using Frag = typename M::Frag;
@@ -470,7 +476,7 @@ __device__ __forceinline__ void ds_scale(uint32_t largest, float& down, float& u
 // dq: the forward's shape; p is taken from the saved lse. delta = sum_d do o of each row on the
 // way, kept for dk.
 template <typename T, int DP, int RW>
-__global__ __launch_bounds__(kThreads, (sizeof(T) == 2 && DP <= 64 ? (RW == 1 ? 2 : 3) : 1)) void k_attend_dq(Args a) {
+__global__ __launch_bounds__(kThreads, (sizeof(T) == 2 ? (DP > 64 || RW == 1 ? 2 : 3) : 1)) void k_attend_dq(Args a) {
   using M = Mma<T>;
   using L = Tile<T, DP>;
   using Frag = typename M::Frag;
@@ -613,15 +619,19 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 2 && DP <= 64 ? (RW == 1 ? 
 
 // dk, dv of one key block: RW waves hold 32 keys each, 4 / RW take turns at the 32-query units of
 // the tiles that chose the block (their bits, some at a time) and are joined at the end. Every sum
-// has one order: no atomics on the gradients.
+// has one order: no atomics on the gradients. (Few blocks with long lists: gridDim.y parts of each, every
+// gridDim.y-th step.)
 constexpr int kTiles = 1024;  // tiles listed at a time
+template <typename T>
+constexpr int kDkvBuffers = 1;
 template <typename T, int DP, int RW>
-__global__ __launch_bounds__(kThreads) void k_attend_dkv(Args a) {
+__global__ __launch_bounds__(kThreads, (sizeof(T) == 2 ? (DP <= 64 ? (RW == 1 ? 2 : 3) : DP == 128 && RW == 1 ? 1 : 2) : 1)) void k_attend_dkv(Args a) {
   using M = Mma<T>;
   using L = Tile<T, DP>;
   using Frag = typename M::Frag;
-  constexpr int QW = 4 / RW, NS = DP / 16, ND = DP / 32, NB = kBuffers<T, DP, QW>;
-  constexpr int kAhead = sizeof(T) == 2 && DP <= 64 ? 2 : 1;  // steps whose rows are on their way
+  constexpr int QW = 4 / RW, NS = DP / 16, ND = DP / 32, NB = kDkvBuffers<T>;
+  constexpr int kAhead = 1;  // steps whose rows are on their way
+  constexpr bool KEEP = sizeof(T) == 4;
   extern __shared__ __align__(16) char lds[];
   __shared__ int32_t tiles[kTiles];
   __shared__ int count;
@@ -633,15 +643,37 @@ __global__ __launch_bounds__(kThreads) void k_attend_dkv(Args a) {
   const int64_t nq = length_of(a.q_lengths, b, a.Lq), nk = length_of(a.kv_lengths, b, a.Lk);
   const int64_t key = (int64_t)blk * a.block + 32 * rw + col;
   const bool exists = key < a.Lk, valid = key < nk;
-  const int64_t kr = valid ? key : 0;
-  const T* kp = (const T*)a.k.p + b * a.k.b + kr * a.k.l + hk * a.k.h;
-  const T* vp = (const T*)a.v.p + b * a.v.b + kr * a.v.l + hk * a.v.h;
-  Frag kf[NS], vf[NS];
+  // the block's keys and values: f32 in registers, 16 bits in LDS (from there they cost a third more of its
+  // reads and leave the registers to a third wave per SIMD)
+  char* tkv = lds + NB * 2 * QW * L::kUnit;
+  Frag kf[KEEP ? NS : 1], vf[KEEP ? NS : 1];
+  if constexpr (KEEP) {
+    const int64_t kr = valid ? key : 0;
+    const T* kp = (const T*)a.k.p + b * a.k.b + kr * a.k.l + hk * a.k.h;
+    const T* vp = (const T*)a.v.p + b * a.v.b + kr * a.v.l + hk * a.v.h;
 #pragma unroll
-  for (int s = 0; s < NS; ++s) {
-    kf[s] = row_frag<T>(kp, 16 * s + 8 * half, a.D, valid);
-    if (a.scale < 0.f) kf[s] = -kf[s];
-    vf[s] = row_frag<T>(vp, 16 * s + 8 * half, a.D, valid);
+    for (int s = 0; s < NS; ++s) {
+      kf[s] = row_frag<T>(kp, 16 * s + 8 * half, a.D, valid);
+      if (a.scale < 0.f) kf[s] = -kf[s];
+      vf[s] = row_frag<T>(vp, 16 * s + 8 * half, a.D, valid);
+    }
+  } else {
+    Stage<T, DP, RW> sk, sv;
+    const T *pk[RW], *pv[RW];
+    int have[RW];
+#pragma unroll
+    for (int j = 0; j < RW; ++j) {
+      const int64_t k0 = (int64_t)blk * a.block + 32 * j;
+      have[j] = (int)max((int64_t)0, min((int64_t)32, nk - k0));
+      pk[j] = (const T*)a.k.p + b * a.k.b + k0 * a.k.l + hk * a.k.h;
+      pv[j] = (const T*)a.v.p + b * a.v.b + k0 * a.v.l + hk * a.v.h;
+    }
+    sk.load(pk, have, a.k.l, a.D);
+    sv.load(pv, have, a.v.l, a.D);
+    if (a.scale < 0.f) sk.negate();
+    sk.store(tkv);
+    sv.store(tkv + RW * L::kUnit);
+    tkv += rw * L::kUnit;
   }
   float down = 1.f, up = 1.f;
   if constexpr (kFewExponents<T>) ds_scale(*a.gmax, down, up);
@@ -649,6 +681,7 @@ __global__ __launch_bounds__(kThreads) void k_attend_dkv(Args a) {
   const int upt = a.G << a.lg, words = (a.Tq + 31) / 32;  // units per tile
   const uint32_t* bits = a.bits + (((int64_t)b * a.Hkv + hk) * a.Tk + blk) * words;
   const bool any = (int64_t)blk * a.block < nk;
+  const int u0 = blockIdx.y * QW, stride = gridDim.y * QW;  // this part's steps
   int step = 0;
   for (int w0 = 0; any && w0 < words; w0 += kTiles / 32) {
     __syncthreads();
@@ -717,15 +750,15 @@ __global__ __launch_bounds__(kThreads) void k_attend_dkv(Args a) {
       }
       __syncthreads();
       const int live = f.live, buffer = step++ % NB;
-      if (u + kAhead * QW < units) fetch(f, u + kAhead * QW);
+      if (u + kAhead * stride < units) fetch(f, u + kAhead * stride);
       if (live == 0) return;
       tq += qw * L::kUnit;
       tg += qw * L::kUnit;
       f32x16 x = {}, dp = {};
 #pragma unroll
       for (int s = 0; s < NS; ++s) {
-        x = M::mma(L::row(tq, s, col, half), kf[s], x);
-        dp = M::mma(L::row(tg, s, col, half), vf[s], dp);
+        x = M::mma(L::row(tq, s, col, half), KEEP ? kf[KEEP ? s : 0] : L::row(tkv, s, col, half), x);
+        dp = M::mma(L::row(tg, s, col, half), KEEP ? vf[KEEP ? s : 0] : L::row(tkv + RW * L::kUnit, s, col, half), dp);
       }
       // (lanes whose key is none hold columns that are not written)
 #pragma unroll
@@ -753,11 +786,11 @@ __global__ __launch_bounds__(kThreads) void k_attend_dkv(Args a) {
     Ahead f[kAhead] = {};
 #pragma unroll
     for (int k = 0; k < kAhead; ++k)
-      if (k * QW < units) fetch(f[k], k * QW);
-    for (int u = 0; u < units; u += kAhead * QW)
+      if (u0 + k * stride < units) fetch(f[k], u0 + k * stride);
+    for (int u = u0; u < units; u += kAhead * stride)
 #pragma unroll
       for (int k = 0; k < kAhead; ++k)
-        if (u + k * QW < units) turn(f[k], u + k * QW);
+        if (u + k * stride < units) turn(f[k], u + k * stride);
   }
   if constexpr (QW > 1) {
     float* jo = (float*)lds + (rw * 32 + col) * (DP + 1);
@@ -781,6 +814,21 @@ __global__ __launch_bounds__(kThreads) void k_attend_dkv(Args a) {
   }
   if (qw != 0 || !exists) return;
   const int64_t off = (((int64_t)b * a.Lk + key) * a.Hkv + hk) * a.D;
+  if (gridDim.y > 1) {  // one of several parts: k_attend_dkv_join adds them up
+    const int64_t n = (int64_t)(gridDim.x / a.Tk / a.Hkv) * a.Lk * a.Hkv * a.D;
+    float *pk = a.part + (int64_t)blockIdx.y * 2 * n + off, *pv = pk + n;
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const int e = 32 * d + 8 * c + 4 * half;
+        if (e >= a.D) continue;
+        store4<float>(pk + e, dk[d][4 * c] * a.scale * up, dk[d][4 * c + 1] * a.scale * up, dk[d][4 * c + 2] * a.scale * up,
+                      dk[d][4 * c + 3] * a.scale * up);
+        store4<float>(pv + e, dv[d][4 * c], dv[d][4 * c + 1], dv[d][4 * c + 2], dv[d][4 * c + 3]);
+      }
+    return;
+  }
   const float f = a.scale * up;
 #pragma unroll
   for (int d = 0; d < ND; ++d)
@@ -834,7 +882,7 @@ struct Dq {
 template <typename T, int DP, int RW>
 struct Dkv {
   static int go(const Args& a, dim3 grid, hipStream_t st) {
-    return launch(k_attend_dkv<T, DP, RW>, a, grid, kTileBytes<T, DP, 4 / RW>, st, "k_attend_dkv");
+    return launch(k_attend_dkv<T, DP, RW>, a, grid, (kDkvBuffers<T> * 2 * (4 / RW) + (sizeof(T) == 2 ? 2 * RW : 0)) * Tile<T, DP>::kUnit, st, "k_attend_dkv");
   }
 };
 template <template <typename, int, int> class F, typename T, int DP>
