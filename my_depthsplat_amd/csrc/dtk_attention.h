@@ -75,10 +75,13 @@ struct Args {
   int32_t* order;
 };
 
-__device__ __forceinline__ int64_t length_of(const int32_t* lengths, int b, int64_t L) {
-  if (!lengths) return L;
-  const int64_t n = lengths[b];
-  return n < 0 ? 0 : n < L ? n : L;
+__device__ __forceinline__ int length_of(const int32_t* lengths, int b, int64_t L) {  // fewer than 2^31 (the host checks)
+  return lengths ? min(max(lengths[b], 0), (int)L) : (int)L;
+}
+// Row r of rows that start at p: token numbers and their strides fit 32 bits, their product is one unsigned 64-bit one.
+template <typename T>
+__device__ __forceinline__ const T* row_at(const T* p, int r, int64_t stride) {
+  return p + (uint64_t)(uint32_t)r * (uint32_t)stride;
 }
 
 // 8 channels of a row from d0 on, zeros behind D and for rows that do not count (what stands
@@ -245,13 +248,12 @@ __device__ __forceinline__ Where where(const Args& a) {
 // A tile's units of 32 keys: unit u is part u % (block / 32) of the list's block u / (block / 32).
 template <int U>
 struct Span {
-  int64_t first[U];
+  int first[U];
   int n[U];  // keys that count
 };
 struct Keys {
   const int32_t* list;
-  int block, lg, units;
-  int64_t nk;
+  int lg, units, nk;
   template <int U>
   __device__ __forceinline__ Span<U> span(int u) const {
     int b[U];
@@ -260,9 +262,8 @@ struct Keys {
     for (int j = 0; j < U; ++j) b[j] = list[min(u + j, units - 1) >> lg];
 #pragma unroll
     for (int j = 0; j < U; ++j) {
-      s.first[j] = (int64_t)uniform(b[j]) * block + 32 * ((u + j) & ((1 << lg) - 1));
-      const int64_t left = nk - s.first[j];
-      s.n[j] = u + j < units ? (int)max((int64_t)0, min((int64_t)32, left)) : 0;
+      s.first[j] = ((uniform(b[j]) << lg) + ((u + j) & ((1 << lg) - 1))) * 32;
+      s.n[j] = u + j < units ? max(0, min(32, nk - s.first[j])) : 0;
     }
     return s;
   }
@@ -300,15 +301,15 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 2 ? (DP > 64 || RW == 1 ? 2
   const int first_places = idx[min((int)threadIdx.x & 63, a.top - 1)];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, col = lane & 31;
   const int rw = uniform(wave) % RW, kw = uniform(wave) / RW;
-  const int64_t nq = length_of(a.q_lengths, at.b, a.Lq), nk = length_of(a.kv_lengths, at.b, a.Lk);
+  const int nq = length_of(a.q_lengths, at.b, a.Lq), nk = length_of(a.kv_lengths, at.b, a.Lk);
   const int row = (at.rt * RW + rw) * 32 + col;
   const int g = row / a.Lt;
   const int64_t i = (int64_t)at.t * a.block + row % a.Lt;
   const bool exists = g < a.G && i < a.Lq, valid = exists && i < nq;
   const int h = at.hk * a.G + (g < a.G ? g : 0);
-  const int blocks = (int)min((int64_t)a.Tk, (nk + a.block - 1) / a.block);
+  const int blocks = (nk >> (5 + a.lg)) + ((nk & (a.block - 1)) != 0);
   int n = 0;
-  if ((int64_t)at.t * a.block < nq) n = block_list(idx, first_places, a.top, blocks, list, &count);
+  if (at.t * a.block < nq) n = block_list(idx, first_places, a.top, blocks, list, &count);
 
   const T* qp = (const T*)a.q.p + at.b * a.q.b + (valid ? i : 0) * a.q.l + h * a.q.h;
   Frag qf[NS];
@@ -328,15 +329,15 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 2 ? (DP > 64 || RW == 1 ? 2
   const int units = n << a.lg;
   const int per = (units + a.splits - 1) / a.splits;
   const int u0 = min(units, at.split * per), u1 = min(units, u0 + per);
-  const Keys where_ = {list, a.block, a.lg, u1, nk};
+  const Keys where_ = {list, a.lg, u1, nk};
   Stage<T, DP, KW> sk, sv;
   const auto fetch = [&](int u) {
     const Span<KW> s = where_.span<KW>(u);
     const T *pk[KW], *pv[KW];
 #pragma unroll
     for (int j = 0; j < KW; ++j) {
-      pk[j] = kp + s.first[j] * a.k.l;
-      pv[j] = vp + s.first[j] * a.v.l;
+      pk[j] = row_at(kp, s.first[j], a.k.l);
+      pv[j] = row_at(vp, s.first[j], a.v.l);
     }
     sk.load(pk, s.n, a.k.l, a.D);
     sv.load(pv, s.n, a.v.l, a.D);
@@ -489,15 +490,15 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 2 ? (DP > 64 || RW == 1 ? 2
   const int first_places = idx[min((int)threadIdx.x & 63, a.top - 1)];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, col = lane & 31;
   const int rw = uniform(wave) % RW, kw = uniform(wave) / RW;
-  const int64_t nq = length_of(a.q_lengths, at.b, a.Lq), nk = length_of(a.kv_lengths, at.b, a.Lk);
+  const int nq = length_of(a.q_lengths, at.b, a.Lq), nk = length_of(a.kv_lengths, at.b, a.Lk);
   const int row = (at.rt * RW + rw) * 32 + col;
   const int g = row / a.Lt;
   const int64_t i = (int64_t)at.t * a.block + row % a.Lt;
   const bool exists = g < a.G && i < a.Lq, valid = exists && i < nq;
   const int h = at.hk * a.G + (g < a.G ? g : 0);
-  const int blocks = (int)min((int64_t)a.Tk, (nk + a.block - 1) / a.block);
+  const int blocks = (nk >> (5 + a.lg)) + ((nk & (a.block - 1)) != 0);
   int n = 0;
-  if ((int64_t)at.t * a.block < nq) n = block_list(idx, first_places, a.top, blocks, list, &count);
+  if (at.t * a.block < nq) n = block_list(idx, first_places, a.top, blocks, list, &count);
 
   const int64_t ir = valid ? i : 0;
   const T* qp = (const T*)a.q.p + at.b * a.q.b + ir * a.q.l + h * a.q.h;
@@ -535,15 +536,15 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 2 ? (DP > 64 || RW == 1 ? 2
 
   f32x16 dq[ND] = {};
   const int units = n << a.lg;
-  const Keys where_ = {list, a.block, a.lg, units, nk};
+  const Keys where_ = {list, a.lg, units, nk};
   Stage<T, DP, KW> sk, sv;
   const auto fetch = [&](int u) {
     const Span<KW> s = where_.span<KW>(u);
     const T *pk[KW], *pv[KW];
 #pragma unroll
     for (int j = 0; j < KW; ++j) {
-      pk[j] = kp + s.first[j] * a.k.l;
-      pv[j] = vp + s.first[j] * a.v.l;
+      pk[j] = row_at(kp, s.first[j], a.k.l);
+      pv[j] = row_at(vp, s.first[j], a.v.l);
     }
     sk.load(pk, s.n, a.k.l, a.D);
     sv.load(pv, s.n, a.v.l, a.D);
@@ -640,7 +641,7 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 2 ? (DP <= 64 ? (RW == 1 ? 
   const int blk = item % a.Tk, hk = item / a.Tk % a.Hkv, b = item / a.Tk / a.Hkv;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, col = lane & 31;
   const int rw = uniform(wave) % RW, qw = uniform(wave) / RW;
-  const int64_t nq = length_of(a.q_lengths, b, a.Lq), nk = length_of(a.kv_lengths, b, a.Lk);
+  const int nq = length_of(a.q_lengths, b, a.Lq), nk = length_of(a.kv_lengths, b, a.Lk);
   const int64_t key = (int64_t)blk * a.block + 32 * rw + col;
   const bool exists = key < a.Lk, valid = key < nk;
   // the block's keys and values: f32 in registers, 16 bits in LDS (from there they cost a third more of its
@@ -664,7 +665,7 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 2 ? (DP <= 64 ? (RW == 1 ? 
 #pragma unroll
     for (int j = 0; j < RW; ++j) {
       const int64_t k0 = (int64_t)blk * a.block + 32 * j;
-      have[j] = (int)max((int64_t)0, min((int64_t)32, nk - k0));
+      have[j] = (int)max((int64_t)0, min((int64_t)32, (int64_t)nk - k0));
       pk[j] = (const T*)a.k.p + b * a.k.b + k0 * a.k.l + hk * a.k.h;
       pv[j] = (const T*)a.v.p + b * a.v.b + k0 * a.v.l + hk * a.v.h;
     }
@@ -680,7 +681,9 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 2 ? (DP <= 64 ? (RW == 1 ? 
   f32x16 dk[ND] = {}, dv[ND] = {};
   const int upt = a.G << a.lg, words = (a.Tq + 31) / 32;  // units per tile
   const uint32_t* bits = a.bits + (((int64_t)b * a.Hkv + hk) * a.Tk + blk) * words;
-  const bool any = (int64_t)blk * a.block < nk;
+  const bool any = blk * a.block < nk;
+  const T* qb = (const T*)a.q.p + b * a.q.b + (int64_t)hk * a.G * a.q.h;
+  const T* gb = (const T*)a.g.p + b * a.g.b + (int64_t)hk * a.G * a.g.h;
   const int u0 = blockIdx.y * QW, stride = gridDim.y * QW;  // this part's steps
   int step = 0;
   for (int w0 = 0; any && w0 < words; w0 += kTiles / 32) {
@@ -714,11 +717,11 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 2 ? (DP <= 64 ? (RW == 1 ? 
       for (int j = 0; j < QW; ++j) tile[j] = tiles[pos(min(u + j, units - 1))];
 #pragma unroll
       for (int j = 0; j < QW; ++j) {
-        const int64_t i0 = (int64_t)uniform(tile[j]) * a.block + 32 * ((u + j) & ((1 << a.lg) - 1));
-        const int h = hk * a.G + ((u + j) >> a.lg) - pos(u + j) * a.G;
-        pq[j] = (const T*)a.q.p + b * a.q.b + i0 * a.q.l + h * a.q.h;
-        pg[j] = (const T*)a.g.p + b * a.g.b + i0 * a.g.l + h * a.g.h;
-        have[j] = u + j < units ? (int)max((int64_t)0, min((int64_t)32, nq - i0)) : 0;
+        const int i0 = ((uniform(tile[j]) << a.lg) + ((u + j) & ((1 << a.lg) - 1))) * 32;
+        const int64_t g = ((u + j) >> a.lg) - pos(u + j) * a.G;
+        pq[j] = row_at(qb, i0, a.q.l) + g * a.q.h;
+        pg[j] = row_at(gb, i0, a.g.l) + g * a.g.h;
+        have[j] = u + j < units ? max(0, min(32, nq - i0)) : 0;
       }
       f.q.load(pq, have, a.q.l, a.D);
       f.g.load(pg, have, a.g.l, a.D);
@@ -727,7 +730,7 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 2 ? (DP <= 64 ? (RW == 1 ? 
         f.lse = -INFINITY;
         if (uj < units) {
           const int at = pos(uj);
-          const int64_t i = (int64_t)tiles[at] * a.block + 32 * (uj & ((1 << a.lg) - 1)) + r;
+          const int i = ((tiles[at] << a.lg) + (uj & ((1 << a.lg) - 1))) * 32 + r;
           if (i < nq) {
             const int64_t stat = ((int64_t)b * a.Hq + hk * a.G + (uj >> a.lg) - at * a.G) * a.Lq + i;
             f.lse = a.lse[stat];

@@ -133,7 +133,7 @@ int check(const dtk_attention* c, const char* who) {
   DSPLAT_REQUIRE(c->Hq / c->Hkv <= 1024, "%s: more than 1024 query heads per key head", who);
   for (const int64_t* s : {c->q_strides, c->k_strides, c->v_strides})
     DSPLAT_REQUIRE(s[1] >= 0 && s[1] < (1LL << 24), "%s: a token stride must be below 2^24 elements", who);
-  DSPLAT_REQUIRE(c->Lq < (1LL << 31) && c->Lk < (1LL << 31) && c->Hq < 65536 && c->B < 65536, "%s: too large", who);
+  DSPLAT_REQUIRE(c->Lq <= (1LL << 31) - 256 && c->Lk <= (1LL << 31) - 256 && c->Hq < 65536 && c->B < 65536, "%s: too large", who);
   DSPLAT_REQUIRE(c->B == 0 || c->Lq == 0 || (c->q && c->o && c->index && (c->Lk == 0 || (c->k && c->v))), "%s: null pointer", who);
   return 0;
 }
