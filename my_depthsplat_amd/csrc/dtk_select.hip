@@ -32,9 +32,17 @@ struct PoolArgs {
   int64_t L[2];
   int group[2];  // heads that share a pooled row
   int Tq, D, pitch, block;
-  double* out[2];  // [B, Hkv, tiles, pitch]: zeros from D on
+  double* out[2];  // [B, Hkv], packed (below): zeros from D on
 };
 inline int pitch_of(int D) { return (D + 7) & ~7; }
+__host__ __device__ inline int64_t padded(int64_t tiles) { return (tiles + 15) & ~(int64_t)15; }
+// Where channel d of pooled row t lies: 16 rows together, in the order in which the matrix instruction's lanes read
+// them (lane group lane / 16 takes a quarter of the channels, two at a time), so that a load is 1 KB in a row. (Rows one
+// after the other put the 64 lanes of a load on 64 lines: the scores of 360 x 360 and 1440 x 1440 took 28 us instead of 17 on average.)
+__device__ __forceinline__ int64_t packed(int t, int d, int pitch) {
+  const int per = pitch / 4, quarter = d / per, i = d % per;
+  return ((int64_t)(t / 16) * (per / 2) + i / 2) * 128 + (quarter * 16 + t % 16) * 2 + i % 2;
+}
 
 // One workgroup per tile: a thread sums one 16-byte piece of every (256 / pieces)-th row, the
 // threads of a piece are folded through LDS in a fixed order.
@@ -67,19 +75,18 @@ __global__ __launch_bounds__(NT) void k_pool(PoolArgs a) {
 #pragma unroll
   for (int e = 0; e < N; ++e) red[e * NT + threadIdx.x] = s[e];
   __syncthreads();
-  double* out = a.out[which] + (((int64_t)b * gridDim.y + hk) * tiles + t) * a.pitch;
+  double* out = a.out[which] + ((int64_t)b * gridDim.y + hk) * padded(tiles) * a.pitch;
   const double inv = n ? 1.0 / (double)(n * group) : 0.0;
   for (int d = threadIdx.x; d < a.pitch; d += NT) {
     double v = 0.0;
     if (d < a.D)
       for (int k = 0; k < parts; ++k) v += red[(d % N) * NT + k * pieces + d / N];
-    out[d] = v * inv;
+    out[packed(t, d, a.pitch)] = v * inv;
   }
 }
 
 // Scores on the 64-bit matrix instruction (16 x 16 x 4): a wave takes 32 query tiles x 64 key
-// blocks, the workgroup's 4 waves stand side by side over 256 blocks. Lane group lane / 16 takes a
-// quarter of the channels in order, so each lane reads its pooled rows as 16-byte vectors.
+// blocks, the workgroup's 4 waves stand side by side over 256 blocks.
 typedef double f64x4 __attribute__((ext_vector_type(4)));
 typedef double f64x2 __attribute__((ext_vector_type(2)));
 __global__ __launch_bounds__(NT) void k_scores(int Tq, int Tk, int pitch, const double* __restrict__ qm,
@@ -88,20 +95,21 @@ __global__ __launch_bounds__(NT) void k_scores(int Tq, int Tk, int pitch, const 
   const int lane = threadIdx.x & 63, col = lane & 15, quarter = lane >> 4;
   const int q0 = blockIdx.y * 32, k0 = (blockIdx.x * 4 + (threadIdx.x >> 6)) * 64;
   if (k0 >= Tk) return;
-  const int per = pitch / 4;
+  const int steps = pitch / 8;
+  const int qlast = (int)padded(Tq) - 16, klast = (int)padded(Tk) - 16;  // groups behind the last are read as the last
   const double *ap[2], *bp[4];
 #pragma unroll
-  for (int i = 0; i < 2; ++i) ap[i] = qm + (z * Tq + min(q0 + 16 * i + col, Tq - 1)) * pitch + quarter * per;
+  for (int i = 0; i < 2; ++i) ap[i] = qm + (z * padded(Tq) + min(q0 + 16 * i, qlast)) * pitch + lane * 2;
 #pragma unroll
-  for (int j = 0; j < 4; ++j) bp[j] = km + (z * Tk + min(k0 + 16 * j + col, Tk - 1)) * pitch + quarter * per;
+  for (int j = 0; j < 4; ++j) bp[j] = km + (z * padded(Tk) + min(k0 + 16 * j, klast)) * pitch + lane * 2;
   f64x4 acc[2][4] = {};
 #pragma unroll 2
-  for (int d = 0; d < per; d += 2) {
+  for (int d = 0; d < steps; ++d) {
     f64x2 av[2], bv[4];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) av[i] = *(const f64x2*)(ap[i] + d);
+    for (int i = 0; i < 2; ++i) av[i] = *(const f64x2*)(ap[i] + d * 128);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) bv[j] = *(const f64x2*)(bp[j] + d);
+    for (int j = 0; j < 4; ++j) bv[j] = *(const f64x2*)(bp[j] + d * 128);
 #pragma unroll
     for (int e = 0; e < 2; ++e)
 #pragma unroll
@@ -114,9 +122,11 @@ __global__ __launch_bounds__(NT) void k_scores(int Tq, int Tk, int pitch, const 
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int q = q0 + 16 * i + 4 * r + quarter;
+      if (q >= Tq) continue;
+      double* out = score + (z * Tq + q) * Tk + k0 + col;
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        if (q < Tq && k0 + 16 * j + col < Tk) score[(z * Tq + q) * Tk + k0 + 16 * j + col] = acc[i][j][r];
+        if (k0 + 16 * j + col < Tk) out[16 * j] = acc[i][j][r];
     }
 }
 
@@ -141,7 +151,8 @@ struct ChooseArgs {
 // A wave per tile, 64 NV >= Tk keys in registers (place 64 j + lane in slot j). The key of the last chosen
 // place is found from its highest bit down: a bit is kept if at least `top` keys reach the number with
 // it. As soon as exactly `top` do, they are the answer: for scores that differ early, as they
-// do, well before the lower 32 bits are looked at.
+// do, well before the lower 32 bits are looked at. (Halving the interval of the scores instead takes
+// fewer turns, but they are not what the time goes into: 27 and 13 us against 28 and 12.5 for 1440 and 360 blocks.)
 template <int NV>
 __global__ __launch_bounds__(NT) void k_choose(ChooseArgs a) {
   const int64_t row = (int64_t)blockIdx.x * (NT / 64) + (threadIdx.x >> 6);
@@ -152,12 +163,23 @@ __global__ __launch_bounds__(NT) void k_choose(ChooseArgs a) {
   const int blocks = (int64_t)t * a.block < nq ? (int)((nk + a.block - 1) / a.block) : 0;  // blocks with a key
   const double* score = a.score + row * a.Tk;
   const uint8_t* may = a.allowed ? a.allowed + (int64_t)t * a.Tk : nullptr;
+  if (blocks == 0) {  // (there may be no scores at all: nothing is read)
+    for (int i = lane; i < a.top; i += 64) out[i] = -1;
+    return;
+  }
   uint32_t hi[NV], lo[NV];
   int have = 0;
+  double v[NV];
+  uint8_t ok[NV];
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {  // all on their way together
+    const int i = min(64 * j + lane, a.Tk - 1);
+    v[j] = score[i];
+    ok[j] = may ? may[i] : 1;
+  }
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
-    const int i = 64 * j + lane;
-    const uint64_t k = i < blocks && (!may || may[i]) ? order_key(score[i]) : 0;
+    const uint64_t k = 64 * j + lane < blocks && ok[j] ? order_key(v[j]) : 0;
     hi[j] = (uint32_t)(k >> 32);
     lo[j] = (uint32_t)k;
     have += __popcll(__ballot(k != 0));
@@ -306,7 +328,7 @@ extern "C" {
 size_t dtk_select_blocks_workspace_size(int B, int64_t Lq, int64_t Lk, int Hkv, int D, int block) {
   if (B <= 0 || Lq <= 0 || Lk <= 0 || Hkv <= 0 || D <= 0 || block <= 0) return 0;
   const size_t tq = tiles_of(Lq, block), tk = tiles_of(Lk, block);
-  return (size_t)B * Hkv * ((tq + tk) * pitch_of(D) + tq * tk) * sizeof(double);
+  return (size_t)B * Hkv * ((padded(tq) + padded(tk)) * pitch_of(D) + tq * tk) * sizeof(double);
 }
 
 int dtk_select_blocks(int B, int64_t Lq, int64_t Lk, int Hq, int Hkv, int D, int block, int top, int dtype,
@@ -325,8 +347,8 @@ int dtk_select_blocks(int B, int64_t Lq, int64_t Lk, int Hq, int Hkv, int D, int
   hipStream_t st = (hipStream_t)stream;
   const int pitch = pitch_of(D);
   double* qm = (double*)workspace;
-  double* km = qm + (size_t)B * Hkv * Tq * pitch;
-  double* score = km + (size_t)B * Hkv * Tk * pitch;
+  double* km = qm + (size_t)B * Hkv * padded(Tq) * pitch;
+  double* score = km + (size_t)B * Hkv * padded(Tk) * pitch;
   if (Lk > 0) {
     const PoolArgs a = {{{q, q_strides[0], q_strides[1], q_strides[2], q_lengths}, {k, k_strides[0], k_strides[1], k_strides[2], kv_lengths}},
                         {Lq, Lk}, {Hq / Hkv, 1}, Tq, D, pitch, block, {qm, km}};
@@ -343,6 +365,8 @@ int dtk_select_blocks(int B, int64_t Lq, int64_t Lk, int Hq, int Hkv, int D, int
   const unsigned waves = (unsigned)((a.rows + NT / 64 - 1) / (NT / 64));
   if (Tk <= 64 * 2) k_choose<2><<<waves, NT, 0, st>>>(a);
   else if (Tk <= 64 * 8) k_choose<8><<<waves, NT, 0, st>>>(a);
+  else if (Tk <= 64 * 16) k_choose<16><<<waves, NT, 0, st>>>(a);
+  else if (Tk <= 64 * 24) k_choose<24><<<waves, NT, 0, st>>>(a);
   else if (Tk <= 64 * 32) k_choose<32><<<waves, NT, 0, st>>>(a);
   else k_choose_long<<<(unsigned)a.rows, NT, 0, st>>>(a);
   return dsplat::check_launch("k_choose");
