@@ -71,8 +71,9 @@ struct Args {
   float *lse;                // [B, Hq, Lq], base 2; -inf for rows without a key
   float *part, *part_m, *part_l;
   float* delta;
-  uint32_t *bits, *gmax, *chosen;  // chosen, order: NULL where every workgroup of dk/dv fits the chip at once
-  int32_t* order;
+  uint32_t *bits, *gmax, *chosen;
+  int4 *plan, *split;  // NULL where every list is short and every workgroup of dk/dv fits the chip at once
+  int* planned;        // how many of each
 };
 
 __device__ __forceinline__ int length_of(const int32_t* lengths, int b, int64_t L) {  // fewer than 2^31 (the host checks)
@@ -620,8 +621,8 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 2 ? (DP > 64 || RW == 1 ? 2
 
 // dk, dv of one key block: RW waves hold 32 keys each, 4 / RW take turns at the 32-query units of
 // the tiles that chose the block (their bits, some at a time) and are joined at the end. Every sum
-// has one order: no atomics on the gradients. (Few blocks with long lists: gridDim.y parts of each, every
-// gridDim.y-th step.)
+// has one order: no atomics on the gradients. A long list is worked off by several workgroups, each taking every
+// parts-th step.
 constexpr int kTiles = 1024;  // tiles listed at a time
 template <typename T>
 constexpr int kDkvBuffers = 1;
@@ -637,7 +638,15 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 2 ? (DP <= 64 ? (RW == 1 ? 
   __shared__ int32_t tiles[kTiles];
   __shared__ int count;
   __shared__ __align__(16) float stats[NB][2][QW * 32];  // lse and delta of the staged rows
-  const int item = a.order ? a.order[blockIdx.x] : (int)blockIdx.x;
+  int item = blockIdx.x, part = 0, parts = 1, slot = 0;
+  if (a.plan) {
+    if ((int)blockIdx.x >= a.planned[0]) return;
+    const int4 e = a.plan[blockIdx.x];
+    item = e.x;
+    part = e.y;
+    parts = e.z;
+    slot = e.w;
+  }
   const int blk = item % a.Tk, hk = item / a.Tk % a.Hkv, b = item / a.Tk / a.Hkv;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, col = lane & 31;
   const int rw = uniform(wave) % RW, qw = uniform(wave) / RW;
@@ -684,7 +693,7 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 2 ? (DP <= 64 ? (RW == 1 ? 
   const bool any = blk * a.block < nk;
   const T* qb = (const T*)a.q.p + b * a.q.b + (int64_t)hk * a.G * a.q.h;
   const T* gb = (const T*)a.g.p + b * a.g.b + (int64_t)hk * a.G * a.g.h;
-  const int u0 = blockIdx.y * QW, stride = gridDim.y * QW;  // this part's steps
+  const int u0 = part * QW, stride = parts * QW;  // this part's steps
   int step = 0;
   for (int w0 = 0; any && w0 < words; w0 += kTiles / 32) {
     __syncthreads();
@@ -817,9 +826,9 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 2 ? (DP <= 64 ? (RW == 1 ? 
   }
   if (qw != 0 || !exists) return;
   const int64_t off = (((int64_t)b * a.Lk + key) * a.Hkv + hk) * a.D;
-  if (gridDim.y > 1) {  // one of several parts: k_attend_dkv_join adds them up
-    const int64_t n = (int64_t)(gridDim.x / a.Tk / a.Hkv) * a.Lk * a.Hkv * a.D;
-    float *pk = a.part + (int64_t)blockIdx.y * 2 * n + off, *pv = pk + n;
+  if (parts > 1) {  // k_attend_dkv_join adds them up
+    float* pk = a.part + (((int64_t)slot + part) * 2 * a.block + 32 * rw + col) * a.D;
+    float* pv = pk + (int64_t)a.block * a.D;
 #pragma unroll
     for (int d = 0; d < ND; ++d)
 #pragma unroll

@@ -67,54 +67,85 @@ __global__ __launch_bounds__(NT) void k_attend_mark(Args a) {
   }
 }
 
-// The blocks with the longest lists first: they are workgroups of dk/dv, the longest of which would
-// otherwise run on alone at the end (a popular block is chosen several times as often as the mean). One
-// workgroup sorts by the list's length, eight steps to a power of two; the order within a step does not matter.
-constexpr int kSteps = 264, kOrderThreads = 1024;
-__device__ __forceinline__ int length_step(uint32_t n) {  // 0 for the longest
-  if (n < 8) return kSteps - 1 - (int)n;
+// The workgroups of dk/dv: a popular block is chosen several times as often as the mean, so a list of more than `most`
+// steps is cut into equal parts, and the longest parts come first (whatever starts last then ends soon). One
+// workgroup sorts by the steps of a part, eight grades to a power of two; the order within a grade does not matter.
+constexpr int kGrades = 264, kPlanThreads = 1024;
+__device__ __forceinline__ int grade_of(uint32_t n) {  // 0 for the longest
+  if (n < 8) return kGrades - 1 - (int)n;
   const int e = 31 - __clz(n);
-  return kSteps - 1 - (8 * (e - 2) + (int)((n >> (e - 3)) & 7));
+  return kGrades - 1 - (8 * (e - 2) + (int)((n >> (e - 3)) & 7));
 }
-__global__ __launch_bounds__(kOrderThreads) void k_attend_order(Args a, int items) {
-  __shared__ int at[kSteps];
-  for (int i = threadIdx.x; i < kSteps; i += kOrderThreads) at[i] = 0;
+__global__ __launch_bounds__(kPlanThreads) void k_attend_plan(Args a, int items, int most) {
+  __shared__ int at[kGrades];
+  __shared__ int all, slots, splits;
+  for (int i = threadIdx.x; i < kGrades; i += kPlanThreads) at[i] = 0;
+  if (threadIdx.x == 0) slots = splits = 0;
+  const int units = a.G << a.lg, together = 128 / a.block;  // of a tile, in a step
+  const auto parts_of = [&](int i, int& grade) {
+    const int64_t steps = ((int64_t)a.chosen[i] * units + together - 1) / together;
+    const int n = (int)max((int64_t)1, (steps + most - 1) / most);
+    grade = grade_of((uint32_t)((steps + n - 1) / n));
+    return n;
+  };
   __syncthreads();
-  for (int i = threadIdx.x; i < items; i += kOrderThreads) atomicAdd(&at[length_step(a.chosen[i])], 1);
-  __syncthreads();
-  if (threadIdx.x < 64) {  // exclusive sums, 64 steps at a time
-    int before = 0;
-    for (int base = 0; base < kSteps; base += 64) {
-      const int i = base + (int)threadIdx.x;
-      const int n = i < kSteps ? at[i] : 0;
-      const int incl = (int)dsplat::wave_incl_scan((uint32_t)n, threadIdx.x);
-      if (i < kSteps) at[i] = before + incl - n;
-      before += __shfl(incl, 63, 64);
-    }
+  for (int i = threadIdx.x; i < items; i += kPlanThreads) {
+    int grade;
+    const int n = parts_of(i, grade);
+    atomicAdd(&at[grade], n);
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < items; i += kOrderThreads) a.order[atomicAdd(&at[length_step(a.chosen[i])], 1)] = i;
+  if (threadIdx.x < 64) {  // exclusive sums, 64 grades at a time
+    int before = 0;
+    for (int base = 0; base < kGrades; base += 64) {
+      const int i = base + (int)threadIdx.x;
+      const int n = i < kGrades ? at[i] : 0;
+      const int incl = (int)dsplat::wave_incl_scan((uint32_t)n, threadIdx.x);
+      if (i < kGrades) at[i] = before + incl - n;
+      before += __shfl(incl, 63, 64);
+    }
+    if (threadIdx.x == 0) all = before;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < items; i += kPlanThreads) {
+    int grade, slot = 0;
+    const int n = parts_of(i, grade), to = atomicAdd(&at[grade], n);
+    if (n > 1) {
+      slot = atomicAdd(&slots, n);
+      a.split[atomicAdd(&splits, 1)] = make_int4(i, slot, n, 0);
+    }
+    for (int k = 0; k < n; ++k) a.plan[to + k] = make_int4(i, k, n, slot);
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    a.planned[0] = all;
+    a.planned[1] = splits;
+  }
 }
 
 // Adds up the parts of dk and dv in order: four channels of a key per thread; 0 behind the lengths.
 template <typename T>
-__global__ __launch_bounds__(NT) void k_attend_dkv_join(Args a, int64_t n, int parts) {
-  const int64_t i = ((int64_t)blockIdx.x * NT + threadIdx.x) * 4;
-  if (i >= n) return;
-  const int64_t key = i / ((int64_t)a.Hkv * a.D), b = key / a.Lk;
-  const bool valid = key - b * a.Lk < length_of(a.kv_lengths, (int)b, a.Lk);
+__global__ __launch_bounds__(NT) void k_attend_dkv_join(Args a) {
+  if ((int)blockIdx.x >= a.planned[1]) return;
+  const int4 e = a.split[blockIdx.x];
+  const int blk = e.x % a.Tk, hk = e.x / a.Tk % a.Hkv, b = e.x / a.Tk / a.Hkv;
+  const int per = a.D / 4, i = blockIdx.y * NT + threadIdx.x, row = i / per, d = (i - row * per) * 4;
+  const int64_t key = (int64_t)blk * a.block + row;
+  if (row >= a.block || key >= a.Lk) return;
+  const bool valid = key < length_of(a.kv_lengths, b, a.Lk);
+  const int64_t n = (int64_t)a.block * a.D, to = ((b * a.Lk + key) * a.Hkv + hk) * a.D + d;
 #pragma unroll
   for (int which = 0; which < 2; ++which) {
     float s[4] = {};
     if (valid)
-      for (int k = 0; k < parts; ++k) {
-        const float4 v = *(const float4*)(a.part + (2 * k + which) * n + i);
+      for (int k = 0; k < e.z; ++k) {
+        const float4 v = *(const float4*)(a.part + (2 * ((int64_t)e.y + k) + which) * n + (int64_t)row * a.D + d);
         s[0] += v.x;
         s[1] += v.y;
         s[2] += v.z;
         s[3] += v.w;
       }
-    store4<T>((T*)(which ? a.dv : a.dk) + i, s[0], s[1], s[2], s[3]);
+    store4<T>((T*)(which ? a.dv : a.dk) + to, s[0], s[1], s[2], s[3]);
   }
 }
 
@@ -170,30 +201,34 @@ Args args_of(const dtk_attention* c) {
 }
 size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
 
-// The backward's workspace: delta, then what is cleared (the largest |do|, the lists' bits and lengths), the order.
+// The backward's workspace: delta, what is cleared (the largest |do|, the lists' bits and lengths), the plan of dk/dv,
+// the parts in f32.
 struct BwdLayout {
-  size_t gmax, bits, chosen, order, end;
-  size_t part;
-  int64_t items;
-  bool sorted;
-  int parts;
+  size_t gmax, bits, chosen, planned, plan, split, part, end;
+  int64_t items, slots;  // slots: parts of split lists, at most
+  int most;              // steps of a part; 0: no plan
 };
 BwdLayout layout_of(const dtk_attention* c, const Args& a) {
   BwdLayout l;
+  const int64_t together = 128 / a.block, units = (int64_t)a.G << a.lg;
   l.items = (int64_t)c->B * c->Hkv * a.Tk;
-  l.sorted = l.items > 512;
+  // Steps of all lists, at most (a list entry that stands twice counts once).
+  const int64_t steps = (int64_t)c->B * c->Hkv * a.Tq * (a.top < a.Tk ? a.top : a.Tk) * units / together;
+  // A part: a 1024th of all (a few per CU, whatever the lists' lengths), and 8 steps or more. 16 scenes of 2048 f32
+  // tokens of 128 channels, 512 blocks: whole lists in any order 304 us, parts of 8 steps 208 us and 9 us for their join, of
+  // 4 steps 230 + 16. 4 scenes of 32256 bf16 tokens, 4032 blocks: whole lists, the longest first, 293 us; 512ths 296,
+  // 1024ths 264, 2048ths 265.
+  const int64_t most = steps / 1024 > 8 ? steps / 1024 : 8;
+  l.most = l.items > 512 || a.Tq * units > most * together ? (int)(most < (1 << 30) ? most : 1 << 30) : 0;
+  l.slots = l.most ? 2 * steps / l.most + 1 : 0;  // a list of n > most steps has fewer than 2 n / most parts
   l.gmax = align256((size_t)c->B * c->Hq * c->Lq * 4);
   l.bits = l.gmax + 256;
   l.chosen = l.bits + (size_t)l.items * ((a.Tq + 31) / 32) * 4;
-  l.order = l.chosen + (l.sorted ? (size_t)l.items * 4 : 0);
-  // Parts of the lists, in f32: where the blocks are too few to fill the chip and to even out their lists, down to
-  // 8 steps of the mean list each. (2 x 16384 tokens, 4 heads on one: 512 workgroups of 128 steps 390 us, four
-  // parts 215 us and 27 us for their join.)
-  const int64_t steps = a.Tk ? (int64_t)a.Tq * a.top * a.G * (a.block / 32) / a.Tk / (4 * 32 / a.block ? 4 * 32 / a.block : 1) : 0;
-  l.parts = 1;
-  while (l.items * l.parts < 2048 && l.parts * 16 <= steps) l.parts *= 2;
-  l.part = align256(l.order + (l.sorted ? (size_t)l.items * 4 : 0));
-  l.end = l.part + (l.parts > 1 ? (size_t)l.parts * 2 * c->B * c->Lk * c->Hkv * c->D * 4 : 0);
+  l.planned = align256(l.chosen + (l.most ? (size_t)l.items * 4 : 0));
+  l.plan = l.planned + 256;
+  l.split = l.plan + (l.most ? (size_t)(l.items + l.slots) * sizeof(int4) : 0);
+  l.part = align256(l.split + (size_t)(l.slots / 2) * sizeof(int4));
+  l.end = l.part + (size_t)l.slots * 2 * a.block * c->D * 4;
   return l;
 }
 
@@ -254,15 +289,18 @@ int dtk_block_sparse_attention_bwd(const dtk_attention* c, const void* dout, con
   a.dv = dv;
   char* ws = (char*)workspace;
   const BwdLayout l = layout_of(c, a);
-  DSPLAT_REQUIRE(l.items < (1LL << 31), "dtk_block_sparse_attention_bwd: too large");
+  DSPLAT_REQUIRE(l.items + l.slots < (1LL << 31), "dtk_block_sparse_attention_bwd: too large");
   a.delta = (float*)ws;
   a.gmax = (uint32_t*)(ws + l.gmax);
   a.bits = (uint32_t*)(ws + l.bits);
-  if (l.sorted) {
+  if (l.most) {
     a.chosen = (uint32_t*)(ws + l.chosen);
-    a.order = (int32_t*)(ws + l.order);
+    a.planned = (int*)(ws + l.planned);
+    a.plan = (int4*)(ws + l.plan);
+    a.split = (int4*)(ws + l.split);
+    a.part = (float*)(ws + l.part);
   }
-  if (int e = dsplat::zero_async(a.gmax, l.order - l.gmax, st, "dtk_block_sparse_attention_bwd")) return e;
+  if (int e = dsplat::zero_async(a.gmax, l.planned - l.gmax, st, "dtk_block_sparse_attention_bwd")) return e;
   if (c->Lq) {
     const dim3 grid(a.Tq * a.rowtiles, a.Hkv, c->B);
     if (int e = by_type(c->dtype, attend_dq<float>, attend_dq<bf16>, attend_dq<f16>)(a, row_waves(a), grid, st)) return e;
@@ -272,18 +310,16 @@ int dtk_block_sparse_attention_bwd(const dtk_attention* c, const void* dout, con
     }
   }
   if (!a.Tk) return 0;
-  if (l.sorted) {
-    k_attend_order<<<1, kOrderThreads, 0, st>>>(a, (int)l.items);
-    if (int e = dsplat::check_launch("k_attend_order")) return e;
+  if (l.most) {
+    k_attend_plan<<<1, kPlanThreads, 0, st>>>(a, (int)l.items, l.most);
+    if (int e = dsplat::check_launch("k_attend_plan")) return e;
   }
-  a.part = (float*)(ws + l.part);
-  if (int e = by_type(c->dtype, attend_dkv<float>, attend_dkv<bf16>, attend_dkv<f16>)(a, a.block / 32, dim3((unsigned)l.items, l.parts), st)) return e;
-  if (l.parts == 1) return 0;
-  const int64_t n = (int64_t)c->B * c->Lk * c->Hkv * c->D;
-  const unsigned blocks = (unsigned)((n / 4 + NT - 1) / NT);
-  if (c->dtype == DTK_F32) k_attend_dkv_join<float><<<blocks, NT, 0, st>>>(a, n, l.parts);
-  else if (c->dtype == DTK_BF16) k_attend_dkv_join<bf16><<<blocks, NT, 0, st>>>(a, n, l.parts);
-  else k_attend_dkv_join<f16><<<blocks, NT, 0, st>>>(a, n, l.parts);
+  if (int e = by_type(c->dtype, attend_dkv<float>, attend_dkv<bf16>, attend_dkv<f16>)(a, a.block / 32, dim3((unsigned)(l.items + l.slots)), st)) return e;
+  if (l.slots < 2) return 0;
+  const dim3 blocks((unsigned)(l.slots / 2), (a.block * a.D / 4 + NT - 1) / NT);
+  if (c->dtype == DTK_F32) k_attend_dkv_join<float><<<blocks, NT, 0, st>>>(a);
+  else if (c->dtype == DTK_BF16) k_attend_dkv_join<bf16><<<blocks, NT, 0, st>>>(a);
+  else k_attend_dkv_join<f16><<<blocks, NT, 0, st>>>(a);
   return dsplat::check_launch("k_attend_dkv_join");
 }
 
