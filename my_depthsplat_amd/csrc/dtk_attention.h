@@ -289,7 +289,7 @@ struct Join {
 // of 32 keys and are joined at the end. The rows of a tile are its queries of all heads that
 // share the key head (few queries: they fill the instruction's columns together).
 template <typename T, int DP, int RW>
-__global__ __launch_bounds__(kThreads, (sizeof(T) == 2 ? (DP > 64 || RW == 1 ? 2 : 4) : 1)) void k_attend_fwd(Args a) {
+__global__ __launch_bounds__(kThreads, (sizeof(T) == 2 ? (DP > 64 || RW == 1 ? 2 : 4) : 2)) void k_attend_fwd(Args a) {
   using M = Mma<T>;
   using L = Tile<T, DP>;
   using Frag = typename M::Frag;
@@ -331,36 +331,51 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 2 ? (DP > 64 || RW == 1 ? 2
   const int per = (units + a.splits - 1) / a.splits;
   const int u0 = min(units, at.split * per), u1 = min(units, u0 + per);
   const Keys where_ = {list, a.lg, u1, nk};
+  // A step's keys and values come together, while the step before is worked on; or, for f32 rows of more than 64
+  // channels, in turn through the same registers, the values during the first product and the next keys during
+  // the second (which take 4096 cycles each at 128 channels), so that two waves per SIMD fit: 16 scenes of
+  // 2048 tokens of 128 channels, 8 blocks of 64 each, 91 us instead of 106. (Where both fit anyway, the second barrier costs:
+  // 2 x 16384 tokens of 64 channels, 4 heads on one: 320 us instead of 287.)
+  constexpr bool TURNS = sizeof(T) == 4 && DP > 64;
   Stage<T, DP, KW> sk, sv;
-  const auto fetch = [&](int u) {
-    const Span<KW> s = where_.span<KW>(u);
-    const T *pk[KW], *pv[KW];
+  const auto load = [&](Stage<T, DP, KW>& to, const Span<KW>& s, const T* p, int64_t stride) {
+    const T* rows[KW];
 #pragma unroll
-    for (int j = 0; j < KW; ++j) {
-      pk[j] = row_at(kp, s.first[j], a.k.l);
-      pv[j] = row_at(vp, s.first[j], a.v.l);
-    }
-    sk.load(pk, s.n, a.k.l, a.D);
-    sv.load(pv, s.n, a.v.l, a.D);
-    return pick(s.n, kw);
+    for (int j = 0; j < KW; ++j) rows[j] = row_at(p, s.first[j], stride);
+    to.load(rows, s.n, stride, a.D);
   };
-  int ahead = u0 < u1 ? fetch(u0) : 0;
+  Span<KW> next = {};
+  const auto fetch = [&](int u) {
+    next = where_.span<KW>(u);
+    load(sk, next, kp, a.k.l);
+    if (!TURNS) load(sv, next, vp, a.v.l);
+  };
+  if (u0 < u1) fetch(u0);
   bool begun = false;
   for (int u = u0, step = 0; u < u1; u += KW, ++step) {
     char* tk = lds + (step % NB) * 2 * KW * L::kUnit;
     char* tv = tk + KW * L::kUnit;
-    if (NB == 1) __syncthreads();
+    if (NB == 1 && !TURNS) __syncthreads();
     sk.store(tk);
-    sv.store(tv);
+    if (!TURNS) sv.store(tv);
     __syncthreads();
-    const int left = ahead;
-    if (u + KW < u1) ahead = fetch(u + KW);
+    const int left = pick(next.n, kw);
+    if (TURNS) load(sk, next, vp, a.v.l);
+    else if (u + KW < u1) fetch(u + KW);
     tk += kw * L::kUnit;
-    tv += kw * L::kUnit;
-    if (left == 0) continue;
+    if (!TURNS && left == 0) continue;
     f32x16 x = {};
+    if (!TURNS || left > 0) {
 #pragma unroll
-    for (int s = 0; s < NS; ++s) x = M::mma(L::row(tk, s, col, half), qf[s], x);
+      for (int s = 0; s < NS; ++s) x = M::mma(L::row(tk, s, col, half), qf[s], x);
+    }
+    if (TURNS) {
+      sk.store(tv);  // every wave is past the products of the values before
+      if (u + KW < u1) fetch(u + KW);
+      __syncthreads();  // (and of these keys)
+    }
+    tv += kw * L::kUnit;
+    if (TURNS && left == 0) continue;
     if (left < 32) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) x[r] = acc_row(r, half) < left ? x[r] : -INFINITY;
@@ -478,7 +493,7 @@ __device__ __forceinline__ void ds_scale(uint32_t largest, float& down, float& u
 // dq: the forward's shape; p is taken from the saved lse. delta = sum_d do o of each row on the
 // way, kept for dk.
 template <typename T, int DP, int RW>
-__global__ __launch_bounds__(kThreads, (sizeof(T) == 2 ? (DP > 64 || RW == 1 ? 2 : 3) : 1)) void k_attend_dq(Args a) {
+__global__ __launch_bounds__(kThreads, (sizeof(T) == 2 ? (DP > 64 || RW == 1 ? 2 : 3) : DP <= 64 ? 2 : 1)) void k_attend_dq(Args a) {
   using M = Mma<T>;
   using L = Tile<T, DP>;
   using Frag = typename M::Frag;
@@ -627,7 +642,7 @@ constexpr int kTiles = 1024;  // tiles listed at a time
 template <typename T>
 constexpr int kDkvBuffers = 1;
 template <typename T, int DP, int RW>
-__global__ __launch_bounds__(kThreads, (sizeof(T) == 2 ? (DP <= 64 ? (RW == 1 ? 2 : 3) : DP == 128 && RW == 1 ? 1 : 2) : 1)) void k_attend_dkv(Args a) {
+__global__ __launch_bounds__(kThreads, (sizeof(T) == 2 ? (DP <= 64 ? (RW == 1 ? 2 : 3) : DP == 128 && RW == 1 ? 1 : 2) : DP == 32 ? 2 : 1)) void k_attend_dkv(Args a) {
   using M = Mma<T>;
   using L = Tile<T, DP>;
   using Frag = typename M::Frag;
