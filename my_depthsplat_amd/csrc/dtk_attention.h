@@ -639,16 +639,19 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 2 ? (DP > 64 || RW == 1 ? 2
 // has one order: no atomics on the gradients. A long list is worked off by several workgroups, each taking every
 // parts-th step.
 constexpr int kTiles = 1024;  // tiles listed at a time
-template <typename T>
-constexpr int kDkvBuffers = 1;
+// Where a key block's rows stay while its list is worked off: in LDS, from where they cost a third more of its reads and
+// leave the registers to another wave per SIMD, or in registers, where that makes no room (f32: more than 64 channels'
+// sums fill a SIMD with one wave; 64 channels of 32 or 128 keys fill the LDS).
 template <typename T, int DP, int RW>
-__global__ __launch_bounds__(kThreads, (sizeof(T) == 2 ? (DP <= 64 ? (RW == 1 ? 2 : 3) : DP == 128 && RW == 1 ? 1 : 2) : DP == 32 ? 2 : 1)) void k_attend_dkv(Args a) {
+constexpr bool kRowsInLds = sizeof(T) == 2 || (DP == 64 && RW == 2);
+template <typename T, int DP, int RW>
+__global__ __launch_bounds__(kThreads, (sizeof(T) == 2 ? (DP <= 64 ? (RW == 1 ? 2 : 3) : DP == 128 && RW == 1 ? 1 : 2) : DP <= 64 && RW > 1 || DP == 32 ? 2 : 1)) void k_attend_dkv(Args a) {
   using M = Mma<T>;
   using L = Tile<T, DP>;
   using Frag = typename M::Frag;
-  constexpr int QW = 4 / RW, NS = DP / 16, ND = DP / 32, NB = kDkvBuffers<T>;
+  constexpr int QW = 4 / RW, NS = DP / 16, ND = DP / 32, NB = 1;
   constexpr int kAhead = 1;  // steps whose rows are on their way
-  constexpr bool KEEP = sizeof(T) == 4;
+  constexpr bool KEEP = !kRowsInLds<T, DP, RW>;
   extern __shared__ __align__(16) char lds[];
   __shared__ int32_t tiles[kTiles];
   __shared__ int count;
@@ -668,8 +671,6 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 2 ? (DP <= 64 ? (RW == 1 ? 
   const int nq = length_of(a.q_lengths, b, a.Lq), nk = length_of(a.kv_lengths, b, a.Lk);
   const int64_t key = (int64_t)blk * a.block + 32 * rw + col;
   const bool exists = key < a.Lk, valid = key < nk;
-  // the block's keys and values: f32 in registers, 16 bits in LDS (from there they cost a third more of its
-  // reads and leave the registers to a third wave per SIMD)
   char* tkv = lds + NB * 2 * QW * L::kUnit;
   Frag kf[KEEP ? NS : 1], vf[KEEP ? NS : 1];
   if constexpr (KEEP) {
@@ -909,7 +910,7 @@ struct Dq {
 template <typename T, int DP, int RW>
 struct Dkv {
   static int go(const Args& a, dim3 grid, hipStream_t st) {
-    return launch(k_attend_dkv<T, DP, RW>, a, grid, (kDkvBuffers<T> * 2 * (4 / RW) + (sizeof(T) == 2 ? 2 * RW : 0)) * Tile<T, DP>::kUnit, st, "k_attend_dkv");
+    return launch(k_attend_dkv<T, DP, RW>, a, grid, (2 * (4 / RW) + (kRowsInLds<T, DP, RW> ? 2 * RW : 0)) * Tile<T, DP>::kUnit, st, "k_attend_dkv");
   }
 };
 template <template <typename, int, int> class F, typename T, int DP>
