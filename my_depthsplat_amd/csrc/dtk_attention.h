@@ -202,6 +202,12 @@ constexpr int kTileBytes = 2 * kBuffers<T, DP, U> * U * Tile<T, DP>::kUnit;
 
 __device__ __forceinline__ int acc_row(int r, int half) { return 8 * (r >> 2) + 4 * half + (r & 3); }
 
+// Units of keys that a wave of dq works off per step: where all four waves stand side by side over the rows, two, so that a
+// barrier and a step's addresses serve 64 keys (4 scenes of 32256 bf16 tokens, 16 blocks of 64: 183 us with one, 166 with
+// two; the forward has no registers for it at four waves per SIMD, 128 us either way).
+template <typename T, int RW>
+constexpr int kEach = sizeof(T) == 2 && RW == 4 ? 2 : 1;
+
 // The tile's list without places that are no block or stand in it already, in LDS, in order. One wave, 64 places at
 // a time: each is compared with those before it by broadcasts within the wave (from memory, one after the other, it took
 // longer than the attention of few queries itself), and with the list so far.
@@ -497,10 +503,10 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 2 ? (DP > 64 || RW == 1 ? 2
   using M = Mma<T>;
   using L = Tile<T, DP>;
   using Frag = typename M::Frag;
-  constexpr int KW = 4 / RW, NS = DP / 16, ND = DP / 32, NB = kBuffers<T, DP, KW>;
+  constexpr int KW = 4 / RW, NS = DP / 16, ND = DP / 32, EACH = kEach<T, RW>, U = KW * EACH, NB = kBuffers<T, DP, U>;
   extern __shared__ __align__(16) char lds[];
   __shared__ int count;
-  int32_t* list = (int32_t*)(lds + kTileBytes<T, DP, KW>);
+  int32_t* list = (int32_t*)(lds + kTileBytes<T, DP, U>);
   const Where at = where(a);
   const int32_t* idx = a.index + (((int64_t)at.b * a.Hkv + at.hk) * a.Tq + at.t) * a.top;
   const int first_places = idx[min((int)threadIdx.x & 63, a.top - 1)];
@@ -553,52 +559,55 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 2 ? (DP > 64 || RW == 1 ? 2
   f32x16 dq[ND] = {};
   const int units = n << a.lg;
   const Keys where_ = {list, a.lg, units, nk};
-  Stage<T, DP, KW> sk, sv;
+  Stage<T, DP, U> sk, sv;
+  Span<U> next = {};
   const auto fetch = [&](int u) {
-    const Span<KW> s = where_.span<KW>(u);
-    const T *pk[KW], *pv[KW];
+    next = where_.span<U>(u);
+    const T *pk[U], *pv[U];
 #pragma unroll
-    for (int j = 0; j < KW; ++j) {
-      pk[j] = row_at(kp, s.first[j], a.k.l);
-      pv[j] = row_at(vp, s.first[j], a.v.l);
+    for (int j = 0; j < U; ++j) {
+      pk[j] = row_at(kp, next.first[j], a.k.l);
+      pv[j] = row_at(vp, next.first[j], a.v.l);
     }
-    sk.load(pk, s.n, a.k.l, a.D);
-    sv.load(pv, s.n, a.v.l, a.D);
-    return pick(s.n, kw);
+    sk.load(pk, next.n, a.k.l, a.D);
+    sv.load(pv, next.n, a.v.l, a.D);
   };
-  int ahead = units ? fetch(0) : 0;
-  for (int u = 0, step = 0; u < units; u += KW, ++step) {
-    char* tk = lds + (step % NB) * 2 * KW * L::kUnit;
-    char* tv = tk + KW * L::kUnit;
+  if (units) fetch(0);
+  for (int u = 0, step = 0; u < units; u += U, ++step) {
+    char* tk = lds + (step % NB) * 2 * U * L::kUnit;
+    char* tv = tk + U * L::kUnit;
     if (NB == 1) __syncthreads();
     sk.store(tk);
     sv.store(tv);
     __syncthreads();
-    const int left = ahead;
-    if (u + KW < units) ahead = fetch(u + KW);
-    tk += kw * L::kUnit;
-    tv += kw * L::kUnit;
-    if (left == 0) continue;
-    f32x16 x = {}, dp = {};
+    const Span<U> now = next;
+    if (u + U < units) fetch(u + U);
+#pragma unroll 1
+    for (int e = 0; e < EACH; ++e) {
+      const char *uk = tk + (e * KW + kw) * L::kUnit, *uv = tv + (e * KW + kw) * L::kUnit;
+      const int left = pick(now.n, e * KW + kw);
+      if (left == 0) continue;
+      f32x16 x = {}, dp = {};
 #pragma unroll
-    for (int s = 0; s < NS; ++s) {
-      x = M::mma(L::row(tk, s, col, half), qf[s], x);
-      dp = M::mma(L::row(tv, s, col, half), gf[s], dp);
-    }
-    if (left < 32) {
+      for (int s = 0; s < NS; ++s) {
+        x = M::mma(L::row(uk, s, col, half), qf[s], x);
+        dp = M::mma(L::row(uv, s, col, half), gf[s], dp);
+      }
+      if (left < 32) {
 #pragma unroll
-      for (int r = 0; r < 16; ++r) x[r] = acc_row(r, half) < left ? x[r] : -INFINITY;
-    }
+        for (int r = 0; r < 16; ++r) x[r] = acc_row(r, half) < left ? x[r] : -INFINITY;
+      }
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(x[r], a.scale2, -lse));
-      x[r] = p * (kFewExponents<T> ? (dp[r] - delta) * down : dp[r] - delta);
-    }
-    const Frag s0 = acc_frag<T>(x, 0), s1 = acc_frag<T>(x, 1);
+      for (int r = 0; r < 16; ++r) {
+        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(x[r], a.scale2, -lse));
+        x[r] = p * (kFewExponents<T> ? (dp[r] - delta) * down : dp[r] - delta);
+      }
+      const Frag s0 = acc_frag<T>(x, 0), s1 = acc_frag<T>(x, 1);
 #pragma unroll
-    for (int d = 0; d < ND; ++d) {
-      dq[d] = M::mma(L::col(tk, 0, d, lane), s0, dq[d]);
-      dq[d] = M::mma(L::col(tk, 1, d, lane), s1, dq[d]);
+      for (int d = 0; d < ND; ++d) {
+        dq[d] = M::mma(L::col(uk, 0, d, lane), s0, dq[d]);
+        dq[d] = M::mma(L::col(uk, 1, d, lane), s1, dq[d]);
+      }
     }
   }
   if constexpr (KW > 1) {
@@ -904,7 +913,7 @@ struct Fwd {
 template <typename T, int DP, int RW>
 struct Dq {
   static int go(const Args& a, dim3 grid, hipStream_t st) {
-    return launch(k_attend_dq<T, DP, RW>, a, grid, kTileBytes<T, DP, 4 / RW> + a.top * sizeof(int32_t), st, "k_attend_dq");
+    return launch(k_attend_dq<T, DP, RW>, a, grid, kTileBytes<T, DP, 4 / RW * kEach<T, RW>> + a.top * sizeof(int32_t), st, "k_attend_dq");
   }
 };
 template <typename T, int DP, int RW>

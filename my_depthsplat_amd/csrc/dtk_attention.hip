@@ -57,10 +57,10 @@ __global__ __launch_bounds__(NT) void k_attend_mark(Args a) {
   const int t = blockIdx.x, hk = blockIdx.y, b = blockIdx.z;
   if ((int64_t)t * a.block >= length_of(a.q_lengths, b, a.Lq)) return;
   const int32_t* idx = a.index + (((int64_t)b * a.Hkv + hk) * a.Tq + t) * a.top;
-  const int words = (a.Tq + 31) / 32;
+  const int words = (a.Tq + 31) / 32, nk = length_of(a.kv_lengths, b, a.Lk);
   for (int j = threadIdx.x; j < a.top; j += NT) {
     const int v = idx[j];
-    if (v < 0 || v >= a.Tk) continue;
+    if (v < 0 || v >= a.Tk || v * a.block >= nk) continue;
     const int64_t item = ((int64_t)b * a.Hkv + hk) * a.Tk + v;
     const uint32_t bit = 1u << (t % 32);
     if (!(atomicOr(a.bits + item * words + t / 32, bit) & bit) && a.chosen) atomicAdd(a.chosen + item, 1u);
