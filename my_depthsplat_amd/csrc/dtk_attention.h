@@ -521,6 +521,12 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 2 ? (DP > 64 || RW == 1 ? 2
   const int blocks = (nk >> (5 + a.lg)) + ((nk & (a.block - 1)) != 0);
   int n = 0;
   if (at.t * a.block < nq) n = block_list(idx, first_places, a.top, blocks, list, &count);
+  if (at.rt == 0)  // for dk, dv: which tiles chose a block (bits [B, Hkv, Tk, ceil(Tq / 32)]), and how many did
+    for (int j = threadIdx.x; j < n; j += kThreads) {
+      const int64_t item = ((int64_t)at.b * a.Hkv + at.hk) * a.Tk + list[j];
+      atomicOr(a.bits + item * ((a.Tq + 31) / 32) + at.t / 32, 1u << (at.t % 32));
+      if (a.chosen) atomicAdd(a.chosen + item, 1u);
+    }
 
   const int64_t ir = valid ? i : 0;
   const T* qp = (const T*)a.q.p + at.b * a.q.b + ir * a.q.l + h * a.q.h;

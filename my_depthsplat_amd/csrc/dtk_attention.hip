@@ -1,5 +1,5 @@
-// dtk_attention.hip — the C ABI of attention over chosen blocks (kernels: dtk_attention.h), the join of
-// split lists, and who chose which block for the backward.
+// dtk_attention.hip — the C ABI of attention over chosen blocks (kernels: dtk_attention.h), the joins of
+// split lists, and the plan of dk/dv.
 #include "dtk_attention.h"
 
 namespace {
@@ -49,22 +49,6 @@ __global__ __launch_bounds__(NT) void k_attend_join(Args a, int64_t rows) {
   const float inv = valid && l > 0.f ? 1.f / l : (l != l ? l : 0.f);
   store4<T>((T*)a.out + ((b * a.Lq + i) * a.Hq + h) * a.D + d, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
   if (d == 0 && a.lse) a.lse[r] = valid ? m + log2f(l) : -INFINITY;
-}
-
-// Which tiles chose a block: bits [B, Hkv, Tk, ceil(Tq / 32)]; and how many did (a block named twice counts
-// once: whoever sets the bit counts it).
-__global__ __launch_bounds__(NT) void k_attend_mark(Args a) {
-  const int t = blockIdx.x, hk = blockIdx.y, b = blockIdx.z;
-  if ((int64_t)t * a.block >= length_of(a.q_lengths, b, a.Lq)) return;
-  const int32_t* idx = a.index + (((int64_t)b * a.Hkv + hk) * a.Tq + t) * a.top;
-  const int words = (a.Tq + 31) / 32, nk = length_of(a.kv_lengths, b, a.Lk);
-  for (int j = threadIdx.x; j < a.top; j += NT) {
-    const int v = idx[j];
-    if (v < 0 || v >= a.Tk || v * a.block >= nk) continue;
-    const int64_t item = ((int64_t)b * a.Hkv + hk) * a.Tk + v;
-    const uint32_t bit = 1u << (t % 32);
-    if (!(atomicOr(a.bits + item * words + t / 32, bit) & bit) && a.chosen) atomicAdd(a.chosen + item, 1u);
-  }
 }
 
 // The workgroups of dk/dv: a popular block is chosen several times as often as the mean, so a list of more than `most`
@@ -304,10 +288,6 @@ int dtk_block_sparse_attention_bwd(const dtk_attention* c, const void* dout, con
   if (c->Lq) {
     const dim3 grid(a.Tq * a.rowtiles, a.Hkv, c->B);
     if (int e = by_type(c->dtype, attend_dq<float>, attend_dq<bf16>, attend_dq<f16>)(a, row_waves(a), grid, st)) return e;
-    if (a.Tk) {
-      k_attend_mark<<<dim3(a.Tq, a.Hkv, c->B), NT, 0, st>>>(a);
-      if (int e = dsplat::check_launch("k_attend_mark")) return e;
-    }
   }
   if (!a.Tk) return 0;
   if (l.most) {
