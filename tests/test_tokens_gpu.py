@@ -439,6 +439,39 @@ def test_attention_of_many_tiles_of_one_block(gpu):
     check_attention(gpu, F32, 1, 70 * 32 - 3, 96, 1, 1, 32, 32, 2, index=index)
 
 
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("block", [32, 64, 128])
+def test_attention_of_popular_blocks_in_padded_batches(gpu, t, block):
+    """Block 1 is in every tile's list (it is worked off in parts, its rows behind the last key stay 0), block 3 stands
+    in half of them twice; the sequences end before, inside and behind them."""
+    L, Lk = 40 * block - 3, 4 * block + 5
+    index = random_index(3, 2, 40, 5, 4, block, holes=0.5)
+    index[..., 1] = 1
+    index[..., ::2, 2:] = 3
+    check_attention(gpu, t, 3, L, Lk, 4, 2, 40, block, 4, index=index, seed=block,
+                    lengths=([L, 1 + L // 3, L - block], [Lk, block - 1, block + 7]))
+
+
+@pytest.mark.parametrize("t", TYPES)
+def test_attention_of_more_blocks_than_workgroups_at_once(gpu, t):
+    """Some 1200 key blocks, most of which nobody chose; one is in every list."""
+    index = random_index(2, 1, 20, 600, 5, 3)
+    index[..., 0] = 7
+    check_attention(gpu, t, 2, 20 * 32, 600 * 32 - 9, 2, 1, 24, 32, 5, index=index)
+
+
+def test_attention_gradients_of_popular_blocks_are_the_same_bits_every_time(gpu):
+    T = tokens()
+    index = random_index(2, 2, 60, 60, 6, 5).to(gpu)
+    index[..., 0] = 11
+    q, k, v, do = (torch.randn(2, 60 * 32, h, 64, device=gpu).to(BF16).requires_grad_(True) for h in (4, 2, 2, 4))
+    first = None
+    for _ in range(5):
+        got = torch.autograd.grad(T.block_sparse_attention(q, k, v, index, block=32), (q, k, v), do)
+        first = first or got
+        assert all(torch.equal(a, b) for a, b in zip(got, first))
+
+
 def test_attention_f16_gradients_far_from_one(gpu):
     """f16 gradients of 2^-12 and 2^8 of the usual size: ds stays within its type's exponents."""
     T = tokens()
