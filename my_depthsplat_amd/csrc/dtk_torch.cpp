@@ -257,6 +257,7 @@ struct AddLayerNorm : torch::autograd::Function<AddLayerNorm> {
 void check_norm(const Tensor& x, const Tensor& weight, const Tensor& bias, double eps) {
   row_type(x);
   TORCH_CHECK_VALUE(x.dim() > 0 && x.size(-1) > 0, "layer norm needs rows [..., width > 0], got ", x.sizes());
+  TORCH_CHECK_VALUE(x.size(-1) <= (1LL << 28) && x.numel() / x.size(-1) < (1LL << 31), "x is too large: ", x.sizes());
   TORCH_CHECK_VALUE(eps >= 0.0, "eps must not be negative, got ", eps);
   for (const auto& [name, w] : {std::pair<const char*, const Tensor*>{"weight", &weight}, {"bias", &bias}})
     if (w->defined()) {
@@ -299,13 +300,21 @@ std::pair<Tensor, Tensor> dropout_add_layer_norm(const Tensor& x, const Tensor& 
 
 // ---- rotary positions ---------------------------------------------------------------------------------------------
 
+// the token stride: of a single token it may be any number, and is not used
+int64_t token_stride(const Tensor& t) { return t.size(1) > 1 ? t.stride(1) : 0; }
 // rows whose channels are dense, and whose token stride the kernels take
-Tensor dense_rows(const Tensor& t) { return t.stride(-1) == 1 && t.stride(1) < (1LL << 24) ? t : t.contiguous(); }
+Tensor dense_rows(const Tensor& t) { return t.stride(-1) == 1 && token_stride(t) < (1LL << 24) ? t : t.contiguous(); }
 
 struct Strides {
   int64_t s[3];
-  explicit Strides(const Tensor& t) : s{t.stride(0), t.stride(1), t.stride(2)} {}
+  explicit Strides(const Tensor& t) : s{t.stride(0), token_stride(t), t.stride(2)} {}
 };
+
+// Sizes that the C ABI takes as 32-bit numbers.
+void check_sizes(const Tensor& t, const char* name) {
+  TORCH_CHECK_VALUE(t.size(0) < 65536 && t.size(1) <= (1LL << 31) - 256 && t.size(2) < 65536 && t.size(3) < (1LL << 20), name,
+                    " is too large: ", t.sizes());
+}
 
 std::pair<Tensor, Tensor> run_rotary(const Tensor& q, const Tensor& k, const Tensor& positions, const Tensor& freqs, bool interleaved,
                                      double factor, bool backward) {
@@ -350,6 +359,8 @@ std::pair<Tensor, MaybeTensor> rotary(const Tensor& q_, const MaybeTensor& k_, T
   TORCH_CHECK_VALUE(q.dim() == 4, "q must be [B,L,Hq,D], got ", q.sizes());
   TORCH_CHECK_VALUE(!k.defined() || (k.dim() == 4 && k.size(0) == q.size(0) && k.size(1) == q.size(1) && k.size(3) == q.size(3)),
                     "k must be [B,L,Hk,D] beside q ", q.sizes(), ", got ", k.defined() ? k.sizes() : q.sizes());
+  check_sizes(q, "q");
+  if (k.defined()) check_sizes(k, "k");
   row_type(q, "q");
   TORCH_CHECK_VALUE(!k.defined() || k.scalar_type() == q.scalar_type(), "q and k must have one type");
   const int64_t B = q.size(0), L = q.size(1), D = q.size(3);
@@ -362,6 +373,7 @@ std::pair<Tensor, MaybeTensor> rotary(const Tensor& q_, const MaybeTensor& k_, T
   TORCH_CHECK_VALUE(freqs.scalar_type() == at::kDouble && freqs.dim() == 1 && 2 * F <= D && axes > 0 && F % axes == 0,
                     "freqs must be float64 [F], 2 F <= ", D, ", F a multiple of the ", axes, " axes, got ", freqs.scalar_type(), " ",
                     freqs.sizes());
+  TORCH_CHECK_VALUE(!wants_grad({&positions, &freqs}), "positions and freqs have no gradient: detach them");
   same_device(q, {{"k", &k}, {"positions", &positions}, {"freqs", &freqs}});
   q = dense_rows(q);
   if (k.defined()) k = dense_rows(k);
@@ -381,6 +393,8 @@ void check_heads(const Tensor& q, const Tensor& k, int64_t block) {
                     "q must be [B,Lq,Hq,D] and k [B,Lk,Hkv,D], got ", q.sizes(), " and ", k.sizes());
   TORCH_CHECK_VALUE(k.size(2) > 0 && q.size(2) > 0 && q.size(2) % k.size(2) == 0, "the ", q.size(2),
                     " query heads must be a multiple of the ", k.size(2), " key heads");
+  check_sizes(q, "q");
+  check_sizes(k, "k");
   row_type(q, "q");
   TORCH_CHECK_VALUE(k.scalar_type() == q.scalar_type(), "q, k and v must have one type");
 }
@@ -435,10 +449,11 @@ dtk_attention attention_of(const Tensor& q, const Tensor& k, const Tensor& v, co
   a.q = ptr(q);
   a.k = ptr(k);
   a.v = ptr(v);
+  const Strides sq(q), sk(k), sv(v);
   for (int i = 0; i < 3; ++i) {
-    a.q_strides[i] = q.stride(i);
-    a.k_strides[i] = k.stride(i);
-    a.v_strides[i] = v.stride(i);
+    a.q_strides[i] = sq.s[i];
+    a.k_strides[i] = sk.s[i];
+    a.v_strides[i] = sv.s[i];
   }
   a.index = (const int32_t*)ptr(index);
   a.q_lengths = (const int32_t*)ptr(q_lengths);

@@ -504,6 +504,23 @@ def test_attention_of_slices_and_same_bits(gpu):
         assert torch.equal(g, want)
 
 
+def test_single_tokens_of_any_token_stride(gpu):
+    """The stride of a dimension of one token is any number; it is not used."""
+    T = tokens()
+    any_stride = lambda x: x.as_strided(x.shape, (x.stride(0), 1 << 40, x.stride(2), 1))  # noqa: E731
+    q, k, v = (torch.randn(1, 1, h, 16, device=gpu) for h in (4, 2, 2))
+    aq, ak, av = (any_stride(x).requires_grad_(True) for x in (q, k, v))
+    index = torch.zeros(1, 2, 1, 1, dtype=torch.int32, device=gpu)
+    o = T.block_sparse_attention(aq, ak, av, index)
+    assert torch.equal(o, v.repeat_interleave(2, 2))
+    grads = torch.autograd.grad(o, (aq, ak, av), any_stride(torch.ones_like(q)))
+    # one key: p = 1 and dp = delta, two sums of 16 products: off by 2 * 16 * 2^-24 * sum |v| (< 32) * scale * |k| (< 4)
+    assert torch.equal(grads[2], torch.full_like(v, 2.0)) and all(float(g.abs().max()) < 2 * 16 * 2.0 ** -24 * 32 for g in grads[:2])
+    assert torch.equal(T.select_blocks(aq, ak, 1), index)
+    pos, freqs = torch.tensor([3], device=gpu), T.rotary_frequencies(16, device=gpu)
+    assert all(torch.equal(a, b) for a, b in zip(T.rotary(aq, ak, pos, freqs), T.rotary(q, k, pos, freqs)))
+
+
 def test_gradients_are_not_differentiable_twice(gpu):
     T = tokens()
     x = torch.randn(4, 8, device=gpu, requires_grad=True)

@@ -98,6 +98,8 @@ half = torch.float16
     lambda: tokens.dropout_add_layer_norm(x, x[:, :5], w, w),
     lambda: tokens.dropout_add_layer_norm(x, x.to(half), w, w),
     lambda: tokens.dropout_add_layer_norm(x, x, w, w, p=0.5),
+    lambda: tokens.layer_norm(x[:1, :1].expand(1, (1 << 32) + 16)),
+    lambda: tokens.layer_norm(x[:1, :2].expand(1 << 31, 2)),
 ])
 def test_row_refusals(call):
     with pytest.raises(ValueError):
@@ -121,6 +123,10 @@ pos, fr = torch.zeros(5, dtype=torch.int64), torch.ones(4, dtype=torch.float64)
     lambda: tokens.rotary(q4, k4, pos, torch.ones(9, dtype=torch.float64)),
     lambda: tokens.rotary(q4, k4, torch.zeros(5, 3, dtype=torch.int64), fr),
     lambda: tokens.rotary(q4, k4, torch.zeros(5, 0, dtype=torch.int64), fr),
+    lambda: tokens.rotary(q4, k4, pos.float().requires_grad_(True), fr),
+    lambda: tokens.rotary(q4, k4, pos, fr.clone().requires_grad_(True)),
+    lambda: tokens.rotary(q4[:, :, :1].expand(2, 5, 65536, 16), None, pos, fr),
+    lambda: tokens.rotary(q4, k4[:, :, :1].expand(2, 5, (1 << 32) + 2, 16), pos, fr),
 ])
 def test_rotary_refusals(call):
     with pytest.raises(ValueError):
@@ -134,6 +140,8 @@ idx = torch.zeros(2, 2, 1, 3, dtype=torch.int32)
     lambda: tokens.select_blocks(q4, k4, 2, block=16),
     lambda: tokens.select_blocks(q4, k4, 0),
     lambda: tokens.select_blocks(q4[:, :, :3], k4, 2),
+    lambda: tokens.select_blocks(q4[:, :, :1].expand(2, 5, (1 << 32) + 2, 16), k4, 2),
+    lambda: tokens.select_blocks(q4, k4[:, :1].expand(2, 1 << 31, 2, 16), 2),
     lambda: tokens.select_blocks(q4, k4[:, :, :0], 2),
     lambda: tokens.select_blocks(q4, k4.to(half), 2),
     lambda: tokens.select_blocks(torch.zeros(1, 2, 1, 257), torch.zeros(1, 2, 1, 257), 2),
