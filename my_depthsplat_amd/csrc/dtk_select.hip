@@ -31,7 +31,8 @@ struct PoolArgs {
   Rows x[2];
   int64_t L[2];
   int group[2];  // heads that share a pooled row
-  int Tq, D, pitch, block;
+  int tiles[2];
+  int D, pitch, block;
   double* out[2];  // [B, Hkv], packed (below): zeros from D on
 };
 inline int pitch_of(int D) { return (D + 7) & ~7; }
@@ -44,44 +45,54 @@ __device__ __forceinline__ int64_t packed(int t, int d, int pitch) {
   return ((int64_t)(t / 16) * (per / 2) + i / 2) * 128 + (quarter * 16 + t % 16) * 2 + i % 2;
 }
 
-// One workgroup per tile: a thread sums one 16-byte piece of every (256 / pieces)-th row, the
-// threads of a piece are folded through LDS in a fixed order.
+// One wave per tile: a lane sums one 16-byte piece of every (64 / pieces)-th row, the lanes of a piece are folded through
+// LDS in a fixed order.
 template <typename T, bool VEC>
 __global__ __launch_bounds__(NT) void k_pool(PoolArgs a) {
   constexpr int N = VEC ? Vec<T>::N : 1;
-  __shared__ double red[NT * N];
-  const int which = (int)blockIdx.x >= a.Tq, t = (int)blockIdx.x - (which ? a.Tq : 0);
-  const int hk = blockIdx.y, b = blockIdx.z, tiles = which ? gridDim.x - a.Tq : a.Tq, group = a.group[which];
+  __shared__ double folds[NT / 64][N * 64];
+  const int lane = threadIdx.x & 63, number = blockIdx.x * (NT / 64) + (threadIdx.x >> 6);
+  if (number >= a.tiles[0] + a.tiles[1]) return;  // (the waves share nothing)
+  const int which = number >= a.tiles[0], t = number - (which ? a.tiles[0] : 0);
+  const int hk = blockIdx.y, b = blockIdx.z, tiles = a.tiles[which], group = a.group[which];
+  double* red = folds[threadIdx.x >> 6];
   const Rows x = a.x[which];
   const int64_t lo = (int64_t)t * a.block;
   const int n = (int)max((int64_t)0, min((int64_t)a.block, length_of(x.lengths, b, a.L[which]) - lo));
-  const int pieces = a.D / N, parts = NT / pieces;  // D <= 256
-  const int c = threadIdx.x % pieces, part = threadIdx.x / pieces;
-  const T* p = (const T*)x.p + (int64_t)b * x.b + (int64_t)hk * group * x.h + lo * x.l + c * N;
-  double s[N] = {};
-  if (part < parts) {
-    if constexpr (VEC) {
-      for (int g = 0; g < group; ++g)
-#pragma unroll 4
-        for (int i = part; i < n; i += parts) {
-          const Vec<T> v = load_vec(p + i * x.l + g * x.h);
-#pragma unroll
-          for (int e = 0; e < N; ++e) s[e] += (double)(float)v.v[e];
-        }
-    } else {
-      for (int i = part; i < n * group; i += parts) s[0] += (double)(float)p[(i / group) * x.l + (i % group) * x.h];
-    }
-  }
-#pragma unroll
-  for (int e = 0; e < N; ++e) red[e * NT + threadIdx.x] = s[e];
-  __syncthreads();
+  const T* rows = (const T*)x.p + (int64_t)b * x.b + (int64_t)hk * group * x.h + lo * x.l;
   double* out = a.out[which] + ((int64_t)b * gridDim.y + hk) * padded(tiles) * a.pitch;
   const double inv = n ? 1.0 / (double)(n * group) : 0.0;
-  for (int d = threadIdx.x; d < a.pitch; d += NT) {
-    double v = 0.0;
-    if (d < a.D)
-      for (int k = 0; k < parts; ++k) v += red[(d % N) * NT + k * pieces + d / N];
-    out[packed(t, d, a.pitch)] = v * inv;
+  for (int first = 0; first < a.pitch; first += 64 * N) {  // (once where rows are vectors: D <= 256)
+    const int pieces = max(1, min(64, a.D / N - first / N)), parts = 64 / pieces;
+    const int c = lane % pieces, part = lane / pieces;
+    const T* p = rows + first + c * N;
+    double s[N] = {};
+    if (part < parts && first + c * N < a.D) {
+      for (int g = 0; g < group; ++g)
+#pragma unroll 8
+        for (int i = part; i < n; i += parts) {
+          if constexpr (VEC) {
+            const Vec<T> v = load_vec(p + i * x.l + g * x.h);
+#pragma unroll
+            for (int e = 0; e < N; ++e) s[e] += (double)(float)v.v[e];
+          } else {
+            s[0] += (double)(float)p[i * x.l + g * x.h];
+          }
+        }
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();  // the sums before are read
+#pragma unroll
+    for (int e = 0; e < N; ++e) red[e * 64 + lane] = s[e];
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    const int end = min(a.pitch, first + 64 * N);
+    for (int d = first + lane; d < end; d += 64) {
+      double v = 0.0;
+      if (d < a.D)
+        for (int k = 0; k < parts; ++k) v += red[(d - first) % N * 64 + k * pieces + (d - first) / N];
+      out[packed(t, d, a.pitch)] = v * inv;
+    }
   }
 }
 
@@ -351,8 +362,8 @@ int dtk_select_blocks(int B, int64_t Lq, int64_t Lk, int Hq, int Hkv, int D, int
   double* score = km + (size_t)B * Hkv * padded(Tk) * pitch;
   if (Lk > 0) {
     const PoolArgs a = {{{q, q_strides[0], q_strides[1], q_strides[2], q_lengths}, {k, k_strides[0], k_strides[1], k_strides[2], kv_lengths}},
-                        {Lq, Lk}, {Hq / Hkv, 1}, Tq, D, pitch, block, {qm, km}};
-    const dim3 grid(Tq + Tk, Hkv, B);
+                        {Lq, Lk}, {Hq / Hkv, 1}, {Tq, Tk}, D, pitch, block, {qm, km}};
+    const dim3 grid((Tq + Tk + NT / 64 - 1) / (NT / 64), Hkv, B);
     if (dtype == DTK_F32) pool<float>(a, grid, st);
     else if (dtype == DTK_BF16) pool<bf16>(a, grid, st);
     else pool<f16>(a, grid, st);
