@@ -155,7 +155,8 @@ struct ChooseArgs {
   int64_t Lq, Lk, rows;
   const int32_t *q_lengths, *kv_lengths;
   const uint8_t* allowed;
-  const double* score;
+  const double *score, *qm, *km;
+  int pitch;
   int32_t* index;
 };
 
@@ -164,9 +165,12 @@ struct ChooseArgs {
 // it. As soon as exactly `top` do, they are the answer: for scores that differ early, as they
 // do, well before the lower 32 bits are looked at. (Halving the interval of the scores instead takes
 // fewer turns, but they are not what the time goes into: 27 and 13 us against 28 and 12.5 for 1440 and 360 blocks.)
-template <int NV>
+// SCORE: the wave takes its tile's scores itself, a lane those of its blocks: a launch less. (2 x 2048 tokens, 2 heads of
+// 64 channels, blocks of 64: a whole call 11.3 us instead of 17.3, 4 x 8192 tokens 12.7 instead of 19.3. Every wave reads all
+// pooled rows of its head, so with more than 128 blocks the matrix instructions' tiles serve them better.)
+template <int NV, bool SCORE>
 __global__ __launch_bounds__(NT) void k_choose(ChooseArgs a) {
-  const int64_t row = (int64_t)blockIdx.x * (NT / 64) + (threadIdx.x >> 6);
+  const int64_t row = (int64_t)blockIdx.x * (NT / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if (row >= a.rows) return;
   const int lane = threadIdx.x & 63, t = (int)(row % a.Tq), b = (int)(row / a.Tq / a.Hkv);
   const int64_t nq = length_of(a.q_lengths, b, a.Lq), nk = length_of(a.kv_lengths, b, a.Lk);
@@ -185,8 +189,30 @@ __global__ __launch_bounds__(NT) void k_choose(ChooseArgs a) {
 #pragma unroll
   for (int j = 0; j < NV; ++j) {  // all on their way together
     const int i = min(64 * j + lane, a.Tk - 1);
-    v[j] = score[i];
+    if (!SCORE) v[j] = score[i];
     ok[j] = may ? may[i] : 1;
+  }
+  if constexpr (SCORE) {
+    const int64_t z = row / a.Tq;
+    const double *q = a.qm + z * padded(a.Tq) * a.pitch, *k = a.km + z * padded(a.Tk) * a.pitch;
+    const double* kp[NV];
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      v[j] = 0.0;
+      kp[j] = k + packed(min(64 * j + lane, a.Tk - 1), 0, a.pitch);
+    }
+    q += packed(t, 0, a.pitch);
+    for (int quarter = 0; quarter < 4; ++quarter)
+#pragma unroll 4
+      for (int i = 0; i < a.pitch / 8; ++i) {  // two channels each
+        const f64x2 qv = *(const f64x2*)(q + quarter * 32 + i * 128);
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+          const f64x2 kv = *(const f64x2*)(kp[j] + quarter * 32 + i * 128);
+          v[j] = fma(qv[0], kv[0], v[j]);
+          v[j] = fma(qv[1], kv[1], v[j]);
+        }
+      }
   }
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
@@ -324,6 +350,7 @@ __global__ __launch_bounds__(NT) void k_choose_long(ChooseArgs a) {
   for (int i = min(have, a.top) + threadIdx.x; i < a.top; i += NT) out[i] = -1;
 }
 
+constexpr int kScoredByChoice = 64 * 2;  // blocks
 inline int64_t tiles_of(int64_t L, int block) { return (L + block - 1) / block; }
 
 template <typename T>
@@ -368,17 +395,19 @@ int dtk_select_blocks(int B, int64_t Lq, int64_t Lk, int Hq, int Hkv, int D, int
     else if (dtype == DTK_BF16) pool<bf16>(a, grid, st);
     else pool<f16>(a, grid, st);
     if (int e = dsplat::check_launch("k_pool")) return e;
-    k_scores<<<dim3((Tk + 255) / 256, (Tq + 31) / 32, B * Hkv), NT, 0, st>>>(Tq, Tk, pitch, qm, km, score);
-    if (int e = dsplat::check_launch("k_scores")) return e;
+    if (Tk > kScoredByChoice) {
+      k_scores<<<dim3((Tk + 255) / 256, (Tq + 31) / 32, B * Hkv), NT, 0, st>>>(Tq, Tk, pitch, qm, km, score);
+      if (int e = dsplat::check_launch("k_scores")) return e;
+    }
   }
-  const ChooseArgs a = {Tq, Tk, Hkv, block, top, Lq, Lk, (int64_t)B * Hkv * Tq, q_lengths, kv_lengths, allowed, score, index};
+  const ChooseArgs a = {Tq, Tk, Hkv, block, top, Lq, Lk, (int64_t)B * Hkv * Tq, q_lengths, kv_lengths, allowed, score, qm, km, pitch, index};
   DSPLAT_REQUIRE(a.rows < (1LL << 31), "dtk_select_blocks: too large");
   const unsigned waves = (unsigned)((a.rows + NT / 64 - 1) / (NT / 64));
-  if (Tk <= 64 * 2) k_choose<2><<<waves, NT, 0, st>>>(a);
-  else if (Tk <= 64 * 8) k_choose<8><<<waves, NT, 0, st>>>(a);
-  else if (Tk <= 64 * 16) k_choose<16><<<waves, NT, 0, st>>>(a);
-  else if (Tk <= 64 * 24) k_choose<24><<<waves, NT, 0, st>>>(a);
-  else if (Tk <= 64 * 32) k_choose<32><<<waves, NT, 0, st>>>(a);
+  if (Tk <= kScoredByChoice) k_choose<2, true><<<waves, NT, 0, st>>>(a);
+  else if (Tk <= 64 * 8) k_choose<8, false><<<waves, NT, 0, st>>>(a);
+  else if (Tk <= 64 * 16) k_choose<16, false><<<waves, NT, 0, st>>>(a);
+  else if (Tk <= 64 * 24) k_choose<24, false><<<waves, NT, 0, st>>>(a);
+  else if (Tk <= 64 * 32) k_choose<32, false><<<waves, NT, 0, st>>>(a);
   else k_choose_long<<<(unsigned)a.rows, NT, 0, st>>>(a);
   return dsplat::check_launch("k_choose");
 }
