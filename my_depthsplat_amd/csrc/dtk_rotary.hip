@@ -9,6 +9,9 @@
 // and reduced to one turn there (a far position times a frequency needs more digits than 32
 // bits hold); the sine and cosine are then of a small number in 32 bits. A thread takes the
 // sines of its channels once and turns every head of its token with them.
+//
+// Measured: 92160 tokens, 2 + 2 heads of 64 bf16, two axes: 22 us a direction, 4.3 TB/s (a copy of 256 MB 5.4); 16 single tokens
+// of 8 + 2 heads 4.0 us, a launch and the chain position, frequency, sine.
 
 #include "dtk_common.h"
 

@@ -7,6 +7,10 @@
 // The means, products and scores are held in 64 bits: the answer is a set of whole numbers, and
 // near scores change places with the rounding of a 32-bit sum (and so with the order in which a
 // kernel adds). The work is small next to reading q and k: T_q T_k D products per key head.
+//
+// Measured, pooled rows / scores / choice: 4 scenes of 32256 bf16 tokens (504 x 504 blocks of 64), 2 heads of 64: 13.5 us
+// (4.0 TB/s), 11.5 us, 12.5 us; 92160 tokens (1440 x 1440): 13 us, 22.5 us (24 TFLOP/s in 64 bits and 33 MB of scores), 28 us. The
+// scores' and the choice's time goes into the latency of reads behind the L2 (two thirds of the choice's cycles wait).
 
 #include "dtk_common.h"
 

@@ -10,7 +10,8 @@ needs between the features and the cost volume or the head.
   dropout_rng, rotary_frequencies, view_positions: the inputs they take
 
 float32, bfloat16 or float16 rows; HIP kernels forward and backward (include/dsplat_hip.h, dtk_*;
-argument checks and autograd nodes: csrc/dtk_torch.cpp), on torch's current stream of the tensors' device, without host synchronisation (capturable).
+argument checks and autograd nodes: csrc/dtk_torch.cpp), on torch's current stream of the
+tensors' device, without host synchronisation (capturable).
 Gradients are the same bits every time (no atomics on them). Not differentiable twice.
 """
 from __future__ import annotations
@@ -85,7 +86,8 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, fre
     """Turn pair i of every head by positions[..., axis(i)] * freqs[i], axis(i) = i / (F / axes), times
     `factor` -> (q', k'). q [B,L,Hq,D], k [B,L,Hk,D] or None; positions [L], [L,axes] or [B,L,axes]
     (int64, int32 or float32); freqs float64 [F], 2 F <= D (rotary_frequencies()); pairs (i, i + F), or
-    (2i, 2i + 1) if interleaved; the channels behind 2 F stay. Angles are taken in 64 bits."""
+    (2i, 2i + 1) if interleaved; the channels behind 2 F stay. Angles are taken in 64 bits. positions and
+    freqs have no gradient: those that ask for one are refused."""
     return _lib.load_torch().rotary(q, k, positions, freqs, interleaved, factor)
 
 
@@ -107,7 +109,7 @@ def block_sparse_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, in
                            scale: float | None = None) -> torch.Tensor:
     """softmax(scale q k^T) v of the queries of each tile over the keys of its blocks -> [B,Lq,Hq,D].
     q [B,Lq,Hq,D], k, v [B,Lk,Hkv,D] (any strides with dense channels; D a multiple of 8 up to 128; query
-    head h reads key head h / (Hq / Hkv)); index int32 [B, Hkv, ceil(Lq / block), top <= 1024], as
+    head h reads key head h / (Hq / Hkv), at most 1024 to one); index int32 [B, Hkv, ceil(Lq / block), top <= 1024], as
     select_blocks gives it: places outside the sequence's blocks, and second ones of a block, count
     for nothing. lengths [B] as there: o is 0 behind q_lengths and for queries that see no key.
     scale: 1 / sqrt(D) by default."""
