@@ -756,9 +756,10 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 2 ? (DP <= 64 ? (RW == 1 ? 
     }
     __syncthreads();
     const int units = uniform(count) * upt;
-    // unit u: 32 rows (part u % (block / 32)) of a head of the group of a listed tile
-    const auto pos = [&](int u) {  // exact: u >> lg < 2^20 and G <= 1024
-      return a.G == 1 ? u >> a.lg : (int)__umulhi((uint32_t)(u >> a.lg), a.group_magic);
+    // Unit u: 32 rows (part u % RW; a block is RW units of keys and a tile RW units of queries) of a head of the group of a
+    // listed tile. With two or four units to a tile, a step's units are of one tile and head.
+    const auto listed = [&](int p) {  // p-th tile and head -> place in the list; exact: p < 2^20 and G <= 1024
+      return a.G == 1 ? p : (int)__umulhi((uint32_t)p, a.group_magic);
     };
     // What is on its way: the rows of the units u .. u + QW - 1 and their statistics.
     struct Ahead {
@@ -766,34 +767,50 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 2 ? (DP <= 64 ? (RW == 1 ? 
       float lse, delta;
       int live;
     };
+    const int64_t stats0 = ((int64_t)b * a.Hq + hk * a.G) * a.Lq;
     const auto fetch = [&](Ahead& f, int u) {
       const T *pq[QW], *pg[QW];
-      int tile[QW], have[QW];
+      int have[QW];
+      f.lse = -INFINITY;
+      if constexpr (RW == 1) {
+        int tile[QW];
 #pragma unroll
-      for (int j = 0; j < QW; ++j) tile[j] = tiles[pos(min(u + j, units - 1))];
+        for (int j = 0; j < QW; ++j) tile[j] = tiles[listed(min(u + j, units - 1))];
 #pragma unroll
-      for (int j = 0; j < QW; ++j) {
-        const int i0 = ((uniform(tile[j]) << a.lg) + ((u + j) & ((1 << a.lg) - 1))) * 32;
-        const int64_t g = ((u + j) >> a.lg) - pos(u + j) * a.G;
-        pq[j] = row_at(qb, i0, a.q.l) + g * a.q.h;
-        pg[j] = row_at(gb, i0, a.g.l) + g * a.g.h;
-        have[j] = u + j < units ? max(0, min(32, nq - i0)) : 0;
-      }
-      f.q.load(pq, have, a.q.l, a.D);
-      f.g.load(pg, have, a.g.l, a.D);
-      if (threadIdx.x < QW * 32) {
-        const int r = threadIdx.x % 32, uj = u + threadIdx.x / 32;
-        f.lse = -INFINITY;
-        if (uj < units) {
-          const int at = pos(uj);
-          const int i = ((tiles[at] << a.lg) + (uj & ((1 << a.lg) - 1))) * 32 + r;
+        for (int j = 0; j < QW; ++j) {
+          const int i0 = uniform(tile[j]) * 32;
+          const int64_t g = u + j - listed(u + j) * a.G;
+          pq[j] = row_at(qb, i0, a.q.l) + g * a.q.h;
+          pg[j] = row_at(gb, i0, a.g.l) + g * a.g.h;
+          have[j] = u + j < units ? max(0, min(32, nq - i0)) : 0;
+        }
+        const int uj = u + threadIdx.x / 32;
+        if (threadIdx.x < QW * 32 && uj < units) {
+          const int at = listed(uj), i = tiles[at] * 32 + threadIdx.x % 32;
           if (i < nq) {
-            const int64_t stat = ((int64_t)b * a.Hq + hk * a.G + (uj >> a.lg) - at * a.G) * a.Lq + i;
+            const int64_t stat = stats0 + (int64_t)(uj - at * a.G) * a.Lq + i;
             f.lse = a.lse[stat];
             f.delta = a.delta[stat];
           }
         }
+      } else {
+        const int p = (int)((uint32_t)u / RW), at = listed(p), g = p - at * a.G;
+        const int i0 = (uniform(tiles[at]) * RW + (int)((uint32_t)u % RW)) * 32;
+        const T *q0 = row_at(qb, i0, a.q.l) + g * a.q.h, *g0 = row_at(gb, i0, a.g.l) + g * a.g.h;
+#pragma unroll
+        for (int j = 0; j < QW; ++j) {
+          pq[j] = q0 + j * 32 * a.q.l;
+          pg[j] = g0 + j * 32 * a.g.l;
+          have[j] = max(0, min(32, nq - i0 - 32 * j));
+        }
+        if (threadIdx.x < QW * 32 && i0 + (int)threadIdx.x < nq) {
+          const int64_t stat = stats0 + (int64_t)g * a.Lq + i0;
+          f.lse = (a.lse + stat)[threadIdx.x];
+          f.delta = (a.delta + stat)[threadIdx.x];
+        }
       }
+      f.q.load(pq, have, a.q.l, a.D);
+      f.g.load(pg, have, a.g.l, a.D);
       f.live = pick(have, qw);
     };
     const auto turn = [&](Ahead& f, int u) {
