@@ -94,10 +94,11 @@ struct Args {
 __device__ __forceinline__ int length_of(const int32_t* lengths, int b, int64_t L) {  // fewer than 2^31 (the host checks)
   return lengths ? min(max(lengths[b], 0), (int)L) : (int)L;
 }
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 // Row r of rows that start at p: token numbers and their strides fit 32 bits, their product is one unsigned 64-bit one.
 template <typename T>
 __device__ __forceinline__ const T* row_at(const T* p, int r, int64_t stride) {
-  return p + (uint64_t)(uint32_t)r * (uint32_t)stride;
+  return p + (uint64_t)(uint32_t)uniform(r) * (uint32_t)uniform((int)stride);
 }
 
 // 8 channels of a row from d0 on, zeros behind D and for rows that do not count (what stands
@@ -156,8 +157,6 @@ struct Tile {
     return f;
   }
 };
-
-__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
 // The workgroup's share of U units (32 rows each) on the way from memory to LDS: loaded into
 // registers while the tile before is worked on, then stored. Rows that do not count and channels
@@ -345,10 +344,10 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 2 ? (DP > 64 || RW == 1 ? 2
   const T* vp = (const T*)a.v.p + at.b * a.v.b + at.hk * a.v.h;
 
   f32x16 o[ND] = {};
-  // The exponents are taken relative to base2, which follows the running maximum m only when a sum of 16
-  // has passed 2^12: p stays in every type's range, the fast path needs no maximum, and o is
-  // rarely rescaled. (l <= 2^12 x keys, o likewise: far inside 32 bits.)
-  float m = -INFINITY, base2 = 0.f, l = 0.f;
+  // The exponents are taken relative to base2 (in powers of two), which is set to the largest score so far only when a sum of
+  // 16 has passed 2^12, or at first, when it is -inf and every sum passes everything: p stays in every type's range, the
+  // fast path needs no maximum, and o is rarely rescaled. (l <= 2^12 x keys, o likewise: far inside 32 bits.)
+  float base2 = -INFINITY, l = 0.f;
   const int units = n << a.lg;
   const int per = (units + a.splits - 1) / a.splits;
   const int u0 = min(units, at.split * per), u1 = min(units, u0 + per);
@@ -373,7 +372,6 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 2 ? (DP > 64 || RW == 1 ? 2
     if (!TURNS) load(sv, next, vp, a.v.l);
   };
   if (u0 < u1) fetch(u0);
-  bool begun = false;
   for (int u = u0, step = 0; u < u1; u += KW, ++step) {
     char* tk = lds + (step % NB) * 2 * KW * L::kUnit;
     char* tv = tk + KW * L::kUnit;
@@ -404,30 +402,26 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 2 ? (DP > 64 || RW == 1 ? 2
     }
     f32x16 p;
     float sum = 0.f;
-    if (begun) {
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        p[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[r], a.scale2, -base2));
-        sum += p[r];
-      }
+    for (int r = 0; r < 16; ++r) {
+      p[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[r], a.scale2, -base2));
+      sum += p[r];
     }
-    if (!begun || __any(!(sum <= 4096.f))) {
-      begun = true;
+    if (__any(!(sum <= 4096.f))) {
       float mx = x[0];
 #pragma unroll
       for (int r = 1; r < 16; ++r) mx = fmaxf(mx, x[r]);
       mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-      const float mn = fmaxf(m, mx), b2 = mn == -INFINITY ? 0.f : mn * a.scale2;
-      const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(base2 - b2);
-      m = mn;
-      base2 = b2;
+      const float top = fmaxf(base2, mx * a.scale2);  // -inf as long as every score was
+      const float to = top == -INFINITY ? 0.f : top, alpha = __builtin_amdgcn_exp2f(base2 - to);
+      base2 = top;
       l *= alpha;
 #pragma unroll
       for (int d = 0; d < ND; ++d) o[d] *= alpha;
       sum = 0.f;
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        p[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[r], a.scale2, -base2));
+        p[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[r], a.scale2, -to));
         sum += p[r];
       }
     }
@@ -452,17 +446,16 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 2 ? (DP > 64 || RW == 1 ? 2
 #pragma unroll
           for (int r = 0; r < 16; ++r) jo[32 * d + acc_row(r, half)] = o[d][r];
         if (half == 0) {
-          join.m[rw * 32 + col] = m == -INFINITY ? m : base2;
+          join.m[rw * 32 + col] = base2;
           join.l[rw * 32 + col] = l;
         }
       }
       __syncthreads();
       if (kw == 0) {
-        const float mo = join.m[rw * 32 + col], lo = join.l[rw * 32 + col], me = m == -INFINITY ? m : base2;
-        const float mn = fmaxf(me, mo), b2 = mn == -INFINITY ? 0.f : mn;
-        const float fa = __builtin_amdgcn_exp2f(me - b2), fb = __builtin_amdgcn_exp2f(mo - b2);
-        m = mn;  // from here on in powers of two
-        base2 = b2;
+        const float mo = join.m[rw * 32 + col], lo = join.l[rw * 32 + col];
+        const float top = fmaxf(base2, mo), to = top == -INFINITY ? 0.f : top;
+        const float fa = __builtin_amdgcn_exp2f(base2 - to), fb = __builtin_amdgcn_exp2f(mo - to);
+        base2 = top;
         l = l * fa + lo * fb;
 #pragma unroll
         for (int d = 0; d < ND; ++d)
@@ -472,7 +465,6 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 2 ? (DP > 64 || RW == 1 ? 2
     }
   }
   if (kw != 0 || !exists) return;
-  const float top2 = m == -INFINITY ? m : base2;
   if (a.splits > 1) {
     const int64_t r = ((int64_t)at.b * a.Hq + h) * a.Lq + i, rows = (int64_t)(gridDim.z / a.splits) * a.Hq * a.Lq;
     float* po = a.part + (at.split * rows + r) * a.D;
@@ -483,7 +475,7 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 2 ? (DP > 64 || RW == 1 ? 2
         if (32 * d + 8 * c + 4 * half < a.D)
           store4<float>(po + 32 * d + 8 * c + 4 * half, o[d][4 * c], o[d][4 * c + 1], o[d][4 * c + 2], o[d][4 * c + 3]);
     if (half == 0) {
-      a.part_m[at.split * rows + r] = top2;
+      a.part_m[at.split * rows + r] = base2;
       a.part_l[at.split * rows + r] = l;
     }
     return;
@@ -497,7 +489,7 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 2 ? (DP > 64 || RW == 1 ? 2
       if (32 * d + 8 * c + 4 * half < a.D)
         store4<T>(op + 32 * d + 8 * c + 4 * half, o[d][4 * c] * inv, o[d][4 * c + 1] * inv, o[d][4 * c + 2] * inv,
                   o[d][4 * c + 3] * inv);
-  if (half == 0 && a.lse) a.lse[((int64_t)at.b * a.Hq + h) * a.Lq + i] = valid ? top2 + log2f(l) : -INFINITY;
+  if (half == 0 && a.lse) a.lse[((int64_t)at.b * a.Hq + h) * a.Lq + i] = valid ? base2 + log2f(l) : -INFINITY;
 }
 
 // ds is rounded to the inputs' type for its products. f16 has few exponents, so ds is taken there

@@ -424,6 +424,33 @@ def test_attention_of_large_and_small_scores(gpu, t):
 
 
 @pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("Lq,Hq,block", [(64, 1, 64), (128, 1, 128), (32, 1, 32), (1, 2, 64), (64, 4, 64)])
+def test_attention_of_scores_that_are_minus_infinity(gpu, t, Lq, Hq, block):
+    """Keys whose score is -inf count for nothing, wherever in the list they stand: the answer is that of the others, 0
+    for a row that has no others. A score of +inf gives no number."""
+    T = tokens()
+    rnd = make(gpu, block + Lq)
+    (q, _), (k, _), (v, _) = rnd(1, Lq, Hq, 32, t=t), rnd(1, 5 * block, 1, 32, t=t), rnd(1, 5 * block, 1, 32, t=t)
+    q[..., 3] = q[..., 3].abs() + 0.5
+    index = torch.arange(5, device=gpu, dtype=torch.int32).expand(1, 1, 1, 5).contiguous()
+    k[:, :block, :, 3] = -float("inf")
+    k[:, 2 * block:3 * block - 7, :, 3] = -float("inf")
+    keep = k[0, :, 0, 3].isfinite()
+    x = torch.einsum("lhd,kd->hlk", q[0].double().cpu(), k[0, :, 0].double().cpu().nan_to_num(neginf=0.0)) / 32 ** 0.5
+    p = torch.softmax(x.masked_fill(~keep.cpu(), -float("inf")), -1)
+    want = (p @ v[0, :, 0].double().cpu()).transpose(0, 1)[None]
+    got = T.block_sparse_attention(q, k, v, index, block=block)
+    # p is rounded to v's type, o too; the exponents' sums of 32 products are off by 2^-24 * 32 * max |x| (< 32) at most
+    eps = torch.finfo(t).eps / 2
+    top = float(v.abs().max())
+    assert float((got.double().cpu() - want).abs().max()) <= (2 * eps + 2 * 2.0 ** -24 * 32 * 32) * top
+    none = torch.zeros_like(index)
+    assert not T.block_sparse_attention(q, k, v, none, block=block).any()
+    k[:, 3 * block, :, 3] = float("inf")
+    assert T.block_sparse_attention(q, k, v, index, block=block).isnan().all()
+
+
+@pytest.mark.parametrize("t", TYPES)
 @pytest.mark.parametrize("Lq,Hq,Hkv,B,top", [(1, 8, 2, 3, 40), (1, 1, 1, 1, 60), (5, 4, 1, 2, 33), (40, 1, 1, 1, 64)])
 def test_attention_of_few_queries_is_split_and_joined(gpu, t, Lq, Hq, Hkv, B, top):
     check_attention(gpu, t, B, Lq, 64 * 70 - 5, Hq, Hkv, 64, 64, top, seed=top, train=Lq > 1)
