@@ -17,10 +17,10 @@
 //
 // Measured (products taken, rate; a large bf16 product reaches 1060 TFLOP/s, f32 153):
 //   4 scenes of 32256 bf16 tokens (lengths from half of that on), 4 heads of 64 channels on 2, 16 blocks of 64:
-//     forward 128 us 560 TFLOP/s, dq 168 us 640, dk/dv 250 us 570
+//     forward 128 us 560 TFLOP/s, dq 170 us 630, dk/dv 231 us 620
 //   16 scenes of 2048 f32 tokens, one head of 128 channels, 8 blocks of 64: 90 us 92, 143 us 87, 208 us 80
 //   12 views of 92160 bf16 tokens, 2 heads of 64, 16 blocks of 64, forward: 104 us 465
-// What bounds them: the forward and dq at 64 channels the vector unit (118 of its instructions per 32 x 32 scores, half of
+// What bounds them: the forward and dq at 64 channels the vector unit (some 110 of its instructions per 32 x 32 scores, half of
 // its cycles, for 8 matrix instructions, a quarter of theirs; with 128 channels the forward comes to 730 TFLOP/s);
 // dk/dv the rows of far tiles from behind the L2 (half of its reads miss; 4.6 TB/s) at three waves per SIMD; the
 // 12 views' forward likewise (6 TB/s: one head's 64 queries share a tile); f32 the matrix instructions and the
@@ -355,8 +355,8 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 2 ? (DP > 64 || RW == 1 ? 2
   // A step's keys and values come together, while the step before is worked on; or, for f32 rows of more than 64
   // channels, in turn through the same registers, the values during the first product and the next keys during
   // the second (which take 4096 cycles each at 128 channels), so that two waves per SIMD fit: 16 scenes of
-  // 2048 tokens of 128 channels, 8 blocks of 64 each, 91 us instead of 106. (Where both fit anyway, the second barrier costs:
-  // 2 x 16384 tokens of 64 channels, 4 heads on one: 320 us instead of 287.)
+  // 2048 tokens of 128 channels, 8 blocks of 64 each, 91 us instead of 106. (At 64 channels three
+  // waves fit as it is.)
   constexpr bool TURNS = sizeof(T) == 4 && DP > 64;
   Stage<T, DP, KW> sk, sv;
   const auto load = [&](Stage<T, DP, KW>& to, const Span<KW>& s, const T* p, int64_t stride) {
