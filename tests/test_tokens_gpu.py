@@ -424,6 +424,13 @@ def test_attention_of_large_and_small_scores(gpu, t):
 
 
 @pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("block", [32, 128])
+def test_attention_of_scores_of_thousands(gpu, t, block):
+    check_attention(gpu, t, 1, 200, 300, 2, 1, 64, block, 4, scale=30.0, train=False, seed=block)
+    check_attention(gpu, t, 1, 40, 300, 1, 1, 64, block, 4, scale=-300.0, train=False, seed=block)
+
+
+@pytest.mark.parametrize("t", TYPES)
 @pytest.mark.parametrize("Lq,Hq,block", [(64, 1, 64), (128, 1, 128), (32, 1, 32), (1, 2, 64), (64, 4, 64)])
 def test_attention_of_scores_that_are_minus_infinity(gpu, t, Lq, Hq, block):
     """Keys whose score is -inf count for nothing, wherever in the list they stand: the answer is that of the others, 0
