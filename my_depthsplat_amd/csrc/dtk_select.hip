@@ -169,9 +169,8 @@ struct ChooseArgs {
 // it. As soon as exactly `top` do, they are the answer: for scores that differ early, as they
 // do, well before the lower 32 bits are looked at. (Halving the interval of the scores instead takes
 // fewer turns, but they are not what the time goes into: 27 and 13 us against 28 and 12.5 for 1440 and 360 blocks.)
-// SCORE: the wave takes its tile's scores itself, a lane those of its blocks: a launch less. (2 x 2048 tokens, 2 heads of
-// 64 channels, blocks of 64: a whole call 11.3 us instead of 17.3, 4 x 8192 tokens 12.7 instead of 19.3. Every wave reads all
-// pooled rows of its head, so with more than 128 blocks the matrix instructions' tiles serve them better.)
+// SCORE: the wave takes its tile's scores itself, a lane those of its blocks, a launch less (scored_by_choice: where that
+// pays).
 template <int NV, bool SCORE>
 __global__ __launch_bounds__(NT) void k_choose(ChooseArgs a) {
   const int64_t row = (int64_t)blockIdx.x * (NT / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -354,7 +353,11 @@ __global__ __launch_bounds__(NT) void k_choose_long(ChooseArgs a) {
   for (int i = min(have, a.top) + threadIdx.x; i < a.top; i += NT) out[i] = -1;
 }
 
-constexpr int kScoredByChoice = 64 * 2;  // blocks
+// Every wave of the choice that takes its scores itself reads all pooled rows of its head; the matrix instructions' tiles read
+// them a 32nd as often and cost a launch. 64 channels, a whole call with and without: 2 x 2048 tokens 11 and 17 us, 4 x 16000
+// 23 and 27, 8 x 16000 (64 M products) 34 and 33, 16 x 16000 57 and 49; 128 channels: 4 x 16000 36 and 38, 8 x 16000 58 and
+// 49; 504 blocks, eight to a lane, 53 and 24.
+inline bool scored_by_choice(int64_t rows, int Tk, int pitch) { return Tk <= 64 * 4 && rows * Tk * pitch <= 1 << 26; }
 inline int64_t tiles_of(int64_t L, int block) { return (L + block - 1) / block; }
 
 template <typename T>
@@ -388,6 +391,9 @@ int dtk_select_blocks(int B, int64_t Lq, int64_t Lk, int Hq, int Hkv, int D, int
   DSPLAT_REQUIRE(index && (Lk == 0 || (q && k && q_strides && k_strides && workspace)), "dtk_select_blocks: null pointer");
   hipStream_t st = (hipStream_t)stream;
   const int pitch = pitch_of(D);
+  const int64_t rows = (int64_t)B * Hkv * Tq;
+  DSPLAT_REQUIRE(rows < (1LL << 31), "dtk_select_blocks: too large");
+  const bool fused = scored_by_choice(rows, Tk, pitch);
   double* qm = (double*)workspace;
   double* km = qm + (size_t)B * Hkv * padded(Tq) * pitch;
   double* score = km + (size_t)B * Hkv * padded(Tk) * pitch;
@@ -399,15 +405,15 @@ int dtk_select_blocks(int B, int64_t Lq, int64_t Lk, int Hq, int Hkv, int D, int
     else if (dtype == DTK_BF16) pool<bf16>(a, grid, st);
     else pool<f16>(a, grid, st);
     if (int e = dsplat::check_launch("k_pool")) return e;
-    if (Tk > kScoredByChoice) {
+    if (!fused) {
       k_scores<<<dim3((Tk + 255) / 256, (Tq + 31) / 32, B * Hkv), NT, 0, st>>>(Tq, Tk, pitch, qm, km, score);
       if (int e = dsplat::check_launch("k_scores")) return e;
     }
   }
-  const ChooseArgs a = {Tq, Tk, Hkv, block, top, Lq, Lk, (int64_t)B * Hkv * Tq, q_lengths, kv_lengths, allowed, score, qm, km, pitch, index};
-  DSPLAT_REQUIRE(a.rows < (1LL << 31), "dtk_select_blocks: too large");
+  const ChooseArgs a = {Tq, Tk, Hkv, block, top, Lq, Lk, rows, q_lengths, kv_lengths, allowed, score, qm, km, pitch, index};
   const unsigned waves = (unsigned)((a.rows + NT / 64 - 1) / (NT / 64));
-  if (Tk <= kScoredByChoice) k_choose<2, true><<<waves, NT, 0, st>>>(a);
+  if (fused && Tk <= 64 * 2) k_choose<2, true><<<waves, NT, 0, st>>>(a);
+  else if (fused) k_choose<4, true><<<waves, NT, 0, st>>>(a);
   else if (Tk <= 64 * 8) k_choose<8, false><<<waves, NT, 0, st>>>(a);
   else if (Tk <= 64 * 16) k_choose<16, false><<<waves, NT, 0, st>>>(a);
   else if (Tk <= 64 * 24) k_choose<24, false><<<waves, NT, 0, st>>>(a);

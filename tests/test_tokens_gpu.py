@@ -319,6 +319,34 @@ def test_select_blocks(gpu, t, B, Lq, Lk, Hq, Hkv, D, block, top):
     assert torch.equal(got.cpu(), orc.select_blocks(q64, k64, top, block, ql, kl, may))
 
 
+@pytest.mark.parametrize("blocks", [128, 129, 256, 257, 512, 513, 1024, 1025, 1536, 1537, 2048, 2049])
+def test_select_blocks_of_every_number_of_blocks(gpu, blocks):
+    """Both sides of each limit between the kernels, with tiles that end inside a group of 16, equal scores and none."""
+    T = tokens()
+    rnd = make(gpu, blocks)
+    Lq, Lk = 18 * 32 + 5, blocks * 32 - 3
+    (q, q64), (k, k64) = rnd(2, Lq, 4, 24, t=F16), rnd(2, Lk, 2, 24, t=F16)
+    k[:, 32 * 50:32 * 60] = k[:, 32 * 40:32 * 41].repeat(1, 10, 1, 1)
+    k64[:, 32 * 50:32 * 60] = k64[:, 32 * 40:32 * 41].repeat(1, 10, 1, 1)
+    g = torch.Generator().manual_seed(blocks)
+    may = torch.rand(19, blocks, generator=g) < 0.8
+    may[3] = False
+    ql, kl = torch.tensor([Lq, 260]), torch.tensor([Lk - 40, Lk // 2])
+    for top in (1, 16, 200):
+        got = T.select_blocks(q, k, top, block=32, q_lengths=ql.to(gpu), kv_lengths=kl.to(gpu), allowed=may.to(gpu))
+        assert torch.equal(got.cpu(), orc.select_blocks(q64, k64, top, 32, ql, kl, may))
+
+
+def test_select_blocks_of_many_rows(gpu):
+    """So many rows that few blocks' scores come from the matrix instruction: the same choice as scene by scene."""
+    T = tokens()
+    q, k = (torch.randn(70, 260 * 32, 1, 128, device=gpu).to(BF16) for _ in range(2))
+    k = k[:, :120 * 32]
+    got = T.select_blocks(q, k, 6, block=32)
+    for b in (0, 33, 69):
+        assert torch.equal(got[b:b + 1], T.select_blocks(q[b:b + 1], k[b:b + 1], 6, block=32))
+
+
 def test_select_blocks_ties_padding_and_no_numbers(gpu):
     """Equal scores go to the lowest blocks, of either sign of zero; rows behind the length do not count, whatever they
     hold; a score that is no number ranks below every other; nothing allowed gives -1."""
