@@ -205,6 +205,40 @@ def test_captured_and_replayed(gpu, name):
 
 
 @gpu_only
+def test_captured_backward_of_lists_that_change(gpu):
+    """Two graphs whose key blocks' lists, and so the parts of dk and dv that are worked off by themselves, differ at every replay."""
+    from my_depthsplat_amd import tokens as T
+    r = lambda *s: torch.randn(*s, device=gpu).to(BF16)  # noqa: E731
+    calls, graphs = [], []
+    for _ in range(2):
+        q, k, v, do = r(2, 1900, 2, 32).requires_grad_(True), r(2, 700, 1, 32).requires_grad_(True), r(2, 700, 1, 32).requires_grad_(True), r(2, 1900, 2, 32)
+        index = torch.zeros(2, 1, 60, 5, dtype=torch.int32, device=gpu)
+
+        def f(q=q, k=k, v=v, do=do, index=index):
+            return torch.autograd.grad(T.block_sparse_attention(q, k, v, index, block=32), (q, k, v), do)
+
+        calls.append((index, f))
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            f()
+        torch.cuda.current_stream().wait_stream(side)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            held = f()
+        graphs.append((graph, held))
+    for turn in range(4):
+        for (index, f), (graph, held) in zip(calls, graphs):
+            index.copy_(torch.randint(-3, 22, index.shape, device=gpu))
+            index[:, :, :, 0] = 5 * turn  # a popular block, another one each time
+            graph.replay()
+            torch.cuda.synchronize()
+            got = [t.clone() for t in held]
+            assert all(torch.equal(a, e) for a, e in zip(got, f())), turn
+
+
+@gpu_only
 @pytest.mark.parametrize("name", ["norm", "add_norm", "dropout", "rotary", "attend", "few"])
 def test_on_another_stream_and_from_two_threads(gpu, name):
     calls = [ops(gpu, s)[name] for s in (3, 4)]
