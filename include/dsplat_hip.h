@@ -610,7 +610,8 @@ int dtk_rotary(int64_t B, int64_t L, int Hq, int Hk, int D, int F, int axes, int
  * block), in 64 bits; index [B,Hkv,ceil(Lq/block),top] = the top blocks of the highest score among
  * the allowed ones (allowed [ceil(Lq/block), ceil(Lk/block)] bytes, NULL: all) that hold a key, ties to
  * the lowest block, ascending, -1 behind. A score that is no number ranks lowest. q_lengths,
- * kv_lengths [B] (NULL: all of Lq, Lk): rows behind them do not count. D <= 256. */
+ * kv_lengths [B] (NULL: all of Lq, Lk): rows behind them do not count. D <= 256; Lq, Lk below 2^31, Hq and
+ * B * Hkv below 2^16. */
 size_t dtk_select_blocks_workspace_size(int B, int64_t Lq, int64_t Lk, int Hkv, int D, int block);
 int dtk_select_blocks(int B, int64_t Lq, int64_t Lk, int Hq, int Hkv, int D, int block, int top, int dtype,
                       const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,

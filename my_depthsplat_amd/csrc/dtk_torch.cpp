@@ -359,8 +359,10 @@ std::pair<Tensor, MaybeTensor> rotary(const Tensor& q_, const MaybeTensor& k_, T
   TORCH_CHECK_VALUE(q.dim() == 4, "q must be [B,L,Hq,D], got ", q.sizes());
   TORCH_CHECK_VALUE(!k.defined() || (k.dim() == 4 && k.size(0) == q.size(0) && k.size(1) == q.size(1) && k.size(3) == q.size(3)),
                     "k must be [B,L,Hk,D] beside q ", q.sizes(), ", got ", k.defined() ? k.sizes() : q.sizes());
-  check_sizes(q, "q");
-  if (k.defined()) check_sizes(k, "k");
+  for (const Tensor* t : {&q, &k})  // (any number of sequences)
+    TORCH_CHECK_VALUE(!t->defined() || (t->size(0) <= INT32_MAX && t->size(1) <= INT32_MAX && t->size(0) * t->size(1) <= INT32_MAX &&
+                                        t->size(2) < 65536 && t->size(3) < (1LL << 20)),
+                      "too many tokens, heads or channels: ", t->sizes());
   row_type(q, "q");
   TORCH_CHECK_VALUE(!k.defined() || k.scalar_type() == q.scalar_type(), "q and k must have one type");
   const int64_t B = q.size(0), L = q.size(1), D = q.size(3);

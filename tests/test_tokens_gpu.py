@@ -300,6 +300,14 @@ def test_rotary_of_slices(gpu):
     assert torch.equal(none, dq) and T.rotary(packed[0], None, pos, fr)[1] is None
 
 
+def test_rotary_of_many_sequences(gpu):
+    """One token in each of 70001 sequences: the same bits as one sequence of so many tokens."""
+    T = tokens()
+    q, pos, freqs = torch.randn(70001, 1, 2, 16, device=gpu).to(BF16), torch.arange(70001, device=gpu), T.rotary_frequencies(16, device=gpu)
+    got = T.rotary(q, None, pos.view(-1, 1, 1), freqs)[0]
+    assert torch.equal(got.view(1, 70001, 2, 16), T.rotary(q.view(1, 70001, 2, 16), None, pos, freqs)[0])
+
+
 # ---- block choice ---------------------------------------------------------------------------
 
 
