@@ -480,15 +480,16 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 2 ? (DP > 64 || RW == 1 ? 2
     }
     return;
   }
-  const float inv = valid && l > 0.f ? 1.f / l : (l != l ? l : 0.f);
+  // a row behind the length is written as 0: its zeros beside an infinite key or value are no number
+  const float inv = l > 0.f ? 1.f / l : (l != l ? l : 0.f);
   T* op = (T*)a.out + (((int64_t)at.b * a.Lq + i) * a.Hq + h) * a.D;
 #pragma unroll
   for (int d = 0; d < ND; ++d)
 #pragma unroll
     for (int c = 0; c < 4; ++c)
       if (32 * d + 8 * c + 4 * half < a.D)
-        store4<T>(op + 32 * d + 8 * c + 4 * half, o[d][4 * c] * inv, o[d][4 * c + 1] * inv, o[d][4 * c + 2] * inv,
-                  o[d][4 * c + 3] * inv);
+        store4<T>(op + 32 * d + 8 * c + 4 * half, valid ? o[d][4 * c] * inv : 0.f, valid ? o[d][4 * c + 1] * inv : 0.f,
+                  valid ? o[d][4 * c + 2] * inv : 0.f, valid ? o[d][4 * c + 3] * inv : 0.f);
   if (half == 0 && a.lse) a.lse[((int64_t)at.b * a.Hq + h) * a.Lq + i] = valid ? base2 + log2f(l) : -INFINITY;
 }
 

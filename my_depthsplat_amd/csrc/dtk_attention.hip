@@ -47,8 +47,9 @@ __global__ __launch_bounds__(NT) void k_attend_join(Args a, int64_t rows) {
   }
   const int64_t i = r % a.Lq, bh = r / a.Lq, b = bh / a.Hq, h = bh % a.Hq;
   const bool valid = i < length_of(a.q_lengths, (int)b, a.Lq);
-  const float inv = valid && l > 0.f ? 1.f / l : (l != l ? l : 0.f);
-  store4<T>((T*)a.out + ((b * a.Lq + i) * a.Hq + h) * a.D + d, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
+  const float inv = l > 0.f ? 1.f / l : (l != l ? l : 0.f);  // (as k_attend_fwd: 0 behind the length whatever the sums are)
+  store4<T>((T*)a.out + ((b * a.Lq + i) * a.Hq + h) * a.D + d, valid ? o[0] * inv : 0.f, valid ? o[1] * inv : 0.f,
+            valid ? o[2] * inv : 0.f, valid ? o[3] * inv : 0.f);
   if (d == 0 && a.lse) a.lse[r] = valid ? m + log2f(l) : -INFINITY;
 }
 
