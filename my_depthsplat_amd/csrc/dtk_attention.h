@@ -843,6 +843,13 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 2 ? (DP <= 64 ? (RW == 1 ? 
           dp[r] = x[r] * (kFewExponents<T> ? (dp[r] - de) * down : dp[r] - de);
         }
       }
+      if (live < 32) {  // rows behind the length: zeros, which beside an infinite key or value are no number
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          x[r] = acc_row(r, half) < live ? x[r] : 0.f;
+          dp[r] = acc_row(r, half) < live ? dp[r] : 0.f;
+        }
+      }
       const Frag p0 = acc_frag<T>(x, 0), p1 = acc_frag<T>(x, 1), s0 = acc_frag<T>(dp, 0), s1 = acc_frag<T>(dp, 1);
 #pragma unroll
       for (int d = 0; d < ND; ++d) {

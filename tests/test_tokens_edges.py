@@ -48,3 +48,22 @@ def test_attention_is_0_behind_the_lengths_whatever_the_keys_hold(gpu, t, Lq, Hq
     for b, n in enumerate(lengths):
         assert float((o[b, :n].double().cpu() - want[b, :n]).abs().amax()) <= bound if n else True
         assert not o[b, n:].any() and not inf[b, n:].any()  # (no number would count)
+
+
+@gpu_only
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("Lq,Hq,block,n", [(100, 2, 64, 70), (150, 1, 128, 130), (64, 1, 32, 33), (130, 3, 64, 65)])
+def test_gradients_of_keys_take_nothing_from_rows_behind_the_lengths(gpu, t, Lq, Hq, block, n):
+    """dk and dv beside keys of -inf: those of the call that ends at the last row (the same rows in the same units of 32, added in the
+    same order)."""
+    q, k, v = masked_by_keys(gpu, t, Lq, 3 * block - 3, Hq, Lq)
+    index = torch.arange(3, device=gpu, dtype=torch.int32).expand(2, 1, -(-Lq // block), 3).contiguous()
+    do = torch.randn(2, Lq, Hq, 32, device=gpu).to(t)
+    k.requires_grad_(True), v.requires_grad_(True)
+    short = q[:, :n].contiguous()
+    want = torch.autograd.grad(tokens.block_sparse_attention(short, k, v, index[:, :, :-(-n // block)].contiguous(), block=block), (k, v), do[:, :n])
+    assert all(bool(x.isfinite().all()) and bool((x != 0).any()) for x in want)
+    lens = torch.tensor([n, n], device=gpu)
+    got = torch.autograd.grad(tokens.block_sparse_attention(q, k, v, index, block=block, q_lengths=lens), (k, v), do)
+    for name, a, b in zip(("dk", "dv"), got, want):
+        assert torch.equal(a, b), name
