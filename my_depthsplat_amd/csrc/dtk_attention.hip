@@ -37,7 +37,8 @@ __global__ __launch_bounds__(NT) void k_attend_join(Args a, int64_t rows) {
     for (int e = 0; e < 4; ++e) o[e] *= f0;
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-      const float f = s0 + k < a.splits ? exp2f(pm[k] - base) : 0.f;
+      if (s0 + k >= a.splits) break;  // (the last part's again: 0 times its infinities would be no number)
+      const float f = exp2f(pm[k] - base);
       l += pl[k] * f;
       o[0] += po[k].x * f;
       o[1] += po[k].y * f;

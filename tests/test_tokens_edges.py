@@ -67,3 +67,16 @@ def test_gradients_of_keys_take_nothing_from_rows_behind_the_lengths(gpu, t, Lq,
     got = torch.autograd.grad(tokens.block_sparse_attention(q, k, v, index, block=block, q_lengths=lens), (k, v), do)
     for name, a, b in zip(("dk", "dv"), got, want):
         assert torch.equal(a, b), name
+
+
+@gpu_only
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("Lq,blocks", [(1, 1), (1, 5), (1, 9), (1, 17), (7, 33), (70, 6)])
+def test_attention_of_infinite_values_in_split_lists(gpu, t, Lq, blocks):
+    """A value of inf, in the last block and in the first, is the answer in its channel, and in no other; lists of one part to
+    eight."""
+    q, k, v = (torch.randn(2, n, h, 32, device=gpu).to(t) for n, h in ((Lq, 2), (blocks * 64, 1), (blocks * 64, 1)))
+    v[:, -1, :, 0], v[:, 3, :, 1] = math.inf, -math.inf
+    index = torch.arange(blocks, device=gpu, dtype=torch.int32).expand(2, 1, -(-Lq // 64), blocks).contiguous()
+    o = tokens.block_sparse_attention(q, k, v, index)
+    assert bool((o[..., 0] == math.inf).all()) and bool((o[..., 1] == -math.inf).all()) and bool(o[..., 2:].isfinite().all())
