@@ -86,7 +86,7 @@ struct Args {
   float *lse;                // [B, Hq, Lq], base 2; -inf for rows without a key
   float *part, *part_m, *part_l;
   float* delta;
-  uint32_t *bits, *gmax, *chosen;
+  uint32_t *bits, *chosen;
   int4 *plan, *split;  // NULL where every list is short and every workgroup of dk/dv fits the chip at once
   int* planned;        // how many of each
 };
@@ -493,16 +493,43 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 2 ? (DP > 64 || RW == 1 ? 2
   if (half == 0 && a.lse) a.lse[((int64_t)at.b * a.Hq + h) * a.Lq + i] = valid ? base2 + log2f(l) : -INFINITY;
 }
 
-// ds is rounded to the inputs' type for its products. f16 has few exponents, so ds is taken there
-// relative to a power of two at the largest |do| (exact, undone in 32 bits): of the row in dq, of all rows
-// in dk.
+// ds is rounded to the inputs' type for its products. f16 has few exponents (its normal numbers end at 2^-14), so ds is taken
+// there times a power of two of its own for each column, which is a query in dq and a key in dk: it starts at 2^60 and
+// falls where the column's ds would pass 2^15, to put the largest at 2^12 to 2^13; what is summed so far is
+// scaled with it, in 32 bits, and all is undone at the end. So a column's terms keep f16's 11 bits down to 2^-26 of its largest,
+// whatever other rows, heads and scenes hold. (|ds| <= 2 D 65504^2 < 2^40: in 32 bits 2^60 times that is still a number.) p <= 1 is
+// taken times 2^12 for dv, for unlikely keys: by the exponent's base, at no cost.
+// 4 scenes of 32256 f16 tokens, 4 heads on 2 of 64, 16 blocks of 64: dq 349 us, dk/dv 470, where one power of two of the row (dq) and
+// of the whole call (dk), at the largest |do|, took 356 and 444 and lost the digits of a scene of 2^-13 of another's gradients.
 template <typename T>
 constexpr bool kFewExponents = __is_same(T, f16);
-__device__ __forceinline__ void ds_scale(uint32_t largest, float& down, float& up) {
-  const int e = (int)((largest >> 23) & 255);
-  const bool ok = e > 27 && e < 227;
-  down = ok ? __uint_as_float((uint32_t)(254 - e) << 23) : 1.f;
-  up = ok ? __uint_as_float((uint32_t)e << 23) : 1.f;
+constexpr int kFirstPower = 60, kLikely = 12;
+// ds: 16 rows of this lane's column, the others in the lane 32 further. ldexp by 0 leaves what is no number as it is.
+template <int ND>
+__device__ __forceinline__ bool keep_in_range(f32x16& ds, f32x16 (&sum)[ND], int& power) {
+  float most = 0.f;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) most = fmaxf(most, fabsf(ds[r]));
+  const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(most), __float_as_uint(most), false, false);
+  most = fmaxf(__uint_as_float(both[0]), __uint_as_float(both[1]));
+  const bool far = most >= 32768.f && most < INFINITY;
+  if (!__any(far)) return false;
+  const int down = far ? 12 - ((int)(__float_as_uint(most) >> 23) - 127) : 0;
+  power += down;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) ds[r] = __builtin_amdgcn_ldexpf(ds[r], down);
+#pragma unroll
+  for (int d = 0; d < ND; ++d)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) sum[d][r] = __builtin_amdgcn_ldexpf(sum[d][r], down);
+  return true;
+}
+template <int ND>
+__device__ __forceinline__ void shift(f32x16 (&sum)[ND], int power) {
+#pragma unroll
+  for (int d = 0; d < ND; ++d)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) sum[d][r] = __builtin_amdgcn_ldexpf(sum[d][r], power);
 }
 
 // dq: the forward's shape; p is taken from the saved lse. delta = sum_d do o of each row on the
@@ -542,7 +569,7 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 2 ? (DP > 64 || RW == 1 ? 2
   const T* gp = (const T*)a.g.p + at.b * a.g.b + ir * a.g.l + h * a.g.h;
   const T* op = (const T*)a.o.p + at.b * a.o.b + ir * a.o.l + h * a.o.h;
   Frag qf[NS], gf[NS];
-  float delta = 0.f, most = 0.f;
+  float delta = 0.f;
 #pragma unroll
   for (int s = 0; s < NS; ++s) {
     qf[s] = row_frag<T>(qp, 16 * s + 8 * half, a.D, valid);
@@ -550,20 +577,9 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 2 ? (DP > 64 || RW == 1 ? 2
     gf[s] = row_frag<T>(gp, 16 * s + 8 * half, a.D, valid);
     const Frag of = row_frag<T>(op, 16 * s + 8 * half, a.D, valid);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      delta += (float)gf[s][j] * (float)of[j];
-      if (kFewExponents<T>) most = fmaxf(most, fabsf((float)gf[s][j]));
-    }
+    for (int j = 0; j < 8; ++j) delta += (float)gf[s][j] * (float)of[j];
   }
   delta += __shfl_xor(delta, 32, 64);
-  float down = 1.f, up = 1.f;
-  if constexpr (kFewExponents<T>) {
-    most = fmaxf(most, __shfl_xor(most, 32, 64));
-    ds_scale(__float_as_uint(most), down, up);
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) most = fmaxf(most, __shfl_xor(most, off, 64));
-    if (kw == 0 && lane == 0 && most > 0.f) atomicMax(a.gmax, __float_as_uint(most));  // any order, the same answer
-  }
   const int64_t stat = ((int64_t)at.b * a.Hq + h) * a.Lq + ir;
   // rows that see nothing: relative to +inf every p is 0
   const float saved = valid ? a.lse[stat] : -INFINITY, lse = saved == -INFINITY ? INFINITY : saved;
@@ -572,6 +588,8 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 2 ? (DP > 64 || RW == 1 ? 2
   const T* vp = (const T*)a.v.p + at.b * a.v.b + at.hk * a.v.h;
 
   f32x16 dq[ND] = {};
+  int power = kFirstPower;  // f16: of this query's ds
+  float times = __builtin_amdgcn_ldexpf(1.f, power);
   const int units = n << a.lg;
   const Keys where_ = {list, a.lg, units, nk};
   Stage<T, DP, U> sk, sv;
@@ -615,8 +633,10 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 2 ? (DP > 64 || RW == 1 ? 2
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(x[r], a.scale2, -lse));
-        x[r] = p * (kFewExponents<T> ? (dp[r] - delta) * down : dp[r] - delta);
+        x[r] = p * (kFewExponents<T> ? (dp[r] - delta) * times : dp[r] - delta);
       }
+      if constexpr (kFewExponents<T>)
+        if (keep_in_range(x, dq, power)) times = __builtin_amdgcn_ldexpf(1.f, power);
       const Frag s0 = acc_frag<T>(x, 0), s1 = acc_frag<T>(x, 1);
 #pragma unroll
       for (int d = 0; d < ND; ++d) {
@@ -625,6 +645,7 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 2 ? (DP > 64 || RW == 1 ? 2
       }
     }
   }
+  if constexpr (kFewExponents<T>) shift(dq, -power);
   if constexpr (KW > 1) {
     float* jo = (float*)lds + (rw * 32 + col) * (DP + 1);
     for (int k = 1; k < KW; ++k) {
@@ -644,7 +665,7 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 2 ? (DP > 64 || RW == 1 ? 2
   }
   if (kw != 0 || !exists) return;
   T* out = (T*)a.dq + (((int64_t)at.b * a.Lq + i) * a.Hq + h) * a.D;
-  const float f = a.scale * up;
+  const float f = a.scale;
 #pragma unroll
   for (int d = 0; d < ND; ++d)
 #pragma unroll
@@ -725,9 +746,9 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 2 ? (DP <= 64 ? (RW == 1 ? 
     sv.store(tkv + RW * L::kUnit);
     tkv += rw * L::kUnit;
   }
-  float down = 1.f, up = 1.f;
-  if constexpr (kFewExponents<T>) ds_scale(*a.gmax, down, up);
   f32x16 dk[ND] = {}, dv[ND] = {};
+  int power = kFirstPower;  // f16: of this key's ds, p's included
+  float times = __builtin_amdgcn_ldexpf(1.f, power - kLikely);
   const int upt = a.G << a.lg, words = (a.Tq + 31) / 32;  // units per tile
   const uint32_t* bits = a.bits + (((int64_t)b * a.Hkv + hk) * a.Tk + blk) * words;
   const bool any = blk * a.block < nk;
@@ -814,7 +835,7 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 2 ? (DP <= 64 ? (RW == 1 ? 
       f.g.store(tg);
       if (threadIdx.x < QW * 32) {
         // rows that see nothing, or are none: relative to +inf every p is 0
-        stats[step % NB][0][threadIdx.x] = f.lse == -INFINITY ? INFINITY : f.lse;
+        stats[step % NB][0][threadIdx.x] = f.lse == -INFINITY ? INFINITY : kFewExponents<T> ? f.lse - kLikely : f.lse;
         stats[step % NB][1][threadIdx.x] = f.delta;
       }
       __syncthreads();
@@ -840,7 +861,7 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 2 ? (DP <= 64 ? (RW == 1 ? 
           const float ls = e == 0 ? lse.x : e == 1 ? lse.y : e == 2 ? lse.z : lse.w;
           const float de = e == 0 ? delta.x : e == 1 ? delta.y : e == 2 ? delta.z : delta.w;
           x[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[r], a.scale2, -ls));
-          dp[r] = x[r] * (kFewExponents<T> ? (dp[r] - de) * down : dp[r] - de);
+          dp[r] = x[r] * (kFewExponents<T> ? (dp[r] - de) * times : dp[r] - de);
         }
       }
       if (live < 32) {  // rows behind the length: zeros, which beside an infinite key or value are no number
@@ -850,6 +871,8 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 2 ? (DP <= 64 ? (RW == 1 ? 
           dp[r] = acc_row(r, half) < live ? dp[r] : 0.f;
         }
       }
+      if constexpr (kFewExponents<T>)
+        if (keep_in_range(dp, dk, power)) times = __builtin_amdgcn_ldexpf(1.f, power - kLikely);
       const Frag p0 = acc_frag<T>(x, 0), p1 = acc_frag<T>(x, 1), s0 = acc_frag<T>(dp, 0), s1 = acc_frag<T>(dp, 1);
 #pragma unroll
       for (int d = 0; d < ND; ++d) {
@@ -867,6 +890,10 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 2 ? (DP <= 64 ? (RW == 1 ? 
 #pragma unroll
       for (int k = 0; k < kAhead; ++k)
         if (u + k * stride < units) turn(f[k], u + k * stride);
+  }
+  if constexpr (kFewExponents<T>) {
+    shift(dk, -power);
+    shift(dv, -kLikely);
   }
   if constexpr (QW > 1) {
     float* jo = (float*)lds + (rw * 32 + col) * (DP + 1);
@@ -899,13 +926,13 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 2 ? (DP <= 64 ? (RW == 1 ? 
       for (int c = 0; c < 4; ++c) {
         const int e = 32 * d + 8 * c + 4 * half;
         if (e >= a.D) continue;
-        store4<float>(pk + e, dk[d][4 * c] * a.scale * up, dk[d][4 * c + 1] * a.scale * up, dk[d][4 * c + 2] * a.scale * up,
-                      dk[d][4 * c + 3] * a.scale * up);
+        store4<float>(pk + e, dk[d][4 * c] * a.scale, dk[d][4 * c + 1] * a.scale, dk[d][4 * c + 2] * a.scale,
+                      dk[d][4 * c + 3] * a.scale);
         store4<float>(pv + e, dv[d][4 * c], dv[d][4 * c + 1], dv[d][4 * c + 2], dv[d][4 * c + 3]);
       }
     return;
   }
-  const float f = a.scale * up;
+  const float f = a.scale;
 #pragma unroll
   for (int d = 0; d < ND; ++d)
 #pragma unroll

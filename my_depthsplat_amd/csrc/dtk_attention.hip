@@ -190,10 +190,10 @@ Args args_of(const dtk_attention* c) {
 }
 size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
 
-// The backward's workspace: delta, what is cleared (the largest |do|, the lists' bits and lengths), the plan of dk/dv,
+// The backward's workspace: delta, what is cleared (the lists' bits and lengths), the plan of dk/dv,
 // the parts in f32.
 struct BwdLayout {
-  size_t gmax, bits, chosen, planned, plan, split, part, end;
+  size_t bits, chosen, planned, plan, split, part, end;
   int64_t items, slots;  // slots: parts of split lists, at most
   int most;              // steps of a part; 0: no plan
 };
@@ -210,8 +210,7 @@ BwdLayout layout_of(const dtk_attention* c, const Args& a) {
   const int64_t most = steps / 1024 > 8 ? steps / 1024 : 8;
   l.most = l.items > 512 || a.Tq * units > most * together ? (int)(most < (1 << 30) ? most : 1 << 30) : 0;
   l.slots = l.most ? 2 * steps / l.most + 1 : 0;  // a list of n > most steps has fewer than 2 n / most parts
-  l.gmax = align256((size_t)c->B * c->Hq * c->Lq * 4);
-  l.bits = l.gmax + 256;
+  l.bits = align256((size_t)c->B * c->Hq * c->Lq * 4);
   l.chosen = l.bits + (size_t)l.items * ((a.Tq + 31) / 32) * 4;
   l.planned = align256(l.chosen + (l.most ? (size_t)l.items * 4 : 0));
   l.plan = l.planned + 256;
@@ -280,7 +279,6 @@ int dtk_block_sparse_attention_bwd(const dtk_attention* c, const void* dout, con
   const BwdLayout l = layout_of(c, a);
   DSPLAT_REQUIRE(l.items + l.slots < (1LL << 31), "dtk_block_sparse_attention_bwd: too large");
   a.delta = (float*)ws;
-  a.gmax = (uint32_t*)(ws + l.gmax);
   a.bits = (uint32_t*)(ws + l.bits);
   if (l.most) {
     a.chosen = (uint32_t*)(ws + l.chosen);
@@ -289,7 +287,7 @@ int dtk_block_sparse_attention_bwd(const dtk_attention* c, const void* dout, con
     a.split = (int4*)(ws + l.split);
     a.part = (float*)(ws + l.part);
   }
-  if (int e = dsplat::zero_async(a.gmax, l.planned - l.gmax, st, "dtk_block_sparse_attention_bwd")) return e;
+  if (int e = dsplat::zero_async(a.bits, l.planned - l.bits, st, "dtk_block_sparse_attention_bwd")) return e;
   if (c->Lq) {
     const dim3 grid(a.Tq * a.rowtiles, a.Hkv, c->B);
     if (int e = by_type(c->dtype, attend_dq<float>, attend_dq<bf16>, attend_dq<f16>)(a, row_waves(a), grid, st)) return e;

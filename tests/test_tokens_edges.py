@@ -6,6 +6,7 @@ import math
 import pytest
 import torch
 
+import token_oracle as orc
 from my_depthsplat_amd import tokens
 
 gpu_only = pytest.mark.gpu
@@ -80,3 +81,118 @@ def test_attention_of_infinite_values_in_split_lists(gpu, t, Lq, blocks):
     index = torch.arange(blocks, device=gpu, dtype=torch.int32).expand(2, 1, -(-Lq // 64), blocks).contiguous()
     o = tokens.block_sparse_attention(q, k, v, index)
     assert bool((o[..., 0] == math.inf).all()) and bool((o[..., 1] == -math.inf).all()) and bool(o[..., 2:].isfinite().all())
+
+
+# ---- f16: gradients of very different sizes ------------------------------------------------
+
+
+def f16_gradients(q, k, v, do, see, scale):
+    """64-bit inputs of one head each, q, do [L, D], k, v [Lk, D], see [L, Lk] -> name -> (gradient, bound). Each row's
+    terms are counted by its own |do|: p and ds are rounded to f16 for their products, half a step of their value or, far
+    below the largest of their column, of f16's smallest numbers relative to it: the column's largest is
+    taken to 2^12 at least, so 2^-25 / 2^12 of it; p is at most 1 and taken times 2^12."""
+    h = orc.half_step(F16)
+    x = (q @ k.T * scale).masked_fill(~see, -math.inf)
+    p = torch.softmax(x, -1)
+    o, dp = p @ v, do @ v.T
+    ds = p * (dp - (do * o).sum(-1, keepdim=True))
+    noise = (2 * q.shape[1] + int(see.sum(-1).max()) + 32) * orc.E32 * (1 + float((q.abs() @ k.abs().T).max()) * abs(scale))
+    # delta is of o as it was rounded
+    e = h * ds.abs() + p * (h * (do.abs() * o.abs()).sum(-1, keepdim=True)
+                            + noise * (do.abs() @ v.abs().T + (do.abs() * (p @ v.abs())).sum(-1, keepdim=True)))
+    low = 2.0 ** -37
+    eq, ek = (e + see * low * ds.abs().amax(1, keepdim=True)), (e + see * low * ds.abs().amax(0, keepdim=True))
+    ep = (h + noise) * p + see * low
+    rows = q.shape[0] * orc.E32
+    out = {"dq": (ds @ k * scale, eq @ k.abs() * abs(scale)),
+           "dk": (ds.T @ q * scale, (ek + rows * ds.abs()).T @ q.abs() * abs(scale)),
+           "dv": (p.T @ do, (ep + rows * p).T @ do.abs())}
+    return {n: (g, b + h * g.abs() + orc.tiny(F16)) for n, (g, b) in out.items()}
+
+
+def check_f16_gradients(gpu, q, k, v, do, index, block, scale, only=("dq", "dk", "dv")):
+    """[B, L, D] f16 host tensors of one head"""
+    leaves = [x[:, :, None].to(gpu).requires_grad_(True) for x in (q, k, v)]
+    o = tokens.block_sparse_attention(*leaves, index.to(gpu), block=block, scale=scale)
+    got = torch.autograd.grad(o, leaves, do[:, :, None].to(gpu))
+    for b in range(q.shape[0]):
+        see = torch.zeros(q.shape[1], k.shape[1], dtype=torch.bool)
+        for tile in range(index.shape[2]):
+            for j in index[b, 0, tile].tolist():
+                if j >= 0:
+                    see[tile * block:(tile + 1) * block, j * block:(j + 1) * block] = True
+        want = f16_gradients(*(x[b].double() for x in (q, k, v, do)), see, scale)
+        for name, g in zip(("dq", "dk", "dv"), got):
+            if name in only:
+                orc.assert_within(g[b, :, 0], *want[name], f"{name} of scene {b}")
+
+
+def f16(*shape, seed=0, scale=1.0):
+    return (torch.randn(*shape, generator=torch.Generator().manual_seed(seed)) * scale).to(F16)
+
+
+@gpu_only
+@pytest.mark.parametrize("D,block", [(32, 32), (64, 64), (96, 128), (128, 64)])
+def test_f16_gradients_of_a_scene_do_not_depend_on_anothers(gpu, D, block):
+    """Scenes whose do are 2^8, 1 and 2^-8: each within its own roundings, and the bits of the scene by itself."""
+    L = 4 * block
+    q, k, v, do = (f16(3, L, D, seed=i) for i in range(4))
+    do = do * torch.tensor([2.0 ** 8, 1.0, 2.0 ** -8]).to(F16)[:, None, None]
+    # (few of f16's smallest numbers in do itself: those stay as they are)
+    index = torch.arange(4, dtype=torch.int32).expand(3, 1, 4, 4).contiguous()
+    check_f16_gradients(gpu, q, k, v, do, index, block, D ** -0.5)
+    together = [x[:, :, None].to(gpu).requires_grad_(True) for x in (q, k, v)]
+    gd = do[:, :, None].to(gpu)
+    all_of = torch.autograd.grad(tokens.block_sparse_attention(*together, index.to(gpu), block=block), together, gd)
+    for b in range(3):
+        alone = [x[b:b + 1].detach().requires_grad_(True) for x in together]
+        one = torch.autograd.grad(tokens.block_sparse_attention(*alone, index[b:b + 1].to(gpu), block=block), alone, gd[b:b + 1])
+        assert all(torch.equal(x[b:b + 1], y) for x, y in zip(all_of, one)), b
+
+
+@gpu_only
+@pytest.mark.parametrize("block,Lq,G", [(32, 128, 1), (64, 256, 1), (128, 256, 1), (64, 1, 1)])
+def test_f16_gradients_of_a_row_do_not_depend_on_its_neighbours(gpu, block, Lq, G):
+    """Every other row has a do of 2^10 and zeros in the second half of q's channels, so dk's second half comes from the rows between
+    alone, whose do is 2^-4; the large rows come first in some units and last in others."""
+    D, L = 64, Lq
+    q, k, v, do = f16(1, L, D, seed=1), f16(1, 3 * block, D, seed=2), f16(1, 3 * block, D, seed=3), f16(1, L, D, seed=4)
+    large = torch.zeros(L, dtype=torch.bool)
+    large[::2] = True
+    large[32:64] = False
+    large[64:96] = True
+    q[:, large, D // 2:] = 0
+    do = torch.where(large[:, None], do * 2.0 ** 10, do * 2.0 ** -4).to(F16)
+    index = torch.arange(3, dtype=torch.int32).expand(1, 1, -(-L // block), 3).contiguous()
+    check_f16_gradients(gpu, q, k, v, do, index, block, D ** -0.5)
+
+
+@gpu_only
+@pytest.mark.parametrize("block", [32, 64, 128])
+def test_f16_gradients_of_unlikely_keys(gpu, block):
+    """The second block's keys get a share of 2^-17 each: below f16's normal numbers, yet their gradients, of a do of 2^10, are not."""
+    D, L = 32, 2 * block
+    q, k, v, do = f16(1, L, D, seed=1, scale=0.3), f16(1, L, D, seed=2, scale=0.3), f16(1, L, D, seed=3), f16(1, L, D, seed=4, scale=2.0 ** 10)
+    q[..., 0], k[:, :block, 0], k[:, block:, 0] = 1.0, 0.0, -(17 - math.log2(block)) * math.log(2)
+    index = torch.arange(2, dtype=torch.int32).expand(1, 1, 2, 2).contiguous()
+    check_f16_gradients(gpu, q, k, v, do, index, block, 1.0)
+
+
+@gpu_only
+def test_f16_gradients_of_infinite_and_zero_rows(gpu):
+    """Rows whose do is 0 give 0; one of infinity in one scene leaves the others' gradients as they are."""
+    q, k, v, do = (f16(2, 128, 1, 64, seed=i).to(gpu) for i in range(4))
+    index = torch.arange(2, device=gpu, dtype=torch.int32).expand(2, 1, 2, 2).contiguous()
+
+    def grads(g):
+        leaves = [x.detach().requires_grad_(True) for x in (q, k, v)]
+        return torch.autograd.grad(tokens.block_sparse_attention(*leaves, index), leaves, g)
+
+    want = grads(do)
+    bad = do.clone()
+    bad[0, 5, 0, 3] = math.inf
+    got = grads(bad)
+    assert all(torch.equal(a[1], b[1]) for a, b in zip(got, want))
+    keep = [i for i in range(128) if i != 5]
+    assert torch.equal(got[0][0, keep], want[0][0, keep]) and not got[0][0, 5].isfinite().all()
+    assert all(not x.any() for x in grads(torch.zeros_like(do)))
