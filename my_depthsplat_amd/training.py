@@ -100,11 +100,22 @@ class GaussianHead(nn.Module):
         self.layers = None
         if token_layers:
             from .token_layer import ViewTokenLayer
-            from .tokens import rotary_frequencies
             self.layers = nn.ModuleList(ViewTokenLayer(2 * width, token_heads, top=token_top, p=token_dropout)
                                         for _ in range(token_layers))
-            self.register_buffer("freqs", rotary_frequencies(self.layers[0].part(2), 2, device="cpu"), persistent=False)
+            self.register_buffer("freqs", self._frequencies("cpu"), persistent=False)
             self.register_buffer("rng", torch.tensor([seed, 0], dtype=torch.int64))
+
+    def _apply(self, fn, recurse=True):
+        freqs = getattr(self, "freqs", None)
+        super()._apply(fn, recurse)
+        if freqs is not None:  # angles are taken in 64 bits: the frequencies follow the device, never a cast
+            device = self.freqs.device
+            self.freqs = freqs if device == freqs.device else self._frequencies(device)
+        return self
+
+    def _frequencies(self, device) -> torch.Tensor:
+        from .tokens import rotary_frequencies
+        return rotary_frequencies(self.layers[0].part(2), 2, device=device)
 
     def _view_tokens(self, x: torch.Tensor, views: int) -> torch.Tensor:
         """[BV, C, h, w] -> the same, through the token layers over the V h w tokens of each scene."""

@@ -196,3 +196,44 @@ def test_f16_gradients_of_infinite_and_zero_rows(gpu):
     keep = [i for i in range(128) if i != 5]
     assert torch.equal(got[0][0, keep], want[0][0, keep]) and not got[0][0, 5].isfinite().all()
     assert all(not x.any() for x in grads(torch.zeros_like(do)))
+
+
+# ---- the head and its layer -----------------------------------------------------------------
+
+
+def small_head(**kw):
+    from my_depthsplat_amd.training import GaussianHead
+    torch.manual_seed(0)
+    return GaussianHead(10, **{**dict(width=24, down=2, token_layers=2, token_heads=2, token_top=2, seed=7), **kw})
+
+
+def scene(gpu, t=F32):
+    torch.manual_seed(1)
+    return torch.rand(2, 3, 3, 24, 16, device=gpu).to(t), torch.rand(2, 3, 24 * 16, 1, 1, device=gpu).to(t)
+
+
+@pytest.mark.parametrize("cast", [lambda m: m.bfloat16(), lambda m: m.half(), lambda m: m.float(), lambda m: m.double().float(),
+                                  lambda m: m.to(BF16), lambda m: m.to("meta").to_empty(device="cpu")])
+def test_head_frequencies_keep_64_bits_through_casts(cast):
+    want = small_head().freqs.clone()
+    head = cast(small_head())
+    assert head.freqs.dtype == torch.float64 and torch.equal(head.freqs, want)
+    assert head.rng.dtype == torch.int64 and "freqs" not in head.state_dict()
+    kept = head.freqs
+    assert head.float().freqs is kept and head.cpu().freqs is kept  # (a captured graph may hold it)
+    assert small_head(token_layers=0).bfloat16().layers is None
+
+
+@gpu_only
+@pytest.mark.parametrize("t", TYPES)
+def test_head_in_each_type_trains(gpu, t):
+    """A module cast: every parameter gets a finite gradient, and the output is within a tenth of the f32 head's norm (some 20
+    roundings of 2^-8 in turn)."""
+    head = small_head(token_dropout=0.1)
+    want = small_head(token_dropout=0.1).to(gpu)(*scene(gpu)).detach()
+    head = head.to(gpu).to(t)
+    y = head(*scene(gpu, t))
+    assert float((y.detach().float() - want).norm() / want.norm()) < 0.1
+    y.float().square().sum().backward()
+    for n, p in head.named_parameters():
+        assert p.grad is not None and p.grad.dtype == t and bool(p.grad.isfinite().all()) and bool((p.grad != 0).any()), n
