@@ -53,6 +53,7 @@ class ViewTokenLayer(nn.Module):
         at = dict(block=self.block, q_lengths=lengths, kv_lengths=lengths)
         index = tokens.select_blocks(q, k, self.top, allowed=allowed, **at)
         o = tokens.block_sparse_attention(q, k, v, index, **at)
-        s, y = tokens.dropout_add_layer_norm(self.out(o.flatten(2)), x, self.norm2.weight, self.norm2.bias, p=p, rng=rng,
+        # (under autocast the projections come in 16 bits: the sum over the layers stays in the rows' own type)
+        s, y = tokens.dropout_add_layer_norm(self.out(o.flatten(2)).to(x.dtype), x, self.norm2.weight, self.norm2.bias, p=p, rng=rng,
                                              call=call, eps=self.norm2.eps)
-        return tokens.dropout(self.fc2(F.gelu(self.fc1(y))), p, rng, call + 1, residual=s)
+        return tokens.dropout(self.fc2(F.gelu(self.fc1(y))).to(x.dtype), p, rng, call + 1, residual=s)

@@ -237,3 +237,27 @@ def test_head_in_each_type_trains(gpu, t):
     y.float().square().sum().backward()
     for n, p in head.named_parameters():
         assert p.grad is not None and p.grad.dtype == t and bool(p.grad.isfinite().all()) and bool((p.grad != 0).any()), n
+
+
+@gpu_only
+@pytest.mark.parametrize("t", [BF16, F16])
+def test_head_and_layer_under_autocast(gpu, t):
+    """The products in 16 bits, the sum of the layers in the rows' own type: within a tenth of the result without (some 20 roundings
+    of 2^-8 in turn), finite gradients in the parameters' type; the layer by itself keeps its input's type."""
+    head = small_head(token_dropout=0.1).to(gpu)
+    want = small_head(token_dropout=0.1).to(gpu)(*scene(gpu)).detach()
+    with torch.autocast("cuda", t):
+        y = head(*scene(gpu))
+    assert float((y.detach().float() - want).norm() / want.norm()) < 0.1
+    y.float().square().sum().backward()
+    for n, p in head.named_parameters():
+        assert p.grad is not None and p.grad.dtype == F32 and bool(p.grad.isfinite().all()), n
+    layer, freqs = head.layers[0].eval(), head.freqs
+    pos = tokens.view_positions(2, 5, 6, gpu)
+    x = torch.randn(2, 60, 48, device=gpu, requires_grad=True)
+    plain = layer(x, pos, freqs).detach()
+    with torch.autocast("cuda", t):
+        z = layer(x, pos, freqs)
+    assert z.dtype == F32 and float((z.detach() - plain).norm() / plain.norm()) < 0.05
+    (g,) = torch.autograd.grad(z.square().sum(), x)
+    assert g.dtype == F32 and bool(g.isfinite().all())
