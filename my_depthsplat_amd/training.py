@@ -84,7 +84,10 @@ class GaussianHead(nn.Module):
     token_layers > 0: that many ViewTokenLayers over the tokens of all views of a scene between the body
     and the output (GPU only), with `token_heads` heads, `token_top` key blocks per tile and dropout
     `token_dropout` from the generator state `rng` (seed, step): a buffer, so a checkpoint resumes it; the step
-    goes up with every training forward."""
+    goes up with every training forward. The mask is a function of the state and of the element's place in the rank's own
+    batch: data-parallel ranks need seeds of their own (after loading one rank's checkpoint too: head.rng[0] = seed).
+    Under activation checkpointing the state has to be an argument (forward(rng=head.next_rng())); a recomputed forward
+    without it is refused."""
 
     def __init__(self, d_out: int, width: int = 108, down: int = 8, token_layers: int = 0, token_heads: int = 3,
                  token_top: int = 16, token_dropout: float = 0.0, seed: int = 0):
@@ -117,26 +120,42 @@ class GaussianHead(nn.Module):
         from .tokens import rotary_frequencies
         return rotary_frequencies(self.layers[0].part(2), 2, device=device)
 
-    def _view_tokens(self, x: torch.Tensor, views: int) -> torch.Tensor:
+    def next_rng(self) -> torch.Tensor:
+        """The generator state of one training forward, for forward(rng=...); the step goes up."""
+        rng = self.rng.clone()  # the backward reads it again, after the step below
+        self.rng[1] += 1
+        return rng
+
+    def _own_rng(self) -> torch.Tensor:
+        again = torch._C._current_graph_task_id() != -1  # inside a backward pass
+        if self.training and not again:
+            return self.next_rng()
+        if self.training and any(layer.p > 0.0 for layer in self.layers):
+            raise RuntimeError("GaussianHead: a forward that a backward pass computes again (activation checkpointing) would draw "
+                               "another step's dropout masks: pass rng=head.next_rng() through the checkpoint")
+        return self.rng.clone()
+
+    def _view_tokens(self, x: torch.Tensor, views: int, rng: torch.Tensor | None) -> torch.Tensor:
         """[BV, C, h, w] -> the same, through the token layers over the V h w tokens of each scene."""
         from .tokens import view_positions
         BV, C, h, w = x.shape
         t = x.view(BV // views, views, C, h * w).transpose(2, 3).reshape(BV // views, views * h * w, C)
         positions = view_positions(views, h, w, x.device)
-        rng = self.rng.clone()  # the backward reads it again, after the step below
+        if rng is None:
+            rng = self._own_rng()
         for i, layer in enumerate(self.layers):
             t = layer(t, positions, self.freqs, rng, 2 * i)
-        if self.training:
-            self.rng[1] += 1
         return t.view(BV, h * w, C).transpose(1, 2).reshape(BV, C, h, w)
 
-    def forward(self, images: torch.Tensor, depths: torch.Tensor) -> torch.Tensor:
+    def forward(self, images: torch.Tensor, depths: torch.Tensor, rng: torch.Tensor | None = None) -> torch.Tensor:
+        """rng (with token layers): the generator state to draw from, as next_rng() gives it; None: the head's own,
+        whose step goes up while training."""
         B, V, _, H, W = images.shape
         x = torch.cat([images, depths.reshape(B, V, 1, H, W)], 2).reshape(B * V, 4, H, W)
         x = F.avg_pool2d(x, self.down)
         x = self.body(self.stem(x))
         if self.layers is not None:
-            x = self._view_tokens(x, V)
+            x = self._view_tokens(x, V, rng)
         x = self.out(x)                                         # [BV, d_out r^2, h, w], r = down
         # pixel shuffle + "(b v) c h w -> b v (h w) c" in one pass (head_rows):
         # out[b, v, (hh r + i) W + ww r + j, c] = x[bv, c r^2 + i r + j, hh, ww]

@@ -261,3 +261,38 @@ def test_head_and_layer_under_autocast(gpu, t):
     assert z.dtype == F32 and float((z.detach() - plain).norm() / plain.norm()) < 0.05
     (g,) = torch.autograd.grad(z.square().sum(), x)
     assert g.dtype == F32 and bool(g.isfinite().all())
+
+
+@gpu_only
+@pytest.mark.parametrize("reentrant", [False, True])
+def test_head_under_activation_checkpointing(gpu, reentrant):
+    """A forward that is computed again draws the same masks if its generator state is an argument: the gradients of the call
+    without, in several steps at once; without that argument it is an error, not another step's masks."""
+    from torch.utils.checkpoint import checkpoint
+    images, depths = scene(gpu)
+    images.requires_grad_(True)  # (a reentrant checkpoint needs an input that asks for a gradient)
+    head = small_head(token_dropout=0.3).to(gpu)
+
+    def grads(run):
+        head.zero_grad()
+        head.rng.copy_(torch.tensor([7, 0]))
+        outs = [run(head.next_rng()) for _ in range(2)]
+        assert head.rng.tolist() == [7, 2]
+        sum((y * y).sum() for y in outs).backward()
+        assert head.rng.tolist() == [7, 2]
+        return [y.detach() for y in outs], [p.grad.clone() for p in head.parameters()]
+
+    want, want_grads = grads(lambda rng: head(images, depths, rng))
+    got, got_grads = grads(lambda rng: checkpoint(head, images, depths, rng, use_reentrant=reentrant))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    # (torch's convolutions' weight gradients may add in any order)
+    assert all(float((a - b).norm()) <= 1e-5 * float(b.norm()) for a, b in zip(got_grads, want_grads))
+    y = checkpoint(head, images, depths, use_reentrant=reentrant)
+    with pytest.raises(RuntimeError, match="next_rng"):
+        y.sum().backward()
+    with torch.no_grad():
+        head.rng.copy_(torch.tensor([7, 0]))
+        assert torch.equal(head(images, depths), want[0]) and head.rng.tolist() == [7, 1]
+    dry = small_head(token_dropout=0.0).to(gpu)  # nothing is drawn, so nothing can differ
+    checkpoint(dry, images, depths, use_reentrant=reentrant).sum().backward()
+    assert dry.rng.tolist() == [7, 1]
