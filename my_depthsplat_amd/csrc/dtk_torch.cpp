@@ -5,8 +5,8 @@
 // 5 - 60 us, and the Python layers took 90 - 120 us of host time forward and backward (11 us forward alone) against
 // torch's own 45 us for any node (its engine's thread). From here it is that and the launches.
 //
-// Errors: ValueError for arguments, DsplatError (my_depthsplat_amd._lib) for tensors that are not on a GPU and for a
-// status of the C ABI.
+// Errors: ValueError for arguments, NotImplementedError for forward-mode derivatives, DsplatError (my_depthsplat_amd._lib) for
+// tensors that are not on a GPU and for a status of the C ABI.
 #include <torch/extension.h>
 
 #include <c10/hip/HIPStream.h>
@@ -92,6 +92,15 @@ bool wants_grad(std::initializer_list<const Tensor*> ts) {
   return false;
 }
 
+// A forward-mode derivative would be lost on the way to the result, which is a derivative of 0: refused. (A look at the
+// tensors' own data; no dispatch.)
+void no_tangent(std::initializer_list<const Tensor*> ts) {
+  if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+  for (const Tensor* t : ts)
+    TORCH_CHECK_NOT_IMPLEMENTED(!t->defined() || !t->_fw_grad(/*level=*/0).defined(),
+                                "the view-token operators have no forward-mode derivatives: take the tangent off (unpack_dual)");
+}
+
 // A backward's gradients. Where a graph of the backward is being made, differentiating them is an error, not zeros.
 variable_list once(variable_list grads) {
   if (!at::GradMode::is_enabled()) return grads;
@@ -159,6 +168,7 @@ Tensor dropout(const Tensor& x, double p, const MaybeTensor& rng_, int64_t call,
   TORCH_CHECK_VALUE(!residual.defined() || (residual.sizes() == x.sizes() && residual.scalar_type() == x.scalar_type()),
                     "residual does not match x: ", x.scalar_type(), " ", x.sizes());
   if (p == 0.0) rng = Tensor();
+  if (p > 0.0 || residual.defined()) no_tangent({&x, &residual});  // (else x is returned with all it has)
   same_device(x, {{"residual", &residual}, {"rng", &rng}});
   if (p == 0.0 && !residual.defined()) return x;
   residual = contiguous(residual);
@@ -272,6 +282,7 @@ void check_norm(const Tensor& x, const Tensor& weight, const Tensor& bias, doubl
 Tensor layer_norm(const Tensor& x, const MaybeTensor& weight_, const MaybeTensor& bias_, double eps) {
   Tensor weight = or_none(weight_), bias = or_none(bias_);
   check_norm(x, weight, bias, eps);
+  no_tangent({&x, &weight, &bias});
   same_device(x, {{"weight", &weight}, {"bias", &bias}});
   weight = contiguous(weight);
   bias = contiguous(bias);
@@ -287,6 +298,7 @@ std::pair<Tensor, Tensor> dropout_add_layer_norm(const Tensor& x, const Tensor& 
   TORCH_CHECK_VALUE(residual.sizes() == x.sizes() && residual.scalar_type() == x.scalar_type(),
                     "residual does not match x: ", x.scalar_type(), " ", x.sizes());
   if (p == 0.0) rng = Tensor();
+  no_tangent({&x, &residual, &weight, &bias});
   same_device(x, {{"residual", &residual}, {"weight", &weight}, {"bias", &bias}, {"rng", &rng}});
   weight = contiguous(weight);
   bias = contiguous(bias);
@@ -376,6 +388,7 @@ std::pair<Tensor, MaybeTensor> rotary(const Tensor& q_, const MaybeTensor& k_, T
                     "freqs must be float64 [F], 2 F <= ", D, ", F a multiple of the ", axes, " axes, got ", freqs.scalar_type(), " ",
                     freqs.sizes());
   TORCH_CHECK_VALUE(!wants_grad({&positions, &freqs}), "positions and freqs have no gradient: detach them");
+  no_tangent({&q, &k, &positions, &freqs});
   same_device(q, {{"k", &k}, {"positions", &positions}, {"freqs", &freqs}});
   q = dense_rows(q);
   if (k.defined()) k = dense_rows(k);
@@ -516,6 +529,7 @@ Tensor block_sparse_attention(const Tensor& q_, const Tensor& k_, const Tensor& 
                     "index must be int32 [", B, ", ", Hkv, ", ", Tq, ", 1..1024], got ", index_.scalar_type(), " ", index_.sizes());
   check_lengths(q_lengths, "q_lengths", B);
   check_lengths(kv_lengths, "kv_lengths", B);
+  no_tangent({&q_, &k_, &v_});
   same_device(q_, {{"k", &k_}, {"v", &v_}, {"index", &index_}, {"q_lengths", &q_lengths}, {"kv_lengths", &kv_lengths}});
   const Tensor q = dense_rows(q_), k = dense_rows(k_), v = dense_rows(v_), index = index_.contiguous();
   q_lengths = int32(q_lengths);

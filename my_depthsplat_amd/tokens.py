@@ -13,7 +13,7 @@ float32, bfloat16 or float16 rows; HIP kernels forward and backward (include/dsp
 argument checks and autograd nodes: csrc/dtk_torch.cpp), on torch's current stream of the
 tensors' device, without host synchronisation (capturable; a backward pass, as torch has it,
 with leaves that no graph made outside the capture holds).
-Gradients are the same bits every time (no atomics on them). Not differentiable twice.
+Gradients are the same bits every time (no atomics on them). Not differentiable twice, nor in forward mode (an error).
 """
 from __future__ import annotations
 

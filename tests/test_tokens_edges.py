@@ -7,7 +7,7 @@ import pytest
 import torch
 
 import token_oracle as orc
-from my_depthsplat_amd import tokens
+from my_depthsplat_amd import _lib, tokens
 
 gpu_only = pytest.mark.gpu
 F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
@@ -296,3 +296,47 @@ def test_head_under_activation_checkpointing(gpu, reentrant):
     dry = small_head(token_dropout=0.0).to(gpu)  # nothing is drawn, so nothing can differ
     checkpoint(dry, images, depths, use_reentrant=reentrant).sum().backward()
     assert dry.rng.tolist() == [7, 1]
+
+
+# ---- calls that are refused -----------------------------------------------------------------
+
+
+def dual_calls():
+    x, w = torch.randn(4, 8), torch.ones(8)
+    q, k = torch.randn(2, 5, 4, 16), torch.randn(2, 5, 2, 16)
+    rng, index = torch.zeros(2, dtype=torch.int64), torch.zeros(2, 2, 1, 1, dtype=torch.int32)
+    pos, freqs = torch.zeros(5), torch.ones(4, dtype=torch.float64)
+    T = tokens
+    return [((x,), lambda a: T.layer_norm(a)), ((w,), lambda a: T.layer_norm(x, a)), ((w,), lambda a: T.layer_norm(x, w, a)),
+            ((x,), lambda a: T.dropout(a, 0.5, rng)), ((x,), lambda a: T.dropout(x, 0.0, residual=a)),
+            ((x,), lambda a: T.dropout_add_layer_norm(a, x)), ((x,), lambda a: T.dropout_add_layer_norm(x, a)),
+            ((w,), lambda a: T.dropout_add_layer_norm(x, x, a)), ((w,), lambda a: T.dropout_add_layer_norm(x, x, w, a)),
+            ((q,), lambda a: T.rotary(a, k, pos, freqs)), ((k,), lambda a: T.rotary(q, a, pos, freqs)),
+            ((pos,), lambda a: T.rotary(q, k, a, freqs)), ((freqs,), lambda a: T.rotary(q, k, pos, a)),
+            ((q,), lambda a: T.block_sparse_attention(a, k, k, index)), ((k,), lambda a: T.block_sparse_attention(q, a, k, index)),
+            ((k,), lambda a: T.block_sparse_attention(q, k, a, index))]
+
+
+@pytest.mark.parametrize("case", range(16))
+def test_forward_mode_derivatives_are_refused(case):
+    """A tangent that the result would lose is an error, not a derivative of 0; outside its level nothing is refused for it."""
+    import torch.autograd.forward_ad as fw
+    if not _lib.LIB_PATH.exists():
+        pytest.skip("extension not built")
+    (t,), call = dual_calls()[case]
+    with fw.dual_level():
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            call(fw.make_dual(t, torch.ones_like(t)))
+    with pytest.raises(_lib.DsplatError):  # a CPU tensor
+        call(t)
+
+
+@gpu_only
+def test_forward_mode_derivatives_where_nothing_is_done(gpu):
+    """p = 0 returns x with its tangent; a tangent taken off is no obstacle."""
+    import torch.autograd.forward_ad as fw
+    x = torch.randn(4, 8, device=gpu)
+    with fw.dual_level():
+        d = fw.make_dual(x, torch.ones_like(x))
+        assert tokens.dropout(d, 0.0) is d
+        assert torch.equal(tokens.layer_norm(fw.unpack_dual(d).primal), tokens.layer_norm(x))
