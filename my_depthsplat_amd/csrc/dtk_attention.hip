@@ -150,6 +150,7 @@ int check(const dtk_attention* c, const char* who) {
   DSPLAT_REQUIRE(c->D > 0 && c->D <= 128 && c->D % 8 == 0, "%s: the head size must be a multiple of 8 up to 128", who);
   DSPLAT_REQUIRE(c->block == 32 || c->block == 64 || c->block == 128, "%s: block must be 32, 64 or 128", who);
   DSPLAT_REQUIRE(type_ok(c->dtype), "%s: bad type", who);
+  DSPLAT_REQUIRE(fabsf(c->scale) < INFINITY, "%s: the scale must be a finite number", who);
   DSPLAT_REQUIRE(c->Hq / c->Hkv <= 1024, "%s: more than 1024 query heads per key head", who);
   for (const int64_t* s : {c->q_strides, c->k_strides, c->v_strides})
     DSPLAT_REQUIRE(s[1] >= 0 && s[1] < (1LL << 24), "%s: a token stride must be below 2^24 elements", who);

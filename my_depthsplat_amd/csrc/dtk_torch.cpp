@@ -529,12 +529,13 @@ Tensor block_sparse_attention(const Tensor& q_, const Tensor& k_, const Tensor& 
                     "index must be int32 [", B, ", ", Hkv, ", ", Tq, ", 1..1024], got ", index_.scalar_type(), " ", index_.sizes());
   check_lengths(q_lengths, "q_lengths", B);
   check_lengths(kv_lengths, "kv_lengths", B);
+  const double scale = scale_.has_value() ? *scale_ : 1.0 / std::sqrt((double)D);
+  TORCH_CHECK_VALUE(std::isfinite((float)scale), "scale must be a finite 32-bit number, got ", scale);
   no_tangent({&q_, &k_, &v_});
   same_device(q_, {{"k", &k_}, {"v", &v_}, {"index", &index_}, {"q_lengths", &q_lengths}, {"kv_lengths", &kv_lengths}});
   const Tensor q = dense_rows(q_), k = dense_rows(k_), v = dense_rows(v_), index = index_.contiguous();
   q_lengths = int32(q_lengths);
   kv_lengths = int32(kv_lengths);
-  const double scale = scale_.has_value() ? *scale_ : 1.0 / std::sqrt((double)D);
   if (wants_grad({&q, &k, &v})) return Attention::apply(q, k, v, index, block, maybe(q_lengths), maybe(kv_lengths), scale);
   return run_attention(q, k, v, index, block, q_lengths, kv_lengths, scale, false).first;
 }

@@ -1,6 +1,7 @@
 """View-token operators and their layer at the edges of what they allow."""
 from __future__ import annotations
 
+import ctypes
 import math
 
 import pytest
@@ -340,3 +341,15 @@ def test_forward_mode_derivatives_where_nothing_is_done(gpu):
         d = fw.make_dual(x, torch.ones_like(x))
         assert tokens.dropout(d, 0.0) is d
         assert torch.equal(tokens.layer_norm(fw.unpack_dual(d).primal), tokens.layer_norm(x))
+
+
+@pytest.mark.parametrize("scale", [math.nan, math.inf, -math.inf])
+def test_attention_scale_that_is_no_number_is_refused(scale):
+    if not _lib.LIB_PATH.exists():
+        pytest.skip("extension not built")
+    q, index = torch.zeros(1, 5, 1, 8), torch.zeros(1, 1, 1, 1, dtype=torch.int32)
+    with pytest.raises(ValueError, match="scale"):
+        tokens.block_sparse_attention(q, q, q, index, scale=scale)
+    a = _lib.Attention(Lq=9, Lk=9, B=1, Hq=2, Hkv=1, D=8, block=64, top=2, dtype=0, scale=scale)
+    assert _lib.load().dtk_block_sparse_attention_fwd(ctypes.byref(a), None, None) == 1
+    assert b"scale" in _lib.load().dsplat_last_error()
