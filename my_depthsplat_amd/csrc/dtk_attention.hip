@@ -143,7 +143,8 @@ F* by_type(int dtype, F* f32, F* b16, F* h16) {
   return dtype == DTK_F32 ? f32 : dtype == DTK_BF16 ? b16 : h16;
 }
 
-int check(const dtk_attention* c, const char* who) {
+// What the sizes by themselves have to keep to (the workspace sizes of others are 0).
+int check_sizes(const dtk_attention* c, const char* who) {
   DSPLAT_REQUIRE(c, "%s: null pointer", who);
   DSPLAT_REQUIRE(c->B >= 0 && c->Lq >= 0 && c->Lk >= 0 && c->Hkv > 0 && c->Hq > 0 && c->Hq % c->Hkv == 0 && c->top > 0 && c->top <= 1024,
                  "%s: bad sizes", who);
@@ -152,9 +153,13 @@ int check(const dtk_attention* c, const char* who) {
   DSPLAT_REQUIRE(type_ok(c->dtype), "%s: bad type", who);
   DSPLAT_REQUIRE(fabsf(c->scale) < INFINITY, "%s: the scale must be a finite number", who);
   DSPLAT_REQUIRE(c->Hq / c->Hkv <= 1024, "%s: more than 1024 query heads per key head", who);
+  DSPLAT_REQUIRE(c->Lq <= (1LL << 31) - 256 && c->Lk <= (1LL << 31) - 256 && c->Hq < 65536 && c->B < 65536, "%s: too large", who);
+  return 0;
+}
+int check(const dtk_attention* c, const char* who) {
+  if (int e = check_sizes(c, who)) return e;
   for (const int64_t* s : {c->q_strides, c->k_strides, c->v_strides})
     DSPLAT_REQUIRE(s[1] >= 0 && s[1] < (1LL << 24), "%s: a token stride must be below 2^24 elements", who);
-  DSPLAT_REQUIRE(c->Lq <= (1LL << 31) - 256 && c->Lk <= (1LL << 31) - 256 && c->Hq < 65536 && c->B < 65536, "%s: too large", who);
   DSPLAT_REQUIRE(c->B == 0 || c->Lq == 0 || (c->q && c->o && c->index && (c->Lk == 0 || (c->k && c->v))), "%s: null pointer", who);
   return 0;
 }
@@ -226,7 +231,7 @@ BwdLayout layout_of(const dtk_attention* c, const Args& a) {
 extern "C" {
 
 size_t dtk_block_sparse_attention_fwd_workspace_size(const dtk_attention* c) {
-  if (!c || c->B <= 0 || c->Lq <= 0 || c->Hq <= 0 || c->Hkv <= 0 || c->block <= 0) return 0;
+  if (check_sizes(c, "dtk_block_sparse_attention_fwd_workspace_size") || c->B == 0 || c->Lq == 0) return 0;
   const Args a = args_of(c);
   if (a.splits == 1) return 0;
   return (size_t)a.splits * c->B * c->Hq * c->Lq * (c->D + 2) * sizeof(float);
@@ -255,7 +260,7 @@ int dtk_block_sparse_attention_fwd(const dtk_attention* c, void* workspace, void
 }
 
 size_t dtk_block_sparse_attention_bwd_workspace_size(const dtk_attention* c) {
-  if (!c || c->B <= 0 || c->Lq < 0 || c->Lk < 0 || c->Hq <= 0 || c->Hkv <= 0 || c->block <= 0) return 0;
+  if (check_sizes(c, "dtk_block_sparse_attention_bwd_workspace_size") || c->B == 0) return 0;
   const Args a = args_of(c);
   return layout_of(c, a).end;
 }

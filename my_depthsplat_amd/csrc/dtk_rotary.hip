@@ -148,7 +148,7 @@ extern "C" int dtk_rotary(int64_t B, int64_t L, int Hq, int Hk, int D, int F, in
                           const double* freqs, float factor, void* q_out, void* k_out, void* stream) {
   DSPLAT_REQUIRE(B >= 0 && L >= 0 && (L == 0 || B < (1LL << 31) / L) && Hq >= 0 && Hk >= 0 && D > 0 && Hq < 65536 && Hk < 65536 && D < (1 << 20),
                  "dtk_rotary: bad sizes");
-  DSPLAT_REQUIRE(F >= 0 && 2 * F <= D && axes > 0 && F % axes == 0, "dtk_rotary: bad number of frequencies");
+  DSPLAT_REQUIRE(F >= 0 && F <= D / 2 && axes > 0 && F % axes == 0, "dtk_rotary: bad number of frequencies");
   DSPLAT_REQUIRE(type_ok(dtype) && (ptype == DTK_I64 || ptype == DTK_I32 || ptype == DTK_F32), "dtk_rotary: bad types");
   if (B == 0 || L == 0 || Hq + Hk == 0) return 0;
   DSPLAT_REQUIRE((!Hq || (q && q_strides && q_out)) && (!Hk || (k && k_strides && k_out)) &&

@@ -359,6 +359,7 @@ __global__ __launch_bounds__(NT) void k_choose_long(ChooseArgs a) {
 // 49; 504 blocks, eight to a lane, 53 and 24.
 inline bool scored_by_choice(int64_t rows, int Tk, int pitch) { return Tk <= 64 * 4 && rows * Tk * pitch <= 1 << 26; }
 inline int64_t tiles_of(int64_t L, int block) { return (L + block - 1) / block; }
+inline bool block_ok(int block) { return block == 32 || block == 64 || block == 128; }
 
 template <typename T>
 void pool(const PoolArgs& a, dim3 grid, hipStream_t st) {
@@ -371,7 +372,7 @@ void pool(const PoolArgs& a, dim3 grid, hipStream_t st) {
 extern "C" {
 
 size_t dtk_select_blocks_workspace_size(int B, int64_t Lq, int64_t Lk, int Hkv, int D, int block) {
-  if (B <= 0 || Lq <= 0 || Lk <= 0 || Hkv <= 0 || D <= 0 || block <= 0) return 0;
+  if (B <= 0 || Lq <= 0 || Lk <= 0 || Hkv <= 0 || D <= 0 || D > 256 || !block_ok(block) || Lq >= (1LL << 31) || Lk >= (1LL << 31)) return 0;
   const size_t tq = tiles_of(Lq, block), tk = tiles_of(Lk, block);
   return (size_t)B * Hkv * ((padded(tq) + padded(tk)) * pitch_of(D) + tq * tk) * sizeof(double);
 }
@@ -382,7 +383,7 @@ int dtk_select_blocks(int B, int64_t Lq, int64_t Lk, int Hq, int Hkv, int D, int
                       void* workspace, void* stream) {
   DSPLAT_REQUIRE(B >= 0 && Lq >= 0 && Lk >= 0 && Hkv > 0 && Hq > 0 && Hq % Hkv == 0 && D > 0 && D <= 256 && top > 0,
                  "dtk_select_blocks: bad sizes");
-  DSPLAT_REQUIRE(block == 32 || block == 64 || block == 128, "dtk_select_blocks: block must be 32, 64 or 128");
+  DSPLAT_REQUIRE(block_ok(block), "dtk_select_blocks: block must be 32, 64 or 128");
   DSPLAT_REQUIRE(type_ok(dtype), "dtk_select_blocks: bad type");
   DSPLAT_REQUIRE(Lq < (1LL << 31) && Lk < (1LL << 31) && (int64_t)B * Hkv < 65536 && Hq < 65536, "dtk_select_blocks: too large");
   if (B == 0 || Lq == 0) return 0;

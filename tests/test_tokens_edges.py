@@ -353,3 +353,25 @@ def test_attention_scale_that_is_no_number_is_refused(scale):
     a = _lib.Attention(Lq=9, Lk=9, B=1, Hq=2, Hkv=1, D=8, block=64, top=2, dtype=0, scale=scale)
     assert _lib.load().dtk_block_sparse_attention_fwd(ctypes.byref(a), None, None) == 1
     assert b"scale" in _lib.load().dsplat_last_error()
+
+
+def test_abi_sizes_that_do_not_fit_end_no_process():
+    """Workspace sizes of arguments that the call itself refuses are 0 (no division by 0); 2 F past 32 bits is refused."""
+    if not _lib.LIB_PATH.exists():
+        pytest.skip("extension not built")
+    lib = _lib.load()
+    at = lambda **kw: _lib.Attention(**{**dict(Lq=900, Lk=900, B=1, Hq=2, Hkv=1, D=8, block=64, top=2, dtype=0, scale=1.0), **kw})  # noqa: E731
+    sizes = (lib.dtk_block_sparse_attention_fwd_workspace_size, lib.dtk_block_sparse_attention_bwd_workspace_size)
+    assert sizes[1](ctypes.byref(at())) > 0
+    for kw in (dict(Hq=1, Hkv=2), dict(Hq=3, Hkv=2), dict(block=256), dict(block=48), dict(block=1 << 30), dict(D=0), dict(D=4096),
+               dict(top=0), dict(top=-5), dict(top=2000), dict(Hq=2000), dict(Lq=1 << 40), dict(Lk=1 << 40), dict(B=1 << 20),
+               dict(B=-1), dict(dtype=7)):
+        for size in sizes:
+            assert size(ctypes.byref(at(**kw))) == 0, kw
+    assert all(size(None) == 0 for size in sizes)
+    buf, s3 = ctypes.create_string_buffer(4096), (ctypes.c_int64 * 3)(1, 1, 1)
+    for F in (1 << 30, (1 << 30) + 4, 0x7FFFFFFF):
+        rc = lib.dtk_rotary(1, 2, 1, 0, 8, F, 1, 0, 0, 0, 4, buf, s3, None, None, buf, s3, buf, 1.0, buf, None, None)
+        assert rc == 1 and b"bad number" in lib.dsplat_last_error(), F
+    assert lib.dtk_select_blocks_workspace_size(1, 1 << 40, 9, 1, 8, 64) == 0
+    assert lib.dtk_select_blocks_workspace_size(1, 9, 9, 1, 8, 48) == 0
