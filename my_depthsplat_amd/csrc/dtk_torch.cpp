@@ -417,7 +417,11 @@ void check_lengths(const Tensor& t, const char* name, int64_t B) {
   TORCH_CHECK_VALUE(!t.defined() || (t.dim() == 1 && t.size(0) == B && (t.scalar_type() == at::kInt || t.scalar_type() == at::kLong)),
                     name, " must be int32 or int64 [B=", B, "]");
 }
-Tensor int32(const Tensor& t) { return t.defined() ? t.to(at::kInt).contiguous() : t; }
+// Lengths as the kernels take them: 64 bits are cut to what 32 hold (all of a sequence, or nothing), not to their lower half.
+Tensor int32(const Tensor& t) {
+  if (!t.defined()) return t;
+  return (t.scalar_type() == at::kLong ? t.clamp(0, INT32_MAX).to(at::kInt) : t).contiguous();
+}
 int64_t tiles_of(int64_t n, int64_t block) { return (n + block - 1) / block; }
 
 Tensor select_blocks(const Tensor& q_, const Tensor& k_, int64_t top, int64_t block, const MaybeTensor& q_lengths_,

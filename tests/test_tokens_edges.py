@@ -375,3 +375,16 @@ def test_abi_sizes_that_do_not_fit_end_no_process():
         assert rc == 1 and b"bad number" in lib.dsplat_last_error(), F
     assert lib.dtk_select_blocks_workspace_size(1, 1 << 40, 9, 1, 8, 64) == 0
     assert lib.dtk_select_blocks_workspace_size(1, 9, 9, 1, 8, 48) == 0
+
+
+@gpu_only
+@pytest.mark.parametrize("long,short", [(2 ** 32, 300), (2 ** 40 + 7, 300), (2 ** 31, 300), (-2 ** 32 + 50, 0), (-2 ** 31 - 1, 0)])
+def test_64_bit_lengths_past_32_bits(gpu, long, short):
+    """Lengths are counted as they are: one behind the sequence's end means all of it, a negative one nothing."""
+    q, k = torch.randn(1, 300, 1, 16, device=gpu), torch.randn(1, 300, 1, 16, device=gpu)
+    far, near = (dict(q_lengths=torch.tensor([n], device=gpu), kv_lengths=torch.tensor([n], device=gpu)) for n in (long, short))
+    index = tokens.select_blocks(q, k, 3, block=32, **near)
+    assert torch.equal(tokens.select_blocks(q, k, 3, block=32, **far), index)
+    index = tokens.select_blocks(q, k, 3, block=32)
+    assert torch.equal(tokens.block_sparse_attention(q, k, k, index, block=32, **far),
+                       tokens.block_sparse_attention(q, k, k, index, block=32, **near))
