@@ -65,7 +65,8 @@ __global__ __launch_bounds__(NT) void k_pool(PoolArgs a) {
   const int n = (int)max((int64_t)0, min((int64_t)a.block, length_of(x.lengths, b, a.L[which]) - lo));
   const T* rows = (const T*)x.p + (int64_t)b * x.b + (int64_t)hk * group * x.h + lo * x.l;
   double* out = a.out[which] + ((int64_t)b * gridDim.y + hk) * padded(tiles) * a.pitch;
-  const double inv = n ? 1.0 / (double)(n * group) : 0.0;
+  // (a division: a mean by the rounded reciprocal of 75 rows may be above their common value, and equal blocks no tie)
+  const double count = n ? (double)n * group : 1.0;
   for (int first = 0; first < a.pitch; first += 64 * N) {  // (once where rows are vectors: D <= 256)
     const int pieces = max(1, min(64, a.D / N - first / N)), parts = 64 / pieces;
     const int c = lane % pieces, part = lane / pieces;
@@ -95,7 +96,7 @@ __global__ __launch_bounds__(NT) void k_pool(PoolArgs a) {
       double v = 0.0;
       if (d < a.D)
         for (int k = 0; k < parts; ++k) v += red[(d - first) % N * 64 + k * pieces + (d - first) / N];
-      out[packed(t, d, a.pitch)] = v * inv;
+      out[packed(t, d, a.pitch)] = v / count;
     }
   }
 }

@@ -388,3 +388,21 @@ def test_64_bit_lengths_past_32_bits(gpu, long, short):
     index = tokens.select_blocks(q, k, 3, block=32)
     assert torch.equal(tokens.block_sparse_attention(q, k, k, index, block=32, **far),
                        tokens.block_sparse_attention(q, k, k, index, block=32, **near))
+
+
+# ---- the choice of blocks -------------------------------------------------------------------
+
+
+@gpu_only
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("blocks", [3, 200, 700, 2100])
+@pytest.mark.parametrize("block,rows,value", [(128, 75, 1.75), (128, 91, 1.5), (64, 49, -1.0), (32, 13, 1.375), (128, 127, -1.25)])
+def test_a_shorter_last_block_ties_with_the_others(gpu, t, blocks, block, rows, value):
+    """Rows all equal: every block's mean is that value (a mean by a rounded reciprocal is not), so the lowest are chosen, of
+    either sign."""
+    k = torch.zeros(1, (blocks - 1) * block + rows, 1, 8, device=gpu, dtype=t)
+    k[..., 0] = value
+    q = torch.zeros(1, block + rows, 1, 8, device=gpu, dtype=t)
+    q[..., 0] = 1.0
+    for sign in (1, -1):
+        assert tokens.select_blocks(q * sign, k, 2, block=block).flatten().tolist() == [0, 1] * 2
