@@ -297,13 +297,12 @@ __global__ __launch_bounds__(kThreads, waves_of(NI, ADD)) void k_norm_bwd(BwdArg
     if (row < a.rows) fetch(next, row);
     float xh[NI][N], g[NI][N];
     float s1 = 0.f, s2 = 0.f;
-    const float shift = -cur.mu * cur.r;
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
       const C c(lane + i * LPR, width);
 #pragma unroll
       for (int e = 0; e < N; ++e) {
-        xh[i][e] = __builtin_fmaf((float)cur.z[i].v[e], cur.r, shift);
+        xh[i][e] = ((float)cur.z[i].v[e] - cur.mu) * cur.r;  // (the forward's: z r - mu r loses a large mean's digits)
         const float d = (float)cur.dy[i].v[e];
         dw[i][e] = __builtin_fmaf(d, xh[i][e], dw[i][e]);
         db[i][e] += d;

@@ -406,3 +406,27 @@ def test_a_shorter_last_block_ties_with_the_others(gpu, t, blocks, block, rows, 
     q[..., 0] = 1.0
     for sign in (1, -1):
         assert tokens.select_blocks(q * sign, k, 2, block=block).flatten().tolist() == [0, 1] * 2
+
+
+# ---- layer norm -----------------------------------------------------------------------------
+
+
+@gpu_only
+@pytest.mark.parametrize("add", [False, True])
+@pytest.mark.parametrize("width", [8, 64, 512, 2048, 8192])
+def test_layer_norm_gradients_beside_a_large_mean(gpu, add, width):
+    """Rows of 1234568 and 1234560 in turn: every sum that the mean takes is exact in 32 bits (4 times whole numbers below 2^24, or
+    such times a power of two), so the backward has no more to lose than its own roundings of numbers near 1 (64 of them in a
+    chain at most; the weights' over 9 rows). (The mean times 1 / deviation, about 308641, rounded and subtracted: 2^-6.)"""
+    g = torch.Generator().manual_seed(width)
+    x = torch.tensor([1234568.0, 1234560.0]).repeat(9, width // 2)
+    w, dy = torch.randn(width, generator=g), torch.randn(9, width, generator=g)
+    leaves = [v.to(gpu).requires_grad_(True) for v in (x, w)]
+    y = (tokens.dropout_add_layer_norm(leaves[0], torch.zeros_like(leaves[0]), leaves[1])[1] if add
+         else tokens.layer_norm(leaves[0], leaves[1]))
+    got = torch.autograd.grad(y, leaves, dy.to(gpu))
+    _, xh, r, _ = orc.layer_norm(x.double(), w.double(), None, 1e-5)
+    dz, dw, _ = orc.layer_norm_grads(xh, r, dy.double(), w.double())
+    a = (dy * w).double().abs()
+    orc.assert_within(got[0], dz, 64 * orc.E32 * (a + 2 * a.mean(-1, keepdim=True)), "dx")
+    orc.assert_within(got[1], dw, 64 * orc.E32 * dy.double().abs().sum(0), "dw")
