@@ -625,7 +625,7 @@ int dtk_select_blocks(int B, int64_t Lq, int64_t Lk, int Hq, int Hkv, int D, int
  * no key and behind q_lengths. lse [B,Hq,Lq] (base 2; NULL when no backward follows). Few tiles: the lists are
  * split over workgroups and joined through the workspace. At most 1024 query heads per key head; token
  * strides below 2^24 elements; Lq, Lk at most 2^31 - 256; B and Hq below 2^16; a finite scale. Backward: dout with its strides; dq,
- * dk, dv contiguous, overwritten (0 behind the lengths), each sum in one order. */
+ * dk, dv contiguous, overwritten (0 behind the lengths), each sum in one order; dk and dv may both be NULL (not taken). */
 typedef struct dtk_attention {
     int64_t Lq, Lk;
     int32_t B, Hq, Hkv, D, block, top, dtype;

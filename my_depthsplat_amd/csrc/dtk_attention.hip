@@ -269,7 +269,7 @@ int dtk_block_sparse_attention_bwd(const dtk_attention* c, const void* dout, con
                                    void* dk, void* dv, void* workspace, void* stream) {
   if (int e = check(c, "dtk_block_sparse_attention_bwd")) return e;
   if (c->B == 0) return 0;
-  DSPLAT_REQUIRE((c->Lq == 0 || (dout && dout_strides && dq && c->lse && workspace)) && (c->Lk == 0 || (dk && dv && workspace)),
+  DSPLAT_REQUIRE((c->Lq == 0 || (dout && dout_strides && dq && c->lse && workspace)) && !dk == !dv && (!dk || workspace),
                  "dtk_block_sparse_attention_bwd: null pointer");
   DSPLAT_REQUIRE(c->Lq == 0 || (dout_strides[1] >= 0 && dout_strides[1] < (1LL << 24)),
                  "dtk_block_sparse_attention_bwd: a token stride must be below 2^24 elements");
@@ -298,7 +298,7 @@ int dtk_block_sparse_attention_bwd(const dtk_attention* c, const void* dout, con
     const dim3 grid(a.Tq * a.rowtiles, a.Hkv, c->B);
     if (int e = by_type(c->dtype, attend_dq<float>, attend_dq<bf16>, attend_dq<f16>)(a, row_waves(a), grid, st)) return e;
   }
-  if (!a.Tk) return 0;
+  if (!a.Tk || !dk) return 0;
   if (l.most) {
     k_attend_plan<<<1, kPlanThreads, 0, st>>>(a, (int)l.items, l.most);
     if (int e = dsplat::check_launch("k_attend_plan")) return e;

@@ -356,7 +356,8 @@ struct Rotary : torch::autograd::Function<Rotary> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     variable_list none(6);
-    const Tensor dq = grads[0], dk = grads.size() > 1 ? grads[1] : Tensor();
+    Needs need{ctx};
+    const Tensor dq = need(true) ? grads[0] : Tensor(), dk = need(grads.size() > 1) ? grads[1] : Tensor();
     if (!dq.defined() && !dk.defined()) return none;
     const auto v = ctx->get_saved_variables();
     std::tie(none[0], none[1]) = run_rotary(dq.defined() ? dense_rows(dq) : dq, dk.defined() ? dense_rows(dk) : dk, v[0], v[1],
@@ -505,16 +506,19 @@ struct Attention : torch::autograd::Function<Attention> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const auto s = ctx->get_saved_variables();
     const Tensor g = dense_rows(grads[0]);
-    Tensor dq = empty_as(s[0]), dk = empty_as(s[1]), dv = empty_as(s[2]);
+    Needs need{ctx};
+    const bool nq = need(true), nk = need(true), nv = need(true), keys = nk || nv;
+    // (dq's kernel finds the lists that dk's reads; dk and dv are one kernel's)
+    Tensor dq = empty_as(s[0]), dk = keys ? empty_as(s[1]) : Tensor(), dv = keys ? empty_as(s[2]) : Tensor();
     const dtk_attention a = attention_of(s[0], s[1], s[2], s[3], ctx->saved_data["block"].toInt(), s[4], s[5],
                                          ctx->saved_data["scale"].toDouble(), s[6], s[7]);
     const Tensor ws = bytes(g, api.attention_bwd_workspace_size(&a));
     const Strides sg(g);
     launch("dtk_block_sparse_attention_bwd", g, api.attention_bwd, &a, ptr(g), sg.s, out(dq), out(dk), out(dv), out(ws));
     variable_list none(8);
-    none[0] = dq;
-    none[1] = dk;
-    none[2] = dv;
+    if (nq) none[0] = dq;
+    if (nk) none[1] = dk;
+    if (nv) none[2] = dv;
     return once(std::move(none));
   }
 };

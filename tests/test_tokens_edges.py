@@ -430,3 +430,37 @@ def test_layer_norm_gradients_beside_a_large_mean(gpu, add, width):
     a = (dy * w).double().abs()
     orc.assert_within(got[0], dz, 64 * orc.E32 * (a + 2 * a.mean(-1, keepdim=True)), "dx")
     orc.assert_within(got[1], dw, 64 * orc.E32 * dy.double().abs().sum(0), "dw")
+
+
+@gpu_only
+@pytest.mark.parametrize("t", TYPES)
+def test_attention_gradients_that_nobody_asks_for_are_not_taken(gpu, t):
+    """Each subset's gradients are those of all three, to the bit; with frozen keys and values no memory is taken for theirs."""
+    q, do = (torch.randn(1, 64, 2, 64, device=gpu).to(t) for _ in range(2))
+    k, v = (torch.randn(1, 1 << 16, 1, 64, device=gpu).to(t) for _ in range(2))
+    index = torch.tensor([[[[3, 700, 1023, 5]]]], dtype=torch.int32, device=gpu)
+
+    def grads(asked):
+        leaves = [x.detach().requires_grad_(n in asked) for n, x in zip("qkv", (q, k, v))]
+        o = tokens.block_sparse_attention(*leaves, index)
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats()
+        held = torch.cuda.memory_allocated()
+        o.backward(do)
+        torch.cuda.synchronize()
+        return [x.grad for x in leaves], torch.cuda.max_memory_allocated() - held
+
+    want, _ = grads("qkv")
+    for asked in ("q", "k", "v", "qk", "qv", "kv"):
+        got, more = grads(asked)
+        assert all((a is None) == (n not in asked) and (a is None or torch.equal(a, b)) for n, a, b in zip("qkv", got, want)), asked
+        if asked == "q":
+            assert more < k.numel() * k.element_size(), more
+    qr, kr = (torch.randn(1, 5, 2, 16, device=gpu) for _ in range(2))
+    pos, freqs = torch.arange(5, device=gpu), tokens.rotary_frequencies(16, device=gpu)
+    both = [x.clone().requires_grad_(True) for x in (qr, kr)]
+    want = torch.autograd.grad(sum(x.sum() for x in tokens.rotary(*both, pos, freqs)), both)
+    for i in range(2):
+        one = [x.clone().requires_grad_(j == i) for j, x in enumerate((qr, kr))]
+        (got,) = torch.autograd.grad(sum(x.sum() for x in tokens.rotary(*one, pos, freqs)), one[i])
+        assert torch.equal(got, want[i])
