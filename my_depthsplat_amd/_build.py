@@ -32,10 +32,11 @@ CFLAGS = [
 # (hipcc's host pass warns that it does not know the feature).
 CFLAGS += ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
-# Per-file extra flags. The rasterizer's per-lane pixel math is scalar by design (its packed
-# FP32 is written out with explicit vector types); the SLP vectorizer re-packs the scalar
-# parts with register shuffles that cost more than they save (k_render_bwd 119 -> 109 us
-# without it at config B).
+# Per-file extra flags. The rasterizer's per-lane pixel math is scalar by design (pairs of list
+# entries are written out with explicit vector types, which this build lowers to scalar FMAs);
+# the SLP vectorizer packs the scalar parts with register shuffles (k_render_bwd 119 -> 109 us
+# without it at config B while packed FP32 was on; without that 90.6 K views/s against 90.3 K
+# with the vectorizer, 16 scenes of 2 views at 256 x 256).
 FILE_FLAGS = {"dsr_raster.hip": ["-fno-slp-vectorize"],
               # nothing there has to match another kernel bit for bit (the fused norm matches the plain one)
               **{f: ["-ffp-contract=fast"] for f in ("dtk_rotary.hip", "dtk_attention.hip", "dtk_attention_f32.hip",

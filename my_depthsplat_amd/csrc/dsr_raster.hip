@@ -2496,14 +2496,15 @@ __device__ __forceinline__ bool conic_pd(float A, float B, float C) { return A <
 __device__ __forceinline__ float fall_p2(const PixUV& p, float F, float D, float E, float A, float B, float C) {
   return fmaf(A, p.uu, fmaf(C, p.vv, fmaf(B, p.uv, fmaf(D, p.u, fmaf(E, p.v, F)))));
 }
-// Two consecutive list entries with their fields interleaved, so the falloff of both runs
-// as packed FP32 (v_pk_fma/mul) with no operand shuffling; per-element results are the same
+// Two consecutive list entries with their fields interleaved, so the falloff of both runs as
+// two independent chains of FMAs on whole 16-byte reads, with no operand shuffling (one
+// instruction per element: the build has no packed FP32); per-element results are the same
 // IEEE operations as fall_p2 (the backward's decisions agree).
 struct __align__(16) PairRec {
-  f2v F, D, E, A, C, B;  // falloff fields of entries 0 and 1, interleaved (packed math); F holds
+  f2v F, D, E, A, C, B;  // falloff fields of entries 0 and 1, interleaved; F holds
                          // F + lo, lo = log2(opacity) (pair_put)
   f2v b;
-  f2v rg[2];             // (r, g) of entry j: one packed FMA into the pixel's (R, G)
+  f2v rg[2];             // (r, g) of entry j: one two-element FMA into the pixel's (R, G)
   f2v o;                 // lo (the power test of an indefinite conic only): last, so the common
                          // loop reads the fields before it as whole 16-byte vectors
 };
@@ -2514,7 +2515,7 @@ struct __align__(16) WaveList {
   PairRec rec[(CH + 8) / 2];
   uint32_t pos[CH + 8];
 };
-// the pixel terms stay scalars; the packed FMAs broadcast them (op_sel), no duplicated registers
+// the pixel terms stay scalars: both elements' FMAs read the same registers
 typedef PixUV PixUV2;
 __device__ __forceinline__ PixUV2 pix_uv2(const PixUV& p) { return p; }
 __device__ __forceinline__ f2v fall_p2x2(const PixUV2& p, const PairRec& P) {
@@ -2644,7 +2645,7 @@ __device__ bool tail_reaches_live(const float* __restrict__ gv, const uint64_t* 
 
 // One chunk of the walk: keep the entries of [base, base + CH) (this lane's record q, r, b)
 // whose alpha >= 1/255 region reaches the live pixels' box in the wave's LDS list (ballot
-// compaction, list order kept, entry pairs field-interleaved for packed math, 8 zero-opacity
+// compaction, list order kept, entry pairs field-interleaved, 8 zero-opacity
 // pad entries after the end), then composite that list four entries per step with the next
 // four read ahead.
 template <bool LAST>

@@ -14,9 +14,9 @@
 // element's number.
 //
 // Measured (a copy of 256 MB runs at 5.4 TB/s): 42240 x 768 bf16 forward 26 us (5.0 TB/s), backward 35 us (5.6 TB/s) and
-// 5.5 us for the fold of the weights' gradients; fused with dropout, 20001 x 1001 f16: forward 38 us (4.2 TB/s),
-// backward 56 us (3.6 TB/s) + 5: rows of no whole number of vectors, and the generator (a third of its time); 512 x 128 f32
-// forward 2.4 us, a launch.
+// 5.5 us for the fold of the weights' gradients; fused with dropout, 20001 x 1001 f16: forward 37.5 us (4.3 TB/s;
+// without the generator 32.6), backward 56.5 us (3.5 TB/s) + 5: rows of no whole number of vectors, which take three groups
+// of the generator per vector instead of two; 512 x 128 f32 forward 2.4 us, a launch.
 
 #pragma once
 #include "dtk_common.h"

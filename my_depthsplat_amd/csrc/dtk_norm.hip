@@ -41,9 +41,9 @@ __device__ __forceinline__ void drop_vec(Vec<T>& v, const Vec<T>& r, const Drop&
     v.v[e] = rounded<T>(add ? f + (float)r.v[e] : f);
   }
 }
-// One vector per thread. The generator's 20 products per vector (f32: 10) come to about half the time that the
-// vector's bytes take. (129024 x 512 bf16, forward with a residual and backward together 118 us, 5.6 TB/s;
-// 2048 x 128 f32 2.6 us, a launch.)
+// One vector per thread. The generator takes two products a round, ten rounds per four elements: 40 per vector (f32: 20),
+// which fit beside the vector's bytes (129024 x 512 bf16 with a residual: 69 us, 5.7 TB/s, with the generator and without).
+// Forward with a residual and backward together 118 us, 5.6 TB/s; 2048 x 128 f32 2.6 us, a launch.
 template <typename T>
 __global__ __launch_bounds__(NT) void k_dropout(int64_t n, const T* __restrict__ x, const T* __restrict__ residual,
                                                 Drop drop, T* __restrict__ y) {
