@@ -9,6 +9,7 @@ import torch
 
 import token_oracle as orc
 from my_depthsplat_amd import _lib, tokens
+from test_tokens_gpu import check_attention
 
 gpu_only = pytest.mark.gpu
 F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
@@ -464,3 +465,55 @@ def test_attention_gradients_that_nobody_asks_for_are_not_taken(gpu, t):
         one = [x.clone().requires_grad_(j == i) for j, x in enumerate((qr, kr))]
         (got,) = torch.autograd.grad(sum(x.sum() for x in tokens.rotary(*one, pos, freqs)), one[i])
         assert torch.equal(got, want[i])
+
+
+# ---- the largest groups of heads and lists, a first call that is captured, a cache that sequences share ---------------
+
+
+@gpu_only
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("block,Lq,D", [(32, 3, 8), (64, 1, 128), (128, 33, 24)])
+def test_attention_of_1024_heads_to_one(gpu, t, block, Lq, D):
+    check_attention(gpu, t, 1, Lq, 2 * block - 5, 1024, 1, D, block, 3, seed=block)
+
+
+@gpu_only
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("Lq,D,Hq", [(1, 128, 1), (40, 128, 1), (64, 32, 2), (130, 128, 1)])
+def test_attention_of_lists_of_1024(gpu, t, Lq, D, Hq):
+    check_attention(gpu, t, 1, Lq, 1030 * 32 - 9, Hq, 1, D, 32, 1024, seed=Lq)
+
+
+@gpu_only
+@pytest.mark.parametrize("t", [F32, F16])
+def test_attention_captured_without_a_call_before(gpu, t):
+    """Kernels of more LDS than they get unasked, whose first launch is the captured one."""
+    q, k, v, do = (torch.randn(2, 300, h, 104, device=gpu).to(t).requires_grad_(i < 3) for i, h in enumerate((2, 1, 1, 2)))
+    index = torch.arange(3, device=gpu, dtype=torch.int32).expand(2, 1, 5, 3).contiguous()
+
+    def f():
+        return torch.autograd.grad(tokens.block_sparse_attention(q, k, v, index), (q, k, v), do)
+
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = f()
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [x.clone() for x in held]
+        assert all(torch.equal(a, b) for a, b in zip(got, f()))
+
+
+@gpu_only
+def test_attention_of_a_cache_that_the_batch_shares(gpu):
+    """Keys and values expanded over the batch (a stride of 0): the bits of their copies."""
+    q = torch.randn(3, 70, 4, 64, device=gpu, requires_grad=True)
+    cache = torch.randn(1, 200, 2, 64, device=gpu, requires_grad=True)
+    index = torch.arange(4, device=gpu, dtype=torch.int32).expand(3, 2, 2, 4).contiguous()
+    shared, copies = cache.expand(3, -1, -1, -1), cache.detach().repeat(3, 1, 1, 1).requires_grad_(True)
+    outs = [tokens.block_sparse_attention(q, c, c, index) for c in (shared, copies)]
+    assert torch.equal(*outs)
+    do = torch.randn_like(outs[0])
+    a = torch.autograd.grad(outs[0], (q, shared), do)
+    b = torch.autograd.grad(outs[1], (q, copies), do)
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
