@@ -110,7 +110,7 @@ class Attention(ctypes.Structure):
     _fields_ = ([("Lq", _L), ("Lk", _L)] + [(n, ctypes.c_int32) for n in ("B", "Hq", "Hkv", "D", "block", "top", "dtype")]
                 + [("scale", c_float)] + [(n, _P) for n in ("q", "k", "v")]
                 + [(n, _L * 3) for n in ("q_strides", "k_strides", "v_strides")]
-                + [(n, _P) for n in ("index", "q_lengths", "kv_lengths", "o", "lse")])
+                + [(n, _P) for n in ("index", "q_lengths", "kv_lengths", "o", "lse", "o_rest")])
 
 
 _lib = None

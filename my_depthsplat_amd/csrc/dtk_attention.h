@@ -12,13 +12,15 @@
 // permuted as long as both operands agree, so the accumulator's rows (8 (r / 4) + 4 half + r % 4)
 // serve as they are and nothing is shuffled.
 //
-// Probabilities and ds are rounded to the inputs' type for the second products (the matrix instructions' operands), as
-// the inputs themselves were; all sums, the maximum, lse and delta are held in 32 bits. f32 operands stay f32.
+// Probabilities, and ds for dk, are rounded to the inputs' type for the second products (the matrix instructions' operands),
+// as the inputs themselves were: a rounding of each term's own, so o, dv and dk of random rows are 0.0023 - 0.0024 of their
+// norm from 64 bits in bf16, where their own rounding alone makes 0.0017. dq takes ds in two pieces (k_attend_dq).
+// All sums, the maximum, lse and delta are held in 32 bits. f32 operands stay f32.
 //
 // Measured (products taken, rate; a large bf16 product reaches 1060 TFLOP/s, f32 153):
 //   4 scenes of 32256 bf16 tokens (lengths from half of that on), 4 heads of 64 channels on 2, 16 blocks of 64:
-//     forward 128 us 560 TFLOP/s, dq 170 us 630, dk/dv 231 us 620
-//   16 scenes of 2048 f32 tokens, one head of 128 channels, 8 blocks of 64: 90 us 92, 143 us 87, 208 us 80
+//     forward 125 us 570 TFLOP/s (137 us where a backward follows), dq 225 us 640 (four products), dk/dv 235 us 610
+//   16 scenes of 2048 f32 tokens, one head of 128 channels, 8 blocks of 64: 89 us 93, 142 us 87, 208 us 80
 //   12 views of 92160 bf16 tokens, 2 heads of 64, 16 blocks of 64, forward: 104 us 465
 // What bounds them: the forward and dq at 64 channels the vector unit (some 110 of its instructions per 32 x 32 scores, half of
 // its cycles, for 8 matrix instructions, a quarter of theirs; with 128 channels the forward comes to 730 TFLOP/s);
@@ -84,6 +86,7 @@ struct Args {
   const int32_t *index, *q_lengths, *kv_lengths;
   void *out, *dq, *dk, *dv;  // contiguous
   float *lse;                // [B, Hq, Lq], base 2; -inf for rows without a key
+  void *rest;                // what the rounding of o left (kRest times it), for delta; 16-bit types that train, else NULL
   float *part, *part_m, *part_l;
   float* delta;
   uint32_t *bits, *chosen;
@@ -114,6 +117,15 @@ __device__ __forceinline__ typename Mma<T>::Frag acc_frag(const f32x16& p, int s
   typename Mma<T>::Frag f;
 #pragma unroll
   for (int j = 0; j < 8; ++j) f[j] = (T)p[8 * s + j];
+  return f;
+}
+
+// What acc_frag left of it.
+template <typename T>
+__device__ __forceinline__ typename Mma<T>::Frag rest_frag(const f32x16& p, const typename Mma<T>::Frag& of, int s) {
+  typename Mma<T>::Frag f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) f[j] = (T)(p[8 * s + j] - (float)of[j]);
   return f;
 }
 
@@ -250,6 +262,14 @@ template <typename T>
 __device__ __forceinline__ void store4(T* p, float a, float b, float c, float d) {
   T v[4] = {(T)a, (T)b, (T)c, (T)d};
   __builtin_memcpy(p, v, sizeof(v));
+}
+
+// What the rounding of a, b, c, d left, itself rounded; f16's is taken times 2^11, out of its smallest numbers.
+template <typename T>
+constexpr float kRest = __is_same(T, f16) ? 2048.f : 1.f;
+template <typename T>
+__device__ __forceinline__ void store_rest4(T* p, float a, float b, float c, float d) {
+  store4<T>(p, (a - (float)(T)a) * kRest<T>, (b - (float)(T)b) * kRest<T>, (c - (float)(T)c) * kRest<T>, (d - (float)(T)d) * kRest<T>);
 }
 
 // Where a workgroup works: tile, row group, key head, scene, part of the list.
@@ -482,14 +502,19 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 2 ? (DP > 64 || RW == 1 ? 2
   }
   // a row behind the length is written as 0: its zeros beside an infinite key or value are no number
   const float inv = l > 0.f ? 1.f / l : (l != l ? l : 0.f);
-  T* op = (T*)a.out + (((int64_t)at.b * a.Lq + i) * a.Hq + h) * a.D;
+  const int64_t to = (((int64_t)at.b * a.Lq + i) * a.Hq + h) * a.D;
 #pragma unroll
   for (int d = 0; d < ND; ++d)
 #pragma unroll
-    for (int c = 0; c < 4; ++c)
-      if (32 * d + 8 * c + 4 * half < a.D)
-        store4<T>(op + 32 * d + 8 * c + 4 * half, valid ? o[d][4 * c] * inv : 0.f, valid ? o[d][4 * c + 1] * inv : 0.f,
-                  valid ? o[d][4 * c + 2] * inv : 0.f, valid ? o[d][4 * c + 3] * inv : 0.f);
+    for (int c = 0; c < 4; ++c) {
+      const int e = 32 * d + 8 * c + 4 * half;
+      if (e >= a.D) continue;
+      float v[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) v[k] = valid ? o[d][4 * c + k] * inv : 0.f;
+      store4<T>((T*)a.out + to + e, v[0], v[1], v[2], v[3]);
+      if (sizeof(T) == 2 && a.rest) store_rest4<T>((T*)a.rest + to + e, v[0], v[1], v[2], v[3]);
+    }
   if (half == 0 && a.lse) a.lse[((int64_t)at.b * a.Hq + h) * a.Lq + i] = valid ? base2 + log2f(l) : -INFINITY;
 }
 
@@ -499,8 +524,8 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 2 ? (DP > 64 || RW == 1 ? 2
 // scaled with it, in 32 bits, and all is undone at the end. So a column's terms keep f16's 11 bits down to 2^-26 of its largest,
 // whatever other rows, heads and scenes hold. (|ds| <= 2 D 65504^2 < 2^40: in 32 bits 2^60 times that is still a number.) p <= 1 is
 // taken times 2^12 for dv, for unlikely keys: by the exponent's base, at no cost.
-// 4 scenes of 32256 f16 tokens, 4 heads on 2 of 64, 16 blocks of 64: dq 349 us, dk/dv 470, where one power of two of the row (dq) and
-// of the whole call (dk), at the largest |do|, took 356 and 444 and lost the digits of a scene of 2^-13 of another's gradients.
+// 4 scenes of 32256 f16 tokens, 4 heads on 2 of 64, 16 blocks of 64: dk/dv 470 us, where one power of two of the whole call, at the
+// largest |do|, took 444 and lost the digits of a scene of 2^-13 of another's gradients.
 template <typename T>
 constexpr bool kFewExponents = __is_same(T, f16);
 constexpr int kFirstPower = 60, kLikely = 12;
@@ -534,6 +559,14 @@ __device__ __forceinline__ void shift(f32x16 (&sum)[ND], int power) {
 
 // dq: the forward's shape; p is taken from the saved lse. delta = sum_d do o of each row on the
 // way, kept for dk.
+//
+// A row's ds add up to 0, so what all keys have in common falls out of dq = sum ds k, and what all values have in
+// common out of ds = p (dp - delta). A rounding of ds leaves a share of the keys' common part in it, one of o (which delta
+// is made of) a share of both: with keys and values of a mean of 1 (3) times their spread, 1024 bf16 keys, dq was off by 0.037
+// (0.34) of its norm. So, in 16 bits: o comes in two pieces (o, and the rest that the forward saved), ds is taken in two pieces, and
+// c, the mean of some keys (the first block's first 32), is taken off all keys by subtracting (sum ds) c at the end,
+// two matrix instructions a piece. 0.0017 (0.0020) from 64 bits, where the rounding of dq makes 0.0017. (4 scenes of 32256 bf16
+// tokens: 171 us without, 206 with two pieces, 225 with c; the forward's rest 125 -> 137 us.)
 template <typename T, int DP, int RW>
 __global__ __launch_bounds__(kThreads, (sizeof(T) == 2 ? (DP > 64 || RW == 1 ? 2 : 3) : DP <= 64 ? 2 : 1)) void k_attend_dq(Args a) {
   using M = Mma<T>;
@@ -567,7 +600,7 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 2 ? (DP > 64 || RW == 1 ? 2
   const int64_t ir = valid ? i : 0;
   const T* qp = (const T*)a.q.p + at.b * a.q.b + ir * a.q.l + h * a.q.h;
   const T* gp = (const T*)a.g.p + at.b * a.g.b + ir * a.g.l + h * a.g.h;
-  const T* op = (const T*)a.o.p + at.b * a.o.b + ir * a.o.l + h * a.o.h;
+  const int64_t oat = at.b * a.o.b + ir * a.o.l + h * a.o.h;
   Frag qf[NS], gf[NS];
   float delta = 0.f;
 #pragma unroll
@@ -575,9 +608,10 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 2 ? (DP > 64 || RW == 1 ? 2
     qf[s] = row_frag<T>(qp, 16 * s + 8 * half, a.D, valid);
     if (a.scale < 0.f) qf[s] = -qf[s];
     gf[s] = row_frag<T>(gp, 16 * s + 8 * half, a.D, valid);
-    const Frag of = row_frag<T>(op, 16 * s + 8 * half, a.D, valid);
+    const Frag of = row_frag<T>((const T*)a.o.p + oat, 16 * s + 8 * half, a.D, valid);
+    const Frag rest = sizeof(T) == 2 ? row_frag<T>((const T*)a.rest + oat, 16 * s + 8 * half, a.D, valid) : Frag{};
 #pragma unroll
-    for (int j = 0; j < 8; ++j) delta += (float)gf[s][j] * (float)of[j];
+    for (int j = 0; j < 8; ++j) delta += (float)gf[s][j] * ((float)of[j] + (float)rest[j] * (1.f / kRest<T>));
   }
   delta += __shfl_xor(delta, 32, 64);
   const int64_t stat = ((int64_t)at.b * a.Hq + h) * a.Lq + ir;
@@ -605,8 +639,12 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 2 ? (DP > 64 || RW == 1 ? 2
     sk.load(pk, next.n, a.k.l, a.D);
     sv.load(pv, next.n, a.v.l, a.D);
   };
-  if (units) fetch(0);
-  for (int u = 0, step = 0; u < units; u += U, ++step) {
+  // From the list's end to its start: the last step then holds the first block's first unit, which has a key.
+  const int last = units ? (units - 1) / U * U : -1;
+  int step = 0;
+  float total = 0.f;  // 16 bits: of this lane's ds
+  if (units) fetch(last);
+  for (int u = last; u >= 0; u -= U, ++step) {
     char* tk = lds + (step % NB) * 2 * U * L::kUnit;
     char* tv = tk + U * L::kUnit;
     if (NB == 1) __syncthreads();
@@ -614,7 +652,7 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 2 ? (DP > 64 || RW == 1 ? 2
     sv.store(tv);
     __syncthreads();
     const Span<U> now = next;
-    if (u + U < units) fetch(u + U);
+    if (u > 0) fetch(u - U);
 #pragma unroll 1
     for (int e = 0; e < EACH; ++e) {
       const char *uk = tk + (e * KW + kw) * L::kUnit, *uv = tv + (e * KW + kw) * L::kUnit;
@@ -637,12 +675,43 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 2 ? (DP > 64 || RW == 1 ? 2
       }
       if constexpr (kFewExponents<T>)
         if (keep_in_range(x, dq, power)) times = __builtin_amdgcn_ldexpf(1.f, power);
-      const Frag s0 = acc_frag<T>(x, 0), s1 = acc_frag<T>(x, 1);
+      if constexpr (sizeof(T) == 2) {
+        float sum = 0.f;
 #pragma unroll
-      for (int d = 0; d < ND; ++d) {
-        dq[d] = M::mma(L::col(uk, 0, d, lane), s0, dq[d]);
-        dq[d] = M::mma(L::col(uk, 1, d, lane), s1, dq[d]);
+        for (int r = 0; r < 16; ++r) sum += x[r];
+        total += kFewExponents<T> ? __builtin_amdgcn_ldexpf(sum, -power) : sum;
       }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const Frag hi = acc_frag<T>(x, h), lo = sizeof(T) == 2 ? rest_frag<T>(x, hi, h) : Frag{};
+#pragma unroll
+        for (int d = 0; d < ND; ++d) {
+          const Frag k = L::col(uk, h, d, lane);
+          dq[d] = M::mma(k, hi, dq[d]);
+          if constexpr (sizeof(T) == 2) dq[d] = M::mma(k, lo, dq[d]);
+        }
+      }
+    }
+  }
+  if constexpr (sizeof(T) == 2) {
+    if (units) {  // dq -= total c, c the mean of the last step's first unit (rows that do not count are zeros there)
+      total += __shfl_xor(total, 32, 64);
+      float w = total * (-1.f / (float)next.n[0]);
+      f32x16 one = {};
+      if constexpr (kFewExponents<T>) w = __builtin_amdgcn_ldexpf(w, power);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) one[r] = w;
+      if constexpr (kFewExponents<T>) keep_in_range(one, dq, power);
+      const char* uk = lds + ((step - 1) % NB) * 2 * U * L::kUnit;
+      const Frag hi = acc_frag<T>(one, 0), lo = rest_frag<T>(one, hi, 0);
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int d = 0; d < ND; ++d) {
+          const Frag k = L::col(uk, h, d, lane);
+          dq[d] = M::mma(k, hi, dq[d]);
+          dq[d] = M::mma(k, lo, dq[d]);
+        }
     }
   }
   if constexpr (kFewExponents<T>) shift(dq, -power);

@@ -49,8 +49,11 @@ __global__ __launch_bounds__(NT) void k_attend_join(Args a, int64_t rows) {
   const int64_t i = r % a.Lq, bh = r / a.Lq, b = bh / a.Hq, h = bh % a.Hq;
   const bool valid = i < length_of(a.q_lengths, (int)b, a.Lq);
   const float inv = l > 0.f ? 1.f / l : (l != l ? l : 0.f);  // (as k_attend_fwd: 0 behind the length whatever the sums are)
-  store4<T>((T*)a.out + ((b * a.Lq + i) * a.Hq + h) * a.D + d, valid ? o[0] * inv : 0.f, valid ? o[1] * inv : 0.f,
-            valid ? o[2] * inv : 0.f, valid ? o[3] * inv : 0.f);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) o[e] = valid ? o[e] * inv : 0.f;
+  const int64_t to = ((b * a.Lq + i) * a.Hq + h) * a.D + d;
+  store4<T>((T*)a.out + to, o[0], o[1], o[2], o[3]);
+  if (sizeof(T) == 2 && a.rest) store_rest4<T>((T*)a.rest + to, o[0], o[1], o[2], o[3]);
   if (d == 0 && a.lse) a.lse[r] = valid ? m + log2f(l) : -INFINITY;
 }
 
@@ -189,6 +192,7 @@ Args args_of(const dtk_attention* c) {
   a.kv_lengths = c->kv_lengths;
   a.out = c->o;
   a.lse = c->lse;
+  a.rest = c->o_rest;
   const int per = 32 * row_waves(a);
   a.rowtiles = (a.Lt * a.G + per - 1) / per;
   a.splits = splits_of((int64_t)a.Tq * a.rowtiles * a.Hkv * c->B, a.top * (a.block / 32));
@@ -269,7 +273,7 @@ int dtk_block_sparse_attention_bwd(const dtk_attention* c, const void* dout, con
                                    void* dk, void* dv, void* workspace, void* stream) {
   if (int e = check(c, "dtk_block_sparse_attention_bwd")) return e;
   if (c->B == 0) return 0;
-  DSPLAT_REQUIRE((c->Lq == 0 || (dout && dout_strides && dq && c->lse && workspace)) && !dk == !dv && (!dk || workspace),
+  DSPLAT_REQUIRE((c->Lq == 0 || (dout && dout_strides && dq && c->lse && workspace && (c->dtype == DTK_F32 || c->o_rest))) && !dk == !dv && (!dk || workspace),
                  "dtk_block_sparse_attention_bwd: null pointer");
   DSPLAT_REQUIRE(c->Lq == 0 || (dout_strides[1] >= 0 && dout_strides[1] < (1LL << 24)),
                  "dtk_block_sparse_attention_bwd: a token stride must be below 2^24 elements");

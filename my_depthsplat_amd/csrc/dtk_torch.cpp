@@ -454,7 +454,7 @@ Tensor select_blocks(const Tensor& q_, const Tensor& k_, int64_t top, int64_t bl
 }
 
 dtk_attention attention_of(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& index, int64_t block, const Tensor& q_lengths,
-                           const Tensor& kv_lengths, double scale, const Tensor& o, const Tensor& lse) {
+                           const Tensor& kv_lengths, double scale, const Tensor& o, const Tensor& lse, const Tensor& rest) {
   dtk_attention a = {};
   a.Lq = q.size(1);
   a.Lk = k.size(1);
@@ -480,28 +480,36 @@ dtk_attention attention_of(const Tensor& q, const Tensor& k, const Tensor& v, co
   a.kv_lengths = (const int32_t*)ptr(kv_lengths);
   a.o = out(o);
   a.lse = (float*)out(lse);
+  a.o_rest = out(rest);
   return a;
 }
 
-std::pair<Tensor, Tensor> run_attention(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& index, int64_t block,
+struct Attended {
+  Tensor o, lse, rest;
+};
+Attended run_attention(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& index, int64_t block,
                                         const Tensor& q_lengths, const Tensor& kv_lengths, double scale, bool stats) {
-  Tensor o = empty_as(q), lse;
-  if (stats) lse = at::empty({q.size(0), q.size(2), q.size(1)}, q.options().dtype(at::kFloat));
-  const dtk_attention a = attention_of(q, k, v, index, block, q_lengths, kv_lengths, scale, o, lse);
+  Attended r;
+  r.o = empty_as(q);
+  if (stats) {
+    r.lse = at::empty({q.size(0), q.size(2), q.size(1)}, q.options().dtype(at::kFloat));
+    if (q.scalar_type() != at::kFloat) r.rest = empty_as(q);
+  }
+  const dtk_attention a = attention_of(q, k, v, index, block, q_lengths, kv_lengths, scale, r.o, r.lse, r.rest);
   const Tensor ws = bytes(q, api.attention_fwd_workspace_size(&a));
   launch("dtk_block_sparse_attention_fwd", q, api.attention_fwd, &a, out(ws));
-  return {o, lse};
+  return r;
 }
 
 struct Attention : torch::autograd::Function<Attention> {
   static Tensor forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& index, int64_t block,
                         const MaybeTensor& q_lengths_, const MaybeTensor& kv_lengths_, double scale) {
     const Tensor q_lengths = or_none(q_lengths_), kv_lengths = or_none(kv_lengths_);
-    auto [o, lse] = run_attention(q, k, v, index, block, q_lengths, kv_lengths, scale, true);
-    ctx->save_for_backward({q, k, v, index, q_lengths, kv_lengths, o, lse});
+    Attended r = run_attention(q, k, v, index, block, q_lengths, kv_lengths, scale, true);
+    ctx->save_for_backward({q, k, v, index, q_lengths, kv_lengths, r.o, r.lse, r.rest});
     ctx->saved_data["block"] = block;
     ctx->saved_data["scale"] = scale;
-    return o;
+    return r.o;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const auto s = ctx->get_saved_variables();
@@ -511,7 +519,7 @@ struct Attention : torch::autograd::Function<Attention> {
     // (dq's kernel finds the lists that dk's reads; dk and dv are one kernel's)
     Tensor dq = empty_as(s[0]), dk = keys ? empty_as(s[1]) : Tensor(), dv = keys ? empty_as(s[2]) : Tensor();
     const dtk_attention a = attention_of(s[0], s[1], s[2], s[3], ctx->saved_data["block"].toInt(), s[4], s[5],
-                                         ctx->saved_data["scale"].toDouble(), s[6], s[7]);
+                                         ctx->saved_data["scale"].toDouble(), s[6], s[7], s[8]);
     const Tensor ws = bytes(g, api.attention_bwd_workspace_size(&a));
     const Strides sg(g);
     launch("dtk_block_sparse_attention_bwd", g, api.attention_bwd, &a, ptr(g), sg.s, out(dq), out(dk), out(dv), out(ws));
@@ -545,7 +553,7 @@ Tensor block_sparse_attention(const Tensor& q_, const Tensor& k_, const Tensor& 
   q_lengths = int32(q_lengths);
   kv_lengths = int32(kv_lengths);
   if (wants_grad({&q, &k, &v})) return Attention::apply(q, k, v, index, block, maybe(q_lengths), maybe(kv_lengths), scale);
-  return run_attention(q, k, v, index, block, q_lengths, kv_lengths, scale, false).first;
+  return run_attention(q, k, v, index, block, q_lengths, kv_lengths, scale, false).o;
 }
 
 void bind(const std::map<std::string, uintptr_t>& fn) {

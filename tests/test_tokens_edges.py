@@ -517,3 +517,47 @@ def test_attention_of_a_cache_that_the_batch_shares(gpu):
     a = torch.autograd.grad(outs[0], (q, shared), do)
     b = torch.autograd.grad(outs[1], (q, copies), do)
     assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+# ---- 16 bits: values and keys with a mean ------------------------------------------------------------
+
+
+def query_gradient(q, k, v, do, scale, t):
+    """(dq, how far off before it is rounded) in 64 bits. dq's terms are p (dp - delta) (k - c), for any c, as a row's p (dp - delta) add up to 0; c is the mean of
+    the first 32 keys. dp and delta are sums of D 32-bit products, a score likewise, its exponent and logarithm off by 8 steps; ds is
+    two pieces of h each. delta is do . o of an o in two pieces, made of p rounded to h: n roundings of their own, so six
+    standard deviations of their sum (each at most h)."""
+    h, D, n = orc.half_step(t), q.shape[1], k.shape[0]
+    x, dp = q @ k.T * scale, do @ v.T
+    p = torch.softmax(x, -1)
+    o = p @ v
+    delta = (do * o).sum(-1, keepdim=True)
+    ds = p * (dp - delta)
+    e_x = (D * (q.abs() @ k.abs().T) * abs(scale) + 8 * (1 + x.abs())) * orc.E32
+    e_o = 6 * h * (p.square() @ v.square()).sqrt() + (p * (2 * e_x + n * orc.E32)) @ v.abs() + (2 * h * h + 2 * orc.E32) * o.abs()
+    e_delta = (do.abs() * e_o).sum(-1, keepdim=True) + D * orc.E32 * (do.abs() * o.abs()).sum(-1, keepdim=True)
+    e_ds = p * D * orc.E32 * (do.abs() @ v.abs().T) + ds.abs() * (2 * e_x + h * h + (n + 4) * orc.E32)
+    dq, off = ds @ k * scale, k - k[:32].mean(0)
+    return dq, (e_ds @ off.abs() + e_delta * (p @ off).abs()) * abs(scale)
+
+
+@gpu_only
+@pytest.mark.parametrize("t", [BF16, F16])
+@pytest.mark.parametrize("key_mean,value_mean", [(0.0, 0.0), (3.0, 0.0), (0.0, 3.0), (1.0, 1.0), (3.0, 3.0)])
+@pytest.mark.parametrize("L,Hq,block,n,D", [(256, 1, 64, 1024, 64), (40, 2, 32, 500, 32), (130, 1, 128, 900, 128), (16, 2, 64, 4000, 96)])
+def test_query_gradients_of_keys_and_values_with_a_mean(gpu, t, key_mean, value_mean, L, Hq, block, n, D):
+    """dq to its own rounding where every key and every value has a large part in common: none of it belongs in dq, and a rounding of
+    o or of ds times that part would be larger than dq."""
+    g = torch.Generator().manual_seed(n)
+    km, vm = torch.randn(D, generator=g) * key_mean, torch.randn(D, generator=g) * value_mean
+    q, k, v, do = ((torch.randn(1, m, h, D, generator=g) + a).to(t) for m, h, a in ((L, Hq, 0.0), (n, 1, km), (n, 1, vm), (L, Hq, 0.0)))
+    blocks = -(-n // block)
+    index = torch.arange(blocks, device=gpu, dtype=torch.int32).expand(1, 1, -(-L // block), blocks).contiguous()
+    leaves = [x.to(gpu).requires_grad_(True) for x in (q, k, v)]
+    (got,) = torch.autograd.grad(tokens.block_sparse_attention(*leaves, index, block=block), leaves[:1], do.to(gpu))
+    for head in range(Hq):
+        want, off = query_gradient(*(x[0, :, min(head, x.shape[2] - 1)].double() for x in (q, k, v, do)), D ** -0.5, t)
+        h, dq = orc.half_step(t), got[0, :, head]
+        orc.assert_within(dq, want, off + h * want.abs() + orc.tiny(t), "dq")
+        # (roundings are spread evenly over a step: together at most 0.58 of the half step, that of a value just above a power of two)
+        assert float((dq.double().cpu() - want).norm()) < 0.58 * h * float(want.norm()) + float(off.norm())
