@@ -20,7 +20,7 @@
 // Measured (products taken, rate; a large bf16 product reaches 1060 TFLOP/s, f32 153):
 //   4 scenes of 32256 bf16 tokens (lengths from half of that on), 4 heads of 64 channels on 2, 16 blocks of 64:
 //     forward 125 us 570 TFLOP/s (137 us where a backward follows), dq 225 us 640 (four products), dk/dv 235 us 610
-//   16 scenes of 2048 f32 tokens, one head of 128 channels, 8 blocks of 64: 89 us 93, 142 us 87, 208 us 80
+//   16 scenes of 2048 f32 tokens, one head of 128 channels, 8 blocks of 64: 89 us 93, 146 us 85, 208 us 80
 //   12 views of 92160 bf16 tokens, 2 heads of 64, 16 blocks of 64, forward: 104 us 465
 // What bounds them: the forward and dq at 64 channels the vector unit (some 110 of its instructions per 32 x 32 scores, half of
 // its cycles, for 8 matrix instructions, a quarter of theirs; with 128 channels the forward comes to 730 TFLOP/s);
@@ -563,10 +563,11 @@ __device__ __forceinline__ void shift(f32x16 (&sum)[ND], int power) {
 // A row's ds add up to 0, so what all keys have in common falls out of dq = sum ds k, and what all values have in
 // common out of ds = p (dp - delta). A rounding of ds leaves a share of the keys' common part in it, one of o (which delta
 // is made of) a share of both: with keys and values of a mean of 1 (3) times their spread, 1024 bf16 keys, dq was off by 0.037
-// (0.34) of its norm. So, in 16 bits: o comes in two pieces (o, and the rest that the forward saved), ds is taken in two pieces, and
-// c, the mean of some keys (the first block's first 32), is taken off all keys by subtracting (sum ds) c at the end,
-// two matrix instructions a piece. 0.0017 (0.0020) from 64 bits, where the rounding of dq makes 0.0017. (4 scenes of 32256 bf16
-// tokens: 171 us without, 206 with two pieces, 225 with c; the forward's rest 125 -> 137 us.)
+// (0.34) of its norm. So c, the mean of some keys (the first block's first 32), is taken off all keys by subtracting (sum ds) c at
+// the end, a few matrix instructions; and in 16 bits o comes in two pieces (o, and the rest that the forward saved) and ds
+// is taken in two pieces. 0.0017 (0.0020) from 64 bits, where the rounding of dq makes 0.0017; f32 rows of 64 with
+// means of 3: 2e-6, where it was 2e-5 (torch's operations in f32: 3e-6). What it costs: 4 scenes of 32256 bf16 tokens 171 us
+// without, 206 with two pieces, 225 with c, and the forward's rest 125 -> 137 us; 16 of 2048 f32 tokens 143 -> 146 us.
 template <typename T, int DP, int RW>
 __global__ __launch_bounds__(kThreads, (sizeof(T) == 2 ? (DP > 64 || RW == 1 ? 2 : 3) : DP <= 64 ? 2 : 1)) void k_attend_dq(Args a) {
   using M = Mma<T>;
@@ -642,7 +643,7 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 2 ? (DP > 64 || RW == 1 ? 2
   // From the list's end to its start: the last step then holds the first block's first unit, which has a key.
   const int last = units ? (units - 1) / U * U : -1;
   int step = 0;
-  float total = 0.f;  // 16 bits: of this lane's ds
+  float total = 0.f;  // of this lane's ds
   if (units) fetch(last);
   for (int u = last; u >= 0; u -= U, ++step) {
     char* tk = lds + (step % NB) * 2 * U * L::kUnit;
@@ -675,12 +676,10 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 2 ? (DP > 64 || RW == 1 ? 2
       }
       if constexpr (kFewExponents<T>)
         if (keep_in_range(x, dq, power)) times = __builtin_amdgcn_ldexpf(1.f, power);
-      if constexpr (sizeof(T) == 2) {
-        float sum = 0.f;
+      float sum = 0.f;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) sum += x[r];
-        total += kFewExponents<T> ? __builtin_amdgcn_ldexpf(sum, -power) : sum;
-      }
+      for (int r = 0; r < 16; ++r) sum += x[r];
+      total += kFewExponents<T> ? __builtin_amdgcn_ldexpf(sum, -power) : sum;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const Frag hi = acc_frag<T>(x, h), lo = sizeof(T) == 2 ? rest_frag<T>(x, hi, h) : Frag{};
@@ -693,26 +692,24 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 2 ? (DP > 64 || RW == 1 ? 2
       }
     }
   }
-  if constexpr (sizeof(T) == 2) {
-    if (units) {  // dq -= total c, c the mean of the last step's first unit (rows that do not count are zeros there)
-      total += __shfl_xor(total, 32, 64);
-      float w = total * (-1.f / (float)next.n[0]);
-      f32x16 one = {};
-      if constexpr (kFewExponents<T>) w = __builtin_amdgcn_ldexpf(w, power);
+  if (units) {  // dq -= total c, c the mean of the last step's first unit (rows that do not count are zeros there)
+    total += __shfl_xor(total, 32, 64);
+    float w = total * (-1.f / (float)next.n[0]);
+    f32x16 one = {};
+    if constexpr (kFewExponents<T>) w = __builtin_amdgcn_ldexpf(w, power);
 #pragma unroll
-      for (int r = 0; r < 16; ++r) one[r] = w;
-      if constexpr (kFewExponents<T>) keep_in_range(one, dq, power);
-      const char* uk = lds + ((step - 1) % NB) * 2 * U * L::kUnit;
-      const Frag hi = acc_frag<T>(one, 0), lo = rest_frag<T>(one, hi, 0);
+    for (int r = 0; r < 16; ++r) one[r] = w;
+    if constexpr (kFewExponents<T>) keep_in_range(one, dq, power);
+    const char* uk = lds + ((step - 1) % NB) * 2 * U * L::kUnit;
+    const Frag hi = acc_frag<T>(one, 0), lo = sizeof(T) == 2 ? rest_frag<T>(one, hi, 0) : Frag{};
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
+    for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int d = 0; d < ND; ++d) {
-          const Frag k = L::col(uk, h, d, lane);
-          dq[d] = M::mma(k, hi, dq[d]);
-          dq[d] = M::mma(k, lo, dq[d]);
-        }
-    }
+      for (int d = 0; d < ND; ++d) {
+        const Frag k = L::col(uk, h, d, lane);
+        dq[d] = M::mma(k, hi, dq[d]);
+        if constexpr (sizeof(T) == 2) dq[d] = M::mma(k, lo, dq[d]);
+      }
   }
   if constexpr (kFewExponents<T>) shift(dq, -power);
   if constexpr (KW > 1) {

@@ -519,13 +519,13 @@ def test_attention_of_a_cache_that_the_batch_shares(gpu):
     assert all(torch.equal(x, y) for x, y in zip(a, b))
 
 
-# ---- 16 bits: values and keys with a mean ------------------------------------------------------------
+# ---- values and keys with a mean ------------------------------------------------------------
 
 
 def query_gradient(q, k, v, do, scale, t):
     """(dq, how far off before it is rounded) in 64 bits. dq's terms are p (dp - delta) (k - c), for any c, as a row's p (dp - delta) add up to 0; c is the mean of
     the first 32 keys. dp and delta are sums of D 32-bit products, a score likewise, its exponent and logarithm off by 8 steps; ds is
-    two pieces of h each. delta is do . o of an o in two pieces, made of p rounded to h: n roundings of their own, so six
+    two pieces of h each (16 bits). delta is do . o of an o in two pieces, made of p rounded to h: n roundings of their own, so six
     standard deviations of their sum (each at most h)."""
     h, D, n = orc.half_step(t), q.shape[1], k.shape[0]
     x, dp = q @ k.T * scale, do @ v.T
@@ -542,7 +542,7 @@ def query_gradient(q, k, v, do, scale, t):
 
 
 @gpu_only
-@pytest.mark.parametrize("t", [BF16, F16])
+@pytest.mark.parametrize("t", TYPES)
 @pytest.mark.parametrize("key_mean,value_mean", [(0.0, 0.0), (3.0, 0.0), (0.0, 3.0), (1.0, 1.0), (3.0, 3.0)])
 @pytest.mark.parametrize("L,Hq,block,n,D", [(256, 1, 64, 1024, 64), (40, 2, 32, 500, 32), (130, 1, 128, 900, 128), (16, 2, 64, 4000, 96)])
 def test_query_gradients_of_keys_and_values_with_a_mean(gpu, t, key_mean, value_mean, L, Hq, block, n, D):
