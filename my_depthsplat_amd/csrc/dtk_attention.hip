@@ -37,13 +37,13 @@ __global__ __launch_bounds__(NT) void k_attend_join(Args a, int64_t rows) {
     for (int e = 0; e < 4; ++e) o[e] *= f0;
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-      if (s0 + k >= a.splits) break;  // (the last part's again: 0 times its infinities would be no number)
+      const bool part = s0 + k < a.splits;  // else the last part again: left out, as 0 times its infinities would be no number
       const float f = exp2f(pm[k] - base);
-      l += pl[k] * f;
-      o[0] += po[k].x * f;
-      o[1] += po[k].y * f;
-      o[2] += po[k].z * f;
-      o[3] += po[k].w * f;
+      l += part ? pl[k] * f : 0.f;
+      o[0] += part ? po[k].x * f : 0.f;
+      o[1] += part ? po[k].y * f : 0.f;
+      o[2] += part ? po[k].z * f : 0.f;
+      o[3] += part ? po[k].w * f : 0.f;
     }
   }
   const int64_t i = r % a.Lq, bh = r / a.Lq, b = bh / a.Hq, h = bh % a.Hq;
