@@ -33,7 +33,7 @@ CFLAGS = [
 CFLAGS += ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 # Per-file extra flags. The rasterizer's per-lane pixel math is scalar by design (pairs of list
-# entries are written out with explicit vector types, which this build lowers to scalar FMAs);
+# entries are written out with explicit vector types, which compile to scalar FMAs as above);
 # the SLP vectorizer packs the scalar parts with register shuffles (k_render_bwd 119 -> 109 us
 # without it at config B while packed FP32 was on; without that 90.6 K views/s against 90.3 K
 # with the vectorizer, 16 scenes of 2 views at 256 x 256).

@@ -2498,7 +2498,7 @@ __device__ __forceinline__ float fall_p2(const PixUV& p, float F, float D, float
 }
 // Two consecutive list entries with their fields interleaved, so the falloff of both runs as
 // two independent chains of FMAs on whole 16-byte reads, with no operand shuffling (one
-// instruction per element: the build has no packed FP32); per-element results are the same
+// instruction per element: packed FP32 is off); per-element results are the same
 // IEEE operations as fall_p2 (the backward's decisions agree).
 struct __align__(16) PairRec {
   f2v F, D, E, A, C, B;  // falloff fields of entries 0 and 1, interleaved; F holds

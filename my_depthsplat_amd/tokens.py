@@ -112,7 +112,8 @@ def block_sparse_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, in
     q [B,Lq,Hq,D], k, v [B,Lk,Hkv,D] (any strides with dense channels; D a multiple of 8 up to 128; query
     head h reads key head h / (Hq / Hkv), at most 1024 to one); index int32 [B, Hkv, ceil(Lq / block), top <= 1024], as
     select_blocks gives it: places outside the sequence's blocks, and second ones of a block, count
-    for nothing. lengths [B] as there: o is 0 behind q_lengths and for queries that see no key.
-    scale (a finite number): 1 / sqrt(D) by default. Scores and the softmax's statistics are held in 32 bits: past 2^20
+    for nothing. lengths [B] as there: o is 0 behind q_lengths and for queries that see no key. scale (a
+    finite number): 1 / sqrt(D) by default. A call that trains in 16 bits keeps a second tensor of o's size
+    for its backward. Scores and the softmax's statistics are held in 32 bits: past 2^20
     they lose digits that matter, past 2^30 a row may give no number."""
     return _lib.load_torch().block_sparse_attention(q, k, v, index, block, q_lengths, kv_lengths, scale)
