@@ -623,7 +623,8 @@ int dtk_select_blocks(int B, int64_t Lq, int64_t Lk, int Hq, int Hkv, int D, int
  * [B,Lq,Hq,D], k and v [B,Lk,Hkv,D]: element strides (batch, token, head), channels contiguous, D a
  * multiple of 8 up to 128; Hq a multiple of Hkv. o [B,Lq,Hq,D] contiguous: 0 for queries that see
  * no key and behind q_lengths. lse [B,Hq,Lq] (base 2; NULL when no backward follows). o_rest as o: what the rounding
- * of o to 16 bits left (f16: 2^11 times it), which the backward needs (NULL for DTK_F32 or when none follows). Few tiles: the lists are
+ * of o to 16 bits left (f16: 2^11 times it), which the backward needs (NULL for DTK_F32 or when none follows; with it the forward
+ * takes the probabilities in two 16-bit pieces). Few tiles: the lists are
  * split over workgroups and joined through the workspace. At most 1024 query heads per key head; token
  * strides below 2^24 elements; Lq, Lk at most 2^31 - 256; B and Hq below 2^16; a finite scale. Backward: dout with its strides; dq,
  * dk, dv contiguous, overwritten (0 behind the lengths), each sum in one order; dk and dv may both be NULL (not taken). */

@@ -14,13 +14,14 @@
 //
 // Probabilities, and ds for dk, are rounded to the inputs' type for the second products (the matrix instructions' operands),
 // as the inputs themselves were: a rounding of each term's own, so o, dv and dk of random rows are 0.0023 - 0.0024 of their
-// norm from 64 bits in bf16, where their own rounding alone makes 0.0017. dq takes ds in two pieces (k_attend_dq).
+// norm from 64 bits in bf16, where their own rounding alone makes 0.0017. What dq is made of is taken in two pieces: ds, and
+// the probabilities of a forward that trains (k_attend_dq says why); its o and dq are 0.0017 off.
 // All sums, the maximum, lse and delta are held in 32 bits. f32 operands stay f32.
 //
 // Measured (products taken, rate; a large bf16 product reaches 1060 TFLOP/s, f32 153):
 //   4 scenes of 32256 bf16 tokens (lengths from half of that on), 4 heads of 64 channels on 2, 16 blocks of 64:
-//     forward 125 us 570 TFLOP/s (137 us where a backward follows), dq 225 us 640 (four products), dk/dv 235 us 610
-//   16 scenes of 2048 f32 tokens, one head of 128 channels, 8 blocks of 64: 89 us 93, 146 us 85, 208 us 80
+//     forward 125 us 570 TFLOP/s; training forward 171 us 630 (three products), dq 218 us 660 (four), dk/dv 235 us 610
+//   16 scenes of 2048 f32 tokens, one head of 128 channels, 8 blocks of 64: 89 us 93, 144 us 86, 209 us 80
 //   12 views of 92160 bf16 tokens, 2 heads of 64, 16 blocks of 64, forward: 104 us 465
 // What bounds them: the forward and dq at 64 channels the vector unit (some 110 of its instructions per 32 x 32 scores, half of
 // its cycles, for 8 matrix instructions, a quarter of theirs; with 128 channels the forward comes to 730 TFLOP/s);
@@ -169,6 +170,23 @@ struct Tile {
     return f;
   }
 };
+
+// sum += rows^T x for the 32 rows of a unit and an accumulator's 32 x 32 numbers x, which 16-bit types take in two pieces (what rounding
+// the first left is the second).
+template <typename T, int DP>
+__device__ __forceinline__ void add_pieces(f32x16 (&sum)[DP / 32], const f32x16& x, const char* rows, int lane) {
+  using Frag = typename Mma<T>::Frag;
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+    const Frag hi = acc_frag<T>(x, s), lo = sizeof(T) == 2 ? rest_frag<T>(x, hi, s) : Frag{};
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d) {
+      const Frag r = Tile<T, DP>::col(rows, s, d, lane);
+      sum[d] = Mma<T>::mma(r, hi, sum[d]);
+      if constexpr (sizeof(T) == 2) sum[d] = Mma<T>::mma(r, lo, sum[d]);
+    }
+  }
+}
 
 // The workgroup's share of U units (32 rows each) on the way from memory to LDS: loaded into
 // registers while the tile before is worked on, then stored. Rows that do not count and channels
@@ -328,8 +346,9 @@ struct Join {
 // Forward. RW waves stand side by side over 32 rows each, 4 / RW take turns at the list's units
 // of 32 keys and are joined at the end. The rows of a tile are its queries of all heads that
 // share the key head (few queries: they fill the instruction's columns together). Few tiles: the list is split over
-// workgroups (splits_of) and k_attend_join adds them up.
-template <typename T, int DP, int RW>
+// workgroups (splits_of) and k_attend_join adds them up. PIECES: 16-bit p in two pieces, and o's rest, for a backward (an
+// instance of its own: as a branch it spills at four waves per SIMD, 103 -> 182 us for the 12 views).
+template <typename T, int DP, int RW, bool PIECES>
 __global__ __launch_bounds__(kThreads, (sizeof(T) == 2 ? (DP > 64 || RW == 1 ? 2 : 4) : 2)) void k_attend_fwd(Args a) {
   using M = Mma<T>;
   using L = Tile<T, DP>;
@@ -446,11 +465,15 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 2 ? (DP > 64 || RW == 1 ? 2
       }
     }
     l += sum;
-    const Frag p0 = acc_frag<T>(p, 0), p1 = acc_frag<T>(p, 1);
+    if constexpr (PIECES) {
+      add_pieces<T, DP>(o, p, tv, lane);
+    } else {
+      const Frag p0 = acc_frag<T>(p, 0), p1 = acc_frag<T>(p, 1);
 #pragma unroll
-    for (int d = 0; d < ND; ++d) {
-      o[d] = M::mma(L::col(tv, 0, d, lane), p0, o[d]);
-      o[d] = M::mma(L::col(tv, 1, d, lane), p1, o[d]);
+      for (int d = 0; d < ND; ++d) {
+        o[d] = M::mma(L::col(tv, 0, d, lane), p0, o[d]);
+        o[d] = M::mma(L::col(tv, 1, d, lane), p1, o[d]);
+      }
     }
   }
   l += __shfl_xor(l, 32, 64);
@@ -513,7 +536,7 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 2 ? (DP > 64 || RW == 1 ? 2
 #pragma unroll
       for (int k = 0; k < 4; ++k) v[k] = valid ? o[d][4 * c + k] * inv : 0.f;
       store4<T>((T*)a.out + to + e, v[0], v[1], v[2], v[3]);
-      if (sizeof(T) == 2 && a.rest) store_rest4<T>((T*)a.rest + to + e, v[0], v[1], v[2], v[3]);
+      if (PIECES) store_rest4<T>((T*)a.rest + to + e, v[0], v[1], v[2], v[3]);
     }
   if (half == 0 && a.lse) a.lse[((int64_t)at.b * a.Hq + h) * a.Lq + i] = valid ? base2 + log2f(l) : -INFINITY;
 }
@@ -561,13 +584,12 @@ __device__ __forceinline__ void shift(f32x16 (&sum)[ND], int power) {
 // way, kept for dk.
 //
 // A row's ds add up to 0, so what all keys have in common falls out of dq = sum ds k, and what all values have in
-// common out of ds = p (dp - delta). A rounding of ds leaves a share of the keys' common part in it, one of o (which delta
-// is made of) a share of both: with keys and values of a mean of 1 (3) times their spread, 1024 bf16 keys, dq was off by 0.037
-// (0.34) of its norm. So c, the mean of some keys (the first block's first 32), is taken off all keys by subtracting (sum ds) c at
-// the end, a few matrix instructions; and in 16 bits o comes in two pieces (o, and the rest that the forward saved) and ds
-// is taken in two pieces. 0.0017 (0.0020) from 64 bits, where the rounding of dq makes 0.0017; f32 rows of 64 with
-// means of 3: 2e-6, where it was 2e-5 (torch's operations in f32: 3e-6). What it costs: 4 scenes of 32256 bf16 tokens 171 us
-// without, 206 with two pieces, 225 with c, and the forward's rest 125 -> 137 us; 16 of 2048 f32 tokens 143 -> 146 us.
+// common out of ds = p (dp - delta). A rounding of ds leaves a share of the keys' common part in it, one of delta
+// a share of both: with 16-bit ds, and delta of an o made of 16-bit p and rounded itself, bf16 keys and values with a mean of 1 (3) times
+// their spread, 1024 of them, put dq 0.037 (0.34) of its norm off. So ds is two pieces, p of the forward that trains
+// likewise, and that forward keeps what the rounding of o left: 0.0017 (0.0017), which the rounding of dq alone makes. (4 scenes of
+// 32256 bf16 tokens: dq 171 -> 218 us, the forward 125 -> 171. Subtracting (sum ds) times a mean of some keys at the end
+// instead of the forward's second piece takes as long, and lets keys that a row does not see enter its dq.)
 template <typename T, int DP, int RW>
 __global__ __launch_bounds__(kThreads, (sizeof(T) == 2 ? (DP > 64 || RW == 1 ? 2 : 3) : DP <= 64 ? 2 : 1)) void k_attend_dq(Args a) {
   using M = Mma<T>;
@@ -640,12 +662,8 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 2 ? (DP > 64 || RW == 1 ? 2
     sk.load(pk, next.n, a.k.l, a.D);
     sv.load(pv, next.n, a.v.l, a.D);
   };
-  // From the list's end to its start: the last step then holds the first block's first unit, which has a key.
-  const int last = units ? (units - 1) / U * U : -1;
-  int step = 0;
-  float total = 0.f;  // of this lane's ds
-  if (units) fetch(last);
-  for (int u = last; u >= 0; u -= U, ++step) {
+  if (units) fetch(0);
+  for (int u = 0, step = 0; u < units; u += U, ++step) {
     char* tk = lds + (step % NB) * 2 * U * L::kUnit;
     char* tv = tk + U * L::kUnit;
     if (NB == 1) __syncthreads();
@@ -653,7 +671,7 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 2 ? (DP > 64 || RW == 1 ? 2
     sv.store(tv);
     __syncthreads();
     const Span<U> now = next;
-    if (u > 0) fetch(u - U);
+    if (u + U < units) fetch(u + U);
 #pragma unroll 1
     for (int e = 0; e < EACH; ++e) {
       const char *uk = tk + (e * KW + kw) * L::kUnit, *uv = tv + (e * KW + kw) * L::kUnit;
@@ -676,40 +694,8 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 2 ? (DP > 64 || RW == 1 ? 2
       }
       if constexpr (kFewExponents<T>)
         if (keep_in_range(x, dq, power)) times = __builtin_amdgcn_ldexpf(1.f, power);
-      float sum = 0.f;
-#pragma unroll
-      for (int r = 0; r < 16; ++r) sum += x[r];
-      total += kFewExponents<T> ? __builtin_amdgcn_ldexpf(sum, -power) : sum;
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const Frag hi = acc_frag<T>(x, h), lo = sizeof(T) == 2 ? rest_frag<T>(x, hi, h) : Frag{};
-#pragma unroll
-        for (int d = 0; d < ND; ++d) {
-          const Frag k = L::col(uk, h, d, lane);
-          dq[d] = M::mma(k, hi, dq[d]);
-          if constexpr (sizeof(T) == 2) dq[d] = M::mma(k, lo, dq[d]);
-        }
-      }
+      add_pieces<T, DP>(dq, x, uk, lane);
     }
-  }
-  if (units) {  // dq -= total c, c the mean of the last step's first unit (rows that do not count are zeros there)
-    total += __shfl_xor(total, 32, 64);
-    float w = total * (-1.f / (float)next.n[0]);
-    f32x16 one = {};
-    if constexpr (kFewExponents<T>) w = __builtin_amdgcn_ldexpf(w, power);
-#pragma unroll
-    for (int r = 0; r < 16; ++r) one[r] = w;
-    if constexpr (kFewExponents<T>) keep_in_range(one, dq, power);
-    const char* uk = lds + ((step - 1) % NB) * 2 * U * L::kUnit;
-    const Frag hi = acc_frag<T>(one, 0), lo = sizeof(T) == 2 ? rest_frag<T>(one, hi, 0) : Frag{};
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-      for (int d = 0; d < ND; ++d) {
-        const Frag k = L::col(uk, h, d, lane);
-        dq[d] = M::mma(k, hi, dq[d]);
-        if constexpr (sizeof(T) == 2) dq[d] = M::mma(k, lo, dq[d]);
-      }
   }
   if constexpr (kFewExponents<T>) shift(dq, -power);
   if constexpr (KW > 1) {
@@ -1039,7 +1025,10 @@ inline int splits_of(int64_t workgroups, int units) {
 template <typename T, int DP, int RW>
 struct Fwd {
   static int go(const Args& a, dim3 grid, hipStream_t st) {
-    return launch(k_attend_fwd<T, DP, RW>, a, grid, kTileBytes<T, DP, 4 / RW> + a.top * sizeof(int32_t), st, "k_attend_fwd");
+    const size_t lds = kTileBytes<T, DP, 4 / RW> + a.top * sizeof(int32_t);
+    if constexpr (sizeof(T) == 2)
+      if (a.rest) return launch(k_attend_fwd<T, DP, RW, true>, a, grid, lds, st, "k_attend_fwd");
+    return launch(k_attend_fwd<T, DP, RW, false>, a, grid, lds, st, "k_attend_fwd");
   }
 };
 template <typename T, int DP, int RW>

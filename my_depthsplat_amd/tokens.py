@@ -113,7 +113,8 @@ def block_sparse_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, in
     head h reads key head h / (Hq / Hkv), at most 1024 to one); index int32 [B, Hkv, ceil(Lq / block), top <= 1024], as
     select_blocks gives it: places outside the sequence's blocks, and second ones of a block, count
     for nothing. lengths [B] as there: o is 0 behind q_lengths and for queries that see no key. scale (a
-    finite number): 1 / sqrt(D) by default. A call that trains in 16 bits keeps a second tensor of o's size
-    for its backward. Scores and the softmax's statistics are held in 32 bits: past 2^20
+    finite number): 1 / sqrt(D) by default. A call that trains in 16 bits takes the probabilities in two pieces
+    (its o may differ from a call's without gradients by their rounding) and keeps a second tensor of o's
+    size for its backward. Scores and the softmax's statistics are held in 32 bits: past 2^20
     they lose digits that matter, past 2^30 a row may give no number."""
     return _lib.load_torch().block_sparse_attention(q, k, v, index, block, q_lengths, kv_lengths, scale)

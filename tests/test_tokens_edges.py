@@ -522,23 +522,22 @@ def test_attention_of_a_cache_that_the_batch_shares(gpu):
 # ---- values and keys with a mean ------------------------------------------------------------
 
 
-def query_gradient(q, k, v, do, scale, t):
-    """(dq, how far off before it is rounded) in 64 bits. dq's terms are p (dp - delta) (k - c), for any c, as a row's p (dp - delta) add up to 0; c is the mean of
-    the first 32 keys. dp and delta are sums of D 32-bit products, a score likewise, its exponent and logarithm off by 8 steps; ds is
-    two pieces of h each (16 bits). delta is do . o of an o in two pieces, made of p rounded to h: n roundings of their own, so six
-    standard deviations of their sum (each at most h)."""
-    h, D, n = orc.half_step(t), q.shape[1], k.shape[0]
+def query_gradient(q, k, v, do, scale):
+    """(dq, how far off before it is rounded) in 64 bits, for any type. dp, delta and a score are sums of D 32-bit products, the score's
+    exponent and logarithm off by 8 steps. p (for o, which delta is made of), o and ds are 32-bit numbers, or two pieces
+    of 16 bits (bf16's keep 2^-16 of a value; n roundings of p, so six standard deviations of their sum); o and dq are sums over
+    the n keys."""
+    D, n, E, two = q.shape[1], k.shape[0], orc.E32, 2.0 ** -16
     x, dp = q @ k.T * scale, do @ v.T
     p = torch.softmax(x, -1)
     o = p @ v
     delta = (do * o).sum(-1, keepdim=True)
     ds = p * (dp - delta)
-    e_x = (D * (q.abs() @ k.abs().T) * abs(scale) + 8 * (1 + x.abs())) * orc.E32
-    e_o = 6 * h * (p.square() @ v.square()).sqrt() + (p * (2 * e_x + n * orc.E32)) @ v.abs() + (2 * h * h + 2 * orc.E32) * o.abs()
-    e_delta = (do.abs() * e_o).sum(-1, keepdim=True) + D * orc.E32 * (do.abs() * o.abs()).sum(-1, keepdim=True)
-    e_ds = p * D * orc.E32 * (do.abs() @ v.abs().T) + ds.abs() * (2 * e_x + h * h + (n + 4) * orc.E32)
-    dq, off = ds @ k * scale, k - k[:32].mean(0)
-    return dq, (e_ds @ off.abs() + e_delta * (p @ off).abs()) * abs(scale)
+    e_x = (D * (q.abs() @ k.abs().T) * abs(scale) + 8 * (1 + x.abs())) * E
+    e_o = 6 * two * (p.square() @ v.square()).sqrt() + (p * 2 * e_x) @ v.abs() + n * E * (p @ v.abs()) + two * o.abs()
+    e_delta = (do.abs() * e_o).sum(-1, keepdim=True) + D * E * (do.abs() * o.abs()).sum(-1, keepdim=True)
+    e_ds = p * D * E * (do.abs() @ v.abs().T) + ds.abs() * (2 * e_x + two + (n + 4) * E)
+    return ds @ k * scale, (e_ds @ k.abs() + e_delta * (p @ k).abs()) * abs(scale)
 
 
 @gpu_only
@@ -556,7 +555,7 @@ def test_query_gradients_of_keys_and_values_with_a_mean(gpu, t, key_mean, value_
     leaves = [x.to(gpu).requires_grad_(True) for x in (q, k, v)]
     (got,) = torch.autograd.grad(tokens.block_sparse_attention(*leaves, index, block=block), leaves[:1], do.to(gpu))
     for head in range(Hq):
-        want, off = query_gradient(*(x[0, :, min(head, x.shape[2] - 1)].double() for x in (q, k, v, do)), D ** -0.5, t)
+        want, off = query_gradient(*(x[0, :, min(head, x.shape[2] - 1)].double() for x in (q, k, v, do)), D ** -0.5)
         h, dq = orc.half_step(t), got[0, :, head]
         orc.assert_within(dq, want, off + h * want.abs() + orc.tiny(t), "dq")
         # (roundings are spread evenly over a step: together at most 0.58 of the half step, that of a value just above a power of two)
